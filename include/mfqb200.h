@@ -432,6 +432,86 @@ int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_s
 int mfqb_decoder_free(mfqb_decoder* d);
 
 /* ---------------------------------------------------------------------------------
+ * A key/value cache in pages that sequences share, and what a decoder does over it besides one greedy token: it checks a tree
+ * of drafted tokens in one pass, keeps the branch that the model agrees with, and moves beams.  (The reference's cache is one
+ * contiguous buffer per sequence, mfq/kernels/cuda/kv_cache.cu; it has no counterpart of these calls.)
+ *
+ * The view is plain memory of the caller, all of it on the device that is current at the call:
+ *   k, v    bf16 [layers][pages][kv_heads][page][128], 16-byte aligned; page a power of two, 16 to 1024 tokens
+ *   table   int32 [rows][width]: the page that holds positions i * page .. of a sequence, -1 behind its last one
+ *   lens    int32 [rows]: tokens of every sequence in the cache
+ *   refs    int32 [pages]: how many table entries (or other holders) use a page; 0 or less = free
+ * rows <= 1024.  A table entry outside [0, pages) counts as no page: nothing is read or written through it.  A length outside
+ * [0, width * page] is taken as the nearer end.  Head size 128, heads in groups: query head h reads kv head h / (q_heads / kv_heads).
+ *
+ * Pages are written only at positions from lens on, and mfqb_cache_fork leaves every page that is partly filled to one
+ * sequence, so pages that sequences share are never written.  Calls on one cache must be ordered by their streams; calls on
+ * different caches share nothing.  No call allocates memory, none waits for the device: all can be captured.
+ * --------------------------------------------------------------------------------- */
+typedef struct mfqb_cache {
+    void* k;
+    void* v;
+    int32_t* table;
+    int32_t* lens;
+    int32_t* refs;
+    int layers, kv_heads, page, pages, rows, width;
+} mfqb_cache;
+
+/* Reserves pages for tokens[r] more tokens of every sequence r (device int32 [rows]; 0 or less: none).  Free pages go out in
+ * ascending order, to the sequences in ascending order.  status (device int32 [1]): 0, or how many pages were missing in the pool
+ * or in the table: then nothing has changed. */
+int mfqb_cache_extend(const mfqb_cache* c, const int32_t* tokens, int32_t* status, mfqb_stream_t stream);
+
+/* Sequence r goes on as sequence parents[r] (device int32 [rows]; -1: it ends, its pages go back).  Whole pages are shared; a page
+ * that is partly filled stays with the first sequence that goes on with it, the others get copies of its filled part (free pages
+ * in ascending order, to the sequences in ascending order), in all layers.  Pages that were reserved behind the length go back.
+ * status (device int32 [1]): 0; how many pages were missing; or -1 for an entry of parents outside [-1, rows).  Where it is not
+ * 0 nothing has changed.  work: device memory of mfqb_cache_fork_work bytes, 16-byte aligned. */
+int mfqb_cache_fork_work(const mfqb_cache* c, uint64_t* bytes);
+int mfqb_cache_fork(const mfqb_cache* c, const int32_t* parents, int32_t* status, void* work, uint64_t work_bytes, mfqb_stream_t stream);
+
+/* Trees of drafted tokens: parents (device int32 [rows][nodes], nodes <= 64) holds -1 for node 0 (the sequence's last token, which
+ * is not in the cache yet) and an earlier node for every other one.  A node with any other entry, and every node under it, is
+ * unused; a first node that is not -1 leaves the whole row unused.  masks: uint64 [rows][nodes], bit j = node j is the node itself
+ * or above it (0 for unused nodes); depths: int32 [rows][nodes], 0 for the root and for unused nodes. */
+int mfqb_tree_masks(const int32_t* parents, int rows, int nodes, uint64_t* masks, int32_t* depths, mfqb_stream_t stream);
+
+/* Rotary embedding and cache write of the nodes of every sequence: qkv float32 [rows][nodes][(q_heads + 2 kv_heads) * 128] (query
+ * heads, key heads, value heads), halves convention, position lens[r] + depths[r][i], angle position * freqs[j] for pair (j, j + 64)
+ * (freqs: device float64 [64]; the angle is formed and reduced in 64 bits).  The keys and values of node i go to slot
+ * lens[r] + i of the layer, rounded to bf16; q_out: bf16 [rows][nodes][q_heads][128].  lens stays. */
+int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_heads, int nodes, const int32_t* depths, const double* freqs,
+                     void* q_out, mfqb_stream_t stream);
+
+/* Attention of the nodes over the cache: q, out bf16 [rows][nodes][q_heads][128].  Node i of sequence r sees the positions below
+ * lens[r] and those nodes j (at position lens[r] + j) whose bit is set in masks[r][i]; out = softmax(scale * q.k) v over what it sees,
+ * zeros where it sees nothing.  What a node does not see has no effect on it, an infinity or NaN neither.  Scores, maxima and sums
+ * are float32; probabilities are rounded to bf16 once, their sum is that of the rounded ones.
+ * work: device memory of mfqb_tree_attention_work bytes, 16-byte aligned. */
+int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes);
+int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out,
+                        void* work, uint64_t work_bytes, mfqb_stream_t stream);
+
+/* Keeps the branch of every tree that the model agrees with: from the root on, the lowest child whose drafted token ids[r][child] is
+ * the model's own targets[r][node] (device int32 [rows][nodes]).  Keys and values of the branch move together in all layers, to
+ * slots lens[r] .. lens[r] + count[r] - 1.  Per sequence (device int32): count, the branch's nodes with the root; token, the target of
+ * its last node; path [rows][nodes], the nodes, -1 behind them; lens_out = lens + count (it may be lens itself).  An unused row has
+ * count 0, token -1 and keeps its length. */
+int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count,
+                     int32_t* token, int32_t* path, int32_t* lens_out, mfqb_stream_t stream);
+
+/* Beam selection: logits float32 [groups][beams][vocab], scores float32 [groups][beams].  The k best candidates of every group by
+ * scores + log softmax(logits), largest first, into out_scores float32 [groups][k], out_rows int32 (group * beams + beam: what
+ * mfqb_cache_fork takes) and out_tokens int32.  Candidates of one beam are ordered by logit, equal ones by token; candidates of
+ * different beams by score (log sums and scores are compared in 64 bits), equal ones by beam.  A NaN counts as minus infinity.
+ * A beam with a non-zero entry in done (int32 [groups][beams], may be null) has one candidate: the token eos at its own score.
+ * Where a group has fewer than k candidates the rest is row -1, token -1, score minus infinity.  beams <= 128, k <= min(128, vocab),
+ * vocab <= 1048576.  work: device memory of mfqb_beam_select_work bytes, 16-byte aligned. */
+int mfqb_beam_select_work(int groups, int beams, int vocab, int k, uint64_t* bytes);
+int mfqb_beam_select(const float* logits, int groups, int beams, int vocab, const float* scores, const int32_t* done, int eos, int k,
+                     float* out_scores, int32_t* out_rows, int32_t* out_tokens, void* work, uint64_t work_bytes, mfqb_stream_t stream);
+
+/* ---------------------------------------------------------------------------------
  * Host-side self-check of the device layout (no GPU): packs the blob into the device
  * format, reads every code and scale field back through the same accessors the kernels
  * use, and reports the number of mismatches against the file streams.

@@ -38,6 +38,11 @@ class DecoderConfig(C.Structure):
                 ("rope_theta", C.c_float), ("rms_eps", C.c_float)]
 
 
+class CacheView(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("layers", C.c_int),
+                ("kv_heads", C.c_int), ("page", C.c_int), ("pages", C.c_int), ("rows", C.c_int), ("width", C.c_int)]
+
+
 class MoeInfo(C.Structure):
     _fields_ = [("n_experts", C.c_int), ("out_per_expert", C.c_int), ("k", C.c_int), ("expert_begin", C.c_int),
                 ("expert_end", C.c_int), ("n_pools", C.c_int), ("device", C.c_int), ("payload_bytes", C.c_uint64),
@@ -89,6 +94,16 @@ _SIGNATURES = {
     "mfqb_decoder_read_cache": (_i, [_vp, _i, _i, _i, _i, _vp, _vp]),
     "mfqb_decoder_read_logits": (_i, [_vp, _i, _vp, _vp]),
     "mfqb_decoder_free": (_i, [_vp]),
+    "mfqb_cache_extend": (_i, [_P(CacheView), _vp, _vp, _vp]),
+    "mfqb_cache_fork_work": (_i, [_P(CacheView), _P(_u64)]),
+    "mfqb_cache_fork": (_i, [_P(CacheView), _vp, _vp, _vp, _u64, _vp]),
+    "mfqb_tree_masks": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
+    "mfqb_cache_write": (_i, [_P(CacheView), _i, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "mfqb_tree_attention_work": (_i, [_P(CacheView), _i, _i, _P(_u64)]),
+    "mfqb_tree_attention": (_i, [_P(CacheView), _i, _vp, _i, _i, _vp, C.c_float, _vp, _vp, _u64, _vp]),
+    "mfqb_tree_accept": (_i, [_P(CacheView), _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
+    "mfqb_beam_select_work": (_i, [_i, _i, _i, _i, _P(_u64)]),
+    "mfqb_beam_select": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _u64, _vp]),
     "mfqb_mul_mat_host": (_i, [_vp, _vp, _i, _vp, _i]),
     "mfqb_mul_mat_host_multi": (_i, [_P(_vp), _i, _P(_vp), _i, _P(_vp), _i]),
     "mfqb_tp_plan": (_i, [_i64, _i64, _i, _P(C.c_double), _P(_i64), _P(_i64)]),

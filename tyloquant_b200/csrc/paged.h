@@ -1,0 +1,54 @@
+// Checks and launch helpers shared by the kernels on a paged key/value cache (mfqb_cache).
+#pragma once
+#include <algorithm>
+
+#include "cuda_util.h"
+
+namespace mfqb {
+
+constexpr int kHeadDim = 128;
+constexpr int kTreeNodes = 64;    // nodes of a drafted tree: one bit of a mask each
+constexpr int kCacheRows = 1024;  // sequences of a cache: one thread each in the kernels that give out pages
+
+// Throws unless the view describes a cache that the kernels take.  Their index arithmetic relies on these bounds: positions fit 31
+// bits, page numbers and table entries too; offsets into the pools are formed in 64 bits.
+inline void check_cache(const mfqb_cache* c, const char* who) {
+    if (!c) fail(MFQB_ERR_ARG, "%s: null cache", who);
+    if (!c->k || !c->v || !c->table || !c->lens || !c->refs) fail(MFQB_ERR_ARG, "%s: the cache has a null pointer", who);
+    if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) fail(MFQB_ERR_ARG, "%s: key and value pools must be 16-byte aligned", who);
+    if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1))) fail(MFQB_ERR_UNSUPPORTED, "%s: a page must hold 16 to 1024 tokens, a power of two, got %d", who, c->page);
+    if (c->layers < 1 || c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 1024) fail(MFQB_ERR_ARG, "%s: layers, pages and heads must be positive (heads at most 1024)", who);
+    if (c->rows < 1 || c->rows > kCacheRows) fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to %d sequences, got %d", who, kCacheRows, c->rows);
+    if (c->width < 1 || (int64_t)c->width * c->page > (1ll << 30) || (int64_t)c->width * c->rows > (1ll << 30))
+        fail(MFQB_ERR_UNSUPPORTED, "%s: at most 2^30 positions per sequence and table entries, got %d pages of %d", who, c->width, c->page);
+}
+inline void check_nodes(const mfqb_cache* c, int nodes, const char* who) {
+    if (nodes < 1 || nodes > kTreeNodes) fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to %d nodes per sequence, got %d", who, kTreeNodes, nodes);
+    if ((int64_t)nodes > (int64_t)c->width * c->page) fail(MFQB_ERR_ARG, "%s: %d nodes do not fit a table of %d pages of %d", who, nodes, c->width, c->page);
+}
+
+// Launched with the programmatic-dependent-launch attribute: the kernel becomes resident while its predecessor runs and waits
+// (after_predecessor) until that one has completed.
+template <typename... KArgs, typename... Args>
+void launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MFQB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+}
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ void chained_wait() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+#endif
+
+}  // namespace mfqb
