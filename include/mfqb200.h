@@ -486,7 +486,7 @@ int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_hea
 /* Attention of the nodes over the cache: q, out bf16 [rows][nodes][q_heads][128].  Node i of sequence r sees the positions below
  * lens[r] and those nodes j (at position lens[r] + j) whose bit is set in masks[r][i]; out = softmax(scale * q.k) v over what it sees,
  * zeros where it sees nothing.  What a node does not see has no effect on it, an infinity or NaN neither.  Scores, maxima and sums
- * are float32; probabilities are rounded to bf16 once, their sum is that of the rounded ones.
+ * are float32, probabilities are rounded to bf16 once.  scale: positive and finite.
  * work: device memory of mfqb_tree_attention_work bytes, 16-byte aligned. */
 int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes);
 int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out,

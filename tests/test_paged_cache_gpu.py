@@ -2,8 +2,8 @@
 reserved and forked pages, beam selection, and a run of them as a decoder uses them.
 
 Tolerances.  A bf16 result is off by at most half a step, 2^-8 of its size.  Attention rounds each probability to bf16 too, 2^-8 of
-it; the weights are normalised with the sum of the rounded ones, so numerator and denominator move the average by at most
-2 * 2^-8 times the average of |v|.  Float32 scores of 128 terms and the exponentials add less than 2^-12 of that average
+it, and may do so in the sum of the products and in the sum that normalises it: the average moves by at most 2 * 2^-8 times the
+average of |v|.  Float32 scores of 128 terms and the exponentials add less than 2^-12 of that average
 (|score| <= 60 in these tests: 128 * 2^-24 * 60 * log2(e))."""
 
 import numpy as np

@@ -1,65 +1,681 @@
 // Attention of a tree of drafted tokens over a paged key/value cache.
+//
+// Per sequence and kv head the queries of all nodes and of the heads that share the kv head are the rows of one matrix Q (row
+// node * G + head): S = Q K^T, P = exp2(scale' S - m), O = P V over tiles of 128 positions, with a running maximum m and sum l per row.
+// The work is cut into units (sequence, kv head, tile of 128 rows, tile of 128 positions), which are shared out evenly and in
+// order over the CTAs, one per SM, from the lengths as they are on the device: a batch of very different lengths loads
+// the SMs alike, and a captured call follows the lengths of each replay.  A stretch of units of one (sequence, head, row tile) that
+// covers all its positions is written as it is; otherwise the CTA leaves O, m and l, and tree_merge_kernel adds the parts in the order of
+// the context (no atomics: a call repeats bit for bit).
+//
+// Roles in a CTA of eight warps: one asks for pages (bulk tensor copies into a ring of six 32 KB tiles, keys and values in the
+// order of their use, with the 128-byte swizzle), one issues tcgen05.mma, four do the softmax (a row a thread): S comes out of tensor
+// memory, P goes back into it as the A operand of the second product, O stays there.  O is multiplied by a correction
+// only when a row's maximum has grown by more than 2^8 (P then stays below 2^8, which bf16 holds as exactly as values below 1).
+#include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <mutex>
+
 #include "paged.h"
+#include "tc05.cuh"
 
 namespace mfqb {
 
-// CTA (query head, node, sequence), four warps that take every fourth position each.
-__global__ void __launch_bounds__(128) tree_attn_kernel(mfqb_cache c, int layer, const __nv_bfloat16* __restrict__ q, int hq, int nodes,
-                                                        const unsigned long long* __restrict__ masks, float scale, __nv_bfloat16* __restrict__ out) {
-    chained_wait();
-    __shared__ float s_acc[4][kHeadDim], s_m[4], s_l[4];
-    const int h = blockIdx.x, node = blockIdx.y, r = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = h / (hq / c.kv_heads);
-    const int64_t cap = (int64_t)c.width * c.page;
-    const int64_t len = min(max((int64_t)c.lens[r], (int64_t)0), cap), end = min(len + nodes, cap);
-    const int64_t item = ((int64_t)r * nodes + node) * hq + h;
-    const unsigned long long mask = masks[(int64_t)r * nodes + node];
-    auto load4 = [](const __nv_bfloat16* p) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
-    };
-    float4 qv = load4(q + item * kHeadDim + 4 * lane);
-    const float f = scale * 1.4426950408889634f;
-    qv.x *= f; qv.y *= f; qv.z *= f; qv.w *= f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = -INFINITY, l = 0.f;
-    bool seen = false;
-    for (int64_t t = warp; t < end; t += 4) {
-        if (t >= len && !((mask >> (t - len)) & 1ull)) continue;
-        const int page = c.table[(int64_t)r * c.width + t / c.page];
-        if ((unsigned)page >= (unsigned)c.pages) continue;
-        const int64_t off = ((((int64_t)layer * c.pages + page) * c.kv_heads + kvh) * c.page + (t & (c.page - 1))) * kHeadDim + 4 * lane;
-        const float4 kv = load4(static_cast<const __nv_bfloat16*>(c.k) + off), vv = load4(static_cast<const __nv_bfloat16*>(c.v) + off);
-        float s = qv.x * kv.x + qv.y * kv.y + qv.z * kv.z + qv.w * kv.w;
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        seen = true;
-        const float mn = fmaxf(m, s);
-        const float corr = m == -INFINITY ? 0.f : exp2f(m - mn);
-        const float p = __bfloat162float(__float2bfloat16_rn(mn == -INFINITY ? 0.f : exp2f(s - mn)));
-        l = l * corr + p;
-        acc.x = acc.x * corr + p * vv.x; acc.y = acc.y * corr + p * vv.y; acc.z = acc.z * corr + p * vv.z; acc.w = acc.w * corr + p * vv.w;
-        m = mn;
+int* device_status_word(int device);
+
+constexpr int kTreeCtas = 148;                       // one per SM
+constexpr int kTile = 128;                           // rows of Q, positions of a tile
+constexpr int kTreeRing = 6, kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
+constexpr int kTreeThreads = 256, kSoftmaxThreads = 128;
+constexpr size_t kTreeSmem = (size_t)(kTreeRing + 1) * kTileBytes + 1024;   // ring, Q, alignment
+constexpr uint32_t kColS = 0, kColO = 256, kColP = 384;   // tensor memory columns: S twice, O, P twice (64 each)
+
+struct TreeArgs {
+    const int* table;
+    const int* lens;
+    const __nv_bfloat16* q;
+    const unsigned long long* masks;
+    const __nv_bfloat16 *k, *v;   // of the layer
+    __nv_bfloat16* out;
+    float* part;                  // [CTA][first, last][rows of a tile][128], then their (maximum, sum)
+    float2* part_ml;
+    int* error;
+    int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // tile_rows: rows of a part, at most 128
+    float scale_log2;
+};
+
+// Tiles of sequence r (at least one: a sequence has a node), its length and end.
+struct TreeSeq {
+    int64_t len, end;
+    int tiles;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
+    const int64_t cap = (int64_t)a.width * a.page;
+    TreeSeq s;
+    s.len = min(max((int64_t)__ldcg(a.lens + r), (int64_t)0), cap);
+    s.end = min(s.len + a.nodes, cap);
+    s.tiles = (int)((s.end + kTile - 1) / kTile);
+    return s;
+}
+// Sum of tiles of the rows before `row` and of all rows; 256 threads.
+__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int row, int64_t& before, int64_t& total, int64_t (*red)[2]) {
+    int64_t b = 0, t = 0;
+    for (int r = threadIdx.x; r < a.rows; r += 256) {
+        const int n = tree_seq(a, r).tiles;
+        t += n;
+        if (r < row) b += n;
     }
-    if (m == -INFINITY && seen) l = NAN;   // every score minus infinity
-    *reinterpret_cast<float4*>(&s_acc[warp][4 * lane]) = acc;
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+    for (int o = 16; o > 0; o >>= 1) {
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if ((threadIdx.x & 31) == 0) { red[threadIdx.x >> 5][0] = b; red[threadIdx.x >> 5][1] = t; }
     __syncthreads();
-    float mm = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), ll = 0.f, a = 0.f;
-    for (int w = 0; w < 4; ++w) {
-        const float cw = s_m[w] == mm ? 1.f : exp2f(s_m[w] - mm);
-        if (s_m[w] == -INFINITY && mm > -INFINITY) continue;
-        ll += s_l[w] * cw;
-        a += s_acc[w][threadIdx.x] * cw;
-    }
-    out[item * kHeadDim + threadIdx.x] = __float2bfloat16_rn(ll == 0.f ? 0.f : a / ll);
+    before = total = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) { before += red[w][0]; total += red[w][1]; }
 }
 
-static uint64_t tree_attention_work_bytes(const mfqb_cache&, int, int) { return 16; }
+struct TreeShared {
+    uint64_t kv_full[kTreeRing], kv_empty[kTreeRing], q_full, s_full[2], s_free[2], p_full[2], o_done[2], drain, group;
+    unsigned long long bad_nodes;   // nodes of the stretch whose values hold an infinity or NaN
+    int64_t red[8][2], scan[8];
+    int64_t first, last, item_off;  // the CTA's units; offset of its first one in its sequence's
+    int row0;
+    uint32_t tmem;
+    unsigned good[8];               // per tile (index mod 8): bit g = the 16 positions of group g have a page
+    int failed;
+};
+
+// A CTA's stretches in order: sequence, item (kv head, row tile), tiles [t0, t1) of seq.tiles.
+struct TreeWalk {
+    int r, item, t0, t1;
+    int64_t left;
+    TreeSeq seq;
+    __device__ __forceinline__ void start(const TreeArgs& a, const TreeShared& sh) {
+        r = sh.row0;
+        left = sh.last - sh.first;
+        if (left > 0) {
+            seq = tree_seq(a, r);
+            item = (int)(sh.item_off / seq.tiles);
+            t0 = (int)(sh.item_off % seq.tiles);
+            t1 = (int)min((int64_t)seq.tiles, t0 + left);
+        }
+    }
+    __device__ __forceinline__ void next(const TreeArgs& a) {
+        left -= t1 - t0;
+        if (left <= 0) return;
+        if (++item == a.kv_heads * a.row_tiles) {
+            item = 0;
+            seq = tree_seq(a, ++r);
+        }
+        t0 = 0;
+        t1 = (int)min((int64_t)seq.tiles, left);
+    }
+};
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+// D (+)= A B^T, both operands in shared memory.
+__device__ __forceinline__ void tc_mma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// bf16 x bf16 -> f32; B with its K index running over rows of 128 bytes (values: position by position) where mn is set.
+constexpr uint32_t instr_desc_bf16(int m, int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Descriptor of a [positions][64 dims] half in 128-byte rows taken as B operand with the dims as its rows: eight positions 1024
+// bytes apart, the next 64 dims one half further.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(kHalfBytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+#define MFQB_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define MFQB_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+// 32 lanes x 32 columns, a lane's columns in its registers; the load's values may be used after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : MFQB_R8(r, 0), MFQB_R8(r, 8), MFQB_R8(r, 16), MFQB_R8(r, 24)
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::MFQB_W8(r, 0), MFQB_W8(r, 8), MFQB_W8(r, 16), MFQB_W8(r, 24), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MFQB_W8(r, 0), MFQB_W8(r, 8), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
+// Position in the ring's sequence of the key and value tiles of a stretch of n tiles: K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1).
+__device__ __forceinline__ int key_at(int i) { return i ? 2 * i - 1 : 0; }
+__device__ __forceinline__ int value_at(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
+
+// Rare: values of visible nodes that hold an infinity or NaN were taken out of the product (0 in their place, so that rows which do not see
+// the node keep clear of them); here they are added to the row's result, where the row sees them.
+template <typename T>
+__device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long bad, const TreeSeq& seq, int r, int kvh, int row, float mc, T* dst) {
+    const int node = row / a.group, h = kvh * a.group + row % a.group;
+    bad &= a.masks[(int64_t)r * a.nodes + node];
+    for (; bad; bad &= bad - 1) {
+        const int64_t t = seq.len + (__ffsll((long long)bad) - 1);
+        const int page = a.table[(int64_t)r * a.width + t / a.page];
+        const int64_t at = (((int64_t)page * a.kv_heads + kvh) * a.page + (t & (a.page - 1))) * kHeadDim;
+        const __nv_bfloat16* q = a.q + (((int64_t)r * a.nodes + node) * a.hq + h) * kHeadDim;
+        float s = 0.f;
+        for (int d = 0; d < kHeadDim; ++d) s += __bfloat162float(q[d]) * __bfloat162float(a.k[at + d]);
+        const float p = exp2_approx(s * a.scale_log2 - mc);
+        for (int d = 0; d < kHeadDim; ++d) {
+            const float v = __bfloat162float(a.v[at + d]);
+            if (!isfinite(v)) dst[d] = (T)((float)dst[d] + (p > 0.f ? v : NAN));
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                                   const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TreeShared sh;
+    unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* q_tile = ring + (size_t)kTreeRing * kTileBytes;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&sh.kv_full[i], 1); mbar_init(&sh.kv_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.s_free[i], kSoftmaxThreads); mbar_init(&sh.p_full[i], kSoftmaxThreads); mbar_init(&sh.o_done[i], 1); }
+        mbar_init(&sh.q_full, kSoftmaxThreads);
+        mbar_init(&sh.drain, 1);
+        mbar_init(&sh.group, kSoftmaxThreads);
+        sh.bad_nodes = 0;
+        sh.failed = 0;
+        sh.first = sh.last = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(&sh.tmem, 512u);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+    chained_wait();
+    {   // this CTA's units: thread t holds the sequences 4t .. 4t + 3
+        int tiles[4];
+        int64_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            tiles[j] = 4 * tid + j < a.rows ? tree_seq(a, 4 * tid + j).tiles : 0;
+            mine += tiles[j];
+        }
+        int64_t upto = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        if (lane == 31) sh.scan[warp] = upto;
+        __syncthreads();
+        int64_t total = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp) upto += sh.scan[w];
+            total += sh.scan[w];
+        }
+        const int64_t items = (int64_t)a.kv_heads * a.row_tiles, units = total * items, quota = (units + gridDim.x - 1) / gridDim.x;
+        const int64_t first = (int64_t)blockIdx.x * quota, last = min(units, first + quota);
+        int64_t begin = (upto - mine) * items;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t end = begin + tiles[j] * items;
+            if (first < last && begin <= first && first < end) {
+                sh.row0 = 4 * tid + j;
+                sh.item_off = first - begin;
+                sh.first = first;
+                sh.last = last;
+            }
+            begin = end;
+        }
+        __syncthreads();
+    }
+    TreeWalk w;
+    w.start(a, sh);
+    if (warp == 0) {
+        // -------- pages: lane b asks for box b of a tile (a page, or 128 positions of one), then for the same of the other half --------
+        const int box = min(a.page, kTile), boxes = kTile / box;
+        uint32_t issued = 0;   // tiles asked for
+        uint32_t tile_no = 0;
+        bool ok = true;
+        for (; ok && w.left > 0; w.next(a)) {
+            const int kvh = w.item / a.row_tiles, n = w.t1 - w.t0;
+            int kpage = -1, vpage[2] = {-1, -1};   // this lane's page of the key tile, of the value tiles that are still to come
+            for (int s = 0; ok && s < 2 * n; ++s) {
+                // s-th tile of the sequence: keys at 0, 1, 3, 5, ..; values at 2, 4, .. and the last
+                const bool value = s >= 2 * n - 1 ? true : (s && !(s & 1));
+                const int i = value ? (s == 2 * n - 1 ? n - 1 : s / 2 - 1) : (s + 1) / 2;
+                const int64_t pos = (int64_t)(w.t0 + i) * kTile + lane * box;   // this lane's box
+                int page;
+                if (!value) {
+                    kpage = -1;
+                    if (lane < boxes && pos < w.seq.end) kpage = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
+                    if ((unsigned)kpage >= (unsigned)a.pages) kpage = -1;
+                    vpage[i & 1] = page = kpage;
+                    // groups of 16 positions with a page: box b covers groups b * box / 16 ..
+                    unsigned good = 0;
+                    const unsigned have = __ballot_sync(0xffffffffu, kpage >= 0);
+                    for (int g = 0; g < 8; ++g) good |= ((have >> (g * 16 / box)) & 1u) << g;
+                    if (lane == 0) sh.good[tile_no & 7] = good;
+                    ++tile_no;
+                } else {
+                    page = vpage[i & 1];
+                }
+                const uint32_t stage = issued % kTreeRing;
+                if (!warp_wait(&sh.kv_empty[stage], ((issued / kTreeRing) & 1u) ^ 1u)) { ok = false; break; }
+                unsigned char* dst = ring + (size_t)stage * kTileBytes + lane * box * 128;
+                const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+                if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[stage], (uint32_t)__popc(have) * (uint32_t)box * 256u);
+                __syncwarp();
+                if (page >= 0) {
+                    const int y = (int)(pos & (a.page - 1));
+                    tma_load_4d(dst, value ? &vmap : &kmap, 0, y, kvh, page, &sh.kv_full[stage]);
+                    tma_load_4d(dst + kHalfBytes, value ? &vmap : &kmap, 64, y, kvh, page, &sh.kv_full[stage]);
+                }
+                __syncwarp();
+                ++issued;
+            }
+        }
+        if (!ok) sh.failed = 1;
+        for (uint32_t i = 1; i <= min(issued, (uint32_t)kTreeRing); ++i)   // no copy outlives the CTA, whatever became of the other roles
+            if (!warp_wait(&sh.kv_full[(issued - i) % kTreeRing], ((issued - i) / kTreeRing) & 1u)) sh.failed = 1;
+    } else if (warp == 1) {
+        // -------- products: the warp stays together, an elected lane issues --------
+        constexpr uint32_t idesc_s = instr_desc_bf16(kTile, kTile, false), idesc_o = instr_desc_bf16(kTile, kHeadDim, true);
+        const uint32_t q_addr = smem_u32(q_tile), ring_addr = smem_u32(ring);
+        uint32_t base = 0, j = 0, seg = 0;   // ring position of the stretch, its first tile's number, number of the stretch
+        bool ok = true;
+        auto scores = [&](int i) {   // S of tile i
+            const uint32_t at = base + key_at(i), stage = at % kTreeRing, no = j + i;
+            ok = warp_wait(&sh.kv_full[stage], (at / kTreeRing) & 1u) && warp_wait(&sh.s_free[no & 1], ((no >> 1) & 1u) ^ 1u);
+            if (!ok) return;
+            tc_fence_after_sync();
+            const uint32_t k_addr = ring_addr + stage * kTileBytes, d = tmem + kColS + (no & 1) * kTile;
+            if (elect_one()) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    tc_mma_f16_ss(d, smem_desc_sw128(q_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), smem_desc_sw128(k_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), idesc_s, s > 0);
+                tc_commit(&sh.kv_empty[stage]);
+                tc_commit(&sh.s_full[no & 1]);
+            }
+            __syncwarp();
+        };
+        auto values = [&](int i, int n) {   // O += P V of tile i
+            const uint32_t at = base + value_at(i, n), stage = at % kTreeRing, no = j + i;
+            ok = warp_wait(&sh.kv_full[stage], (at / kTreeRing) & 1u) && warp_wait(&sh.p_full[no & 1], (no >> 1) & 1u);
+            if (!ok) return;
+            tc_fence_after_sync();
+            const uint32_t v_addr = ring_addr + stage * kTileBytes, p = tmem + kColP + (no & 1) * (kTile / 2);
+            if (elect_one()) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s) tc_mma_f16_ts(tmem + kColO, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, i > 0 || s > 0);
+                tc_commit(&sh.kv_empty[stage]);
+                tc_commit(&sh.o_done[no & 1]);
+            }
+            __syncwarp();
+        };
+        for (; ok && w.left > 0; w.next(a)) {
+            const int n = w.t1 - w.t0;
+            ok = warp_wait(&sh.q_full, seg & 1u);
+            if (ok) scores(0);
+            for (int i = 1; ok && i < n; ++i) {
+                scores(i);
+                if (ok) values(i - 1, n);
+            }
+            if (ok) values(n - 1, n);
+            base += 2 * n;
+            j += n;
+            ++seg;
+        }
+        if (elect_one()) tc_commit(&sh.drain);   // what was issued still reads the ring and the tensor memory
+        __syncwarp();
+        if (!warp_wait(&sh.drain, 0) || !ok) sh.failed = 1;
+    } else if (warp >= 4) {
+        // -------- softmax: thread = row of the tile --------
+        const int row_l = tid - kSoftmaxThreads;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        uint32_t base = 0, j = 0, groups = 0;
+        bool ok = true;
+        int stretch = 0;
+        auto group_sync = [&]() {   // the four warps, with a bound like every other wait
+            mbar_arrive(&sh.group);
+            ok = ok && warp_wait(&sh.group, groups++ & 1u);
+        };
+        for (; ok && w.left > 0; w.next(a), ++stretch) {
+            const int kvh = w.item / a.row_tiles, rt = w.item % a.row_tiles, n = w.t1 - w.t0;
+            const int row = rt * kTile + row_l, m_rows = a.nodes * a.group;   // row of Q
+            const bool live = row < m_rows, busy = rt * kTile + (warp & 3) * 32 < m_rows;   // busy: some row of the warp is one
+            // Q, 16 threads a row of 256 bytes; the products that read the last stretch's are done (its S has been read)
+            for (int i = row_l; i < kTile * 16; i += kSoftmaxThreads) {
+                const int rr = i >> 4, c = i & 15, qr = rt * kTile + rr;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (qr < m_rows) {
+                    const int node = qr / a.group, h = kvh * a.group + qr % a.group;
+                    v = __ldg(reinterpret_cast<const uint4*>(a.q + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim) + c);
+                }
+                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&sh.q_full);
+            unsigned long long mask = live ? a.masks[(int64_t)w.r * a.nodes + row / a.group] : 0ull;
+            if (a.nodes < 64) mask &= (1ull << a.nodes) - 1ull;
+            float m = -INFINITY, l = 0.f;   // maximum of the scores so far (or less, see above), sum
+            bool seen = false;
+            for (int i = 0; i < n; ++i) {
+                const uint32_t no = j + i, buf = no & 1;
+                ok = warp_wait(&sh.s_full[buf], (no >> 1) & 1u);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const unsigned good = sh.good[no & 7];
+                const int64_t pos0 = (int64_t)(w.t0 + i) * kTile;
+                const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
+                uint32_t s[kTile];
+                if (busy) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(lanes + kColS + buf * kTile + 32 * c, s + 32 * c);
+                    tmem_wait_ld();
+                }
+                tc_fence_before_sync();
+                mbar_arrive(&sh.s_free[buf]);
+                if (!whole) {
+                    // V rows that no row sees (behind the end, no page) are cleared, values of nodes cleaned (see add_bad_nodes)
+                    const uint32_t at = base + value_at(i, n), stage = at % kTreeRing;
+                    ok = warp_wait(&sh.kv_full[stage], (at / kTreeRing) & 1u);
+                    if (!ok) break;
+                    const int64_t pos = pos0 + row_l;
+                    unsigned char* vrow = ring + (size_t)stage * kTileBytes + row_l * 128;
+                    if (pos >= w.seq.end || !((good >> (row_l >> 4)) & 1u)) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(vrow + (c >> 3) * kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    } else if (pos >= w.seq.len) {
+                        bool bad = false;
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            uint4* p = reinterpret_cast<uint4*>(vrow + (c >> 3) * kHalfBytes + (c & 7) * 16);
+                            uint32_t x[4] = {p->x, p->y, p->z, p->w};
+                            bool here = false;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const bool lo = (x[e] & 0x7F80u) == 0x7F80u, hi = (x[e] & 0x7F800000u) == 0x7F800000u;
+                                here |= lo | hi;
+                                x[e] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+                            }
+                            if (here) *p = make_uint4(x[0], x[1], x[2], x[3]);
+                            bad |= here;
+                        }
+                        if (bad) atomicOr(&sh.bad_nodes, 1ull << (pos - w.seq.len));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    // what this row sees of the tile
+                    unsigned any = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int64_t ctx = w.seq.len - (pos0 + 32 * c);   // positions of this quarter before the length
+                        unsigned vis = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << (int)ctx) - 1u;
+                        if (ctx <= 0 && ctx > -64) vis |= (unsigned)(mask >> (int)-ctx);
+                        else if (ctx > 0 && ctx < 32) vis |= (unsigned)(mask << (int)ctx);
+                        vis &= ((good >> (2 * c)) & 1u ? 0x0000FFFFu : 0u) | ((good >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
+                        any |= vis;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!((vis >> e) & 1u)) s[32 * c + e] = 0xFF800000u;
+                    }
+                    seen |= any != 0;
+                } else {
+                    seen = true;
+                }
+                if (busy) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < kTile; ++e) top = fmaxf(top, __uint_as_float(s[e]));
+                    const bool raise = top > -INFINITY && (m == -INFINITY || (top - m) * a.scale_log2 > 8.f);
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float corr = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx((m - top) * a.scale_log2);
+                        if (raise) m = top;
+                        l *= corr;
+                        if (i > 0) {   // O holds the tiles before: all of them, once the last of them is done
+                            ok = warp_wait(&sh.o_done[(no - 1) & 1], ((no - 1) >> 1) & 1u);
+                            if (!ok) break;
+                            tc_fence_after_sync();
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(lanes + kColO + 32 * c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                                tmem_st32(lanes + kColO + 32 * c, o);
+                            }
+                        }
+                    }
+                    if (no >= 2) {   // P's place is free once the tile before the last is done
+                        ok = warp_wait(&sh.o_done[buf], ((no - 2) >> 1) & 1u);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                    }
+                    const float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float x = exp2_approx(fmaf(__uint_as_float(s[32 * c + 2 * e]), a.scale_log2, -mc));
+                            const float y = exp2_approx(fmaf(__uint_as_float(s[32 * c + 2 * e + 1]), a.scale_log2, -mc));
+                            l += x + y;
+                            p[e] = pack_bf16(x, y);
+                        }
+                        tmem_st16(lanes + kColP + buf * (kTile / 2) + 16 * c, p);
+                    }
+                    tmem_wait_st();
+                }
+                tc_fence_before_sync();
+                mbar_arrive(&sh.p_full[buf]);
+            }
+            if (!ok) break;
+            base += 2 * n;
+            j += n;
+            ok = warp_wait(&sh.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1u);
+            if (!ok) break;
+            tc_fence_after_sync();
+            group_sync();   // every tile's bad nodes are known
+            if (!ok) break;
+            const unsigned long long bad = sh.bad_nodes;
+            if (m == -INFINITY) l = seen ? NAN : 0.f;   // every score minus infinity, or nothing seen
+            const float mc = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+            const bool complete = n == w.seq.tiles;
+            if (busy) {
+                const float inv = 1.f / l;
+                const int64_t slot = (int64_t)blockIdx.x * 2 + (stretch > 0);
+                __nv_bfloat16* out = a.out + (((int64_t)w.r * a.nodes + row / a.group) * a.hq + kvh * a.group + row % a.group) * kHeadDim;
+                float* part = a.part + (slot * a.tile_rows + row_l) * kHeadDim;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(lanes + kColO + 32 * c, o);
+                    tmem_wait_ld();
+                    if (live && complete) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const float x = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u]) * inv, y = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u + 1]) * inv;
+                                p[u] = pack_bf16(x, y);
+                            }
+                            *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(p[0], p[1], p[2], p[3]);
+                        }
+                    } else if (live) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (live) {
+                    if (!complete) a.part_ml[slot * a.tile_rows + row_l] = make_float2(mc, l);
+                    if (bad) {
+                        if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, out);
+                        else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, part);
+                    }
+                }
+            }
+            group_sync();   // and have been read
+            if (tid == kSoftmaxThreads) sh.bad_nodes = 0;
+            tc_fence_before_sync();
+        }
+        if (!ok) sh.failed = 1;
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_free(tmem, 512u);
+        if (lane == 0 && sh.failed) atomicExch(a.error, MFQB_ERR_TIMEOUT);
+    }
+}
+
+// Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context.
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int ctas, int per_seq) {
+    chained_wait();
+    __shared__ int64_t red[8][2];
+    const int r = blockIdx.x / per_seq, lane = threadIdx.x & 31;
+    const int local = (blockIdx.x % per_seq) * 8 + (threadIdx.x >> 5);   // kv head, row of Q
+    int64_t before, total;
+    tree_prefix(a, r, before, total, red);
+    const int m_rows = a.nodes * a.group;
+    if (local >= a.kv_heads * m_rows) return;
+    const int kvh = local / m_rows, row = local % m_rows, rt = row / kTile, row_l = row % kTile;
+    const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
+    const int tiles = tree_seq(a, r).tiles;
+    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * tiles, c0 = s0 / quota, c1 = (s0 + tiles - 1) / quota;
+    if (c0 == c1) return;
+    auto slot = [&](int64_t c) { return (c * 2 + (s0 > c * quota ? 1 : 0)) * a.tile_rows + row_l; };
+    float m = -INFINITY;
+    for (int64_t c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, __ldcg(&a.part_ml[slot(c)]).x);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t c = c0; c <= c1; c += 8) {
+        float2 ml[8];
+        float4 o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (c + u <= c1) {
+                const int64_t at = slot(c + u);
+                ml[u] = __ldcg(&a.part_ml[at]);
+                o[u] = __ldcg(reinterpret_cast<const float4*>(a.part + at * kHeadDim) + lane);
+            }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (c + u <= c1 && (ml[u].x > -INFINITY || m == -INFINITY)) {
+                const float f = m == -INFINITY ? 1.f : exp2_approx(ml[u].x - m);
+                l += ml[u].y * f;
+                acc.x += o[u].x * f; acc.y += o[u].y * f; acc.z += o[u].z * f; acc.w += o[u].w * f;
+            }
+    }
+    const float inv = 1.f / l;
+    if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    const int node = row / a.group, h = kvh * a.group + row % a.group;
+    *reinterpret_cast<uint2*>(a.out + (((int64_t)r * a.nodes + node) * a.hq + h) * kHeadDim + 4 * lane) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
+}
+
+// Keys or values of one layer as [page][head][position][128]: boxes of min(page, 128) positions x 64 dims with the 128-byte swizzle.
+static CUtensorMap page_map(const void* base, const mfqb_cache& c) {
+    typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static encode_fn encode = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess)
+            encode = reinterpret_cast<encode_fn>(p);
+    });
+    if (!encode) fail(MFQB_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    CUtensorMap map;
+    const cuuint64_t dims[4] = {kHeadDim, (cuuint64_t)c.page, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {256, (cuuint64_t)c.page * 256, (cuuint64_t)c.kv_heads * c.page * 256};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(c.page, kTile), 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) fail(MFQB_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)rc);
+    return map;
+}
+
+static int tree_rows(const mfqb_cache& c, int q_heads, int nodes) { return std::min(kTile, nodes * (q_heads / c.kv_heads)); }
+static uint64_t tree_attention_work_bytes(const mfqb_cache& c, int q_heads, int nodes) {
+    return (uint64_t)kTreeCtas * 2 * tree_rows(c, q_heads, nodes) * (kHeadDim * 4 + 8);
+}
 static void check_heads(const mfqb_cache* c, int q_heads, const char* who) {
     if (q_heads < 1 || q_heads % c->kv_heads || q_heads / c->kv_heads > 16)
         fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to 16 query heads per kv head, got %d over %d", who, q_heads, c->kv_heads);
+}
+
+static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, void* work,
+                                  cudaStream_t s) {
+    int device = 0;
+    MFQB_CUDA(cudaGetDevice(&device));
+    const int64_t per_layer = (int64_t)c.pages * c.kv_heads * c.page * kHeadDim;
+    TreeArgs a{};
+    a.table = c.table;
+    a.lens = c.lens;
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.masks = reinterpret_cast<const unsigned long long*>(masks);
+    a.k = static_cast<const __nv_bfloat16*>(c.k) + layer * per_layer;
+    a.v = static_cast<const __nv_bfloat16*>(c.v) + layer * per_layer;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.rows = c.rows;
+    a.width = c.width;
+    a.pages = c.pages;
+    a.page = c.page;
+    a.kv_heads = c.kv_heads;
+    a.hq = q_heads;
+    a.group = q_heads / c.kv_heads;
+    a.nodes = nodes;
+    a.row_tiles = (nodes * a.group + kTile - 1) / kTile;
+    a.tile_rows = tree_rows(c, q_heads, nodes);
+    a.part = static_cast<float*>(work);
+    a.part_ml = reinterpret_cast<float2*>(a.part + (int64_t)kTreeCtas * 2 * a.tile_rows * kHeadDim);
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.error = device_status_word(device);
+    const CUtensorMap kmap = page_map(a.k, c), vmap = page_map(a.v, c);
+    static std::once_flag once[64];
+    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem)); });
+    launch_chained(tree_attn_kernel, dim3(kTreeCtas), dim3(kTreeThreads), kTreeSmem, s, a, kmap, vmap);
+    const int per_seq = (c.kv_heads * nodes * a.group + 7) / 8;
+    launch_chained(tree_merge_kernel, dim3((unsigned)(c.rows * per_seq)), dim3(256), 0, s, a, (int)kTreeCtas, per_seq);
 }
 
 }  // namespace mfqb
@@ -88,11 +704,11 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
         if (!q || !masks || !out || !work) fail(MFQB_ERR_ARG, "mfqb_tree_attention: null argument");
         if (((uintptr_t)q & 15) || ((uintptr_t)out & 15)) fail(MFQB_ERR_ARG, "mfqb_tree_attention: q and out must be 16-byte aligned");
         if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "mfqb_tree_attention: layer %d of %d", layer, c->layers);
+        if (!(scale > 0.f) || scale > 1e30f) fail(MFQB_ERR_ARG, "mfqb_tree_attention: scale must be positive and finite");
         if (((uintptr_t)work & 15) || work_bytes < tree_attention_work_bytes(*c, q_heads, nodes))
             fail(MFQB_ERR_ARG, "mfqb_tree_attention: work must be 16-byte aligned and hold %llu bytes, got %llu",
                  (unsigned long long)tree_attention_work_bytes(*c, q_heads, nodes), (unsigned long long)work_bytes);
-        launch_chained(tree_attn_kernel, dim3(q_heads, nodes, c->rows), dim3(128), 0, stream, *c, layer, static_cast<const __nv_bfloat16*>(q), q_heads, nodes,
-                       reinterpret_cast<const unsigned long long*>(masks), scale, static_cast<__nv_bfloat16*>(out));
+        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, work, stream);
     });
 }
 
