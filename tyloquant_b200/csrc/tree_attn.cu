@@ -26,10 +26,10 @@ int* device_status_word(int device);
 
 constexpr int kTreeCtas = 148;                       // one per SM
 constexpr int kTile = 128;                           // rows of Q, positions of a tile
-constexpr int kTreeRing = 6, kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
-constexpr int kTreeThreads = 256, kSoftmaxThreads = 128;
-constexpr size_t kTreeSmem = (size_t)(kTreeRing + 1) * kTileBytes + 1024;   // ring, Q, alignment
-constexpr uint32_t kColS = 0, kColO = 256, kColP = 384;   // tensor memory columns: S twice, O, P twice (64 each)
+constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
+constexpr int kTreeTiles = 7, kTreeRingMax = kTreeTiles - 1;   // 32 KB tiles in shared memory: Q once or twice, the others are the ring
+constexpr int kSoftmaxThreads = 256, kTreeThreads = 128 + kSoftmaxThreads;
+constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory columns: S of the two streams (P takes the place of its first half), O of the two
 
 struct TreeArgs {
     const int* table;
@@ -41,7 +41,7 @@ struct TreeArgs {
     float* part;                  // [CTA][first, last][rows of a tile][128], then their (maximum, sum)
     float2* part_ml;
     int* error;
-    int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // tile_rows: rows of a part, at most 128
+    int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of RT * 128 rows; tile_rows: rows of a part, at most that
     float scale_log2;
 };
 
@@ -78,15 +78,19 @@ __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int row, int64_t&
 }
 
 struct TreeShared {
-    uint64_t kv_full[kTreeRing], kv_empty[kTreeRing], q_full, s_full[2], s_free[2], p_full[2], o_done[2], drain, group;
+    uint64_t kv_full[kTreeRingMax], kv_empty[kTreeRingMax], q_full, s_full[2], p_full[2], o_done[2], drain, group;
     unsigned long long bad_nodes;   // nodes of the stretch whose values hold an infinity or NaN
-    int64_t red[8][2], scan[8];
+    int64_t scan[12];
     int64_t first, last, item_off;  // the CTA's units; offset of its first one in its sequence's
     int row0;
     uint32_t tmem;
     unsigned good[8];               // per tile (index mod 8): bit g = the 16 positions of group g have a page
     int failed;
+    float2 ml[2][kTile];            // the two streams' (maximum in powers of two, sum)
 };
+
+constexpr size_t kTreeSmem = (size_t)kTreeTiles * kTileBytes + sizeof(TreeShared);
+static_assert(kTreeSmem <= 227 * 1024, "one CTA's shared memory");
 
 // A CTA's stretches in order: sequence, item (kv head, row tile), tiles [t0, t1) of seq.tiles.
 struct TreeWalk {
@@ -162,7 +166,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MFQB_W8(r, 0), MFQB_W8(r, 8), "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+#define MFQB_P8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
+// Waits for this thread's loads.  The 32 registers of a load pass through it, so that no use of them can be moved before the wait.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    asm volatile("" : MFQB_P8(r, 0), MFQB_P8(r, 8));
+    asm volatile("" : MFQB_P8(r, 16), MFQB_P8(r, 24));
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r, uint32_t* q) {
+    tmem_wait_ld(r);
+    asm volatile("" : MFQB_P8(q, 0), MFQB_P8(q, 8));
+    asm volatile("" : MFQB_P8(q, 16), MFQB_P8(q, 24));
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -174,14 +189,60 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
-// Position in the ring's sequence of the key and value tiles of a stretch of n tiles: K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1).
-__device__ __forceinline__ int key_at(int i) { return i ? 2 * i - 1 : 0; }
-__device__ __forceinline__ int value_at(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
+// Position in the ring's sequence of the key and value tiles of a stretch of n tiles, which is the order of their use.  RT = 1: K0 K1 V0
+// K2 V1 .. K(n-1) V(n-2) V(n-1); RT = 2: K0 V0 K1 V1 ..
+template <int RT>
+__device__ __forceinline__ int key_at(int i) { return RT == 2 ? 2 * i : i + max(0, i - 1); }
+template <int RT>
+__device__ __forceinline__ int value_at(int i, int n) { return RT == 2 ? 2 * i + 1 : i + min(n, i + 2); }
+
+__device__ __forceinline__ uint64_t pair_f32(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 split_f32(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Scores that a row does not see become minus infinity.
+__device__ __forceinline__ void hide(uint32_t* s, unsigned vis) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+        if (!((vis >> e) & 1u)) s[e] = 0xFF800000u;
+}
+__device__ __forceinline__ float max32(const uint32_t* s) {
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 32; ++e) m[e & 3] = fmaxf(m[e & 3], __uint_as_float(s[e]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// exp2(scale s - mc) of 32 scores, rounded to bf16 into p; their sums into l.
+__device__ __forceinline__ void exp32(const uint32_t* s, uint64_t scale, uint64_t mc, uint64_t (&l)[2], uint32_t* p) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const float2 x = split_f32(fma_f32x2(pair_f32(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale, mc));
+        const float u = exp2_approx(x.x), v = exp2_approx(x.y);
+        l[e & 1] = add_f32x2(l[e & 1], pair_f32(u, v));
+        p[e] = pack_bf16(u, v);
+    }
+}
 
 // Rare: values of visible nodes that hold an infinity or NaN were taken out of the product (0 in their place, so that rows which do not see
 // the node keep clear of them); here they are added to the row's result, where the row sees them.
 template <typename T>
-__device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long bad, const TreeSeq& seq, int r, int kvh, int row, float mc, T* dst) {
+__device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long bad, const TreeSeq& seq, int r, int kvh, int row, float mc, T* dst, int d0, int d1) {
     const int node = row / a.group, h = kvh * a.group + row % a.group;
     bad &= a.masks[(int64_t)r * a.nodes + node];
     for (; bad; bad &= bad - 1) {
@@ -192,23 +253,28 @@ __device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long
         float s = 0.f;
         for (int d = 0; d < kHeadDim; ++d) s += __bfloat162float(q[d]) * __bfloat162float(a.k[at + d]);
         const float p = exp2_approx(s * a.scale_log2 - mc);
-        for (int d = 0; d < kHeadDim; ++d) {
+        for (int d = d0; d < d1; ++d) {
             const float v = __bfloat162float(a.v[at + d]);
             if (!isfinite(v)) dst[d] = (T)((float)dst[d] + (p > 0.f ? v : NAN));
         }
     }
 }
 
+// Two streams of steps take turns on the tensor core, each with its own S, O and four softmax warps: while one stream's scores become
+// probabilities the other's products run.  RT = 1 (up to 128 rows): the streams take alternate tiles of positions and are added at the end
+// of a stretch.  RT = 2: each stream has 128 of 256 rows, both take every tile, which is read once for the two.  Step u of a stretch:
+// stream u & 1; its S waits for the product of step u - 2, whose P lies in S's place.
+template <int RT>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap) {
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ TreeShared sh;
-    unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    unsigned char* q_tile = ring + (size_t)kTreeRing * kTileBytes;
+    constexpr int kRing = kTreeTiles - RT;
+    extern __shared__ __align__(1024) unsigned char ring[];   // the swizzle's pattern repeats every 1024 bytes
+    TreeShared& sh = *reinterpret_cast<TreeShared*>(ring + (size_t)kTreeTiles * kTileBytes);
+    unsigned char* q_tiles = ring + (size_t)kRing * kTileBytes;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&sh.kv_full[i], 1); mbar_init(&sh.kv_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.s_free[i], kSoftmaxThreads); mbar_init(&sh.p_full[i], kSoftmaxThreads); mbar_init(&sh.o_done[i], 1); }
+        for (int i = 0; i < kRing; ++i) { mbar_init(&sh.kv_full[i], 1); mbar_init(&sh.kv_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], kSoftmaxThreads / 2); mbar_init(&sh.o_done[i], 1); }
         mbar_init(&sh.q_full, kSoftmaxThreads);
         mbar_init(&sh.drain, 1);
         mbar_init(&sh.group, kSoftmaxThreads);
@@ -223,12 +289,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     tc_fence_after_sync();
     const uint32_t tmem = sh.tmem;
     chained_wait();
-    {   // this CTA's units: thread t holds the sequences 4t .. 4t + 3
-        int tiles[4];
+    {   // this CTA's units: thread t holds the sequences 3t .. 3t + 2
+        constexpr int kEach = (kCacheRows + kTreeThreads - 1) / kTreeThreads;
+        int tiles[kEach];
         int64_t mine = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            tiles[j] = 4 * tid + j < a.rows ? tree_seq(a, 4 * tid + j).tiles : 0;
+        for (int j = 0; j < kEach; ++j) {
+            tiles[j] = kEach * tid + j < a.rows ? tree_seq(a, kEach * tid + j).tiles : 0;
             mine += tiles[j];
         }
         int64_t upto = mine;
@@ -240,7 +307,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         __syncthreads();
         int64_t total = 0;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
+        for (int w = 0; w < kTreeThreads / 32; ++w) {
             if (w < warp) upto += sh.scan[w];
             total += sh.scan[w];
         }
@@ -248,10 +315,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         const int64_t first = (int64_t)blockIdx.x * quota, last = min(units, first + quota);
         int64_t begin = (upto - mine) * items;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kEach; ++j) {
             const int64_t end = begin + tiles[j] * items;
             if (first < last && begin <= first && first < end) {
-                sh.row0 = 4 * tid + j;
+                sh.row0 = kEach * tid + j;
                 sh.item_off = first - begin;
                 sh.first = first;
                 sh.last = last;
@@ -263,121 +330,129 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     TreeWalk w;
     w.start(a, sh);
     if (warp == 0) {
-        // -------- pages: lane b asks for box b of a tile (a page, or 128 positions of one), then for the same of the other half --------
+        // -------- pages: lane b asks for box b of a tile (a page, or 128 positions of one), both halves --------
         const int box = min(a.page, kTile), boxes = kTile / box;
-        uint32_t issued = 0;   // tiles asked for
-        uint32_t tile_no = 0;
+        uint32_t issued = 0, tile_no = 0;
         bool ok = true;
+        int pages[2] = {-1, -1};   // this lane's page of the last two tiles
+        auto ask = [&](const CUtensorMap* map, int kvh, int64_t pos, int page) {
+            const uint32_t stage = issued % kRing;
+            ok = warp_wait(&sh.kv_empty[stage], ((issued / kRing) & 1u) ^ 1u);
+            if (!ok) return;
+            unsigned char* dst = ring + (size_t)stage * kTileBytes + lane * box * 128;
+            const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[stage], (uint32_t)__popc(have) * (uint32_t)box * 256u);
+            __syncwarp();
+            if (page >= 0) {
+                const int y = (int)(pos & (a.page - 1));
+                tma_load_4d(dst, map, 0, y, kvh, page, &sh.kv_full[stage]);
+                tma_load_4d(dst + kHalfBytes, map, 64, y, kvh, page, &sh.kv_full[stage]);
+            }
+            __syncwarp();
+            ++issued;
+        };
+        auto position = [&](int i) { return (int64_t)(w.t0 + i) * kTile + lane * box; };   // of this lane's box
+        auto keys = [&](int kvh, int i) {
+            const int64_t pos = position(i);
+            int page = -1;
+            if (lane < boxes && pos < w.seq.end) page = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
+            if ((unsigned)page >= (unsigned)a.pages) page = -1;
+            (i & 1 ? pages[1] : pages[0]) = page;
+            unsigned good = 0;   // groups of 16 positions with a page: box b covers groups b * box / 16 ..
+            const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+            for (int g = 0; g < 8; ++g) good |= ((have >> (g * 16 / box)) & 1u) << g;
+            if (lane == 0) sh.good[tile_no & 7] = good;
+            ++tile_no;
+            ask(&kmap, kvh, pos, page);
+        };
+        auto values = [&](int kvh, int i) { ask(&vmap, kvh, position(i), i & 1 ? pages[1] : pages[0]); };
         for (; ok && w.left > 0; w.next(a)) {
             const int kvh = w.item / a.row_tiles, n = w.t1 - w.t0;
-            int kpage = -1, vpage[2] = {-1, -1};   // this lane's page of the key tile, of the value tiles that are still to come
-            for (int s = 0; ok && s < 2 * n; ++s) {
-                // s-th tile of the sequence: keys at 0, 1, 3, 5, ..; values at 2, 4, .. and the last
-                const bool value = s >= 2 * n - 1 ? true : (s && !(s & 1));
-                const int i = value ? (s == 2 * n - 1 ? n - 1 : s / 2 - 1) : (s + 1) / 2;
-                const int64_t pos = (int64_t)(w.t0 + i) * kTile + lane * box;   // this lane's box
-                int page;
-                if (!value) {
-                    kpage = -1;
-                    if (lane < boxes && pos < w.seq.end) kpage = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
-                    if ((unsigned)kpage >= (unsigned)a.pages) kpage = -1;
-                    vpage[i & 1] = page = kpage;
-                    // groups of 16 positions with a page: box b covers groups b * box / 16 ..
-                    unsigned good = 0;
-                    const unsigned have = __ballot_sync(0xffffffffu, kpage >= 0);
-                    for (int g = 0; g < 8; ++g) good |= ((have >> (g * 16 / box)) & 1u) << g;
-                    if (lane == 0) sh.good[tile_no & 7] = good;
-                    ++tile_no;
-                } else {
-                    page = vpage[i & 1];
-                }
-                const uint32_t stage = issued % kTreeRing;
-                if (!warp_wait(&sh.kv_empty[stage], ((issued / kTreeRing) & 1u) ^ 1u)) { ok = false; break; }
-                unsigned char* dst = ring + (size_t)stage * kTileBytes + lane * box * 128;
-                const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
-                if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[stage], (uint32_t)__popc(have) * (uint32_t)box * 256u);
-                __syncwarp();
-                if (page >= 0) {
-                    const int y = (int)(pos & (a.page - 1));
-                    tma_load_4d(dst, value ? &vmap : &kmap, 0, y, kvh, page, &sh.kv_full[stage]);
-                    tma_load_4d(dst + kHalfBytes, value ? &vmap : &kmap, 64, y, kvh, page, &sh.kv_full[stage]);
-                }
-                __syncwarp();
-                ++issued;
+            keys(kvh, 0);
+            for (int i = 0; ok && i < n; ++i) {
+                if (RT == 1 && i + 1 < n) keys(kvh, i + 1);
+                if (ok) values(kvh, i);
+                if (RT == 2 && ok && i + 1 < n) keys(kvh, i + 1);
             }
         }
         if (!ok) sh.failed = 1;
-        for (uint32_t i = 1; i <= min(issued, (uint32_t)kTreeRing); ++i)   // no copy outlives the CTA, whatever became of the other roles
-            if (!warp_wait(&sh.kv_full[(issued - i) % kTreeRing], ((issued - i) / kTreeRing) & 1u)) sh.failed = 1;
+        for (uint32_t i = 1; i <= min(issued, (uint32_t)kRing); ++i)   // no copy outlives the CTA, whatever became of the other roles
+            if (!warp_wait(&sh.kv_full[(issued - i) % kRing], ((issued - i) / kRing) & 1u)) sh.failed = 1;
     } else if (warp == 1) {
         // -------- products: the warp stays together, an elected lane issues --------
         constexpr uint32_t idesc_s = instr_desc_bf16(kTile, kTile, false), idesc_o = instr_desc_bf16(kTile, kHeadDim, true);
-        const uint32_t q_addr = smem_u32(q_tile), ring_addr = smem_u32(ring);
-        uint32_t base = 0, j = 0, seg = 0;   // ring position of the stretch, its first tile's number, number of the stretch
+        const uint32_t q_addr = smem_u32(q_tiles), ring_addr = smem_u32(ring);
+        uint32_t base = 0, stretch = 0, steps[2] = {0, 0};   // ring position of the stretch, its number, steps of each stream before it
         bool ok = true;
-        auto scores = [&](int i) {   // S of tile i
-            const uint32_t at = base + key_at(i), stage = at % kTreeRing, no = j + i;
-            ok = warp_wait(&sh.kv_full[stage], (at / kTreeRing) & 1u) && warp_wait(&sh.s_free[no & 1], ((no >> 1) & 1u) ^ 1u);
+        auto scores = [&](int u) {
+            const int i = RT == 2 ? u >> 1 : u, st = u & 1;
+            const uint32_t at = base + key_at<RT>(i), stage = at % kRing;
+            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
+            if (ok && u >= 2) ok = warp_wait(&sh.o_done[st], ((st ? steps[1] : steps[0]) + (u >> 1) - 1) & 1u);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint32_t k_addr = ring_addr + stage * kTileBytes, d = tmem + kColS + (no & 1) * kTile;
+            const uint32_t k_addr = ring_addr + stage * kTileBytes, q = q_addr + (RT == 2 ? st * kTileBytes : 0), d = tmem + kColS + st * kTile;
             if (elect_one()) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
-                    tc_mma_f16_ss(d, smem_desc_sw128(q_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), smem_desc_sw128(k_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), idesc_s, s > 0);
-                tc_commit(&sh.kv_empty[stage]);
-                tc_commit(&sh.s_full[no & 1]);
+                    tc_mma_f16_ss(d, smem_desc_sw128(q + (s >> 2) * kHalfBytes + (s & 3) * 32), smem_desc_sw128(k_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), idesc_s, s > 0);
+                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
+                tc_commit(&sh.s_full[st]);
             }
             __syncwarp();
         };
-        auto values = [&](int i, int n) {   // O += P V of tile i
-            const uint32_t at = base + value_at(i, n), stage = at % kTreeRing, no = j + i;
-            ok = warp_wait(&sh.kv_full[stage], (at / kTreeRing) & 1u) && warp_wait(&sh.p_full[no & 1], (no >> 1) & 1u);
+        auto values = [&](int u, int n) {
+            const int i = RT == 2 ? u >> 1 : u, st = u & 1;
+            const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
+            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u) && warp_wait(&sh.p_full[st], ((st ? steps[1] : steps[0]) + (u >> 1)) & 1u);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint32_t v_addr = ring_addr + stage * kTileBytes, p = tmem + kColP + (no & 1) * (kTile / 2);
+            const uint32_t v_addr = ring_addr + stage * kTileBytes, p = tmem + kColS + st * kTile, d = tmem + kColO + st * kHeadDim;
             if (elect_one()) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) tc_mma_f16_ts(tmem + kColO, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, i > 0 || s > 0);
-                tc_commit(&sh.kv_empty[stage]);
-                tc_commit(&sh.o_done[no & 1]);
+                for (int s = 0; s < 8; ++s) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, u > 1 || s > 0);
+                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
+                tc_commit(&sh.o_done[st]);
             }
             __syncwarp();
         };
         for (; ok && w.left > 0; w.next(a)) {
-            const int n = w.t1 - w.t0;
-            ok = warp_wait(&sh.q_full, seg & 1u);
+            const int n = w.t1 - w.t0, total = RT * n;
+            ok = warp_wait(&sh.q_full, stretch & 1u);
             if (ok) scores(0);
-            for (int i = 1; ok && i < n; ++i) {
-                scores(i);
-                if (ok) values(i - 1, n);
+            if (ok && total > 1) scores(1);
+            for (int u = 0; ok && u < total; ++u) {
+                values(u, n);
+                if (ok && u + 2 < total) scores(u + 2);
             }
-            if (ok) values(n - 1, n);
             base += 2 * n;
-            j += n;
-            ++seg;
+            steps[0] += (total + 1) >> 1;
+            steps[1] += total >> 1;
+            ++stretch;
         }
         if (elect_one()) tc_commit(&sh.drain);   // what was issued still reads the ring and the tensor memory
         __syncwarp();
         if (!warp_wait(&sh.drain, 0) || !ok) sh.failed = 1;
     } else if (warp >= 4) {
-        // -------- softmax: thread = row of the tile --------
-        const int row_l = tid - kSoftmaxThreads;
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        uint32_t base = 0, j = 0, groups = 0;
+        // -------- softmax: stream = warps 4-7 or 8-11, thread = row of the stream's Q --------
+        const int st = (warp - 4) >> 2, row_l = tid & 127;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lanes + kColS + st * kTile, col_o = lanes + kColO + st * kHeadDim;
+        unsigned char* q_tile = q_tiles + (RT == 2 ? st * kTileBytes : 0);
+        uint32_t base = 0, tile_no = 0, groups = 0, steps[2] = {0, 0};
         bool ok = true;
         int stretch = 0;
-        auto group_sync = [&]() {   // the four warps, with a bound like every other wait
+        auto group_sync = [&]() {   // the eight warps, with a bound like every other wait
             mbar_arrive(&sh.group);
             ok = ok && warp_wait(&sh.group, groups++ & 1u);
         };
+        const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
         for (; ok && w.left > 0; w.next(a), ++stretch) {
             const int kvh = w.item / a.row_tiles, rt = w.item % a.row_tiles, n = w.t1 - w.t0;
-            const int row = rt * kTile + row_l, m_rows = a.nodes * a.group;   // row of Q
-            const bool live = row < m_rows, busy = rt * kTile + (warp & 3) * 32 < m_rows;   // busy: some row of the warp is one
+            const int tile0 = rt * RT * kTile + (RT == 2 ? st * kTile : 0), row = tile0 + row_l, m_rows = a.nodes * a.group;   // first row, this thread's row of Q
+            const bool live = row < m_rows, busy = tile0 + (warp & 3) * 32 < m_rows;   // busy: some row of the warp is one
             // Q, 16 threads a row of 256 bytes; the products that read the last stretch's are done (its S has been read)
-            for (int i = row_l; i < kTile * 16; i += kSoftmaxThreads) {
-                const int rr = i >> 4, c = i & 15, qr = rt * kTile + rr;
+            for (int i = RT == 2 ? row_l : tid - 128; i < kTile * 16; i += RT == 2 ? 128 : 256) {
+                const int rr = i >> 4, c = i & 15, qr = tile0 + rr;
                 uint4 v = make_uint4(0u, 0u, 0u, 0u);
                 if (qr < m_rows) {
                     const int node = qr / a.group, h = kvh * a.group + qr % a.group;
@@ -389,28 +464,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             mbar_arrive(&sh.q_full);
             unsigned long long mask = live ? a.masks[(int64_t)w.r * a.nodes + row / a.group] : 0ull;
             if (a.nodes < 64) mask &= (1ull << a.nodes) - 1ull;
-            float m = -INFINITY, l = 0.f;   // maximum of the scores so far (or less, see above), sum
+            float m = -INFINITY;   // maximum of the scores so far (or less, see above)
+            uint64_t l2[2] = {0ull, 0ull};   // the sum, in four parts
             bool seen = false;
-            for (int i = 0; i < n; ++i) {
-                const uint32_t no = j + i, buf = no & 1;
-                ok = warp_wait(&sh.s_full[buf], (no >> 1) & 1u);
+            const int mine = RT == 2 ? n : (n + 1 - st) >> 1;   // this stream's steps
+            for (int x = 0; x < mine; ++x) {
+                const int i = RT == 2 ? x : 2 * x + st;
+                ok = warp_wait(&sh.s_full[st], ((st ? steps[1] : steps[0]) + x) & 1u);
                 if (!ok) break;
                 tc_fence_after_sync();
-                const unsigned good = sh.good[no & 7];
+                const unsigned good = sh.good[(tile_no + i) & 7];
                 const int64_t pos0 = (int64_t)(w.t0 + i) * kTile;
                 const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
-                uint32_t s[kTile];
-                if (busy) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(lanes + kColS + buf * kTile + 32 * c, s + 32 * c);
-                    tmem_wait_ld();
-                }
-                tc_fence_before_sync();
-                mbar_arrive(&sh.s_free[buf]);
+                unsigned vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
                 if (!whole) {
                     // V rows that no row sees (behind the end, no page) are cleared, values of nodes cleaned (see add_bad_nodes)
-                    const uint32_t at = base + value_at(i, n), stage = at % kTreeRing;
-                    ok = warp_wait(&sh.kv_full[stage], (at / kTreeRing) & 1u);
+                    const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
+                    ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
                     if (!ok) break;
                     const int64_t pos = pos0 + row_l;
                     unsigned char* vrow = ring + (size_t)stage * kTileBytes + row_l * 128;
@@ -419,18 +489,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                         for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(vrow + (c >> 3) * kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     } else if (pos >= w.seq.len) {
                         bool bad = false;
-#pragma unroll
+#pragma unroll 4
                         for (int c = 0; c < 16; ++c) {
                             uint4* p = reinterpret_cast<uint4*>(vrow + (c >> 3) * kHalfBytes + (c & 7) * 16);
-                            uint32_t x[4] = {p->x, p->y, p->z, p->w};
+                            uint32_t y[4] = {p->x, p->y, p->z, p->w};
                             bool here = false;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const bool lo = (x[e] & 0x7F80u) == 0x7F80u, hi = (x[e] & 0x7F800000u) == 0x7F800000u;
+                                const bool lo = (y[e] & 0x7F80u) == 0x7F80u, hi = (y[e] & 0x7F800000u) == 0x7F800000u;
                                 here |= lo | hi;
-                                x[e] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+                                y[e] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
                             }
-                            if (here) *p = make_uint4(x[0], x[1], x[2], x[3]);
+                            if (here) *p = make_uint4(y[0], y[1], y[2], y[3]);
                             bad |= here;
                         }
                         if (bad) atomicOr(&sh.bad_nodes, 1ull << (pos - w.seq.len));
@@ -442,116 +512,154 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int64_t ctx = w.seq.len - (pos0 + 32 * c);   // positions of this quarter before the length
-                        unsigned vis = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << (int)ctx) - 1u;
-                        if (ctx <= 0 && ctx > -64) vis |= (unsigned)(mask >> (int)-ctx);
-                        else if (ctx > 0 && ctx < 32) vis |= (unsigned)(mask << (int)ctx);
-                        vis &= ((good >> (2 * c)) & 1u ? 0x0000FFFFu : 0u) | ((good >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
-                        any |= vis;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!((vis >> e) & 1u)) s[32 * c + e] = 0xFF800000u;
+                        unsigned v = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << (int)ctx) - 1u;
+                        if (ctx <= 0 && ctx > -64) v |= (unsigned)(mask >> (int)-ctx);
+                        else if (ctx > 0 && ctx < 32) v |= (unsigned)(mask << (int)ctx);
+                        v &= ((good >> (2 * c)) & 1u ? 0x0000FFFFu : 0u) | ((good >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
+                        any |= v;
+                        vis[c] = v;
                     }
                     seen |= any != 0;
                 } else {
                     seen = true;
                 }
                 if (busy) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < kTile; ++e) top = fmaxf(top, __uint_as_float(s[e]));
+                    // The maximum over 128 scores, then their exponentials: the second half is read from tensor memory twice, which is
+                    // cheaper than the registers that would hold it.
+                    uint32_t s[64];
+                    tmem_ld32(col_s + 64, s);
+                    tmem_ld32(col_s + 96, s + 32);
+                    tmem_wait_ld(s, s + 32);
+                    if (!whole) { hide(s, vis[2]); hide(s + 32, vis[3]); }
+                    float top = fmaxf(max32(s), max32(s + 32));
+                    tmem_ld32(col_s, s);
+                    tmem_ld32(col_s + 32, s + 32);
+                    tmem_wait_ld(s, s + 32);
+                    if (!whole) { hide(s, vis[0]); hide(s + 32, vis[1]); }
+                    top = fmaxf(top, fmaxf(max32(s), max32(s + 32)));
                     const bool raise = top > -INFINITY && (m == -INFINITY || (top - m) * a.scale_log2 > 8.f);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float corr = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx((m - top) * a.scale_log2);
                         if (raise) m = top;
-                        l *= corr;
-                        if (i > 0) {   // O holds the tiles before: all of them, once the last of them is done
-                            ok = warp_wait(&sh.o_done[(no - 1) & 1], ((no - 1) >> 1) & 1u);
-                            if (!ok) break;
-                            tc_fence_after_sync();
+                        const uint64_t corr2 = pair_f32(corr, corr);
+                        l2[0] = fma_f32x2(l2[0], corr2, 0ull);
+                        l2[1] = fma_f32x2(l2[1], corr2, 0ull);
+                        if (x > 0) {   // O holds the stream's steps before, all complete (this step's S was issued after them)
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t o[32];
-                                tmem_ld32(lanes + kColO + 32 * c, o);
-                                tmem_wait_ld();
+                                tmem_ld32(col_o + 32 * c, o);
+                                tmem_wait_ld(o);
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                tmem_st32(lanes + kColO + 32 * c, o);
+                                tmem_st32(col_o + 32 * c, o);
                             }
                         }
                     }
-                    if (no >= 2) {   // P's place is free once the tile before the last is done
-                        ok = warp_wait(&sh.o_done[buf], ((no - 2) >> 1) & 1u);
-                        if (!ok) break;
-                        tc_fence_after_sync();
-                    }
-                    const float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float x = exp2_approx(fmaf(__uint_as_float(s[32 * c + 2 * e]), a.scale_log2, -mc));
-                            const float y = exp2_approx(fmaf(__uint_as_float(s[32 * c + 2 * e + 1]), a.scale_log2, -mc));
-                            l += x + y;
-                            p[e] = pack_bf16(x, y);
-                        }
-                        tmem_st16(lanes + kColP + buf * (kTile / 2) + 16 * c, p);
-                    }
+                    const float mc = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                    const uint64_t mc2 = pair_f32(mc, mc);
+                    uint32_t t[32], p[16];
+                    tmem_ld32(col_s + 64, t);
+                    exp32(s, scale2, mc2, l2, p);
+                    tmem_st16(col_s, p);   // the first half of S, which has been read
+                    exp32(s + 32, scale2, mc2, l2, p);
+                    tmem_st16(col_s + 16, p);
+                    tmem_wait_ld(t);
+                    tmem_ld32(col_s + 96, s);
+                    if (!whole) hide(t, vis[2]);
+                    exp32(t, scale2, mc2, l2, p);
+                    tmem_st16(col_s + 32, p);
+                    tmem_wait_ld(s);
+                    if (!whole) hide(s, vis[3]);
+                    exp32(s, scale2, mc2, l2, p);
+                    tmem_st16(col_s + 48, p);
                     tmem_wait_st();
                 }
                 tc_fence_before_sync();
-                mbar_arrive(&sh.p_full[buf]);
+                mbar_arrive(&sh.p_full[st]);
             }
             if (!ok) break;
+            const float2 la = split_f32(add_f32x2(l2[0], l2[1]));
+            float l = la.x + la.y, mc = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+            if (m == -INFINITY) l = seen ? NAN : 0.f;   // every score minus infinity, or nothing seen
+            sh.ml[st][row_l] = make_float2(mc, l);
             base += 2 * n;
-            j += n;
-            ok = warp_wait(&sh.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1u);
+            tile_no += n;
+            steps[0] += RT == 2 ? n : (n + 1) >> 1;
+            steps[1] += RT == 2 ? n : n >> 1;
+            // this thread's columns [d0, d0 + width) of its row: RT = 1 adds the streams, each one's warps a half of the columns
+            const bool both = RT == 1 && n > 1;
+            if (mine > 0) ok = warp_wait(&sh.o_done[st], ((st ? steps[1] : steps[0]) - 1) & 1u);
+            group_sync();   // the other stream's maximum, sum and O, every tile's bad nodes
             if (!ok) break;
             tc_fence_after_sync();
-            group_sync();   // every tile's bad nodes are known
-            if (!ok) break;
             const unsigned long long bad = sh.bad_nodes;
-            if (m == -INFINITY) l = seen ? NAN : 0.f;   // every score minus infinity, or nothing seen
-            const float mc = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+            float f0 = 1.f, f1 = 0.f;
+            if (RT == 1) {
+                const float2 a0 = sh.ml[0][row_l], a1 = both ? sh.ml[1][row_l] : make_float2(-INFINITY, 0.f);
+                mc = fmaxf(a0.x, a1.x);
+                f0 = a0.x == -INFINITY ? 0.f : exp2_approx(a0.x - mc);
+                f1 = a1.x == -INFINITY ? 0.f : exp2_approx(a1.x - mc);
+                l = mc == -INFINITY ? a0.y + a1.y : (a0.x == -INFINITY ? 0.f : a0.y * f0) + (a1.x == -INFINITY ? 0.f : a1.y * f1);
+            }
             const bool complete = n == w.seq.tiles;
-            if (busy) {
+            if (busy || RT == 1) {
+                constexpr int kWidth = RT == 1 ? 64 : 128;
+                const int d0 = RT == 1 ? 64 * st : 0;
                 const float inv = 1.f / l;
                 const int64_t slot = (int64_t)blockIdx.x * 2 + (stretch > 0);
+                const int part_row = RT == 2 ? st * kTile + row_l : row_l;
                 __nv_bfloat16* out = a.out + (((int64_t)w.r * a.nodes + row / a.group) * a.hq + kvh * a.group + row % a.group) * kHeadDim;
-                float* part = a.part + (slot * a.tile_rows + row_l) * kHeadDim;
+                float* part = a.part + (slot * a.tile_rows + part_row) * kHeadDim;
+                if (busy) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(lanes + kColO + 32 * c, o);
-                    tmem_wait_ld();
-                    if (live && complete) {
+                    for (int c = 0; c < kWidth; c += 32) {
+                        uint32_t o[32];
+                        if (RT == 1) {
+                            uint32_t q[32];
+                            tmem_ld32(lanes + kColO + d0 + c, o);
+                            if (both) tmem_ld32(lanes + kColO + kHeadDim + d0 + c, q);
+                            tmem_wait_ld(o, q);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint32_t p[4];
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                const float x = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u]) * inv, y = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u + 1]) * inv;
-                                p[u] = pack_bf16(x, y);
+                            for (int e = 0; e < 32; ++e) {
+                                float v = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
+                                if (both && f1 != 0.f) v += __uint_as_float(q[e]) * f1;
+                                o[e] = __float_as_uint(v);
                             }
-                            *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(p[0], p[1], p[2], p[3]);
+                        } else {
+                            tmem_ld32(col_o + c, o);
+                            tmem_wait_ld(o);
                         }
-                    } else if (live) {
+                        if (live && complete) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            for (int e = 0; e < 32; e += 8) {
+                                uint32_t p[4];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    const float y = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u]) * inv, z = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u + 1]) * inv;
+                                    p[u] = pack_bf16(y, z);
+                                }
+                                *reinterpret_cast<uint4*>(out + d0 + c + e) = make_uint4(p[0], p[1], p[2], p[3]);
+                            }
+                        } else if (live) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + d0 + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
                 if (live) {
-                    if (!complete) a.part_ml[slot * a.tile_rows + row_l] = make_float2(mc, l);
+                    if (!complete && (RT == 2 || !st)) a.part_ml[slot * a.tile_rows + part_row] = make_float2(mc, l);
                     if (bad) {
-                        if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, out);
-                        else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, part);
+                        if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, out, d0, d0 + kWidth);
+                        else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, part, d0, d0 + kWidth);
                     }
                 }
             }
-            group_sync();   // and have been read
-            if (tid == kSoftmaxThreads) sh.bad_nodes = 0;
+            __syncwarp();
             tc_fence_before_sync();
+            group_sync();   // sums and bad nodes have been read
+            if (tid == 128) sh.bad_nodes = 0;
         }
         if (!ok) sh.failed = 1;
     }
@@ -575,7 +683,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     tree_prefix(a, r, before, total, red);
     const int m_rows = a.nodes * a.group;
     if (local >= a.kv_heads * m_rows) return;
-    const int kvh = local / m_rows, row = local % m_rows, rt = row / kTile, row_l = row % kTile;
+    const int kvh = local / m_rows, row = local % m_rows, span = m_rows > kTile ? 2 * kTile : kTile, rt = row / span, row_l = row % span;
     const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
     const int tiles = tree_seq(a, r).tiles;
     const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * tiles, c0 = s0 / quota, c1 = (s0 + tiles - 1) / quota;
@@ -634,7 +742,7 @@ static CUtensorMap page_map(const void* base, const mfqb_cache& c) {
     return map;
 }
 
-static int tree_rows(const mfqb_cache& c, int q_heads, int nodes) { return std::min(kTile, nodes * (q_heads / c.kv_heads)); }
+static int tree_rows(const mfqb_cache& c, int q_heads, int nodes) { return std::min(2 * kTile, nodes * (q_heads / c.kv_heads)); }
 static uint64_t tree_attention_work_bytes(const mfqb_cache& c, int q_heads, int nodes) {
     return (uint64_t)kTreeCtas * 2 * tree_rows(c, q_heads, nodes) * (kHeadDim * 4 + 8);
 }
@@ -664,7 +772,8 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.hq = q_heads;
     a.group = q_heads / c.kv_heads;
     a.nodes = nodes;
-    a.row_tiles = (nodes * a.group + kTile - 1) / kTile;
+    const int rt = nodes * a.group > kTile ? 2 : 1;   // see tree_attn_kernel
+    a.row_tiles = (nodes * a.group + rt * kTile - 1) / (rt * kTile);
     a.tile_rows = tree_rows(c, q_heads, nodes);
     a.part = static_cast<float*>(work);
     a.part_ml = reinterpret_cast<float2*>(a.part + (int64_t)kTreeCtas * 2 * a.tile_rows * kHeadDim);
@@ -672,8 +781,11 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.error = device_status_word(device);
     const CUtensorMap kmap = page_map(a.k, c), vmap = page_map(a.v, c);
     static std::once_flag once[64];
-    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem)); });
-    launch_chained(tree_attn_kernel, dim3(kTreeCtas), dim3(kTreeThreads), kTreeSmem, s, a, kmap, vmap);
+    std::call_once(once[device], [] {
+        MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem));
+        MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem));
+    });
+    launch_chained(rt == 2 ? tree_attn_kernel<2> : tree_attn_kernel<1>, dim3(kTreeCtas), dim3(kTreeThreads), kTreeSmem, s, a, kmap, vmap);
     const int per_seq = (c.kv_heads * nodes * a.group + 7) / 8;
     launch_chained(tree_merge_kernel, dim3((unsigned)(c.rows * per_seq)), dim3(256), 0, s, a, (int)kTreeCtas, per_seq);
 }
