@@ -28,7 +28,7 @@ constexpr int kTreeCtas = 148;                       // one per SM
 constexpr int kTile = 128;                           // rows of Q, positions of a tile
 constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
 constexpr int kTreeTiles = 7, kTreeRingMax = kTreeTiles - 1;   // 32 KB tiles in shared memory: Q once or twice, the others are the ring
-constexpr int kSoftmaxThreads = 256, kTreeThreads = 128 + kSoftmaxThreads;
+constexpr int kSoftmaxWarps = 8, kTreeThreads = 128 + 32 * kSoftmaxWarps;
 constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory columns: S of the two streams (P takes the place of its first half), O of the two
 
 struct TreeArgs {
@@ -47,15 +47,14 @@ struct TreeArgs {
 
 // Tiles of sequence r (at least one: a sequence has a node), its length and end.
 struct TreeSeq {
-    int64_t len, end;
-    int tiles;
+    int len, end, tiles;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
-    const int64_t cap = (int64_t)a.width * a.page;
+    const int cap = a.width * a.page;   // at most 2^30
     TreeSeq s;
-    s.len = min(max((int64_t)__ldcg(a.lens + r), (int64_t)0), cap);
+    s.len = min(max(__ldcg(a.lens + r), 0), cap);
     s.end = min(s.len + a.nodes, cap);
-    s.tiles = (int)((s.end + kTile - 1) / kTile);
+    s.tiles = (s.end + kTile - 1) / kTile;
     return s;
 }
 // Sum of tiles of the rows before `row` and of all rows; 256 threads.
@@ -157,13 +156,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
                  : "r"(taddr)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : MFQB_R8(r, 0), MFQB_R8(r, 8)
+                 : "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
                  ::MFQB_W8(r, 0), MFQB_W8(r, 8), MFQB_W8(r, 16), MFQB_W8(r, 24), "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MFQB_W8(r, 0), MFQB_W8(r, 8), "r"(taddr)
                  : "memory");
 }
 #define MFQB_P8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
@@ -172,6 +173,10 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     asm volatile("" : MFQB_P8(r, 0), MFQB_P8(r, 8));
     asm volatile("" : MFQB_P8(r, 16), MFQB_P8(r, 24));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    asm volatile("" : MFQB_P8(r, 0), MFQB_P8(r, 8));
 }
 __device__ __forceinline__ void tmem_wait_ld(uint32_t* r, uint32_t* q) {
     tmem_wait_ld(r);
@@ -186,6 +191,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {   // one arrival for what all lanes have done
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
@@ -217,22 +226,18 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     return r;
 }
 // Scores that a row does not see become minus infinity.
-__device__ __forceinline__ void hide(uint32_t* s, unsigned vis) {
+__device__ __forceinline__ void hide16(uint32_t* s, unsigned vis) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
+    for (int e = 0; e < 16; ++e)
         if (!((vis >> e) & 1u)) s[e] = 0xFF800000u;
 }
-__device__ __forceinline__ float max32(const uint32_t* s) {
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+// exp2(scale s + mc) of 16 scores, rounded to bf16 into p; their sums are added to l, their maxima to top.
+__device__ __forceinline__ void exp16(const uint32_t* s, uint64_t scale, uint64_t mc, uint64_t (&l)[2], float (&top)[2], uint32_t* p) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) m[e & 3] = fmaxf(m[e & 3], __uint_as_float(s[e]));
-    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-}
-// exp2(scale s - mc) of 32 scores, rounded to bf16 into p; their sums into l.
-__device__ __forceinline__ void exp32(const uint32_t* s, uint64_t scale, uint64_t mc, uint64_t (&l)[2], uint32_t* p) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const float2 x = split_f32(fma_f32x2(pair_f32(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale, mc));
+    for (int e = 0; e < 8; ++e) {
+        const float a = __uint_as_float(s[2 * e]), b = __uint_as_float(s[2 * e + 1]);
+        top[e & 1] = fmaxf(fmaxf(top[e & 1], a), b);
+        const float2 x = split_f32(fma_f32x2(pair_f32(a, b), scale, mc));
         const float u = exp2_approx(x.x), v = exp2_approx(x.y);
         l[e & 1] = add_f32x2(l[e & 1], pair_f32(u, v));
         p[e] = pack_bf16(u, v);
@@ -246,7 +251,7 @@ __device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long
     const int node = row / a.group, h = kvh * a.group + row % a.group;
     bad &= a.masks[(int64_t)r * a.nodes + node];
     for (; bad; bad &= bad - 1) {
-        const int64_t t = seq.len + (__ffsll((long long)bad) - 1);
+        const int t = seq.len + (__ffsll((long long)bad) - 1);
         const int page = a.table[(int64_t)r * a.width + t / a.page];
         const int64_t at = (((int64_t)page * a.kv_heads + kvh) * a.page + (t & (a.page - 1))) * kHeadDim;
         const __nv_bfloat16* q = a.q + (((int64_t)r * a.nodes + node) * a.hq + h) * kHeadDim;
@@ -274,10 +279,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) { mbar_init(&sh.kv_full[i], 1); mbar_init(&sh.kv_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], kSoftmaxThreads / 2); mbar_init(&sh.o_done[i], 1); }
-        mbar_init(&sh.q_full, kSoftmaxThreads);
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], kSoftmaxWarps / 2); mbar_init(&sh.o_done[i], 1); }
+        mbar_init(&sh.q_full, kSoftmaxWarps);
         mbar_init(&sh.drain, 1);
-        mbar_init(&sh.group, kSoftmaxThreads);
+        mbar_init(&sh.group, kSoftmaxWarps);
         sh.bad_nodes = 0;
         sh.failed = 0;
         sh.first = sh.last = 0;
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         uint32_t issued = 0, tile_no = 0;
         bool ok = true;
         int pages[2] = {-1, -1};   // this lane's page of the last two tiles
-        auto ask = [&](const CUtensorMap* map, int kvh, int64_t pos, int page) {
+        auto ask = [&](const CUtensorMap* map, int kvh, int pos, int page) {
             const uint32_t stage = issued % kRing;
             ok = warp_wait(&sh.kv_empty[stage], ((issued / kRing) & 1u) ^ 1u);
             if (!ok) return;
@@ -344,16 +349,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[stage], (uint32_t)__popc(have) * (uint32_t)box * 256u);
             __syncwarp();
             if (page >= 0) {
-                const int y = (int)(pos & (a.page - 1));
+                const int y = pos & (a.page - 1);
                 tma_load_4d(dst, map, 0, y, kvh, page, &sh.kv_full[stage]);
                 tma_load_4d(dst + kHalfBytes, map, 64, y, kvh, page, &sh.kv_full[stage]);
             }
             __syncwarp();
             ++issued;
         };
-        auto position = [&](int i) { return (int64_t)(w.t0 + i) * kTile + lane * box; };   // of this lane's box
+        auto position = [&](int i) { return (w.t0 + i) * kTile + lane * box; };   // of this lane's box
         auto keys = [&](int kvh, int i) {
-            const int64_t pos = position(i);
+            const int pos = position(i);
             int page = -1;
             if (lane < boxes && pos < w.seq.end) page = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
             if ((unsigned)page >= (unsigned)a.pages) page = -1;
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         bool ok = true;
         int stretch = 0;
         auto group_sync = [&]() {   // the eight warps, with a bound like every other wait
-            mbar_arrive(&sh.group);
+            warp_arrive(&sh.group);
             ok = ok && warp_wait(&sh.group, groups++ & 1u);
         };
         const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
@@ -450,18 +455,28 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             const int kvh = w.item / a.row_tiles, rt = w.item % a.row_tiles, n = w.t1 - w.t0;
             const int tile0 = rt * RT * kTile + (RT == 2 ? st * kTile : 0), row = tile0 + row_l, m_rows = a.nodes * a.group;   // first row, this thread's row of Q
             const bool live = row < m_rows, busy = tile0 + (warp & 3) * 32 < m_rows;   // busy: some row of the warp is one
-            // Q, 16 threads a row of 256 bytes; the products that read the last stretch's are done (its S has been read)
-            for (int i = RT == 2 ? row_l : tid - 128; i < kTile * 16; i += RT == 2 ? 128 : 256) {
-                const int rr = i >> 4, c = i & 15, qr = tile0 + rr;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (qr < m_rows) {
-                    const int node = qr / a.group, h = kvh * a.group + qr % a.group;
-                    v = __ldg(reinterpret_cast<const uint4*>(a.q + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim) + c);
+            // Q, 16 threads a row of 256 bytes, all loads at once; the products that read the last stretch's are done (its S has been
+            // read).  Rows behind the last one stay as they are: a row of S depends on its own row of Q alone.
+            {
+                constexpr int kStep = RT == 2 ? 8 : 16, kLoads = kTile / kStep;
+                const int c = tid & 15, r0 = (RT == 2 ? row_l : tid - 128) >> 4;
+                uint4 v[kLoads];
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j) {
+                    const int qr = tile0 + r0 + kStep * j;
+                    if (qr < m_rows) {
+                        const int node = qr / a.group, h = kvh * a.group + qr - node * a.group;
+                        v[j] = __ldg(reinterpret_cast<const uint4*>(a.q + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim) + c);
+                    }
                 }
-                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j) {
+                    const int rr = r0 + kStep * j;
+                    if (tile0 + rr < m_rows) *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[j];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&sh.q_full);
+            warp_arrive(&sh.q_full);
             unsigned long long mask = live ? a.masks[(int64_t)w.r * a.nodes + row / a.group] : 0ull;
             if (a.nodes < 64) mask &= (1ull << a.nodes) - 1ull;
             float m = -INFINITY;   // maximum of the scores so far (or less, see above)
@@ -474,7 +489,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 if (!ok) break;
                 tc_fence_after_sync();
                 const unsigned good = sh.good[(tile_no + i) & 7];
-                const int64_t pos0 = (int64_t)(w.t0 + i) * kTile;
+                const int pos0 = (w.t0 + i) * kTile;
                 const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
                 unsigned vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
                 if (!whole) {
@@ -482,7 +497,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                     const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
                     ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
                     if (!ok) break;
-                    const int64_t pos = pos0 + row_l;
+                    const int pos = pos0 + row_l;
                     unsigned char* vrow = ring + (size_t)stage * kTileBytes + row_l * 128;
                     if (pos >= w.seq.end || !((good >> (row_l >> 4)) & 1u)) {
 #pragma unroll
@@ -511,10 +526,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                     unsigned any = 0;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const int64_t ctx = w.seq.len - (pos0 + 32 * c);   // positions of this quarter before the length
-                        unsigned v = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << (int)ctx) - 1u;
-                        if (ctx <= 0 && ctx > -64) v |= (unsigned)(mask >> (int)-ctx);
-                        else if (ctx > 0 && ctx < 32) v |= (unsigned)(mask << (int)ctx);
+                        const int ctx = w.seq.len - (pos0 + 32 * c);   // positions of this quarter before the length
+                        unsigned v = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
+                        if (ctx <= 0 && ctx > -64) v |= (unsigned)(mask >> -ctx);
+                        else if (ctx > 0 && ctx < 32) v |= (unsigned)(mask << ctx);
                         v &= ((good >> (2 * c)) & 1u ? 0x0000FFFFu : 0u) | ((good >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
                         any |= v;
                         vis[c] = v;
@@ -524,23 +539,33 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                     seen = true;
                 }
                 if (busy) {
-                    // The maximum over 128 scores, then their exponentials: the second half is read from tensor memory twice, which is
-                    // cheaper than the registers that would hold it.
-                    uint32_t s[64];
-                    tmem_ld32(col_s + 64, s);
-                    tmem_ld32(col_s + 96, s + 32);
-                    tmem_wait_ld(s, s + 32);
-                    if (!whole) { hide(s, vis[2]); hide(s + 32, vis[3]); }
-                    float top = fmaxf(max32(s), max32(s + 32));
-                    tmem_ld32(col_s, s);
-                    tmem_ld32(col_s + 32, s + 32);
-                    tmem_wait_ld(s, s + 32);
-                    if (!whole) { hide(s, vis[0]); hide(s + 32, vis[1]); }
-                    top = fmaxf(top, fmaxf(max32(s), max32(s + 32)));
-                    const bool raise = top > -INFINITY && (m == -INFINITY || (top - m) * a.scale_log2 > 8.f);
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float corr = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx((m - top) * a.scale_log2);
-                        if (raise) m = top;
+                    // The exponentials are formed with the maximum as it was, the tile's own is found beside them; only where it has grown
+                    // too far (every first tile, few later ones) they are formed again.  P waits in registers meanwhile, S in tensor memory.
+                    uint32_t p[64];
+                    for (;;) {
+                        const float mc = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                        const uint64_t mc2 = pair_f32(mc, mc);
+                        uint64_t sum[2] = {l2[0], l2[1]};
+                        float top[2] = {-INFINITY, -INFINITY};
+                        uint32_t s[2][16];
+                        tmem_ld16_async(col_s, s[0]);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t* now = s[c & 1];
+                            tmem_wait_ld16(now);
+                            if (c < 7) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
+                            if (!whole) hide16(now, vis[c >> 1] >> (16 * (c & 1)));
+                            exp16(now, scale2, mc2, sum, top, p + 8 * c);
+                        }
+                        const float high = fmaxf(top[0], top[1]);
+                        const bool raise = live && high > -INFINITY && (m == -INFINITY || (high - m) * a.scale_log2 > 8.f);
+                        if (!__any_sync(0xffffffffu, raise)) {
+                            l2[0] = sum[0];
+                            l2[1] = sum[1];
+                            break;
+                        }
+                        const float corr = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx((m - high) * a.scale_log2);
+                        if (raise) m = high;
                         const uint64_t corr2 = pair_f32(corr, corr);
                         l2[0] = fma_f32x2(l2[0], corr2, 0ull);
                         l2[1] = fma_f32x2(l2[1], corr2, 0ull);
@@ -556,27 +581,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                             }
                         }
                     }
-                    const float mc = m == -INFINITY ? 0.f : -m * a.scale_log2;
-                    const uint64_t mc2 = pair_f32(mc, mc);
-                    uint32_t t[32], p[16];
-                    tmem_ld32(col_s + 64, t);
-                    exp32(s, scale2, mc2, l2, p);
-                    tmem_st16(col_s, p);   // the first half of S, which has been read
-                    exp32(s + 32, scale2, mc2, l2, p);
-                    tmem_st16(col_s + 16, p);
-                    tmem_wait_ld(t);
-                    tmem_ld32(col_s + 96, s);
-                    if (!whole) hide(t, vis[2]);
-                    exp32(t, scale2, mc2, l2, p);
-                    tmem_st16(col_s + 32, p);
-                    tmem_wait_ld(s);
-                    if (!whole) hide(s, vis[3]);
-                    exp32(s, scale2, mc2, l2, p);
-                    tmem_st16(col_s + 48, p);
+                    tmem_st32(col_s, p);   // in the place of S, all of which has been read
+                    tmem_st32(col_s + 32, p + 32);
                     tmem_wait_st();
                 }
                 tc_fence_before_sync();
-                mbar_arrive(&sh.p_full[st]);
+                warp_arrive(&sh.p_full[st]);
             }
             if (!ok) break;
             const float2 la = split_f32(add_f32x2(l2[0], l2[1]));
