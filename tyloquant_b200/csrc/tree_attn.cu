@@ -29,6 +29,7 @@ constexpr int kTile = 128;                           // rows of Q, positions of 
 constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
 constexpr int kTreeTiles = 7, kTreeRingMax = kTreeTiles - 1;   // 32 KB tiles in shared memory: Q once or twice, the others are the ring
 constexpr int kSoftmaxWarps = 8, kTreeThreads = 128 + 32 * kSoftmaxWarps;
+constexpr int kTreeStart = 2;                         // what starting and ending a stretch takes, in tiles
 constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory columns: S of the two streams (P takes the place of its first half), O of the two
 
 struct TreeArgs {
@@ -48,6 +49,7 @@ struct TreeArgs {
 // Tiles of sequence r (at least one: a sequence has a node), its length and end.
 struct TreeSeq {
     int len, end, tiles;
+    __device__ __forceinline__ int units() const { return tiles + kTreeStart; }
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
     const int cap = a.width * a.page;   // at most 2^30
@@ -57,11 +59,11 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
     s.tiles = (s.end + kTile - 1) / kTile;
     return s;
 }
-// Sum of tiles of the rows before `row` and of all rows; 256 threads.
+// Sum of units of the rows before `row` and of all rows, for one item of each; 256 threads.
 __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int row, int64_t& before, int64_t& total, int64_t (*red)[2]) {
     int64_t b = 0, t = 0;
     for (int r = threadIdx.x; r < a.rows; r += 256) {
-        const int n = tree_seq(a, r).tiles;
+        const int n = tree_seq(a, r).units();
         t += n;
         if (r < row) b += n;
     }
@@ -77,7 +79,7 @@ __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int row, int64_t&
 }
 
 struct TreeShared {
-    uint64_t kv_full[kTreeRingMax], kv_empty[kTreeRingMax], q_full, s_full[2], p_full[2], o_done[2], drain, group;
+    uint64_t kv_full[kTreeRingMax], kv_empty[kTreeRingMax], q_full, s_full[2], p_full[2], o_done[2], drain, all, group[2];
     unsigned long long bad_nodes;   // nodes of the stretch whose values hold an infinity or NaN
     int64_t scan[12];
     int64_t first, last, item_off;  // the CTA's units; offset of its first one in its sequence's
@@ -94,27 +96,37 @@ static_assert(kTreeSmem <= 227 * 1024, "one CTA's shared memory");
 // A CTA's stretches in order: sequence, item (kv head, row tile), tiles [t0, t1) of seq.tiles.
 struct TreeWalk {
     int r, item, t0, t1;
-    int64_t left;
+    int64_t left;   // units from the stretch on; units kTreeStart .. of an item are its tiles
     TreeSeq seq;
     __device__ __forceinline__ void start(const TreeArgs& a, const TreeShared& sh) {
         r = sh.row0;
         left = sh.last - sh.first;
         if (left > 0) {
             seq = tree_seq(a, r);
-            item = (int)(sh.item_off / seq.tiles);
-            t0 = (int)(sh.item_off % seq.tiles);
-            t1 = (int)min((int64_t)seq.tiles, t0 + left);
+            item = (int)(sh.item_off / seq.units());
+            const int u0 = (int)(sh.item_off % seq.units());
+            left += u0;   // as if the item's start were the CTA's too
+            stretch(max(u0 - kTreeStart, 0));
         }
     }
     __device__ __forceinline__ void next(const TreeArgs& a) {
-        left -= t1 - t0;
-        if (left <= 0) return;
+        left -= seq.units();
+        if (left <= kTreeStart) {
+            left = 0;
+            return;
+        }
         if (++item == a.kv_heads * a.row_tiles) {
             item = 0;
             seq = tree_seq(a, ++r);
         }
-        t0 = 0;
-        t1 = (int)min((int64_t)seq.tiles, left);
+        stretch(0);
+    }
+
+private:
+    __device__ __forceinline__ void stretch(int first) {
+        t0 = first;
+        t1 = (int)min((int64_t)seq.tiles, left - kTreeStart);
+        if (t1 <= t0) left = 0;   // nothing but units of the start
     }
 };
 
@@ -165,6 +177,10 @@ __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
                  ::MFQB_W8(r, 0), MFQB_W8(r, 8), MFQB_W8(r, 16), MFQB_W8(r, 24), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MFQB_W8(r, 0), MFQB_W8(r, 8), "r"(taddr)
                  : "memory");
 }
 #define MFQB_P8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
@@ -225,23 +241,48 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// Scores that a row does not see become minus infinity.
-__device__ __forceinline__ void hide16(uint32_t* s, unsigned vis) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-        if (!((vis >> e) & 1u)) s[e] = 0xFF800000u;
-}
-// exp2(scale s + mc) of 16 scores, rounded to bf16 into p; their sums are added to l, their maxima to top.
+// exp2(scale s + mc) of 16 scores, rounded to bf16 into p; their sums are added to l, their maxima to top where TOP.
+template <bool TOP>
 __device__ __forceinline__ void exp16(const uint32_t* s, uint64_t scale, uint64_t mc, uint64_t (&l)[2], float (&top)[2], uint32_t* p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float a = __uint_as_float(s[2 * e]), b = __uint_as_float(s[2 * e + 1]);
-        top[e & 1] = fmaxf(fmaxf(top[e & 1], a), b);
+        if (TOP) top[e & 1] = fmaxf(fmaxf(top[e & 1], a), b);
         const float2 x = split_f32(fma_f32x2(pair_f32(a, b), scale, mc));
         const float u = exp2_approx(x.x), v = exp2_approx(x.y);
         l[e & 1] = add_f32x2(l[e & 1], pair_f32(u, v));
         p[e] = pack_bf16(u, v);
     }
+}
+
+// Values of a tile that is not whole, in shared memory: rows that no row of Q sees (behind the end up to the next 16, without a page)
+// are cleared; an infinity or NaN of a node becomes 0 and the node is noted (add_bad_nodes).  The four warps of a stream; a row of 256
+// bytes is two halves of 128.  Two streams may do the same tile at once: they write the same.
+__device__ __noinline__ void clean_values(TreeShared& sh, unsigned char* tile, TreeSeq seq, int pos0, unsigned good, int quarter, int lane) {
+    const int end = min(kTile, seq.end - pos0), first = max(0, seq.len - pos0);   // nodes are rows first .. end - 1
+    unsigned char* piece = tile + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;
+    const int r0 = 2 * quarter + (lane >> 4);
+    if (good != 0xFFu || (end & 15))
+        for (int r = r0; r < ((end + 15) & ~15); r += 8)
+            if (r >= end || !((good >> (r >> 4)) & 1u)) *reinterpret_cast<uint4*>(piece + r * 128) = make_uint4(0u, 0u, 0u, 0u);
+    for (int r = first + r0; r < end; r += 8) {
+        if (!((good >> (r >> 4)) & 1u)) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(piece + r * 128);
+        uint32_t y[4] = {v.x, v.y, v.z, v.w};
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool lo = (y[e] & 0x7F80u) == 0x7F80u, hi = (y[e] & 0x7F800000u) == 0x7F800000u;
+            bad |= lo | hi;
+            y[e] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+        }
+        if (bad) {
+            *reinterpret_cast<uint4*>(piece + r * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+            atomicOr(&sh.bad_nodes, 1ull << (pos0 + r - seq.len));
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
 }
 
 // Rare: values of visible nodes that hold an infinity or NaN were taken out of the product (0 in their place, so that rows which do not see
@@ -268,8 +309,12 @@ __device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long
 // Two streams of steps take turns on the tensor core, each with its own S, O and four softmax warps: while one stream's scores become
 // probabilities the other's products run.  RT = 1 (up to 128 rows): the streams take alternate tiles of positions and are added at the end
 // of a stretch.  RT = 2: each stream has 128 of 256 rows, both take every tile, which is read once for the two.  Step u of a stretch:
-// stream u & 1; its S waits for the product of step u - 2, whose P lies in S's place.
-template <int RT>
+// stream u & 1; its S waits for the product of step u - 2, whose P lies in S's place.  One warp issues for both: with a
+// warp each the streams fall into step, and the tensor core waits while both do softmax (16 sequences of one token at context 4096 73 us in
+// place of 57).
+// REP: up to 32 (64) rows stand in Q four times (twice), and a copy's warps take a quarter (a half) of every tile's positions: their
+// P is zero elsewhere.  A row's 128 exponentials in one thread are what a tile waits for otherwise.
+template <int RT, int REP>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap) {
     constexpr int kRing = kTreeTiles - RT;
@@ -279,10 +324,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) { mbar_init(&sh.kv_full[i], 1); mbar_init(&sh.kv_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], kSoftmaxWarps / 2); mbar_init(&sh.o_done[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.group[i], kSoftmaxWarps / 2); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], kSoftmaxWarps / 2); mbar_init(&sh.o_done[i], 1); }
         mbar_init(&sh.q_full, kSoftmaxWarps);
+        mbar_init(&sh.all, kSoftmaxWarps);
         mbar_init(&sh.drain, 1);
-        mbar_init(&sh.group, kSoftmaxWarps);
         sh.bad_nodes = 0;
         sh.failed = 0;
         sh.first = sh.last = 0;
@@ -296,12 +341,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     chained_wait();
     {   // this CTA's units: thread t holds the sequences 3t .. 3t + 2
         constexpr int kEach = (kCacheRows + kTreeThreads - 1) / kTreeThreads;
-        int tiles[kEach];
+        int units_of[kEach];
         int64_t mine = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            tiles[j] = kEach * tid + j < a.rows ? tree_seq(a, kEach * tid + j).tiles : 0;
-            mine += tiles[j];
+            units_of[j] = kEach * tid + j < a.rows ? tree_seq(a, kEach * tid + j).units() : 0;
+            mine += units_of[j];
         }
         int64_t upto = mine;
         for (int o = 1; o < 32; o <<= 1) {
@@ -321,7 +366,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         int64_t begin = (upto - mine) * items;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int64_t end = begin + tiles[j] * items;
+            const int64_t end = begin + units_of[j] * items;
             if (first < last && begin <= first && first < end) {
                 sh.row0 = kEach * tid + j;
                 sh.item_off = first - begin;
@@ -392,8 +437,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         auto scores = [&](int u) {
             const int i = RT == 2 ? u >> 1 : u, st = u & 1;
             const uint32_t at = base + key_at<RT>(i), stage = at % kRing;
-            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
-            if (ok && u >= 2) ok = warp_wait(&sh.o_done[st], ((st ? steps[1] : steps[0]) + (u >> 1) - 1) & 1u);
+            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u) && (u < 2 || warp_wait(&sh.o_done[st], ((st ? steps[1] : steps[0]) + (u >> 1) - 1) & 1u));
             if (!ok) return;
             tc_fence_after_sync();
             const uint32_t k_addr = ring_addr + stage * kTileBytes, q = q_addr + (RT == 2 ? st * kTileBytes : 0), d = tmem + kColS + st * kTile;
@@ -401,8 +445,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
                     tc_mma_f16_ss(d, smem_desc_sw128(q + (s >> 2) * kHalfBytes + (s & 3) * 32), smem_desc_sw128(k_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), idesc_s, s > 0);
-                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
                 tc_commit(&sh.s_full[st]);
+                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
             }
             __syncwarp();
         };
@@ -413,11 +457,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             if (!ok) return;
             tc_fence_after_sync();
             const uint32_t v_addr = ring_addr + stage * kTileBytes, p = tmem + kColS + st * kTile, d = tmem + kColO + st * kHeadDim;
+            const int groups = min(8, (w.seq.end - (w.t0 + i) * kTile + 15) >> 4);   // of 16 positions; behind the end nothing is there to be multiplied
             if (elect_one()) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, u > 1 || s > 0);
-                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
+                for (int s = 0; s < 8; ++s)
+                    if (s < groups) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, u > 1 || s > 0);
                 tc_commit(&sh.o_done[st]);
+                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
             }
             __syncwarp();
         };
@@ -439,40 +485,43 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         __syncwarp();
         if (!warp_wait(&sh.drain, 0) || !ok) sh.failed = 1;
     } else if (warp >= 4) {
-        // -------- softmax: stream = warps 4-7 or 8-11, thread = row of the stream's Q --------
-        const int st = (warp - 4) >> 2, row_l = tid & 127;
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lanes + kColS + st * kTile, col_o = lanes + kColO + st * kHeadDim;
+        // -------- softmax: stream = warps 4-7 or 8-11, thread = lane of tensor memory: row lane_l % kSpan of the tile, copy lane_l / kSpan --------
+        constexpr int kSpan = kTile / REP, kCols = kTile / REP;   // rows, a copy's positions of a tile
+        const int st = (warp - 4) >> 2, quarter = warp & 3, lane_l = tid & 127, row_l = lane_l % kSpan, copy = lane_l / kSpan;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), col_s = lanes + kColS + st * kTile, col_o = lanes + kColO + st * kHeadDim;
         unsigned char* q_tile = q_tiles + (RT == 2 ? st * kTileBytes : 0);
-        uint32_t base = 0, tile_no = 0, groups = 0, steps[2] = {0, 0};
+        uint32_t base = 0, tile_no = 0, alls = 0, groups = 0, steps = 0;
         bool ok = true;
         int stretch = 0;
-        auto group_sync = [&]() {   // the eight warps, with a bound like every other wait
-            warp_arrive(&sh.group);
-            ok = ok && warp_wait(&sh.group, groups++ & 1u);
+        auto all_sync = [&]() {   // the eight warps, with a bound like every other wait
+            warp_arrive(&sh.all);
+            ok = ok && warp_wait(&sh.all, alls++ & 1u);
+        };
+        auto group_sync = [&]() {   // the stream's four
+            warp_arrive(&sh.group[st]);
+            ok = ok && warp_wait(&sh.group[st], groups++ & 1u);
         };
         const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
+        const int m_rows = a.nodes * a.group;   // rows of Q in all
         for (; ok && w.left > 0; w.next(a), ++stretch) {
             const int kvh = w.item / a.row_tiles, rt = w.item % a.row_tiles, n = w.t1 - w.t0;
-            const int tile0 = rt * RT * kTile + (RT == 2 ? st * kTile : 0), row = tile0 + row_l, m_rows = a.nodes * a.group;   // first row, this thread's row of Q
-            const bool live = row < m_rows, busy = tile0 + (warp & 3) * 32 < m_rows;   // busy: some row of the warp is one
+            const int tile0 = rt * RT * kTile + (RT == 2 ? st * kTile : 0), row = tile0 + row_l;   // the stream's first row, this thread's
+            const bool live = row < m_rows, busy = tile0 + (quarter * 32) % kSpan < m_rows;   // busy: some row of the warp is one
             // Q, 16 threads a row of 256 bytes, all loads at once; the products that read the last stretch's are done (its S has been
-            // read).  Rows behind the last one stay as they are: a row of S depends on its own row of Q alone.
+            // read).  Rows behind the last one repeat it.
             {
                 constexpr int kStep = RT == 2 ? 8 : 16, kLoads = kTile / kStep;
-                const int c = tid & 15, r0 = (RT == 2 ? row_l : tid - 128) >> 4;
-                uint4 v[kLoads];
+                const int c = tid & 15, r0 = (RT == 2 ? lane_l : tid - 128) >> 4;
+                uint4 v[kLoads / REP];
 #pragma unroll
-                for (int j = 0; j < kLoads; ++j) {
-                    const int qr = tile0 + r0 + kStep * j;
-                    if (qr < m_rows) {
-                        const int node = qr / a.group, h = kvh * a.group + qr - node * a.group;
-                        v[j] = __ldg(reinterpret_cast<const uint4*>(a.q + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim) + c);
-                    }
+                for (int j = 0; j < kLoads / REP; ++j) {
+                    const int qr = min(tile0 + r0 + kStep * j, m_rows - 1), node = qr / a.group, h = kvh * a.group + qr - node * a.group;
+                    v[j] = __ldg(reinterpret_cast<const uint4*>(a.q + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim) + c);
                 }
 #pragma unroll
                 for (int j = 0; j < kLoads; ++j) {
                     const int rr = r0 + kStep * j;
-                    if (tile0 + rr < m_rows) *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[j];
+                    *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[j % (kLoads / REP)];
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -485,104 +534,131 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             const int mine = RT == 2 ? n : (n + 1 - st) >> 1;   // this stream's steps
             for (int x = 0; x < mine; ++x) {
                 const int i = RT == 2 ? x : 2 * x + st;
-                ok = warp_wait(&sh.s_full[st], ((st ? steps[1] : steps[0]) + x) & 1u);
+                ok = warp_wait(&sh.s_full[st], (steps + x) & 1u);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const unsigned good = sh.good[(tile_no + i) & 7];
                 const int pos0 = (w.t0 + i) * kTile;
                 const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
-                unsigned vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
                 if (!whole) {
-                    // V rows that no row sees (behind the end, no page) are cleared, values of nodes cleaned (see add_bad_nodes)
                     const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
                     ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
                     if (!ok) break;
-                    const int pos = pos0 + row_l;
-                    unsigned char* vrow = ring + (size_t)stage * kTileBytes + row_l * 128;
-                    if (pos >= w.seq.end || !((good >> (row_l >> 4)) & 1u)) {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(vrow + (c >> 3) * kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    } else if (pos >= w.seq.len) {
-                        bool bad = false;
-#pragma unroll 4
-                        for (int c = 0; c < 16; ++c) {
-                            uint4* p = reinterpret_cast<uint4*>(vrow + (c >> 3) * kHalfBytes + (c & 7) * 16);
-                            uint32_t y[4] = {p->x, p->y, p->z, p->w};
-                            bool here = false;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const bool lo = (y[e] & 0x7F80u) == 0x7F80u, hi = (y[e] & 0x7F800000u) == 0x7F800000u;
-                                here |= lo | hi;
-                                y[e] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
-                            }
-                            if (here) *p = make_uint4(y[0], y[1], y[2], y[3]);
-                            bad |= here;
-                        }
-                        if (bad) atomicOr(&sh.bad_nodes, 1ull << (pos - w.seq.len));
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    // what this row sees of the tile
+                    clean_values(sh, ring + (size_t)stage * kTileBytes, w.seq, pos0, good, quarter, lane);
+                    // what this row does not see of its copy's positions becomes minus infinity
                     unsigned any = 0;
+#pragma unroll 1
+                    for (int c = 0; c < kCols; c += 32) {
+                        const int p0 = copy * kCols + c, ctx = w.seq.len - (pos0 + p0);   // positions from here on that are before the length
+                        unsigned vis = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
+                        if (ctx <= 0 && ctx > -64) vis |= (unsigned)(mask >> -ctx);
+                        else if (ctx > 0 && ctx < 32) vis |= (unsigned)(mask << ctx);
+                        vis &= ((good >> (p0 >> 4)) & 1u ? 0x0000FFFFu : 0u) | ((good >> ((p0 >> 4) + 1)) & 1u ? 0xFFFF0000u : 0u);
+                        any |= vis;
+                        if (busy && __any_sync(0xffffffffu, vis != 0xFFFFFFFFu)) {
+                            uint32_t s[32];
+                            tmem_ld32(col_s + p0, s);
+                            tmem_wait_ld(s);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int ctx = w.seq.len - (pos0 + 32 * c);   // positions of this quarter before the length
-                        unsigned v = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
-                        if (ctx <= 0 && ctx > -64) v |= (unsigned)(mask >> -ctx);
-                        else if (ctx > 0 && ctx < 32) v |= (unsigned)(mask << ctx);
-                        v &= ((good >> (2 * c)) & 1u ? 0x0000FFFFu : 0u) | ((good >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
-                        any |= v;
-                        vis[c] = v;
+                            for (int e = 0; e < 32; ++e)
+                                if (!((vis >> e) & 1u)) s[e] = 0xFF800000u;
+                            tmem_st32(col_s + p0, s);
+                        }
                     }
+                    tmem_wait_st();
                     seen |= any != 0;
                 } else {
                     seen = true;
                 }
                 if (busy) {
-                    // The exponentials are formed with the maximum as it was, the tile's own is found beside them; only where it has grown
-                    // too far (every first tile, few later ones) they are formed again.  P waits in registers meanwhile, S in tensor memory.
-                    uint32_t p[64];
-                    for (;;) {
-                        const float mc = m == -INFINITY ? 0.f : -m * a.scale_log2;
-                        const uint64_t mc2 = pair_f32(mc, mc);
-                        uint64_t sum[2] = {l2[0], l2[1]};
-                        float top[2] = {-INFINITY, -INFINITY};
-                        uint32_t s[2][16];
-                        tmem_ld16_async(col_s, s[0]);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint32_t* now = s[c & 1];
-                            tmem_wait_ld16(now);
-                            if (c < 7) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
-                            if (!whole) hide16(now, vis[c >> 1] >> (16 * (c & 1)));
-                            exp16(now, scale2, mc2, sum, top, p + 8 * c);
-                        }
-                        const float high = fmaxf(top[0], top[1]);
-                        const bool raise = live && high > -INFINITY && (m == -INFINITY || (high - m) * a.scale_log2 > 8.f);
-                        if (!__any_sync(0xffffffffu, raise)) {
-                            l2[0] = sum[0];
-                            l2[1] = sum[1];
-                            break;
-                        }
+                    auto rescale = [&](float high, bool raise) {   // l and O to a new maximum
                         const float corr = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx((m - high) * a.scale_log2);
                         if (raise) m = high;
                         const uint64_t corr2 = pair_f32(corr, corr);
                         l2[0] = fma_f32x2(l2[0], corr2, 0ull);
                         l2[1] = fma_f32x2(l2[1], corr2, 0ull);
                         if (x > 0) {   // O holds the stream's steps before, all complete (this step's S was issued after them)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
+#pragma unroll 1
+                            for (int c = 0; c < kHeadDim; c += 32) {
                                 uint32_t o[32];
-                                tmem_ld32(col_o + 32 * c, o);
+                                tmem_ld32(col_o + c, o);
                                 tmem_wait_ld(o);
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                tmem_st32(col_o + 32 * c, o);
+                                tmem_st32(col_o + c, o);
                             }
                         }
+                    };
+                    auto too_high = [&](float high) { return live && high > -INFINITY && (m == -INFINITY || (high - m) * a.scale_log2 > 8.f); };
+                    if constexpr (REP > 1) {
+                        uint32_t s[kCols], p[kCols / 2];
+#pragma unroll
+                        for (int c = 0; c < kCols; c += 32) tmem_ld32(col_s + copy * kCols + c, s + c);
+#pragma unroll
+                        for (int c = 0; c < kCols; c += 32) tmem_wait_ld(s + c);
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int e = 0; e < kCols; e += 2) top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+                        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        const bool raise = too_high(high);
+                        if (__any_sync(0xffffffffu, raise)) rescale(high, raise);
+                        const float mc = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                        const uint64_t mc2 = pair_f32(mc, mc);
+                        float unused[2] = {0.f, 0.f};
+#pragma unroll
+                        for (int c = 0; c < kCols; c += 16) exp16<false>(s + c, scale2, mc2, l2, unused, p + c / 2);
+                        // P: this copy's positions, zero for the others'
+                        uint32_t zero[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) zero[e] = 0u;
+#pragma unroll
+                        for (int k = 0; k < REP; ++k)
+#pragma unroll
+                            for (int c = 0; c < kCols / 2; c += 16) tmem_st16(col_s + k * (kCols / 2) + c, k == copy ? p + c : zero);
+                    } else {
+                        // The exponentials are formed with the maximum as it was, the tile's own is found beside them; only where it has grown
+                        // too far they are formed again.  P waits in registers meanwhile, S in tensor memory.
+                        uint32_t p[64];
+                        if (x == 0) {   // there is no maximum yet
+                            float top = -INFINITY;
+#pragma unroll 1
+                            for (int c = 0; c < kTile; c += 32) {
+                                uint32_t s[32];
+                                tmem_ld32(col_s + c, s);
+                                tmem_wait_ld(s);
+                                float t[2] = {top, top};
+#pragma unroll
+                                for (int e = 0; e < 32; e += 2) t[(e >> 1) & 1] = fmaxf(fmaxf(t[(e >> 1) & 1], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+                                top = fmaxf(t[0], t[1]);
+                            }
+                            m = top;
+                        }
+                        for (;;) {
+                            const float mc = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                            const uint64_t mc2 = pair_f32(mc, mc);
+                            uint64_t sum[2] = {l2[0], l2[1]};
+                            float top[2] = {-INFINITY, -INFINITY};
+                            uint32_t s[2][16];
+                            tmem_ld16_async(col_s, s[0]);
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                uint32_t* now = s[c & 1];
+                                tmem_wait_ld16(now);
+                                if (c < 7) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
+                                exp16<true>(now, scale2, mc2, sum, top, p + 8 * c);
+                            }
+                            const float high = fmaxf(top[0], top[1]);
+                            const bool raise = too_high(high);
+                            if (!__any_sync(0xffffffffu, raise)) {
+                                l2[0] = sum[0];
+                                l2[1] = sum[1];
+                                break;
+                            }
+                            rescale(high, raise);
+                        }
+                        tmem_st32(col_s, p);   // in the place of S, all of which has been read
+                        tmem_st32(col_s + 32, p + 32);
                     }
-                    tmem_st32(col_s, p);   // in the place of S, all of which has been read
-                    tmem_st32(col_s + 32, p + 32);
                     tmem_wait_st();
                 }
                 tc_fence_before_sync();
@@ -590,85 +666,112 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             }
             if (!ok) break;
             const float2 la = split_f32(add_f32x2(l2[0], l2[1]));
-            float l = la.x + la.y, mc = m == -INFINITY ? -INFINITY : m * a.scale_log2;
-            if (m == -INFINITY) l = seen ? NAN : 0.f;   // every score minus infinity, or nothing seen
-            sh.ml[st][row_l] = make_float2(mc, l);
+            {
+                // A part without a maximum counts for nothing beside others (its sum says what it is alone: NaN where every score is
+                // minus infinity, 0 where nothing is seen); one with a NaN among its scores makes the row NaN in any company.
+                float l = la.x + la.y;
+                const float mc = m > -INFINITY ? m * a.scale_log2 : l != l ? 0.f : -INFINITY;
+                if (mc == -INFINITY) l = seen ? NAN : 0.f;
+                sh.ml[st][lane_l] = make_float2(mc, l);
+            }
             base += 2 * n;
             tile_no += n;
-            steps[0] += RT == 2 ? n : (n + 1) >> 1;
-            steps[1] += RT == 2 ? n : n >> 1;
-            // this thread's columns [d0, d0 + width) of its row: RT = 1 adds the streams, each one's warps a half of the columns
-            const bool both = RT == 1 && n > 1;
-            if (mine > 0) ok = warp_wait(&sh.o_done[st], ((st ? steps[1] : steps[0]) - 1) & 1u);
-            group_sync();   // the other stream's maximum, sum and O, every tile's bad nodes
+            steps += mine;
+            if (mine > 0) ok = warp_wait(&sh.o_done[st], (steps - 1) & 1u);
+            all_sync();   // the other stream's maximum, sum and O, every tile's bad nodes
             if (!ok) break;
             tc_fence_after_sync();
+            // A row's parts: the copies, of both streams where they share the rows.  RT = 1: each stream's warps add a half of the columns.
             const unsigned long long bad = sh.bad_nodes;
-            float f0 = 1.f, f1 = 0.f;
-            if (RT == 1) {
-                const float2 a0 = sh.ml[0][row_l], a1 = both ? sh.ml[1][row_l] : make_float2(-INFINITY, 0.f);
-                mc = fmaxf(a0.x, a1.x);
-                f0 = a0.x == -INFINITY ? 0.f : exp2_approx(a0.x - mc);
-                f1 = a1.x == -INFINITY ? 0.f : exp2_approx(a1.x - mc);
-                l = mc == -INFINITY ? a0.y + a1.y : (a0.x == -INFINITY ? 0.f : a0.y * f0) + (a1.x == -INFINITY ? 0.f : a1.y * f1);
-            }
-            const bool complete = n == w.seq.tiles;
-            if (busy || RT == 1) {
-                constexpr int kWidth = RT == 1 ? 64 : 128;
-                const int d0 = RT == 1 ? 64 * st : 0;
-                const float inv = 1.f / l;
-                const int64_t slot = (int64_t)blockIdx.x * 2 + (stretch > 0);
-                const int part_row = RT == 2 ? st * kTile + row_l : row_l;
-                __nv_bfloat16* out = a.out + (((int64_t)w.r * a.nodes + row / a.group) * a.hq + kvh * a.group + row % a.group) * kHeadDim;
-                float* part = a.part + (slot * a.tile_rows + part_row) * kHeadDim;
+            const bool both = RT == 1 && n > 1, complete = n == w.seq.tiles;
+            auto joint = [&](int rr) {   // maximum and sum over the parts of row rr
+                float mc = -INFINITY, l = 0.f;
+#pragma unroll
+                for (int k = 0; k < REP; ++k) {
+                    mc = fmaxf(mc, sh.ml[RT == 2 ? st : 0][rr + k * kSpan].x);
+                    if (both) mc = fmaxf(mc, sh.ml[1][rr + k * kSpan].x);
+                }
+#pragma unroll
+                for (int k = 0; k < REP; ++k) {
+                    const float2 a0 = sh.ml[RT == 2 ? st : 0][rr + k * kSpan], a1 = both ? sh.ml[1][rr + k * kSpan] : make_float2(-INFINITY, 0.f);
+                    if (mc == -INFINITY) l += a0.y + a1.y;
+                    else l += (a0.x == -INFINITY ? 0.f : a0.y * exp2_approx(a0.x - mc)) + (a1.x == -INFINITY ? 0.f : a1.y * exp2_approx(a1.x - mc));
+                }
+                return make_float2(mc, l);
+            };
+            const float2 sum = joint(row_l);
+            auto factor = [&](int s) {
+                const float x = sh.ml[s][lane_l].x;
+                return x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
+            };
+            const float f0 = factor(RT == 2 ? st : 0), f1 = both ? factor(1) : 0.f;
+            const int64_t slot = ((int64_t)blockIdx.x * 2 + (stretch > 0)) * a.tile_rows + (RT == 2 ? st * kTile : 0);
+            constexpr int kWidth = RT == 1 ? 64 : 128;
+            const int d0 = RT == 1 ? 64 * st : 0;
+            const int rows_here = min(kSpan, m_rows - tile0);   // may be 0 or less (RT = 2)
+            // 32 columns at a time through 4 KB of the Q tiles' place a warp: a thread has a row of tensor memory, the copies have to be added, and a
+            // store instruction wants neighbouring columns (a row a thread takes a line of the L1 cache per thread and instruction).
+            unsigned char* stage = q_tiles + st * kTileBytes / 2;
+            auto place = [&](int ll, int c) { return reinterpret_cast<float4*>(stage + ll * 128 + ((c ^ (ll & 7)) << 4)); };
+#pragma unroll 1
+            for (int c = 0; c < kWidth; c += 32) {
                 if (busy) {
+                    uint32_t o[32];
+                    if (RT == 1) {
+                        uint32_t q[32];
+                        tmem_ld32(lanes + kColO + d0 + c, o);
+                        if (both) tmem_ld32(lanes + kColO + kHeadDim + d0 + c, q);
+                        tmem_wait_ld(o, q);
 #pragma unroll
-                    for (int c = 0; c < kWidth; c += 32) {
-                        uint32_t o[32];
-                        if (RT == 1) {
-                            uint32_t q[32];
-                            tmem_ld32(lanes + kColO + d0 + c, o);
-                            if (both) tmem_ld32(lanes + kColO + kHeadDim + d0 + c, q);
-                            tmem_wait_ld(o, q);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                float v = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
-                                if (both && f1 != 0.f) v += __uint_as_float(q[e]) * f1;
-                                o[e] = __float_as_uint(v);
-                            }
-                        } else {
-                            tmem_ld32(col_o + c, o);
-                            tmem_wait_ld(o);
+                        for (int e = 0; e < 32; ++e) {
+                            float v = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
+                            if (both && f1 != 0.f) v += __uint_as_float(q[e]) * f1;
+                            o[e] = __float_as_uint(v);
                         }
-                        if (live && complete) {
+                    } else {
+                        tmem_ld32(col_o + c, o);
+                        tmem_wait_ld(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint32_t p[4];
+                        for (int e = 0; e < 32; ++e) o[e] = f0 == 0.f ? 0u : o[e];
+                    }
 #pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                    const float y = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u]) * inv, z = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * u + 1]) * inv;
-                                    p[u] = pack_bf16(y, z);
-                                }
-                                *reinterpret_cast<uint4*>(out + d0 + c + e) = make_uint4(p[0], p[1], p[2], p[3]);
-                            }
-                        } else if (live) {
+                    for (int e = 0; e < 32; e += 4)
+                        *place(lane_l, e >> 2) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                }
+                group_sync();
+                if (!ok) break;
+                for (int idx = lane_l; idx < rows_here * 8; idx += 128) {   // rows x 16-byte pieces
+                    const int rr = idx >> 3, at = tile0 + rr;
+                    float4 v = *place(rr, idx & 7);
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + d0 + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                        }
-                        __syncwarp();
+                    for (int k = 1; k < REP; ++k) {
+                        const float4 u = *place(rr + k * kSpan, idx & 7);
+                        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+                    }
+                    if (complete) {
+                        const float l = joint(rr).y, inv = 1.f / l;
+                        if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        else v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                        const int node = at / a.group, h = kvh * a.group + at - node * a.group;
+                        reinterpret_cast<uint2*>(a.out + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim + d0 + c)[idx & 7] =
+                            make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                    } else {
+                        reinterpret_cast<float4*>(a.part + (slot + rr) * kHeadDim + d0 + c)[idx & 7] = v;
                     }
                 }
-                if (live) {
-                    if (!complete && (RT == 2 || !st)) a.part_ml[slot * a.tile_rows + part_row] = make_float2(mc, l);
-                    if (bad) {
-                        if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, out, d0, d0 + kWidth);
-                        else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, mc, part, d0, d0 + kWidth);
-                    }
+                group_sync();
+                if (!ok) break;
+            }
+            if (!ok) break;
+            if (live && copy == 0) {
+                if (!complete && (RT == 2 || !st)) a.part_ml[slot + row_l] = sum;
+                if (bad) {   // other threads' stores of this row are visible: group_sync
+                    if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + (((int64_t)w.r * a.nodes + row / a.group) * a.hq + kvh * a.group + row % a.group) * kHeadDim, d0, d0 + kWidth);
+                    else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim, d0, d0 + kWidth);
                 }
             }
-            __syncwarp();
             tc_fence_before_sync();
-            group_sync();   // sums and bad nodes have been read
+            all_sync();   // sums and bad nodes have been read
             if (tid == 128) sh.bad_nodes = 0;
         }
         if (!ok) sh.failed = 1;
@@ -695,8 +798,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     if (local >= a.kv_heads * m_rows) return;
     const int kvh = local / m_rows, row = local % m_rows, span = m_rows > kTile ? 2 * kTile : kTile, rt = row / span, row_l = row % span;
     const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
-    const int tiles = tree_seq(a, r).tiles;
-    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * tiles, c0 = s0 / quota, c1 = (s0 + tiles - 1) / quota;
+    const TreeSeq seq = tree_seq(a, r);
+    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units(), c0 = (s0 + kTreeStart) / quota, c1 = (s0 + seq.units() - 1) / quota;
     if (c0 == c1) return;
     auto slot = [&](int64_t c) { return (c * 2 + (s0 > c * quota ? 1 : 0)) * a.tile_rows + row_l; };
     float m = -INFINITY;
@@ -790,12 +893,14 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.scale_log2 = scale * 1.4426950408889634f;
     a.error = device_status_word(device);
     const CUtensorMap kmap = page_map(a.k, c), vmap = page_map(a.v, c);
+    const int m_rows = nodes * a.group;
+    auto* kernel = rt == 2 ? tree_attn_kernel<2, 1> : m_rows > 64 ? tree_attn_kernel<1, 1> : m_rows > 32 ? tree_attn_kernel<1, 2> : tree_attn_kernel<1, 4>;
     static std::once_flag once[64];
     std::call_once(once[device], [] {
-        MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem));
-        MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem));
+        for (auto* k : {tree_attn_kernel<2, 1>, tree_attn_kernel<1, 1>, tree_attn_kernel<1, 2>, tree_attn_kernel<1, 4>})
+            MFQB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem));
     });
-    launch_chained(rt == 2 ? tree_attn_kernel<2> : tree_attn_kernel<1>, dim3(kTreeCtas), dim3(kTreeThreads), kTreeSmem, s, a, kmap, vmap);
+    launch_chained(kernel, dim3(kTreeCtas), dim3(kTreeThreads), kTreeSmem, s, a, kmap, vmap);
     const int per_seq = (c.kv_heads * nodes * a.group + 7) / 8;
     launch_chained(tree_merge_kernel, dim3((unsigned)(c.rows * per_seq)), dim3(256), 0, s, a, (int)kTreeCtas, per_seq);
 }
