@@ -213,6 +213,12 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {   // one arrival fo
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// Both of two barriers; the polls of barriers that are complete (the usual case of one of them) overlap.
+__device__ __forceinline__ bool warp_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+    const bool da = mbar_test(a, pa), db = mbar_test(b, pb);
+    if (__all_sync(0xffffffffu, da && db)) return true;
+    return warp_wait(a, pa) && warp_wait(b, pb);
+}
 
 // Position in the ring's sequence of the key and value tiles of a stretch of n tiles, which is the order of their use.  RT = 1: K0 K1 V0
 // K2 V1 .. K(n-1) V(n-2) V(n-1); RT = 2: K0 V0 K1 V1 ..
@@ -434,13 +440,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         const uint32_t q_addr = smem_u32(q_tiles), ring_addr = smem_u32(ring);
         uint32_t base = 0, stretch = 0, steps[2] = {0, 0};   // ring position of the stretch, its number, steps of each stream before it
         bool ok = true;
+        // What the products' operands are made of is made warp-uniform by the shuffles: an instruction takes some 60 clocks then, its time on the
+        // tensor core, and 120 otherwise.
         auto scores = [&](int u) {
             const int i = RT == 2 ? u >> 1 : u, st = u & 1;
             const uint32_t at = base + key_at<RT>(i), stage = at % kRing;
-            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u) && (u < 2 || warp_wait(&sh.o_done[st], ((st ? steps[1] : steps[0]) + (u >> 1) - 1) & 1u));
+            ok = u < 2 ? warp_wait(&sh.kv_full[stage], (at / kRing) & 1u)
+                       : warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.o_done[st], ((st ? steps[1] : steps[0]) + (u >> 1) - 1) & 1u);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint32_t k_addr = ring_addr + stage * kTileBytes, q = q_addr + (RT == 2 ? st * kTileBytes : 0), d = tmem + kColS + st * kTile;
+            const uint32_t k_addr = __shfl_sync(0xffffffffu, ring_addr + stage * kTileBytes, 0), q = __shfl_sync(0xffffffffu, q_addr + (RT == 2 ? st * kTileBytes : 0), 0);
+            const uint32_t d = __shfl_sync(0xffffffffu, tmem + kColS + st * kTile, 0);
             if (elect_one()) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
@@ -453,15 +463,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         auto values = [&](int u, int n) {
             const int i = RT == 2 ? u >> 1 : u, st = u & 1;
             const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
-            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u) && warp_wait(&sh.p_full[st], ((st ? steps[1] : steps[0]) + (u >> 1)) & 1u);
+            ok = warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.p_full[st], ((st ? steps[1] : steps[0]) + (u >> 1)) & 1u);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint32_t v_addr = ring_addr + stage * kTileBytes, p = tmem + kColS + st * kTile, d = tmem + kColO + st * kHeadDim;
-            const int groups = min(8, (w.seq.end - (w.t0 + i) * kTile + 15) >> 4);   // of 16 positions; behind the end nothing is there to be multiplied
+            const uint32_t v_addr = __shfl_sync(0xffffffffu, ring_addr + stage * kTileBytes, 0), p = __shfl_sync(0xffffffffu, tmem + kColS + st * kTile, 0);
+            const uint32_t d = __shfl_sync(0xffffffffu, tmem + kColO + st * kHeadDim, 0);
+            const bool more = __shfl_sync(0xffffffffu, u > 1, 0);   // there is an O to add to
+            const int groups = __shfl_sync(0xffffffffu, min(8, (w.seq.end - (w.t0 + i) * kTile + 15) >> 4), 0);   // of 16 positions; nothing is behind the end
             if (elect_one()) {
+                if (groups == 8) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (s < groups) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, u > 1 || s > 0);
+                    for (int s = 0; s < 8; ++s) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, s > 0 || more);
+                } else {
+#pragma unroll 1
+                    for (int s = 0; s < groups; ++s) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, s > 0 || more);
+                }
                 tc_commit(&sh.o_done[st]);
                 if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
             }
