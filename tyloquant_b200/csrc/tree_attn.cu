@@ -43,7 +43,14 @@ struct TreeArgs {
     float2* part_ml;
     int* error;
     int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of RT * 128 rows; tile_rows: rows of a part, at most that
+    unsigned group_inv;           // ceil(65536 / group): row / group = row * group_inv >> 16 for rows below 1024, groups up to 16
     float scale_log2;
+    __device__ __forceinline__ int node_of(int row_of_q) const { return (int)((unsigned)row_of_q * group_inv >> 16); }
+    // element offset of a row of Q (or of the output) of sequence r and kv head kvh
+    __device__ __forceinline__ int64_t row_at(int r, int kvh, int row_of_q) const {
+        const int node = node_of(row_of_q);
+        return (((int64_t)r * nodes + node) * hq + kvh * group + row_of_q - node * group) * kHeadDim;
+    }
 };
 
 // Tiles of sequence r (at least one: a sequence has a node), its length and end.
@@ -295,13 +302,12 @@ __device__ __noinline__ void clean_values(TreeShared& sh, unsigned char* tile, T
 // the node keep clear of them); here they are added to the row's result, where the row sees them.
 template <typename T>
 __device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long bad, const TreeSeq& seq, int r, int kvh, int row, float mc, T* dst, int d0, int d1) {
-    const int node = row / a.group, h = kvh * a.group + row % a.group;
-    bad &= a.masks[(int64_t)r * a.nodes + node];
+    const __nv_bfloat16* q = a.q + a.row_at(r, kvh, row);
+    bad &= a.masks[(int64_t)r * a.nodes + a.node_of(row)];
     for (; bad; bad &= bad - 1) {
         const int t = seq.len + (__ffsll((long long)bad) - 1);
         const int page = a.table[(int64_t)r * a.width + t / a.page];
         const int64_t at = (((int64_t)page * a.kv_heads + kvh) * a.page + (t & (a.page - 1))) * kHeadDim;
-        const __nv_bfloat16* q = a.q + (((int64_t)r * a.nodes + node) * a.hq + h) * kHeadDim;
         float s = 0.f;
         for (int d = 0; d < kHeadDim; ++d) s += __bfloat162float(q[d]) * __bfloat162float(a.k[at + d]);
         const float p = exp2_approx(s * a.scale_log2 - mc);
@@ -531,8 +537,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 uint4 v[kLoads / REP];
 #pragma unroll
                 for (int j = 0; j < kLoads / REP; ++j) {
-                    const int qr = min(tile0 + r0 + kStep * j, m_rows - 1), node = qr / a.group, h = kvh * a.group + qr - node * a.group;
-                    v[j] = __ldg(reinterpret_cast<const uint4*>(a.q + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim) + c);
+                    v[j] = __ldg(reinterpret_cast<const uint4*>(a.q + a.row_at(w.r, kvh, min(tile0 + r0 + kStep * j, m_rows - 1))) + c);
                 }
 #pragma unroll
                 for (int j = 0; j < kLoads; ++j) {
@@ -542,7 +547,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&sh.q_full);
-            unsigned long long mask = live ? a.masks[(int64_t)w.r * a.nodes + row / a.group] : 0ull;
+            unsigned long long mask = live ? a.masks[(int64_t)w.r * a.nodes + a.node_of(row)] : 0ull;
             if (a.nodes < 64) mask &= (1ull << a.nodes) - 1ull;
             float m = -INFINITY;   // maximum of the scores so far (or less, see above)
             uint64_t l2[2] = {0ull, 0ull};   // the sum, in four parts
@@ -556,33 +561,38 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 const unsigned good = sh.good[(tile_no + i) & 7];
                 const int pos0 = (w.t0 + i) * kTile;
                 const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
+                int chunks = kTile / 16;      // of 16 positions that are there
+                float known = -INFINITY;      // maximum of this thread's scores of a tile that is not whole
                 if (!whole) {
                     const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
                     ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
                     if (!ok) break;
                     clean_values(sh, ring + (size_t)stage * kTileBytes, w.seq, pos0, good, quarter, lane);
+                    chunks = min(chunks, (w.seq.end - pos0 + 15) >> 4);
                     // what this row does not see of its copy's positions becomes minus infinity
-                    unsigned any = 0;
 #pragma unroll 1
-                    for (int c = 0; c < kCols; c += 32) {
+                    for (int c = 0; c < kCols && copy * kCols + c < 16 * chunks; c += 32) {
                         const int p0 = copy * kCols + c, ctx = w.seq.len - (pos0 + p0);   // positions from here on that are before the length
                         unsigned vis = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
                         if (ctx <= 0 && ctx > -64) vis |= (unsigned)(mask >> -ctx);
                         else if (ctx > 0 && ctx < 32) vis |= (unsigned)(mask << ctx);
                         vis &= ((good >> (p0 >> 4)) & 1u ? 0x0000FFFFu : 0u) | ((good >> ((p0 >> 4) + 1)) & 1u ? 0xFFFF0000u : 0u);
-                        any |= vis;
-                        if (busy && __any_sync(0xffffffffu, vis != 0xFFFFFFFFu)) {
+                        seen |= vis != 0;
+                        if (busy) {
                             uint32_t s[32];
                             tmem_ld32(col_s + p0, s);
                             tmem_wait_ld(s);
+                            float t[2] = {known, known};
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
+                            for (int e = 0; e < 32; ++e) {
                                 if (!((vis >> e) & 1u)) s[e] = 0xFF800000u;
-                            tmem_st32(col_s + p0, s);
+                                t[e & 1] = fmaxf(t[e & 1], __uint_as_float(s[e]));
+                            }
+                            known = fmaxf(t[0], t[1]);
+                            if (__any_sync(0xffffffffu, vis != 0xFFFFFFFFu)) tmem_st32(col_s + p0, s);
                         }
                     }
                     tmem_wait_st();
-                    seen |= any != 0;
                 } else {
                     seen = true;
                 }
@@ -612,6 +622,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                         for (int c = 0; c < kCols; c += 32) tmem_ld32(col_s + copy * kCols + c, s + c);
 #pragma unroll
                         for (int c = 0; c < kCols; c += 32) tmem_wait_ld(s + c);
+                        if (!whole) {   // what lies behind the last chunk has not been hidden
+#pragma unroll
+                            for (int c = 0; c < kCols; c += 32)
+                                if (copy * kCols + c >= 16 * chunks)
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e) s[c + e] = 0xFF800000u;
+                        }
                         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int e = 0; e < kCols; e += 2) top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
@@ -635,7 +652,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                         // The exponentials are formed with the maximum as it was, the tile's own is found beside them; only where it has grown
                         // too far they are formed again.  P waits in registers meanwhile, S in tensor memory.
                         uint32_t p[64];
-                        if (x == 0) {   // there is no maximum yet
+                        if (!whole) {
+                            const bool raise = too_high(known);
+                            if (__any_sync(0xffffffffu, raise)) rescale(known, raise);
+                        } else if (x == 0) {   // there is no maximum yet
                             float top = -INFINITY;
 #pragma unroll 1
                             for (int c = 0; c < kTile; c += 32) {
@@ -658,9 +678,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                             tmem_ld16_async(col_s, s[0]);
 #pragma unroll
                             for (int c = 0; c < 8; ++c) {
+                                if (c >= chunks) break;   // the same for all
                                 uint32_t* now = s[c & 1];
                                 tmem_wait_ld16(now);
-                                if (c < 7) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
+                                if (c < 7 && c + 1 < chunks) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
                                 exp16<true>(now, scale2, mc2, sum, top, p + 8 * c);
                             }
                             const float high = fmaxf(top[0], top[1]);
@@ -716,73 +737,113 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 return make_float2(mc, l);
             };
             const float2 sum = joint(row_l);
+            // What a part's values are multiplied by: its own maximum against the joint one, the sum where the row is complete.
             auto factor = [&](int s) {
-                const float x = sh.ml[s][lane_l].x;
-                return x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
+                const float x = sh.ml[s][lane_l].x, f = x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
+                return complete ? (sum.y == 0.f ? 0.f : f / sum.y) : f;
             };
             const float f0 = factor(RT == 2 ? st : 0), f1 = both ? factor(1) : 0.f;
             const int64_t slot = ((int64_t)blockIdx.x * 2 + (stretch > 0)) * a.tile_rows + (RT == 2 ? st * kTile : 0);
             constexpr int kWidth = RT == 1 ? 64 : 128;
             const int d0 = RT == 1 ? 64 * st : 0;
             const int rows_here = min(kSpan, m_rows - tile0);   // may be 0 or less (RT = 2)
-            // 32 columns at a time through 4 KB of the Q tiles' place a warp: a thread has a row of tensor memory, the copies have to be added, and a
-            // store instruction wants neighbouring columns (a row a thread takes a line of the L1 cache per thread and instruction).
-            unsigned char* stage = q_tiles + st * kTileBytes / 2;
-            auto place = [&](int ll, int c) { return reinterpret_cast<float4*>(stage + ll * 128 + ((c ^ (ll & 7)) << 4)); };
-#pragma unroll 1
-            for (int c = 0; c < kWidth; c += 32) {
+            // 32 columns of this thread's row, its streams added; zero where a part saw nothing (its O may be NaN then)
+            auto take = [&](int c, uint32_t* o) {
+                if (RT == 1) {
+                    uint32_t q[32];
+                    tmem_ld32(lanes + kColO + d0 + c, o);
+                    if (both) tmem_ld32(lanes + kColO + kHeadDim + d0 + c, q);
+                    tmem_wait_ld(o, q);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float v = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
+                        if (both && f1 != 0.f) v = fmaf(__uint_as_float(q[e]), f1, v);
+                        o[e] = __float_as_uint(v);
+                    }
+                } else {
+                    tmem_ld32(col_o + c, o);
+                    tmem_wait_ld(o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = f0 == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f0);
+                }
+            };
+            // Rows leave through the Q tiles' place: a thread has a row of tensor memory, and a store instruction wants neighbouring columns (a row a
+            // thread takes a line of the L1 cache per thread and instruction).
+            if constexpr (REP == 1) {   // 4 KB a warp: its 32 rows, 64 columns of bf16 or 32 of float32
+                unsigned char* stage = q_tiles + (warp - 4) * 4096;
+                auto place = [&](int rr, int c) { return reinterpret_cast<uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4)); };
                 if (busy) {
-                    uint32_t o[32];
-                    if (RT == 1) {
-                        uint32_t q[32];
-                        tmem_ld32(lanes + kColO + d0 + c, o);
-                        if (both) tmem_ld32(lanes + kColO + kHeadDim + d0 + c, q);
-                        tmem_wait_ld(o, q);
+#pragma unroll 1
+                    for (int c = 0; c < kWidth; c += 32) {
+                        uint32_t o[32];
+                        take(c, o);
+                        if (complete) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float v = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
-                            if (both && f1 != 0.f) v += __uint_as_float(q[e]) * f1;
-                            o[e] = __float_as_uint(v);
+                            for (int e = 0; e < 32; e += 8)
+                                *place(lane, ((c & 32) + e) >> 3) =
+                                    make_uint4(pack_bf16(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), pack_bf16(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
+                                               pack_bf16(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])), pack_bf16(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+                            if (!(c & 32)) continue;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) *place(lane, e >> 2) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                         }
-                    } else {
-                        tmem_ld32(col_o + c, o);
-                        tmem_wait_ld(o);
+                        __syncwarp();
+                        uint4 v[8];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = f0 == 0.f ? 0u : o[e];
+                        for (int k = 0; k < 8; ++k) v[k] = *place(4 * k + (lane >> 3), lane & 7);   // four rows of 128 bytes at a time
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int rr = quarter * 32 + 4 * k + (lane >> 3);
+                            if (rr >= rows_here) continue;
+                            if (complete) reinterpret_cast<uint4*>(a.out + a.row_at(w.r, kvh, tile0 + rr) + d0 + (c & ~63))[lane & 7] = v[k];
+                            else reinterpret_cast<uint4*>(a.part + (slot + rr) * kHeadDim + d0 + c)[lane & 7] = v[k];
+                        }
+                        __syncwarp();
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *place(lane_l, e >> 2) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
                 }
-                group_sync();
+            } else {   // 16 KB a stream: the copies of a row are added; up to 16 rows (REP = 4) all 64 columns at once, else 32
+                unsigned char* stage = q_tiles + st * (kTileBytes / 2);
+                const int wide = rows_here * REP <= 64 ? 64 : 32, pieces = wide / 4, shift = wide == 64 ? 4 : 3;
+                auto place = [&](int rr, int cp, int c) { return reinterpret_cast<float4*>(stage + ((cp * rows_here + rr) * pieces + (c ^ (rr & 7))) * 16); };
+#pragma unroll 1
+                for (int c0 = 0; c0 < kWidth; c0 += wide) {
+                    if (c0) group_sync();   // the columns before have been read
+                    if (!ok) break;
+                    if (busy) {
+#pragma unroll 1
+                        for (int c = 0; c < wide; c += 32) {
+                            uint32_t o[32];
+                            take(c0 + c, o);
+                            if (live)
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4)
+                                    *place(row_l, copy, (c + e) >> 2) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                            __syncwarp();
+                        }
+                    }
+                    group_sync();
+                    if (!ok) break;
+                    for (int idx = lane_l; idx < rows_here << shift; idx += 128) {
+                        const int rr = idx >> shift, c = idx & (pieces - 1);
+                        float4 v = *place(rr, 0, c);
+#pragma unroll
+                        for (int k = 1; k < REP; ++k) {
+                            const float4 u = *place(rr, k, c);
+                            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+                        }
+                        if (complete) reinterpret_cast<uint2*>(a.out + a.row_at(w.r, kvh, tile0 + rr) + d0 + c0)[c] = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                        else reinterpret_cast<float4*>(a.part + (slot + rr) * kHeadDim + d0 + c0)[c] = v;
+                    }
+                }
                 if (!ok) break;
-                for (int idx = lane_l; idx < rows_here * 8; idx += 128) {   // rows x 16-byte pieces
-                    const int rr = idx >> 3, at = tile0 + rr;
-                    float4 v = *place(rr, idx & 7);
-#pragma unroll
-                    for (int k = 1; k < REP; ++k) {
-                        const float4 u = *place(rr + k * kSpan, idx & 7);
-                        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-                    }
-                    if (complete) {
-                        const float l = joint(rr).y, inv = 1.f / l;
-                        if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        else v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                        const int node = at / a.group, h = kvh * a.group + at - node * a.group;
-                        reinterpret_cast<uint2*>(a.out + (((int64_t)w.r * a.nodes + node) * a.hq + h) * kHeadDim + d0 + c)[idx & 7] =
-                            make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-                    } else {
-                        reinterpret_cast<float4*>(a.part + (slot + rr) * kHeadDim + d0 + c)[idx & 7] = v;
-                    }
-                }
-                group_sync();
+                if (bad) group_sync();   // the rows' stores, before add_bad_nodes
                 if (!ok) break;
             }
-            if (!ok) break;
             if (live && copy == 0) {
                 if (!complete && (RT == 2 || !st)) a.part_ml[slot + row_l] = sum;
-                if (bad) {   // other threads' stores of this row are visible: group_sync
-                    if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + (((int64_t)w.r * a.nodes + row / a.group) * a.hq + kvh * a.group + row % a.group) * kHeadDim, d0, d0 + kWidth);
+                if (bad) {
+                    if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + a.row_at(w.r, kvh, row), d0, d0 + kWidth);
                     else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim, d0, d0 + kWidth);
                 }
             }
@@ -804,7 +865,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
 
 // Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context.
 __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int ctas, int per_seq) {
-    chained_wait();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ int64_t red[8][2];
     const int r = blockIdx.x / per_seq, lane = threadIdx.x & 31;
     const int local = (blockIdx.x % per_seq) * 8 + (threadIdx.x >> 5);   // kv head, row of Q
@@ -901,6 +963,7 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.hq = q_heads;
     a.group = q_heads / c.kv_heads;
     a.nodes = nodes;
+    a.group_inv = (65536u + a.group - 1) / a.group;
     const int rt = nodes * a.group > kTile ? 2 : 1;   // see tree_attn_kernel
     a.row_tiles = (nodes * a.group + rt * kTile - 1) / (rt * kTile);
     a.tile_rows = tree_rows(c, q_heads, nodes);
