@@ -3,15 +3,15 @@
 // Per sequence and kv head the queries of all nodes and of the heads that share the kv head are the rows of one matrix Q (row
 // node * G + head): S = Q K^T, P = exp2(scale' S - m), O = P V over tiles of 128 positions, with a running maximum m and sum l per row.
 // The work is cut into units (sequence, kv head, tile of 128 rows, tile of 128 positions), which are shared out evenly and in
-// order over the CTAs, one per SM, from the lengths as they are on the device: a batch of very different lengths loads
+// order over the CTAs, which fill the SMs, from the lengths as they are on the device: a batch of very different lengths loads
 // the SMs alike, and a captured call follows the lengths of each replay.  A stretch of units of one (sequence, head, row tile) that
 // covers all its positions is written as it is; otherwise the CTA leaves O, m and l, and tree_merge_kernel adds the parts in the order of
 // the context (no atomics: a call repeats bit for bit).
 //
-// Roles in a CTA of eight warps: one asks for pages (bulk tensor copies into a ring of six 32 KB tiles, keys and values in the
-// order of their use, with the 128-byte swizzle), one issues tcgen05.mma, four do the softmax (a row a thread): S comes out of tensor
-// memory, P goes back into it as the A operand of the second product, O stays there.  O is multiplied by a correction
-// only when a row's maximum has grown by more than 2^8 (P then stays below 2^8, which bf16 holds as exactly as values below 1).
+// Roles in a CTA: one warp asks for pages (bulk tensor copies into a ring of 32 KB tiles, keys and values in the order of their use, with
+// the 128-byte swizzle), one issues tcgen05.mma, four (or eight) do the softmax, a row a thread: S comes out of tensor memory, P goes back
+// into it as the A operand of the second product, O stays there.  O is multiplied by a correction only when a row's maximum has
+// grown by more than 2^8 (P then stays below 2^8, which bf16 holds as exactly as values below 1).
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -24,13 +24,13 @@ namespace mfqb {
 
 int* device_status_word(int device);
 
-constexpr int kTreeCtas = 148;                       // one per SM
+constexpr int kTreeSms = 148;
 constexpr int kTile = 128;                           // rows of Q, positions of a tile
 constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
-constexpr int kTreeTiles = 7, kTreeRingMax = kTreeTiles - 1;   // 32 KB tiles in shared memory: Q once or twice, the others are the ring
-constexpr int kSoftmaxWarps = 8, kTreeThreads = 128 + 32 * kSoftmaxWarps;
+constexpr int tree_ctas(int ns) { return ns == 2 ? kTreeSms : 2 * kTreeSms; }
+constexpr int tree_ring(int ns) { return ns == 2 ? 5 : 2; }   // tiles
+constexpr int tree_threads(int ns) { return 64 + 128 * ns; }
 constexpr int kTreeStart = 2;                         // what starting and ending a stretch takes, in tiles
-constexpr uint32_t kColS = 0, kColO = 256;   // tensor memory columns: S of the two streams (P takes the place of its first half), O of the two
 
 struct TreeArgs {
     const int* table;
@@ -41,8 +41,9 @@ struct TreeArgs {
     __nv_bfloat16* out;
     float* part;                  // [CTA][first, last][rows of a tile][128], then their (maximum, sum)
     float2* part_ml;
+    int64_t* before;              // [rows + 1]: units of one item of each sequence before a sequence; their sum
     int* error;
-    int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of RT * 128 rows; tile_rows: rows of a part, at most that
+    int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of 128 rows a stream; tile_rows: rows of a part, at most that
     unsigned group_inv;           // ceil(65536 / group): row / group = row * group_inv >> 16 for rows below 1024, groups up to 16
     float scale_log2;
     __device__ __forceinline__ int node_of(int row_of_q) const { return (int)((unsigned)row_of_q * group_inv >> 16); }
@@ -66,39 +67,20 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
     s.tiles = (s.end + kTile - 1) / kTile;
     return s;
 }
-// Sum of units of the rows before `row` and of all rows, for one item of each; 256 threads.
-__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int row, int64_t& before, int64_t& total, int64_t (*red)[2]) {
-    int64_t b = 0, t = 0;
-    for (int r = threadIdx.x; r < a.rows; r += 256) {
-        const int n = tree_seq(a, r).units();
-        t += n;
-        if (r < row) b += n;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-        t += __shfl_xor_sync(0xffffffffu, t, o);
-    }
-    if ((threadIdx.x & 31) == 0) { red[threadIdx.x >> 5][0] = b; red[threadIdx.x >> 5][1] = t; }
-    __syncthreads();
-    before = total = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) { before += red[w][0]; total += red[w][1]; }
-}
-
 struct TreeShared {
-    uint64_t kv_full[kTreeRingMax], kv_empty[kTreeRingMax], q_full, s_full[2], p_full[2], o_done[2], drain, all, group[2];
+    uint64_t kv_full[5], kv_empty[5], q_full, s_full[2], p_full[2], o_done[2], drain, all, group[2];
     unsigned long long bad_nodes;   // nodes of the stretch whose values hold an infinity or NaN
-    int64_t scan[12];
+    int64_t scan[10];
     int64_t first, last, item_off;  // the CTA's units; offset of its first one in its sequence's
     int row0;
     uint32_t tmem;
     unsigned good[8];               // per tile (index mod 8): bit g = the 16 positions of group g have a page
     int failed;
-    float2 ml[2][kTile];            // the two streams' (maximum in powers of two, sum)
+    float2 ml[2][kTile];            // the streams' (maximum in powers of two, sum)
 };
 
-constexpr size_t kTreeSmem = (size_t)kTreeTiles * kTileBytes + sizeof(TreeShared);
-static_assert(kTreeSmem <= 227 * 1024, "one CTA's shared memory");
+constexpr size_t tree_smem(int ns) { return (size_t)(tree_ring(ns) + ns) * kTileBytes + sizeof(TreeShared); }   // ring, Q of every stream
+static_assert(tree_smem(2) <= 227 * 1024 && 2 * (tree_smem(1) + 1024) <= 228 * 1024, "shared memory of an SM");
 
 // A CTA's stretches in order: sequence, item (kv head, row tile), tiles [t0, t1) of seq.tiles.
 struct TreeWalk {
@@ -227,13 +209,6 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* a, uint32_t pa, uint64_t* b
     return warp_wait(a, pa) && warp_wait(b, pb);
 }
 
-// Position in the ring's sequence of the key and value tiles of a stretch of n tiles, which is the order of their use.  RT = 1: K0 K1 V0
-// K2 V1 .. K(n-1) V(n-2) V(n-1); RT = 2: K0 V0 K1 V1 ..
-template <int RT>
-__device__ __forceinline__ int key_at(int i) { return RT == 2 ? 2 * i : i + max(0, i - 1); }
-template <int RT>
-__device__ __forceinline__ int value_at(int i, int n) { return RT == 2 ? 2 * i + 1 : i + min(n, i + 2); }
-
 __device__ __forceinline__ uint64_t pair_f32(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -301,7 +276,7 @@ __device__ __noinline__ void clean_values(TreeShared& sh, unsigned char* tile, T
 // Rare: values of visible nodes that hold an infinity or NaN were taken out of the product (0 in their place, so that rows which do not see
 // the node keep clear of them); here they are added to the row's result, where the row sees them.
 template <typename T>
-__device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long bad, const TreeSeq& seq, int r, int kvh, int row, float mc, T* dst, int d0, int d1) {
+__device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long bad, const TreeSeq& seq, int r, int kvh, int row, float mc, T* dst) {
     const __nv_bfloat16* q = a.q + a.row_at(r, kvh, row);
     bad &= a.masks[(int64_t)r * a.nodes + a.node_of(row)];
     for (; bad; bad &= bad - 1) {
@@ -311,48 +286,48 @@ __device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long
         float s = 0.f;
         for (int d = 0; d < kHeadDim; ++d) s += __bfloat162float(q[d]) * __bfloat162float(a.k[at + d]);
         const float p = exp2_approx(s * a.scale_log2 - mc);
-        for (int d = d0; d < d1; ++d) {
+        for (int d = 0; d < kHeadDim; ++d) {
             const float v = __bfloat162float(a.v[at + d]);
             if (!isfinite(v)) dst[d] = (T)((float)dst[d] + (p > 0.f ? v : NAN));
         }
     }
 }
 
-// Two streams of steps take turns on the tensor core, each with its own S, O and four softmax warps: while one stream's scores become
-// probabilities the other's products run.  RT = 1 (up to 128 rows): the streams take alternate tiles of positions and are added at the end
-// of a stretch.  RT = 2: each stream has 128 of 256 rows, both take every tile, which is read once for the two.  Step u of a stretch:
-// stream u & 1; its S waits for the product of step u - 2, whose P lies in S's place.  One warp issues for both: with a
-// warp each the streams fall into step, and the tensor core waits while both do softmax (16 sequences of one token at context 4096 73 us in
-// place of 57).
+// NS = 1 (up to 128 rows): a CTA has one tile of rows, and two CTAs share an SM: while one's scores become probabilities the other's
+// products run, and starts and ends of stretches overlap too (27 nodes of 13 sequences of up to 7000 tokens: 35 us with one CTA whose
+// two halves took alternate tiles of a stretch).  NS = 2: the CTA has the SM and two streams of 128 rows each, which take every
+// tile in turns, so that it is read once for 256 rows.  S of a step waits for the stream's last product, whose P lies in its place.
+// One warp issues for both streams: with a warp each they fall into step, and the tensor core waits while both do softmax.
 // REP: up to 32 (64) rows stand in Q four times (twice), and a copy's warps take a quarter (a half) of every tile's positions: their
 // P is zero elsewhere.  A row's 128 exponentials in one thread are what a tile waits for otherwise.
-template <int RT, int REP>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
-                                                                   const __grid_constant__ CUtensorMap vmap) {
-    constexpr int kRing = kTreeTiles - RT;
+template <int NS, int REP>
+__global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                                                     const __grid_constant__ CUtensorMap vmap) {
+    constexpr int kRing = tree_ring(NS);
+    constexpr uint32_t kColumns = 256 * NS, kColS = 0, kColO = kTile * NS;   // tensor memory: S of the streams (P takes the place of its first half), their O
     extern __shared__ __align__(1024) unsigned char ring[];   // the swizzle's pattern repeats every 1024 bytes
-    TreeShared& sh = *reinterpret_cast<TreeShared*>(ring + (size_t)kTreeTiles * kTileBytes);
+    TreeShared& sh = *reinterpret_cast<TreeShared*>(ring + (size_t)(kRing + NS) * kTileBytes);
     unsigned char* q_tiles = ring + (size_t)kRing * kTileBytes;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) { mbar_init(&sh.kv_full[i], 1); mbar_init(&sh.kv_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh.group[i], kSoftmaxWarps / 2); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], kSoftmaxWarps / 2); mbar_init(&sh.o_done[i], 1); }
-        mbar_init(&sh.q_full, kSoftmaxWarps);
-        mbar_init(&sh.all, kSoftmaxWarps);
+        for (int i = 0; i < NS; ++i) { mbar_init(&sh.group[i], 4); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_done[i], 1); }
+        mbar_init(&sh.q_full, 4 * NS);
+        mbar_init(&sh.all, 4 * NS);
         mbar_init(&sh.drain, 1);
         sh.bad_nodes = 0;
         sh.failed = 0;
         sh.first = sh.last = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc(&sh.tmem, 512u);
+    if (warp == 1) tmem_alloc(&sh.tmem, kColumns);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sh.tmem;
     chained_wait();
-    {   // this CTA's units: thread t holds the sequences 3t .. 3t + 2
-        constexpr int kEach = (kCacheRows + kTreeThreads - 1) / kTreeThreads;
+    {   // this CTA's units: thread t holds the sequences kEach * t ..
+        constexpr int kEach = (kCacheRows + tree_threads(NS) - 1) / tree_threads(NS);
         int units_of[kEach];
         int64_t mine = 0;
 #pragma unroll
@@ -369,7 +344,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         __syncthreads();
         int64_t total = 0;
 #pragma unroll
-        for (int w = 0; w < kTreeThreads / 32; ++w) {
+        for (int w = 0; w < tree_threads(NS) / 32; ++w) {
             if (w < warp) upto += sh.scan[w];
             total += sh.scan[w];
         }
@@ -378,6 +353,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         int64_t begin = (upto - mine) * items;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
+            if (blockIdx.x == 0 && kEach * tid + j < a.rows) a.before[kEach * tid + j] = begin / items;   // for tree_merge_kernel
             const int64_t end = begin + units_of[j] * items;
             if (first < last && begin <= first && first < end) {
                 sh.row0 = kEach * tid + j;
@@ -387,6 +363,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             }
             begin = end;
         }
+        if (blockIdx.x == 0 && tid == 0) a.before[a.rows] = total;
         __syncthreads();
     }
     TreeWalk w;
@@ -396,7 +373,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         const int box = min(a.page, kTile), boxes = kTile / box;
         uint32_t issued = 0, tile_no = 0;
         bool ok = true;
-        int pages[2] = {-1, -1};   // this lane's page of the last two tiles
         auto ask = [&](const CUtensorMap* map, int kvh, int pos, int page) {
             const uint32_t stage = issued % kRing;
             ok = warp_wait(&sh.kv_empty[stage], ((issued / kRing) & 1u) ^ 1u);
@@ -414,27 +390,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             ++issued;
         };
         auto position = [&](int i) { return (w.t0 + i) * kTile + lane * box; };   // of this lane's box
-        auto keys = [&](int kvh, int i) {
-            const int pos = position(i);
-            int page = -1;
-            if (lane < boxes && pos < w.seq.end) page = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
-            if ((unsigned)page >= (unsigned)a.pages) page = -1;
-            (i & 1 ? pages[1] : pages[0]) = page;
-            unsigned good = 0;   // groups of 16 positions with a page: box b covers groups b * box / 16 ..
-            const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
-            for (int g = 0; g < 8; ++g) good |= ((have >> (g * 16 / box)) & 1u) << g;
-            if (lane == 0) sh.good[tile_no & 7] = good;
-            ++tile_no;
-            ask(&kmap, kvh, pos, page);
-        };
-        auto values = [&](int kvh, int i) { ask(&vmap, kvh, position(i), i & 1 ? pages[1] : pages[0]); };
         for (; ok && w.left > 0; w.next(a)) {
             const int kvh = w.item / a.row_tiles, n = w.t1 - w.t0;
-            keys(kvh, 0);
             for (int i = 0; ok && i < n; ++i) {
-                if (RT == 1 && i + 1 < n) keys(kvh, i + 1);
-                if (ok) values(kvh, i);
-                if (RT == 2 && ok && i + 1 < n) keys(kvh, i + 1);
+                const int pos = position(i);
+                int page = -1;
+                if (lane < boxes && pos < w.seq.end) page = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
+                if ((unsigned)page >= (unsigned)a.pages) page = -1;
+                unsigned good = 0;   // groups of 16 positions with a page: box b covers groups b * box / 16 ..
+                const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+                for (int g = 0; g < 8; ++g) good |= ((have >> (g * 16 / box)) & 1u) << g;
+                if (lane == 0) sh.good[tile_no & 7] = good;
+                ++tile_no;
+                ask(&kmap, kvh, pos, page);
+                if (ok) ask(&vmap, kvh, pos, page);
             }
         }
         if (!ok) sh.failed = 1;
@@ -444,37 +413,37 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         // -------- products: the warp stays together, an elected lane issues --------
         constexpr uint32_t idesc_s = instr_desc_bf16(kTile, kTile, false), idesc_o = instr_desc_bf16(kTile, kHeadDim, true);
         const uint32_t q_addr = smem_u32(q_tiles), ring_addr = smem_u32(ring);
-        uint32_t base = 0, stretch = 0, steps[2] = {0, 0};   // ring position of the stretch, its number, steps of each stream before it
+        uint32_t base = 0, stretch = 0, steps = 0;   // ring position of the stretch, its number, tiles before it
         bool ok = true;
         // What the products' operands are made of is made warp-uniform by the shuffles: an instruction takes some 60 clocks then, its time on the
         // tensor core, and 120 otherwise.
         auto scores = [&](int u) {
-            const int i = RT == 2 ? u >> 1 : u, st = u & 1;
-            const uint32_t at = base + key_at<RT>(i), stage = at % kRing;
-            ok = u < 2 ? warp_wait(&sh.kv_full[stage], (at / kRing) & 1u)
-                       : warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.o_done[st], ((st ? steps[1] : steps[0]) + (u >> 1) - 1) & 1u);
+            const int i = u / NS, st = u % NS;
+            const uint32_t at = base + 2 * i, stage = at % kRing;
+            ok = u < NS ? warp_wait(&sh.kv_full[stage], (at / kRing) & 1u)
+                       : warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.o_done[st], (steps + i - 1) & 1u);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint32_t k_addr = __shfl_sync(0xffffffffu, ring_addr + stage * kTileBytes, 0), q = __shfl_sync(0xffffffffu, q_addr + (RT == 2 ? st * kTileBytes : 0), 0);
+            const uint32_t k_addr = __shfl_sync(0xffffffffu, ring_addr + stage * kTileBytes, 0), q = __shfl_sync(0xffffffffu, q_addr + st * kTileBytes, 0);
             const uint32_t d = __shfl_sync(0xffffffffu, tmem + kColS + st * kTile, 0);
             if (elect_one()) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
                     tc_mma_f16_ss(d, smem_desc_sw128(q + (s >> 2) * kHalfBytes + (s & 3) * 32), smem_desc_sw128(k_addr + (s >> 2) * kHalfBytes + (s & 3) * 32), idesc_s, s > 0);
                 tc_commit(&sh.s_full[st]);
-                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
+                if (st == NS - 1) tc_commit(&sh.kv_empty[stage]);
             }
             __syncwarp();
         };
-        auto values = [&](int u, int n) {
-            const int i = RT == 2 ? u >> 1 : u, st = u & 1;
-            const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
-            ok = warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.p_full[st], ((st ? steps[1] : steps[0]) + (u >> 1)) & 1u);
+        auto values = [&](int u) {
+            const int i = u / NS, st = u % NS;
+            const uint32_t at = base + 2 * i + 1, stage = at % kRing;
+            ok = warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.p_full[st], (steps + i) & 1u);
             if (!ok) return;
             tc_fence_after_sync();
             const uint32_t v_addr = __shfl_sync(0xffffffffu, ring_addr + stage * kTileBytes, 0), p = __shfl_sync(0xffffffffu, tmem + kColS + st * kTile, 0);
             const uint32_t d = __shfl_sync(0xffffffffu, tmem + kColO + st * kHeadDim, 0);
-            const bool more = __shfl_sync(0xffffffffu, u > 1, 0);   // there is an O to add to
+            const bool more = __shfl_sync(0xffffffffu, i > 0, 0);   // there is an O to add to
             const int groups = __shfl_sync(0xffffffffu, min(8, (w.seq.end - (w.t0 + i) * kTile + 15) >> 4), 0);   // of 16 positions; nothing is behind the end
             if (elect_one()) {
                 if (groups == 8) {
@@ -485,37 +454,35 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                     for (int s = 0; s < groups; ++s) tc_mma_f16_ts(d, p + s * 8, smem_desc_sw128_mn(v_addr + s * 2048), idesc_o, s > 0 || more);
                 }
                 tc_commit(&sh.o_done[st]);
-                if (RT == 1 || st) tc_commit(&sh.kv_empty[stage]);
+                if (st == NS - 1) tc_commit(&sh.kv_empty[stage]);
             }
             __syncwarp();
         };
         for (; ok && w.left > 0; w.next(a)) {
-            const int n = w.t1 - w.t0, total = RT * n;
+            const int n = w.t1 - w.t0;
             ok = warp_wait(&sh.q_full, stretch & 1u);
-            if (ok) scores(0);
-            if (ok && total > 1) scores(1);
-            for (int u = 0; ok && u < total; ++u) {
-                values(u, n);
-                if (ok && u + 2 < total) scores(u + 2);
+            for (int u = 0; ok && u < NS; ++u) scores(u);
+            for (int u = 0; ok && u < NS * n; ++u) {
+                values(u);
+                if (ok && u + NS < NS * n) scores(u + NS);
             }
             base += 2 * n;
-            steps[0] += (total + 1) >> 1;
-            steps[1] += total >> 1;
+            steps += n;
             ++stretch;
         }
         if (elect_one()) tc_commit(&sh.drain);   // what was issued still reads the ring and the tensor memory
         __syncwarp();
         if (!warp_wait(&sh.drain, 0) || !ok) sh.failed = 1;
-    } else if (warp >= 4) {
-        // -------- softmax: stream = warps 4-7 or 8-11, thread = lane of tensor memory: row lane_l % kSpan of the tile, copy lane_l / kSpan --------
+    } else {
+        // -------- softmax: stream = warps 2-5 or 6-9, thread = lane of tensor memory: row lane_l % kSpan of the tile, copy lane_l / kSpan --------
         constexpr int kSpan = kTile / REP, kCols = kTile / REP;   // rows, a copy's positions of a tile
-        const int st = (warp - 4) >> 2, quarter = warp & 3, lane_l = tid & 127, row_l = lane_l % kSpan, copy = lane_l / kSpan;
+        const int st = (warp - 2) >> 2, quarter = warp & 3, lane_l = quarter * 32 + lane, row_l = lane_l % kSpan, copy = lane_l / kSpan;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), col_s = lanes + kColS + st * kTile, col_o = lanes + kColO + st * kHeadDim;
-        unsigned char* q_tile = q_tiles + (RT == 2 ? st * kTileBytes : 0);
-        uint32_t base = 0, tile_no = 0, alls = 0, groups = 0, steps = 0;
+        unsigned char* q_tile = q_tiles + st * kTileBytes;
+        uint32_t base = 0, alls = 0, groups = 0, steps = 0;   // steps: tiles before the stretch
         bool ok = true;
         int stretch = 0;
-        auto all_sync = [&]() {   // the eight warps, with a bound like every other wait
+        auto all_sync = [&]() {   // all softmax warps, with a bound like every other wait
             warp_arrive(&sh.all);
             ok = ok && warp_wait(&sh.all, alls++ & 1u);
         };
@@ -527,13 +494,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         const int m_rows = a.nodes * a.group;   // rows of Q in all
         for (; ok && w.left > 0; w.next(a), ++stretch) {
             const int kvh = w.item / a.row_tiles, rt = w.item % a.row_tiles, n = w.t1 - w.t0;
-            const int tile0 = rt * RT * kTile + (RT == 2 ? st * kTile : 0), row = tile0 + row_l;   // the stream's first row, this thread's
+            const int tile0 = (rt * NS + st) * kTile, row = tile0 + row_l;   // the stream's first row, this thread's
             const bool live = row < m_rows, busy = tile0 + (quarter * 32) % kSpan < m_rows;   // busy: some row of the warp is one
             // Q, 16 threads a row of 256 bytes, all loads at once; the products that read the last stretch's are done (its S has been
             // read).  Rows behind the last one repeat it.
             {
-                constexpr int kStep = RT == 2 ? 8 : 16, kLoads = kTile / kStep;
-                const int c = tid & 15, r0 = (RT == 2 ? lane_l : tid - 128) >> 4;
+                constexpr int kStep = 8, kLoads = kTile / kStep;
+                const int c = lane_l & 15, r0 = lane_l >> 4;
                 uint4 v[kLoads / REP];
 #pragma unroll
                 for (int j = 0; j < kLoads / REP; ++j) {
@@ -552,19 +519,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             float m = -INFINITY;   // maximum of the scores so far (or less, see above)
             uint64_t l2[2] = {0ull, 0ull};   // the sum, in four parts
             bool seen = false;
-            const int mine = RT == 2 ? n : (n + 1 - st) >> 1;   // this stream's steps
-            for (int x = 0; x < mine; ++x) {
-                const int i = RT == 2 ? x : 2 * x + st;
-                ok = warp_wait(&sh.s_full[st], (steps + x) & 1u);
+            for (int i = 0; i < n; ++i) {
+                ok = warp_wait(&sh.s_full[st], (steps + i) & 1u);
                 if (!ok) break;
                 tc_fence_after_sync();
-                const unsigned good = sh.good[(tile_no + i) & 7];
+                const unsigned good = sh.good[(steps + i) & 7];
                 const int pos0 = (w.t0 + i) * kTile;
                 const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
                 int chunks = kTile / 16;      // of 16 positions that are there
                 float known = -INFINITY;      // maximum of this thread's scores of a tile that is not whole
                 if (!whole) {
-                    const uint32_t at = base + value_at<RT>(i, n), stage = at % kRing;
+                    const uint32_t at = base + 2 * i + 1, stage = at % kRing;
                     ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
                     if (!ok) break;
                     clean_values(sh, ring + (size_t)stage * kTileBytes, w.seq, pos0, good, quarter, lane);
@@ -603,7 +568,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                         const uint64_t corr2 = pair_f32(corr, corr);
                         l2[0] = fma_f32x2(l2[0], corr2, 0ull);
                         l2[1] = fma_f32x2(l2[1], corr2, 0ull);
-                        if (x > 0) {   // O holds the stream's steps before, all complete (this step's S was issued after them)
+                        if (i > 0) {   // O holds the stream's steps before, all complete (this step's S was issued after them)
 #pragma unroll 1
                             for (int c = 0; c < kHeadDim; c += 32) {
                                 uint32_t o[32];
@@ -655,7 +620,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                         if (!whole) {
                             const bool raise = too_high(known);
                             if (__any_sync(0xffffffffu, raise)) rescale(known, raise);
-                        } else if (x == 0) {   // there is no maximum yet
+                        } else if (i == 0) {   // there is no maximum yet
                             float top = -INFINITY;
 #pragma unroll 1
                             for (int c = 0; c < kTile; c += 32) {
@@ -712,102 +677,80 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 sh.ml[st][lane_l] = make_float2(mc, l);
             }
             base += 2 * n;
-            tile_no += n;
-            steps += mine;
-            if (mine > 0) ok = warp_wait(&sh.o_done[st], (steps - 1) & 1u);
-            all_sync();   // the other stream's maximum, sum and O, every tile's bad nodes
+            steps += n;
+            ok = warp_wait(&sh.o_done[st], (steps - 1) & 1u);
+            all_sync();   // the copies' maxima and sums, every tile's bad nodes
             if (!ok) break;
             tc_fence_after_sync();
-            // A row's parts: the copies, of both streams where they share the rows.  RT = 1: each stream's warps add a half of the columns.
             const unsigned long long bad = sh.bad_nodes;
-            const bool both = RT == 1 && n > 1, complete = n == w.seq.tiles;
-            auto joint = [&](int rr) {   // maximum and sum over the parts of row rr
+            const bool complete = n == w.seq.tiles;
+            auto joint = [&](int rr) {   // maximum and sum over the copies of row rr
                 float mc = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int k = 0; k < REP; ++k) {
-                    mc = fmaxf(mc, sh.ml[RT == 2 ? st : 0][rr + k * kSpan].x);
-                    if (both) mc = fmaxf(mc, sh.ml[1][rr + k * kSpan].x);
-                }
+                for (int k = 0; k < REP; ++k) mc = fmaxf(mc, sh.ml[st][rr + k * kSpan].x);
 #pragma unroll
                 for (int k = 0; k < REP; ++k) {
-                    const float2 a0 = sh.ml[RT == 2 ? st : 0][rr + k * kSpan], a1 = both ? sh.ml[1][rr + k * kSpan] : make_float2(-INFINITY, 0.f);
-                    if (mc == -INFINITY) l += a0.y + a1.y;
-                    else l += (a0.x == -INFINITY ? 0.f : a0.y * exp2_approx(a0.x - mc)) + (a1.x == -INFINITY ? 0.f : a1.y * exp2_approx(a1.x - mc));
+                    const float2 x = sh.ml[st][rr + k * kSpan];
+                    l += mc == -INFINITY ? x.y : x.x == -INFINITY ? 0.f : x.y * exp2_approx(x.x - mc);
                 }
                 return make_float2(mc, l);
             };
             const float2 sum = joint(row_l);
-            // What a part's values are multiplied by: its own maximum against the joint one, the sum where the row is complete.
-            auto factor = [&](int s) {
-                const float x = sh.ml[s][lane_l].x, f = x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
-                return complete ? (sum.y == 0.f ? 0.f : f / sum.y) : f;
-            };
-            const float f0 = factor(RT == 2 ? st : 0), f1 = both ? factor(1) : 0.f;
-            const int64_t slot = ((int64_t)blockIdx.x * 2 + (stretch > 0)) * a.tile_rows + (RT == 2 ? st * kTile : 0);
-            constexpr int kWidth = RT == 1 ? 64 : 128;
-            const int d0 = RT == 1 ? 64 * st : 0;
-            const int rows_here = min(kSpan, m_rows - tile0);   // may be 0 or less (RT = 2)
-            // 32 columns of this thread's row, its streams added; zero where a part saw nothing (its O may be NaN then)
-            auto take = [&](int c, uint32_t* o) {
-                if (RT == 1) {
-                    uint32_t q[32];
-                    tmem_ld32(lanes + kColO + d0 + c, o);
-                    if (both) tmem_ld32(lanes + kColO + kHeadDim + d0 + c, q);
-                    tmem_wait_ld(o, q);
+            // What this copy's values are multiplied by: its maximum against the joint one, the sum where the row is complete.
+            const float x = sh.ml[st][lane_l].x, e = x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
+            const float f = !complete ? e : sum.y == 0.f ? 0.f : e / sum.y;
+            const int64_t slot = ((int64_t)blockIdx.x * 2 + (stretch > 0)) * a.tile_rows + st * kTile;
+            const int rows_here = min(kSpan, m_rows - tile0);   // may be 0 or less (NS = 2)
+            auto take = [&](int c, uint32_t* o) {   // 32 columns of this thread's row; zero where it saw nothing (its O may be NaN then)
+                tmem_ld32(col_o + c, o);
+                tmem_wait_ld(o);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float v = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
-                        if (both && f1 != 0.f) v = fmaf(__uint_as_float(q[e]), f1, v);
-                        o[e] = __float_as_uint(v);
-                    }
-                } else {
-                    tmem_ld32(col_o + c, o);
-                    tmem_wait_ld(o);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = f0 == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f0);
-                }
+                for (int k = 0; k < 32; ++k) o[k] = f == 0.f ? 0u : __float_as_uint(__uint_as_float(o[k]) * f);
             };
-            // Rows leave through the Q tiles' place: a thread has a row of tensor memory, and a store instruction wants neighbouring columns (a row a
+            // Rows leave through the Q tile's place: a thread has a row of tensor memory, and a store instruction wants neighbouring columns (a row a
             // thread takes a line of the L1 cache per thread and instruction).
-            if constexpr (REP == 1) {   // 4 KB a warp: its 32 rows, 64 columns of bf16 or 32 of float32
-                unsigned char* stage = q_tiles + (warp - 4) * 4096;
-                auto place = [&](int rr, int c) { return reinterpret_cast<uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4)); };
+            if constexpr (REP == 1) {   // 8 KB a warp: its 32 rows, all columns in bf16 or half of them in float32
+                unsigned char* stage = q_tile + quarter * 8192;
+                auto place = [&](int rr, int c) { return reinterpret_cast<uint4*>(stage + rr * 256 + ((c ^ (rr & 7)) << 4)); };
                 if (busy) {
 #pragma unroll 1
-                    for (int c = 0; c < kWidth; c += 32) {
+                    for (int c = 0; c < kHeadDim; c += 32) {
                         uint32_t o[32];
                         take(c, o);
                         if (complete) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8)
-                                *place(lane, ((c & 32) + e) >> 3) =
-                                    make_uint4(pack_bf16(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), pack_bf16(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
-                                               pack_bf16(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])), pack_bf16(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
-                            if (!(c & 32)) continue;
+                            for (int k = 0; k < 32; k += 8)
+                                *place(lane, (c + k) >> 3) =
+                                    make_uint4(pack_bf16(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), pack_bf16(__uint_as_float(o[k + 2]), __uint_as_float(o[k + 3])),
+                                               pack_bf16(__uint_as_float(o[k + 4]), __uint_as_float(o[k + 5])), pack_bf16(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7])));
+                            if (c < 96) continue;
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) *place(lane, e >> 2) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            for (int k = 0; k < 32; k += 4) *place(lane, ((c & 32) + k) >> 2) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                            if (!(c & 32)) continue;
                         }
                         __syncwarp();
-                        uint4 v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = *place(4 * k + (lane >> 3), lane & 7);   // four rows of 128 bytes at a time
+                        for (int half = 0; half < 2; ++half) {
+                            uint4 v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int rr = quarter * 32 + 4 * k + (lane >> 3);
-                            if (rr >= rows_here) continue;
-                            if (complete) reinterpret_cast<uint4*>(a.out + a.row_at(w.r, kvh, tile0 + rr) + d0 + (c & ~63))[lane & 7] = v[k];
-                            else reinterpret_cast<uint4*>(a.part + (slot + rr) * kHeadDim + d0 + c)[lane & 7] = v[k];
+                            for (int k = 0; k < 8; ++k) v[k] = *place(16 * half + 2 * k + (lane >> 4), lane & 15);   // two rows of 256 bytes at a time
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const int rr = quarter * 32 + 16 * half + 2 * k + (lane >> 4);
+                                if (rr >= rows_here) continue;
+                                if (complete) reinterpret_cast<uint4*>(a.out + a.row_at(w.r, kvh, tile0 + rr))[lane & 15] = v[k];
+                                else reinterpret_cast<uint4*>(a.part + (slot + rr) * kHeadDim + (c & 64))[lane & 15] = v[k];
+                            }
                         }
                         __syncwarp();
                     }
                 }
-            } else {   // 16 KB a stream: the copies of a row are added; up to 16 rows (REP = 4) all 64 columns at once, else 32
-                unsigned char* stage = q_tiles + st * (kTileBytes / 2);
-                const int wide = rows_here * REP <= 64 ? 64 : 32, pieces = wide / 4, shift = wide == 64 ? 4 : 3;
-                auto place = [&](int rr, int cp, int c) { return reinterpret_cast<float4*>(stage + ((cp * rows_here + rr) * pieces + (c ^ (rr & 7))) * 16); };
+            } else {   // 32 KB: the copies of a row are added; all columns at once, or half of them where there are more than 64 rows with the copies
+                const int wide = rows_here * REP <= 64 ? 128 : 64, pieces = wide / 4, shift = wide == 128 ? 5 : 4;
+                auto place = [&](int rr, int cp, int c) { return reinterpret_cast<float4*>(q_tile + ((cp * rows_here + rr) * pieces + (c ^ (rr & 7))) * 16); };
 #pragma unroll 1
-                for (int c0 = 0; c0 < kWidth; c0 += wide) {
+                for (int c0 = 0; c0 < kHeadDim; c0 += wide) {
                     if (c0) group_sync();   // the columns before have been read
                     if (!ok) break;
                     if (busy) {
@@ -817,8 +760,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                             take(c0 + c, o);
                             if (live)
 #pragma unroll
-                                for (int e = 0; e < 32; e += 4)
-                                    *place(row_l, copy, (c + e) >> 2) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                                for (int k = 0; k < 32; k += 4)
+                                    *place(row_l, copy, (c + k) >> 2) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
                             __syncwarp();
                         }
                     }
@@ -832,8 +775,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                             const float4 u = *place(rr, k, c);
                             v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
                         }
-                        if (complete) reinterpret_cast<uint2*>(a.out + a.row_at(w.r, kvh, tile0 + rr) + d0 + c0)[c] = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-                        else reinterpret_cast<float4*>(a.part + (slot + rr) * kHeadDim + d0 + c0)[c] = v;
+                        if (complete) reinterpret_cast<uint2*>(a.out + a.row_at(w.r, kvh, tile0 + rr) + c0)[c] = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                        else reinterpret_cast<float4*>(a.part + (slot + rr) * kHeadDim + c0)[c] = v;
                     }
                 }
                 if (!ok) break;
@@ -841,15 +784,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 if (!ok) break;
             }
             if (live && copy == 0) {
-                if (!complete && (RT == 2 || !st)) a.part_ml[slot + row_l] = sum;
+                if (!complete) a.part_ml[slot + row_l] = sum;
                 if (bad) {
-                    if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + a.row_at(w.r, kvh, row), d0, d0 + kWidth);
-                    else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim, d0, d0 + kWidth);
+                    if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + a.row_at(w.r, kvh, row));
+                    else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim);
                 }
             }
             tc_fence_before_sync();
             all_sync();   // sums and bad nodes have been read
-            if (tid == 128) sh.bad_nodes = 0;
+            if (tid == 64) sh.bad_nodes = 0;
         }
         if (!ok) sh.failed = 1;
     }
@@ -858,25 +801,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     __syncthreads();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_free(tmem, 512u);
+        tmem_free(tmem, kColumns);
         if (lane == 0 && sh.failed) atomicExch(a.error, MFQB_ERR_TIMEOUT);
     }
 }
 
 // Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context.
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int ctas, int per_seq) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ int64_t red[8][2];
-    const int r = blockIdx.x / per_seq, lane = threadIdx.x & 31;
-    const int local = (blockIdx.x % per_seq) * 8 + (threadIdx.x >> 5);   // kv head, row of Q
-    int64_t before, total;
-    tree_prefix(a, r, before, total, red);
-    const int m_rows = a.nodes * a.group;
-    if (local >= a.kv_heads * m_rows) return;
-    const int kvh = local / m_rows, row = local % m_rows, span = m_rows > kTile ? 2 * kTile : kTile, rt = row / span, row_l = row % span;
-    const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int ctas, int streams, int rows) {
+    chained_wait();
+    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5), m_rows = a.nodes * a.group, per_seq = a.kv_heads * m_rows;
+    if (warp >= rows) return;
+    const int r = warp / per_seq, local = warp - r * per_seq, kvh = local / m_rows, row = local - kvh * m_rows;
+    const int64_t before = __ldcg(a.before + r), total = __ldcg(a.before + a.rows);
     const TreeSeq seq = tree_seq(a, r);
+    const int span = streams * kTile, rt = row / span, row_l = row - rt * span;
+    const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
     const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units(), c0 = (s0 + kTreeStart) / quota, c1 = (s0 + seq.units() - 1) / quota;
     if (c0 == c1) return;
     auto slot = [&](int64_t c) { return (c * 2 + (s0 > c * quota ? 1 : 0)) * a.tile_rows + row_l; };
@@ -906,8 +845,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     const float inv = 1.f / l;
     if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
     else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    const int node = row / a.group, h = kvh * a.group + row % a.group;
-    *reinterpret_cast<uint2*>(a.out + (((int64_t)r * a.nodes + node) * a.hq + h) * kHeadDim + 4 * lane) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
+    *reinterpret_cast<uint2*>(a.out + a.row_at(r, kvh, row) + 4 * lane) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
 }
 
 // Keys or values of one layer as [page][head][position][128]: boxes of min(page, 128) positions x 64 dims with the 128-byte swizzle.
@@ -933,9 +871,13 @@ static CUtensorMap page_map(const void* base, const mfqb_cache& c) {
     return map;
 }
 
-static int tree_rows(const mfqb_cache& c, int q_heads, int nodes) { return std::min(2 * kTile, nodes * (q_heads / c.kv_heads)); }
+static int tree_streams(const mfqb_cache& c, int q_heads, int nodes) { return nodes * (q_heads / c.kv_heads) > kTile ? 2 : 1; }
+static int64_t tree_parts(const mfqb_cache& c, int q_heads, int nodes) {   // rows of the parts
+    const int ns = tree_streams(c, q_heads, nodes);
+    return (int64_t)tree_ctas(ns) * 2 * std::min(ns * kTile, nodes * (q_heads / c.kv_heads));
+}
 static uint64_t tree_attention_work_bytes(const mfqb_cache& c, int q_heads, int nodes) {
-    return (uint64_t)kTreeCtas * 2 * tree_rows(c, q_heads, nodes) * (kHeadDim * 4 + 8);
+    return (uint64_t)tree_parts(c, q_heads, nodes) * (kHeadDim * 4 + 8) + 8ull * (c.rows + 1);
 }
 static void check_heads(const mfqb_cache* c, int q_heads, const char* who) {
     if (q_heads < 1 || q_heads % c->kv_heads || q_heads / c->kv_heads > 16)
@@ -964,24 +906,25 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.group = q_heads / c.kv_heads;
     a.nodes = nodes;
     a.group_inv = (65536u + a.group - 1) / a.group;
-    const int rt = nodes * a.group > kTile ? 2 : 1;   // see tree_attn_kernel
-    a.row_tiles = (nodes * a.group + rt * kTile - 1) / (rt * kTile);
-    a.tile_rows = tree_rows(c, q_heads, nodes);
+    const int ns = tree_streams(c, q_heads, nodes), m_rows = nodes * a.group, ctas = tree_ctas(ns);
+    a.row_tiles = (m_rows + ns * kTile - 1) / (ns * kTile);
+    a.tile_rows = std::min(ns * kTile, m_rows);
     a.part = static_cast<float*>(work);
-    a.part_ml = reinterpret_cast<float2*>(a.part + (int64_t)kTreeCtas * 2 * a.tile_rows * kHeadDim);
+    a.part_ml = reinterpret_cast<float2*>(a.part + tree_parts(c, q_heads, nodes) * kHeadDim);
+    a.before = reinterpret_cast<int64_t*>(a.part_ml + tree_parts(c, q_heads, nodes));
     a.scale_log2 = scale * 1.4426950408889634f;
     a.error = device_status_word(device);
     const CUtensorMap kmap = page_map(a.k, c), vmap = page_map(a.v, c);
-    const int m_rows = nodes * a.group;
-    auto* kernel = rt == 2 ? tree_attn_kernel<2, 1> : m_rows > 64 ? tree_attn_kernel<1, 1> : m_rows > 32 ? tree_attn_kernel<1, 2> : tree_attn_kernel<1, 4>;
+    auto* kernel = ns == 2 ? tree_attn_kernel<2, 1> : m_rows > 64 ? tree_attn_kernel<1, 1> : m_rows > 32 ? tree_attn_kernel<1, 2> : tree_attn_kernel<1, 4>;
     static std::once_flag once[64];
     std::call_once(once[device], [] {
-        for (auto* k : {tree_attn_kernel<2, 1>, tree_attn_kernel<1, 1>, tree_attn_kernel<1, 2>, tree_attn_kernel<1, 4>})
-            MFQB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTreeSmem));
+        MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<2, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(2)));
+        for (auto* k : {tree_attn_kernel<1, 1>, tree_attn_kernel<1, 2>, tree_attn_kernel<1, 4>})
+            MFQB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(1)));
     });
-    launch_chained(kernel, dim3(kTreeCtas), dim3(kTreeThreads), kTreeSmem, s, a, kmap, vmap);
-    const int per_seq = (c.kv_heads * nodes * a.group + 7) / 8;
-    launch_chained(tree_merge_kernel, dim3((unsigned)(c.rows * per_seq)), dim3(256), 0, s, a, (int)kTreeCtas, per_seq);
+    launch_chained(kernel, dim3(ctas), dim3(tree_threads(ns)), tree_smem(ns), s, a, kmap, vmap);
+    const int64_t rows = (int64_t)c.rows * c.kv_heads * m_rows;   // at most 1024 x 1024 x 1024
+    launch_chained(tree_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a, ctas, ns, (int)rows);
 }
 
 }  // namespace mfqb
