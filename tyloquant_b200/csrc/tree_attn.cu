@@ -526,17 +526,15 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                 const unsigned good = sh.good[(steps + i) & 7];
                 const int pos0 = (w.t0 + i) * kTile;
                 const bool whole = pos0 + kTile <= w.seq.len && good == 0xFFu;   // every row sees all of the tile
-                int chunks = kTile / 16;      // of 16 positions that are there
-                float known = -INFINITY;      // maximum of this thread's scores of a tile that is not whole
+                float known = -INFINITY;   // maximum of this thread's scores of a tile that is not whole
                 if (!whole) {
                     const uint32_t at = base + 2 * i + 1, stage = at % kRing;
                     ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u);
                     if (!ok) break;
                     clean_values(sh, ring + (size_t)stage * kTileBytes, w.seq, pos0, good, quarter, lane);
-                    chunks = min(chunks, (w.seq.end - pos0 + 15) >> 4);
                     // what this row does not see of its copy's positions becomes minus infinity
 #pragma unroll 1
-                    for (int c = 0; c < kCols && copy * kCols + c < 16 * chunks; c += 32) {
+                    for (int c = 0; c < kCols; c += 32) {
                         const int p0 = copy * kCols + c, ctx = w.seq.len - (pos0 + p0);   // positions from here on that are before the length
                         unsigned vis = ctx >= 32 ? 0xFFFFFFFFu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
                         if (ctx <= 0 && ctx > -64) vis |= (unsigned)(mask >> -ctx);
@@ -587,13 +585,6 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                         for (int c = 0; c < kCols; c += 32) tmem_ld32(col_s + copy * kCols + c, s + c);
 #pragma unroll
                         for (int c = 0; c < kCols; c += 32) tmem_wait_ld(s + c);
-                        if (!whole) {   // what lies behind the last chunk has not been hidden
-#pragma unroll
-                            for (int c = 0; c < kCols; c += 32)
-                                if (copy * kCols + c >= 16 * chunks)
-#pragma unroll
-                                    for (int e = 0; e < 32; ++e) s[c + e] = 0xFF800000u;
-                        }
                         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int e = 0; e < kCols; e += 2) top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
@@ -643,10 +634,9 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                             tmem_ld16_async(col_s, s[0]);
 #pragma unroll
                             for (int c = 0; c < 8; ++c) {
-                                if (c >= chunks) break;   // the same for all
                                 uint32_t* now = s[c & 1];
                                 tmem_wait_ld16(now);
-                                if (c < 7 && c + 1 < chunks) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
+                                if (c < 7) tmem_ld16_async(col_s + 16 * (c + 1), s[(c + 1) & 1]);
                                 exp16<true>(now, scale2, mc2, sum, top, p + 8 * c);
                             }
                             const float high = fmaxf(top[0], top[1]);
