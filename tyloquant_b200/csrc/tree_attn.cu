@@ -420,8 +420,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
         auto scores = [&](int u) {
             const int i = u / NS, st = u % NS;
             const uint32_t at = base + 2 * i, stage = at % kRing;
-            ok = u < NS ? warp_wait(&sh.kv_full[stage], (at / kRing) & 1u)
-                       : warp_wait2(&sh.kv_full[stage], (at / kRing) & 1u, &sh.o_done[st], (steps + i - 1) & 1u);
+            ok = warp_wait(&sh.kv_full[stage], (at / kRing) & 1u) && (u < NS || warp_wait(&sh.o_done[st], (steps + i - 1) & 1u));
             if (!ok) return;
             tc_fence_after_sync();
             const uint32_t k_addr = __shfl_sync(0xffffffffu, ring_addr + stage * kTileBytes, 0), q = __shfl_sync(0xffffffffu, q_addr + st * kTileBytes, 0);
