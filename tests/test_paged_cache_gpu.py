@@ -403,6 +403,24 @@ def test_beam_selection(groups, beams, k, vocab):
     _check_beams(logits, scores, min(k, vocab), done, eos=7, exact_ids=False)
 
 
+def test_the_largest_selections():
+    """128 beams with 128 candidates each; a million tokens: the merge's lists do not fit shared memory, or not all at once."""
+    rng = np.random.default_rng(20)
+    for groups, beams, vocab, k in ((1, 128, 20000, 128), (1, 2, 1 << 20, 128), (1, 70, 1 << 17, 100)):
+        logits = rng.standard_normal((groups, beams, vocab), dtype=np.float32) * 2
+        _check_beams(logits, -rng.random((groups, beams), dtype=np.float32), k, exact_ids=False)
+
+
+def test_rows_with_few_live_tokens():
+    """A vocabulary of which most is masked out: more than a list's worth of equal minus infinities, with and without enough others."""
+    rng = np.random.default_rng(21)
+    for live in (0, 3, 40, 3000):
+        logits = np.full((2, 2, 30000), -np.inf, np.float32)
+        at = rng.permutation(30000)[:live]
+        logits[:, :, at] = rng.standard_normal((2, 2, live)).astype(np.float32)
+        _check_beams(logits, np.array([[0.0, -1.0], [-2.0, 0.0]], np.float32), 20)
+
+
 def test_equal_candidates_go_to_the_lower_beam_and_token():
     """Equal beams on rows of every alignment, equal logits, a row of one value, more equal logits than a thread holds."""
     for vocab in (997, 1000, 20001):

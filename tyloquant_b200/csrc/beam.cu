@@ -1,10 +1,13 @@
 // Beam selection: the k best continuations of a group of beams by score + log softmax(logits), one pass over the logits.
+#include <mutex>
+
 #include "paged.h"
 
 namespace mfqb {
 
 constexpr int kBeamMax = 128, kBeamKeep = 128;   // beams of a group, candidates kept
 constexpr int kSliceThreads = 256, kSliceEach = 32, kSlice = kSliceThreads * kSliceEach;
+constexpr size_t kMergeSmem = 200 * 1024;        // of the merging kernel
 constexpr int kSlicesMax = 128;                  // slices of a row: lists that the 32 lanes of a warp merge, four each
 
 // A slice's record: its largest logit, the sum of exp(logit - largest) and its k best keys, best first.
@@ -26,26 +29,31 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
 
+constexpr int kListMax = 1024;   // candidates of a slice that are ranked by counting
+
 // CTA (slice, row).  A thread keeps its 32 logits in registers: element (j * 256 + thread) * 4 + e of the slice whatever the row's
-// alignment, so that equal rows have equal sums to the last bit and ties between beams are ties.  Of the k best candidates every
-// one is at least the k-th largest of the threads' own best: what reaches that bound (at most 32 k, mostly some k) goes
-// into a list, and a candidate's place is the number of larger ones in it.
-__global__ void __launch_bounds__(kSliceThreads) beam_slice_kernel(const float* __restrict__ logits, const int* __restrict__ done, int vocab, int k, int slices,
+// alignment, so that equal rows have equal sums to the last bit and ties between beams are ties.
+//
+// At least k elements reach the least of the eight warps' ceil(k / 8)-th largest thread maxima, and few others do (some 50 for k = 16):
+// they go into a list, and a candidate's place is the number of larger ones in it.  The bound costs a warp one sort of 32 values; the k-th
+// largest of all 256 maxima, found by counting, took as long as everything else (128 rows of 128256: 73 us in all).  Where too
+// many elements are equal for the list, the best key is taken k times.
+__global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const float* __restrict__ logits, const int* __restrict__ done, int vocab, int k, int slices,
                                                                    bool wide, SliceSum* __restrict__ sums, unsigned long long* __restrict__ keys) {
     chained_wait();
-    extern __shared__ unsigned long long s_list[];   // [kSliceEach * k]
-    __shared__ unsigned long long s_best[kSliceThreads];
-    __shared__ float s_top[8];
+    __shared__ __align__(16) float s_x[kSlice];   // only where the list is too short
+    unsigned long long* s_list = reinterpret_cast<unsigned long long*>(s_x);
+    __shared__ unsigned long long s_round[2][8];
+    __shared__ float s_top[8], s_low[8];
     __shared__ double s_sum[8];
     __shared__ int s_count;
-    __shared__ unsigned long long s_bound;
-    const int t = threadIdx.x, slice = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slice = blockIdx.x;
     const int64_t row = blockIdx.y;
     if (done && done[row]) return;
     const int base = slice * kSlice;
     const float* src = logits + row * vocab + base;
     const int n = min(kSlice, vocab - base);
-    float x[kSliceEach];
+    float x[kSliceEach];   // minus infinity behind the end
 #pragma unroll
     for (int j = 0; j < kSliceEach / 4; ++j) {
         const int i = (j * kSliceThreads + t) * 4;
@@ -57,76 +65,132 @@ __global__ void __launch_bounds__(kSliceThreads) beam_slice_kernel(const float* 
             for (int e = 0; e < 4; ++e) x[4 * j + e] = i + e < n ? __ldcs(src + i + e) : -INFINITY;
         }
     }
-    unsigned long long best = 0ull;
+    if (t == 0) s_count = 0;
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kSliceEach; ++j) {
-        const int i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
-        if (i < n) {
-            best = max(best, beam_key(x[j], (unsigned)(base + i)));
-            top = fmaxf(top, x[j]);
+    for (int j = 0; j < kSliceEach; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
+    // the warp's thread maxima in descending order
+    float sorted = top;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float u = __shfl_xor_sync(0xffffffffu, sorted, o);
+            sorted = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(sorted, u) : fminf(sorted, u);
         }
-    }
-    s_best[t] = best;
-    if (t == 0) s_count = 0;
-    if (t == 0) s_bound = 1ull;
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((t & 31) == 0) s_top[t >> 5] = top;
+    const float low = __shfl_sync(0xffffffffu, sorted, (k + 7) / 8 - 1), high = __shfl_sync(0xffffffffu, sorted, 0);
+    if (lane == 0) { s_top[warp] = high; s_low[warp] = low; }
     __syncthreads();
     top = s_top[0];
+    float bound = s_low[0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, s_top[w]);
-    float part = 0.f;
+    for (int w = 1; w < 8; ++w) {
+        top = fmaxf(top, s_top[w]);
+        bound = fminf(bound, s_low[w]);
+    }
+    // exp(x - top), the exponent in two terms (log2(e) in one float32 is off by 2^-26); NaN where there is a NaN or top is an infinity
+    float part[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kSliceEach; ++j) {
+        const float d = x[j] - top;
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, 1.9259629e-8f, d * 1.44269502f)));
+        part[j & 1] += x[j] == -INFINITY ? 0.f : e;
+    }
+    double sum = (double)part[0] + (double)part[1];
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    // Candidates; a NaN counts as minus infinity, which reaches the bound only where that is minus infinity.
+    unsigned take = 0;
 #pragma unroll
     for (int j = 0; j < kSliceEach; ++j) {
         const int i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
-        if (i < n && x[j] != -INFINITY) part += expf(x[j] - top);
+        if (!(x[j] < bound) && i < n && (x[j] == x[j] || bound == -INFINITY)) take |= 1u << j;
     }
-    double sum = part;
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((t & 31) == 0) s_sum[t >> 5] = sum;
-    int above = 0;
-    for (int j = 0; j < kSliceThreads; ++j) above += s_best[j] > best;
-    if (above == k - 1 && best) s_bound = best;   // keys differ, so one thread at most
+    if (take) {
+        int at = atomicAdd(&s_count, __popc(take));   // the order in the list does not matter
+#pragma unroll
+        for (int j = 0; j < kSliceEach; ++j)
+            if ((take >> j) & 1u) {
+                if (at < kListMax) s_list[at] = beam_key(x[j], (unsigned)(base + ((j >> 2) * kSliceThreads + t) * 4 + (j & 3)));
+                ++at;
+            }
+    }
     __syncthreads();
     if (t == 0) {
         sum = s_sum[0];
         for (int w = 1; w < 8; ++w) sum += s_sum[w];
         sums[row * slices + slice] = SliceSum{sum, top, 0.f};
     }
-    const unsigned long long bound = s_bound;
-    if (best >= bound) {
-#pragma unroll
-        for (int j = 0; j < kSliceEach; ++j) {
-            const int i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
-            if (i < n) {
-                const unsigned long long key = beam_key(x[j], (unsigned)(base + i));
-                if (key >= bound) s_list[atomicAdd(&s_count, 1)] = key;   // the order in the list does not matter
-            }
-        }
-    }
-    __syncthreads();
     const int have = s_count;
     unsigned long long* out = keys + (row * slices + slice) * k;
-    for (int i = t; i < have; i += kSliceThreads) {
-        const unsigned long long key = s_list[i];
-        int rank = 0;
-        for (int j = 0; j < have; ++j) rank += s_list[j] > key;
-        if (rank < k) out[rank] = key;
+    if (have <= kListMax) {
+        for (int i = t; i < have; i += kSliceThreads) {
+            const unsigned long long key = s_list[i];
+            int rank = 0;
+            for (int j = 0; j < have; ++j) rank += s_list[j] > key;
+            if (rank < k) out[rank] = key;
+        }
+        for (int i = have + t; i < k; i += kSliceThreads) out[i] = 0ull;   // a short slice
+        return;
     }
-    for (int i = have + t; i < k; i += kSliceThreads) out[i] = 0ull;   // a short slice
+    // Too many: rounds of the largest key, the logits in shared memory (a loop over registers would have to be unrolled).
+    __syncthreads();   // the list is done with
+#pragma unroll
+    for (int j = 0; j < kSliceEach; ++j) s_x[j * kSliceThreads + t] = x[j];
+    unsigned long long best = 0ull;
+    int from = 0;
+    bool look = true;
+    for (int i = 0; i < k; ++i) {
+        if (look) {   // this thread's best one of what is left
+            best = 0ull;
+#pragma unroll 1
+            for (unsigned left = take; left; left &= left - 1) {
+                const int j = __ffs(left) - 1;
+                const unsigned long long key = beam_key(s_x[j * kSliceThreads + t], (unsigned)(base + ((j >> 2) * kSliceThreads + t) * 4 + (j & 3)));
+                if (key > best) { best = key; from = j; }
+            }
+        }
+        unsigned long long all = best;
+        for (int o = 16; o > 0; o >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
+        if (lane == 0) s_round[i & 1][warp] = all;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) all = max(all, s_round[i & 1][w]);
+        look = all && best == all;   // keys differ, so one thread at most
+        if (look) {
+            take &= ~(1u << from);
+            out[i] = all;
+        }
+    }
 }
 
-// CTA per group.  A warp merges the lists of a beam's slices into the beam's k best, then one warp the beams' lists into the group's.
-__global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restrict__ scores, const int* __restrict__ done, int eos, int beams, int k, int slices,
+// The largest of 32 pairs (high, low word), the same in all lanes.
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
+    const unsigned hi = (unsigned)(v >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+    return (unsigned long long)top << 32 | __reduce_max_sync(0xffffffffu, hi == top ? (unsigned)v : 0u);
+}
+// Doubles in the order of unsigned numbers (a NaN as minus infinity, -0 as 0).
+__device__ __forceinline__ unsigned long long order_f64(double v) {
+    v = v == v ? v + 0.0 : -INFINITY;
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double from_order_f64(unsigned long long o) { return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o)); }
+
+// CTA per group.  A warp merges the lists of a beam's slices into the beam's k best, `at_once` beams at a time, then one warp the beams' lists
+// into the group's.  The lists come into shared memory first where they fit (staged): a warp takes the best head k times, and each time waits
+// for that list's next one.
+__global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restrict__ scores, const int* __restrict__ done, int eos, int beams, int k, int slices, int at_once, bool staged,
                                                           const SliceSum* __restrict__ sums, const unsigned long long* __restrict__ keys,
-                                                          unsigned long long* __restrict__ beam_keys, float* __restrict__ out_scores,
-                                                          int* __restrict__ out_rows, int* __restrict__ out_tokens) {
+                                                          float* __restrict__ out_scores, int* __restrict__ out_rows, int* __restrict__ out_tokens) {
     chained_wait();
-    __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
+    extern __shared__ unsigned long long s_best[];   // the beams' results [beams][k], then [at_once][slices][k] where staged
+    __shared__ double s_score[kBeamMax], s_lse[kBeamMax];
     __shared__ unsigned char s_done[kBeamMax];
     const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = warp; b < beams; b += 32) {
+    for (int b = warp; b < beams; b += at_once) {
+        if (warp >= at_once) break;
         const int64_t row = (int64_t)group * beams + b;
         const bool over = done && done[row];
         if (lane == 0) {
@@ -134,6 +198,12 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restric
             s_score[b] = scores[row];
         }
         if (over) continue;
+        const unsigned long long *src = keys + row * slices * k, *mine = src;
+        if (staged) {
+            unsigned long long* dst = s_best + (size_t)beams * k + (size_t)warp * slices * k;
+            for (int i = lane; i < slices * k; i += 32) dst[i] = src[i];
+            mine = dst;
+        }
         float top = -INFINITY;
         for (int s = lane; s < slices; s += 32) top = fmaxf(top, sums[row * slices + s].top);
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -144,57 +214,37 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restric
         }
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_lse[b] = (double)top + log(sum);
-        const unsigned long long* src = keys + row * slices * k;
-        unsigned long long* dst = beam_keys + row * k;
+        __syncwarp();
         int at[4] = {0, 0, 0, 0};   // next entry of this lane's lists
         unsigned long long head[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) head[j] = lane + 32 * j < slices ? src[(int64_t)(lane + 32 * j) * k] : 0ull;
+        for (int j = 0; j < 4; ++j) head[j] = lane + 32 * j < slices ? mine[(lane + 32 * j) * k] : 0ull;
         for (int i = 0; i < k; ++i) {
-            unsigned long long m = max(max(head[0], head[1]), max(head[2], head[3]));
-            for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (lane == 0) dst[i] = m;
+            const unsigned long long m = warp_max(max(max(head[0], head[1]), max(head[2], head[3])));
+            if (lane == 0) s_best[b * k + i] = m;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (m && head[j] == m) head[j] = ++at[j] < k ? src[(int64_t)(lane + 32 * j) * k + at[j]] : 0ull;
+                if (m && head[j] == m) head[j] = ++at[j] < k ? mine[(lane + 32 * j) * k + at[j]] : 0ull;
         }
+        __syncwarp();
     }
     __syncthreads();
     if (warp) return;
-    // beams lane, lane + 32, ...: head candidate, its score in 64 bits
+    // beams lane, lane + 32, ...: score of the head candidate in 64 bits, as an ordered number; 0 where there is none left
     int at[4] = {0, 0, 0, 0};
-    double head[4];
+    unsigned long long head[4];
     auto fetch = [&](int j) {
         const int b = lane + 32 * j;
-        if (b >= beams || at[j] >= (s_done[b] ? 1 : k)) {
-            at[j] = 1 << 20;   // exhausted
-            return;
-        }
-        double v = s_score[b];
-        if (!s_done[b]) v += (double)key_logit(beam_keys[((int64_t)group * beams + b) * k + at[j]]) - s_lse[b];
-        head[j] = v == v ? v : -INFINITY;
+        head[j] = 0ull;
+        if (b >= beams || at[j] >= (s_done[b] ? 1 : k)) return;
+        head[j] = order_f64(s_done[b] ? s_score[b] : s_score[b] + ((double)key_logit(s_best[b * k + at[j]]) - s_lse[b]));
     };
 #pragma unroll
     for (int j = 0; j < 4; ++j) fetch(j);
     for (int i = 0; i < k; ++i) {
-        double best = 0.0;
-        int from = 1 << 20;   // the beam
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (at[j] < (1 << 20) && (from == (1 << 20) || head[j] > best)) {
-                best = head[j];
-                from = lane + 32 * j;
-            }
-        for (int o = 16; o > 0; o >>= 1) {
-            const double v = __shfl_xor_sync(0xffffffffu, best, o);
-            const int f = __shfl_xor_sync(0xffffffffu, from, o);
-            if (f != (1 << 20) && (from == (1 << 20) || v > best || (v == best && f < from))) {
-                best = v;
-                from = f;
-            }
-        }
+        const unsigned long long best = warp_max(max(max(head[0], head[1]), max(head[2], head[3])));
         const int64_t o = (int64_t)group * k + i;
-        if (from == (1 << 20)) {   // all lists are exhausted
+        if (!best) {   // all lists are exhausted
             if (lane == 0) {
                 out_scores[o] = -INFINITY;
                 out_rows[o] = -1;
@@ -202,33 +252,33 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restric
             }
             continue;
         }
-        if (lane == (from & 31)) {
+        unsigned from = 1u << 20;   // the lowest beam with this score
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j == from >> 5) {
-                    const int64_t row = (int64_t)group * beams + from;
-                    out_scores[o] = (float)best;
-                    out_rows[o] = (int)row;
-                    out_tokens[o] = s_done[from] ? eos : (int)(0xFFFFFFFFu - (unsigned)beam_keys[row * k + at[j]]);
-                    ++at[j];
-                    fetch(j);
-                }
-        }
+        for (int j = 3; j >= 0; --j)
+            if (head[j] == best) from = lane + 32 * j;
+        from = __reduce_min_sync(0xffffffffu, from);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (from == (unsigned)(lane + 32 * j)) {
+                out_scores[o] = (float)from_order_f64(best);
+                out_rows[o] = (int)((int64_t)group * beams + from);
+                out_tokens[o] = s_done[from] ? eos : (int)(0xFFFFFFFFu - (unsigned)s_best[from * k + at[j]]);
+                ++at[j];
+                fetch(j);
+            }
     }
 }
 
 struct BeamWork {
     SliceSum* sums;                  // [rows][slices]
     unsigned long long* keys;        // [rows][slices][k]
-    unsigned long long* beam_keys;   // [rows][k]
 };
 static int beam_slices(int vocab) { return (vocab + kSlice - 1) / kSlice; }
-static uint64_t beam_work_bytes(int64_t rows, int vocab, int k) { return (uint64_t)rows * beam_slices(vocab) * (sizeof(SliceSum) + 8ull * k) + (uint64_t)rows * k * 8ull; }
+static uint64_t beam_work_bytes(int64_t rows, int vocab, int k) { return (uint64_t)rows * beam_slices(vocab) * (sizeof(SliceSum) + 8ull * k); }
 static BeamWork beam_work(void* work, int64_t rows, int vocab, int k) {
     BeamWork w;
     w.sums = static_cast<SliceSum*>(work);
     w.keys = reinterpret_cast<unsigned long long*>(w.sums + rows * beam_slices(vocab));
-    w.beam_keys = w.keys + rows * beam_slices(vocab) * k;
     return w;
 }
 static void check_beams(int groups, int beams, int vocab, int k, const char* who) {
@@ -264,11 +314,23 @@ int mfqb_beam_select(const float* logits, int groups, int beams, int vocab, cons
                  (unsigned long long)work_bytes);
         const BeamWork w = beam_work(work, rows, vocab, k);
         const bool wide = vocab % 4 == 0 && ((uintptr_t)logits & 15) == 0;
-        launch_chained(beam_slice_kernel, dim3(beam_slices(vocab), (unsigned)rows), dim3(kSliceThreads), (size_t)kSliceEach * k * 8, stream, logits,
-                       static_cast<const int*>(done), vocab, k, beam_slices(vocab), wide, w.sums, w.keys);
-        launch_chained(beam_merge_kernel, dim3(groups), dim3(1024), 0, stream, scores, static_cast<const int*>(done), eos, beams, k, beam_slices(vocab),
-                       static_cast<const SliceSum*>(w.sums), static_cast<const unsigned long long*>(w.keys), w.beam_keys, out_scores,
-                       static_cast<int*>(out_rows), static_cast<int*>(out_tokens));
+        const int slices = beam_slices(vocab);
+        launch_chained(beam_slice_kernel, dim3(slices, (unsigned)rows), dim3(kSliceThreads), 0, stream, logits, static_cast<const int*>(done), vocab, k, slices, wide,
+                       w.sums, w.keys);
+        // Beams merged at once: as many as find room for their lists beside the results (at most 128 KB).
+        const size_t each = (size_t)slices * k * 8, results = (size_t)beams * k * 8;
+        const bool staged = results + each <= kMergeSmem;
+        const int at_once = staged ? (int)std::min<size_t>({32, (size_t)beams, (kMergeSmem - results) / each}) : std::min(32, beams);
+        const size_t smem = results + (staged ? at_once * each : 0);
+        if (smem > 40 * 1024) {
+            int device = 0;
+            MFQB_CUDA(cudaGetDevice(&device));
+            static std::once_flag once[64];
+            std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMergeSmem)); });
+        }
+        launch_chained(beam_merge_kernel, dim3(groups), dim3(1024), smem, stream, scores, static_cast<const int*>(done), eos, beams, k, slices, at_once, staged,
+                       static_cast<const SliceSum*>(w.sums), static_cast<const unsigned long long*>(w.keys), out_scores, static_cast<int*>(out_rows),
+                       static_cast<int*>(out_tokens));
     });
 }
 
