@@ -34,17 +34,18 @@ constexpr int kListMax = 1024;   // candidates of a slice that are ranked by cou
 // CTA (slice, row).  A thread keeps its 32 logits in registers: element (j * 256 + thread) * 4 + e of the slice whatever the row's
 // alignment, so that equal rows have equal sums to the last bit and ties between beams are ties.
 //
-// At least k elements reach the least of the eight warps' ceil(k / 8)-th largest thread maxima, and few others do (some 50 for k = 16):
-// they go into a list, and a candidate's place is the number of larger ones in it.  The bound costs a warp one sort of 32 values; the k-th
-// largest of all 256 maxima, found by counting, took as long as everything else (128 rows of 128256: 73 us in all).  Where too
-// many elements are equal for the list, the best key is taken k times.
+// Candidates are the elements that reach a bound which at least k of them do: the j-th largest thread maximum of a warp, j = ceil(k / c), in the
+// c-th best of the eight warps, for the best of c = 8, 4, 2, 1 (some 30 candidates for k = 16; with c = 8 alone some 100).  They go into a list,
+// and a candidate's place is the number of larger ones in it.  The bound costs a warp two sorts by shuffles; the k-th largest of all 256
+// maxima, found by counting, took as long as everything else.  Where too many elements are equal for the list, the best key is taken
+// k times.  128 rows of 128256 (115 of them read): 73 us in all with counting.
 __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const float* __restrict__ logits, const int* __restrict__ done, int vocab, int k, int slices,
-                                                                   bool wide, SliceSum* __restrict__ sums, unsigned long long* __restrict__ keys) {
+                                                                      bool wide, SliceSum* __restrict__ sums, unsigned long long* __restrict__ keys) {
     chained_wait();
     __shared__ __align__(16) float s_x[kSlice];   // only where the list is too short
     unsigned long long* s_list = reinterpret_cast<unsigned long long*>(s_x);
     __shared__ unsigned long long s_round[2][8];
-    __shared__ float s_top[8], s_low[8];
+    __shared__ float s_top[8], s_low[32];
     __shared__ double s_sum[8];
     __shared__ int s_count;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slice = blockIdx.x;
@@ -54,67 +55,85 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     const float* src = logits + row * vocab + base;
     const int n = min(kSlice, vocab - base);
     float x[kSliceEach];   // minus infinity behind the end
+    if (wide && n == kSlice) {
 #pragma unroll
-    for (int j = 0; j < kSliceEach / 4; ++j) {
-        const int i = (j * kSliceThreads + t) * 4;
-        if (wide && i + 4 <= n) {
-            const float4 v = __ldcs(reinterpret_cast<const float4*>(src + i));
+        for (int j = 0; j < kSliceEach / 4; ++j) {
+            const float4 v = __ldcs(reinterpret_cast<const float4*>(src) + j * kSliceThreads + t);
             x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * j + e] = i + e < n ? __ldcs(src + i + e) : -INFINITY;
+        for (int j = 0; j < kSliceEach; ++j) {
+            const int i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
+            x[j] = i < n ? __ldcs(src + i) : -INFINITY;
         }
     }
     if (t == 0) s_count = 0;
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kSliceEach; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
-    // the warp's thread maxima in descending order
-    float sorted = top;
+    // values of `size` neighbouring lanes in descending order
+    auto sort = [&](float v, int width) {
 #pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
+        for (int size = 2; size <= 32; size <<= 1)
+            if (size <= width)
 #pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const float u = __shfl_xor_sync(0xffffffffu, sorted, o);
-            sorted = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(sorted, u) : fminf(sorted, u);
-        }
-    const float low = __shfl_sync(0xffffffffu, sorted, (k + 7) / 8 - 1), high = __shfl_sync(0xffffffffu, sorted, 0);
-    if (lane == 0) { s_top[warp] = high; s_low[warp] = low; }
+                for (int o = size >> 1; o > 0; o >>= 1) {
+                    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+                    v = ((lane & o) == 0) == ((lane & size & (width - 1)) == 0) ? fmaxf(v, u) : fminf(v, u);
+                }
+        return v;
+    };
+    const float sorted = sort(top, 32);
+    if (lane == 0) s_top[warp] = sorted;
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        const int c = 8 >> o, j = (k + c - 1) / c;
+        const float v = __shfl_sync(0xffffffffu, sorted, min(j, 32) - 1);
+        if (lane == 0) s_low[o * 8 + warp] = j <= 32 ? v : -INFINITY;
+    }
     __syncthreads();
     top = s_top[0];
-    float bound = s_low[0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) {
-        top = fmaxf(top, s_top[w]);
-        bound = fminf(bound, s_low[w]);
-    }
-    // exp(x - top), the exponent in two terms (log2(e) in one float32 is off by 2^-26); NaN where there is a NaN or top is an infinity
-    float part[2] = {0.f, 0.f};
+    for (int w = 1; w < 8; ++w) top = fmaxf(top, s_top[w]);
+    float bound = sort(s_low[lane], 8);   // lane 8 o + i: the i-th best warp of choice o
+    bound = (lane & 7) == (8 >> (lane >> 3)) - 1 ? bound : -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kSliceEach; ++j) {
-        const float d = x[j] - top;
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, 1.9259629e-8f, d * 1.44269502f)));
-        part[j & 1] += x[j] == -INFINITY ? 0.f : e;
+    for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+    unsigned take = 0;
+    float part = 0.f;
+    if (top > -INFINITY && top < INFINITY && bound > -INFINITY) {
+        // exp(x - top), the exponent in two terms (log2(e) in one float32 is off by 2^-26); NaN where there is a NaN
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kSliceEach; ++j) {
+            const float d = x[j] - top;
+            float e;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, 1.9259629e-8f, d * 1.44269502f)));
+            sum[j & 1] += e;
+            take |= (unsigned)(x[j] >= bound) << j;
+        }
+        part = sum[0] + sum[1];
+    } else {   // the same for what is out of the ordinary; a NaN counts as minus infinity among the candidates
+#pragma unroll
+        for (int j = 0; j < kSliceEach; ++j) {
+            const int i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
+            if (i >= n) continue;
+            const float d = x[j] - top;
+            if (x[j] != -INFINITY) part += exp2f(fmaf(d, 1.9259629e-8f, d * 1.44269502f));   // infinity - infinity: NaN
+            if (x[j] >= bound || bound == -INFINITY) take |= 1u << j;
+        }
     }
-    double sum = (double)part[0] + (double)part[1];
+    double sum = part;
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
-    // Candidates; a NaN counts as minus infinity, which reaches the bound only where that is minus infinity.
-    unsigned take = 0;
-#pragma unroll
-    for (int j = 0; j < kSliceEach; ++j) {
-        const int i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
-        if (!(x[j] < bound) && i < n && (x[j] == x[j] || bound == -INFINITY)) take |= 1u << j;
-    }
     if (take) {
         int at = atomicAdd(&s_count, __popc(take));   // the order in the list does not matter
-#pragma unroll
-        for (int j = 0; j < kSliceEach; ++j)
-            if ((take >> j) & 1u) {
-                if (at < kListMax) s_list[at] = beam_key(x[j], (unsigned)(base + ((j >> 2) * kSliceThreads + t) * 4 + (j & 3)));
-                ++at;
-            }
+#pragma unroll 1
+        for (unsigned left = take; left && at < kListMax; left &= left - 1, ++at) {   // read again: few, and a loop over registers would have to be unrolled
+            const int j = __ffs(left) - 1, i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
+            s_list[at] = beam_key(__ldg(src + i), (unsigned)(base + i));
+        }
     }
     __syncthreads();
     if (t == 0) {
@@ -128,6 +147,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
         for (int i = t; i < have; i += kSliceThreads) {
             const unsigned long long key = s_list[i];
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < have; ++j) rank += s_list[j] > key;
             if (rank < k) out[rank] = key;
         }
