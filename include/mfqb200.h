@@ -506,7 +506,7 @@ int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* par
  * different beams by score (log sums and scores are compared in 64 bits), equal ones by beam.  A NaN counts as minus infinity.
  * A beam with a non-zero entry in done (int32 [groups][beams], may be null) has one candidate: the token eos at its own score.
  * Where a group has fewer than k candidates the rest is row -1, token -1, score minus infinity.  beams <= 128, k <= min(128, vocab),
- * vocab <= 1048576.  work: device memory of mfqb_beam_select_work bytes, 16-byte aligned. */
+ * beams * k <= 8192, vocab <= 1048576.  work: device memory of mfqb_beam_select_work bytes, 16-byte aligned. */
 int mfqb_beam_select_work(int groups, int beams, int vocab, int k, uint64_t* bytes);
 int mfqb_beam_select(const float* logits, int groups, int beams, int vocab, const float* scores, const int32_t* done, int eos, int k,
                      float* out_scores, int32_t* out_rows, int32_t* out_tokens, void* work, uint64_t work_bytes, mfqb_stream_t stream);

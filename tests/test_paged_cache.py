@@ -71,7 +71,8 @@ def test_arguments_that_are_refused():
 def test_selections_that_are_refused():
     n = C.c_uint64()
     for groups, beams, vocab, k, code, text in ((0, 4, 100, 4, 3, "beams"), (1, 129, 100, 4, 3, "beams"), (1 << 10, 64, 100, 4, 3, "beams"), (1, 4, 0, 1, 3, "tokens"),
-                                                (1, 4, (1 << 20) + 1, 1, 3, "tokens"), (1, 4, 100, 0, 1, "k must"), (1, 4, 1000, 129, 1, "k must"), (1, 4, 5, 6, 1, "k must")):
+                                                (1, 4, (1 << 20) + 1, 1, 3, "tokens"), (1, 4, 100, 0, 1, "k must"), (1, 4, 1000, 129, 1, "k must"), (1, 4, 5, 6, 1, "k must"),
+                                                (1, 100, 1000, 82, 3, "beams times k")):
         _says(code, text, lib.mfqb_beam_select_work(groups, beams, vocab, k, C.byref(n)))
         _says(code, text, lib.mfqb_beam_select(A, groups, beams, vocab, A, None, 0, k, A, A, A, A, 1 << 40, None))
     assert lib.mfqb_beam_select_work(2, 4, 100, 4, C.byref(n)) == 0

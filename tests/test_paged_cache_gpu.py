@@ -404,9 +404,9 @@ def test_beam_selection(groups, beams, k, vocab):
 
 
 def test_the_largest_selections():
-    """128 beams with 128 candidates each; a million tokens: the merge's lists do not fit shared memory, or not all at once."""
+    """128 beams, 128 candidates, a million tokens: the merge's lists do not fit shared memory, or not all at once."""
     rng = np.random.default_rng(20)
-    for groups, beams, vocab, k in ((1, 128, 20000, 128), (1, 2, 1 << 20, 128), (1, 70, 1 << 17, 100)):
+    for groups, beams, vocab, k in ((1, 128, 20000, 64), (1, 2, 1 << 20, 128), (1, 64, 1 << 17, 128), (1, 64, 600000, 128), (2, 40, 3000, 3)):
         logits = rng.standard_normal((groups, beams, vocab), dtype=np.float32) * 2
         _check_beams(logits, -rng.random((groups, beams), dtype=np.float32), k, exact_ids=False)
 

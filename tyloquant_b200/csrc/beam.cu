@@ -5,7 +5,7 @@
 
 namespace mfqb {
 
-constexpr int kBeamMax = 128, kBeamKeep = 128;   // beams of a group, candidates kept
+constexpr int kBeamMax = 128, kBeamKeep = 128, kBeamProduct = 8192;   // beams of a group, candidates kept, one times the other
 constexpr int kSliceThreads = 256, kSliceEach = 32, kSlice = kSliceThreads * kSliceEach;
 constexpr size_t kMergeSmem = 200 * 1024;        // of the merging kernel
 constexpr int kSlicesMax = 128;                  // slices of a row: lists that the 32 lanes of a warp merge, four each
@@ -198,94 +198,108 @@ __device__ __forceinline__ unsigned long long order_f64(double v) {
 }
 __device__ __forceinline__ double from_order_f64(unsigned long long o) { return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o)); }
 
+// A warp merges `lists` sorted lists into their k best: lane l has the lists l, l + 32, .. (NL of them), get(list, i) is entry i of one, 0 behind its
+// end, and put(i, list, at, key) is called by the lane that has the i-th best key: entry `at` of `list`.  Equal keys: the lower list.  A
+// list's next entry is asked for when the one before it comes to its head.  Returns how many there were.
+template <int NL, typename Get, typename Put>
+__device__ __forceinline__ int merge_lists(int lane, int k, Get get, Put put) {
+    int at[NL];
+    unsigned long long head[NL], next[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        at[j] = 0;
+        head[j] = get(lane + 32 * j, 0);
+        next[j] = get(lane + 32 * j, 1);
+    }
+    for (int i = 0; i < k; ++i) {
+        unsigned long long mine = head[0];
+#pragma unroll
+        for (int j = 1; j < NL; ++j) mine = max(mine, head[j]);
+        const unsigned long long best = warp_max(mine);
+        if (!best) return i;
+        unsigned from = 1u << 20;
+#pragma unroll
+        for (int j = NL - 1; j >= 0; --j)
+            if (head[j] == best) from = lane + 32 * j;
+        from = NL == 1 ? (unsigned)(__ffs(__ballot_sync(0xffffffffu, mine == best)) - 1) : __reduce_min_sync(0xffffffffu, from);
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+            if (from == (unsigned)(lane + 32 * j)) {
+                put(i, (int)from, at[j], best);
+                head[j] = next[j];
+                next[j] = get((int)from, ++at[j] + 1);
+            }
+    }
+    return k;
+}
+
 // CTA per group.  A warp merges the lists of a beam's slices into the beam's k best, `at_once` beams at a time, then one warp the beams' lists
-// into the group's.  The lists come into shared memory first where they fit (staged): a warp takes the best head k times, and each time waits
-// for that list's next one.
-__global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restrict__ scores, const int* __restrict__ done, int eos, int beams, int k, int slices, int at_once, bool staged,
-                                                          const SliceSum* __restrict__ sums, const unsigned long long* __restrict__ keys,
+// into the group's.  The lists come into shared memory first where they fit (staged): every one of the k rounds waits for the entry behind
+// the one that it takes.
+template <int NL>
+__global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restrict__ scores, const int* __restrict__ done, int eos, int beams, int k, int slices, int at_once,
+                                                          bool staged, const SliceSum* __restrict__ sums, const unsigned long long* __restrict__ keys,
                                                           float* __restrict__ out_scores, int* __restrict__ out_rows, int* __restrict__ out_tokens) {
     chained_wait();
-    extern __shared__ unsigned long long s_best[];   // the beams' results [beams][k], then [at_once][slices][k] where staged
-    __shared__ double s_score[kBeamMax], s_lse[kBeamMax];
+    extern __shared__ unsigned long long s_best[];   // the beams' results [beams][k]: keys, then scores; then [at_once][slices][k] where staged
+    unsigned long long* s_value = s_best + beams * k;
     __shared__ unsigned char s_done[kBeamMax];
     const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = warp; b < beams; b += at_once) {
-        if (warp >= at_once) break;
-        const int64_t row = (int64_t)group * beams + b;
-        const bool over = done && done[row];
-        if (lane == 0) {
-            s_done[b] = over;
-            s_score[b] = scores[row];
-        }
-        if (over) continue;
-        const unsigned long long *src = keys + row * slices * k, *mine = src;
-        if (staged) {
-            unsigned long long* dst = s_best + (size_t)beams * k + (size_t)warp * slices * k;
-            for (int i = lane; i < slices * k; i += 32) dst[i] = src[i];
-            mine = dst;
-        }
-        float top = -INFINITY;
-        for (int s = lane; s < slices; s += 32) top = fmaxf(top, sums[row * slices + s].top);
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        double sum = 0.0;
-        for (int s = lane; s < slices; s += 32) {
-            const SliceSum v = sums[row * slices + s];
-            sum += v.sum * exp((double)v.top - (double)top);   // NaN where the row holds a NaN, an infinity or nothing above minus infinity
-        }
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s_lse[b] = (double)top + log(sum);
-        __syncwarp();
-        int at[4] = {0, 0, 0, 0};   // next entry of this lane's lists
-        unsigned long long head[4];
+    if (warp < at_once) {
+        for (int b = warp; b < beams; b += at_once) {
+            const int64_t row = (int64_t)group * beams + b;
+            const bool over = done && done[row];
+            const double score = scores[row];
+            if (lane == 0) s_done[b] = over;
+            if (over) {
+                if (lane == 0) s_value[b * k] = order_f64(score);
+                continue;
+            }
+            SliceSum part[NL];
+            float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) head[j] = lane + 32 * j < slices ? mine[(lane + 32 * j) * k] : 0ull;
-        for (int i = 0; i < k; ++i) {
-            const unsigned long long m = warp_max(max(max(head[0], head[1]), max(head[2], head[3])));
-            if (lane == 0) s_best[b * k + i] = m;
+            for (int j = 0; j < NL; ++j) {
+                part[j].top = -INFINITY;
+                part[j].sum = 0.0;
+                if (lane + 32 * j < slices) part[j] = sums[row * slices + lane + 32 * j];
+                top = fmaxf(top, part[j].top);
+            }
+            const unsigned long long *src = keys + row * slices * k, *mine = src;
+            if (staged) {
+                unsigned long long* dst = s_value + (size_t)beams * k + (size_t)warp * slices * k;
+#pragma unroll 4
+                for (int i = lane; i < slices * k; i += 32) dst[i] = src[i];
+                mine = dst;
+            }
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            double sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (m && head[j] == m) head[j] = ++at[j] < k ? mine[(lane + 32 * j) * k + at[j]] : 0ull;
+            for (int j = 0; j < NL; ++j)   // NaN where the row holds a NaN, an infinity or nothing above minus infinity
+                if (lane + 32 * j < slices) sum += part[j].sum * exp((double)part[j].top - (double)top);
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const double lse = (double)top + log(sum);
+            __syncwarp();
+            merge_lists<NL>(
+                lane, k, [&](int list, int i) { return list < slices && i < k ? mine[list * k + i] : 0ull; },
+                [&](int i, int, int, unsigned long long key) { s_best[b * k + i] = key; });
+            __syncwarp();
+            for (int i = lane; i < k; i += 32) s_value[b * k + i] = order_f64(score + ((double)key_logit(s_best[b * k + i]) - lse));
         }
-        __syncwarp();
     }
     __syncthreads();
     if (warp) return;
-    // beams lane, lane + 32, ...: score of the head candidate in 64 bits, as an ordered number; 0 where there is none left
-    int at[4] = {0, 0, 0, 0};
-    unsigned long long head[4];
-    auto fetch = [&](int j) {
-        const int b = lane + 32 * j;
-        head[j] = 0ull;
-        if (b >= beams || at[j] >= (s_done[b] ? 1 : k)) return;
-        head[j] = order_f64(s_done[b] ? s_score[b] : s_score[b] + ((double)key_logit(s_best[b * k + at[j]]) - s_lse[b]));
+    const int64_t o = (int64_t)group * k;
+    auto get = [&](int b, int i) { return b < beams && i < (s_done[b] ? 1 : k) ? s_value[b * k + i] : 0ull; };
+    auto put = [&](int i, int b, int at, unsigned long long value) {
+        out_scores[o + i] = (float)from_order_f64(value);
+        out_rows[o + i] = (int)((int64_t)group * beams + b);
+        out_tokens[o + i] = s_done[b] ? eos : (int)(0xFFFFFFFFu - (unsigned)s_best[b * k + at]);
     };
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fetch(j);
-    for (int i = 0; i < k; ++i) {
-        const unsigned long long best = warp_max(max(max(head[0], head[1]), max(head[2], head[3])));
-        const int64_t o = (int64_t)group * k + i;
-        if (!best) {   // all lists are exhausted
-            if (lane == 0) {
-                out_scores[o] = -INFINITY;
-                out_rows[o] = -1;
-                out_tokens[o] = -1;
-            }
-            continue;
-        }
-        unsigned from = 1u << 20;   // the lowest beam with this score
-#pragma unroll
-        for (int j = 3; j >= 0; --j)
-            if (head[j] == best) from = lane + 32 * j;
-        from = __reduce_min_sync(0xffffffffu, from);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (from == (unsigned)(lane + 32 * j)) {
-                out_scores[o] = (float)from_order_f64(best);
-                out_rows[o] = (int)((int64_t)group * beams + from);
-                out_tokens[o] = s_done[from] ? eos : (int)(0xFFFFFFFFu - (unsigned)s_best[from * k + at[j]]);
-                ++at[j];
-                fetch(j);
-            }
+    const int have = beams <= 32 ? merge_lists<1>(lane, k, get, put) : merge_lists<4>(lane, k, get, put);
+    for (int i = have + lane; i < k; i += 32) {   // all lists are exhausted
+        out_scores[o + i] = -INFINITY;
+        out_rows[o + i] = -1;
+        out_tokens[o + i] = -1;
     }
 }
 
@@ -306,6 +320,7 @@ static void check_beams(int groups, int beams, int vocab, int k, const char* who
         fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to %d beams in each group, at most 65535 in all, got %d groups of %d", who, kBeamMax, groups, beams);
     if (vocab < 1 || vocab > kSlicesMax * kSlice) fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to %d tokens, got %d", who, kSlicesMax * kSlice, vocab);
     if (k < 1 || k > kBeamKeep || k > vocab) fail(MFQB_ERR_ARG, "%s: k must be in [1, min(%d, vocab)], got %d", who, kBeamKeep, k);
+    if (beams * k > kBeamProduct) fail(MFQB_ERR_UNSUPPORTED, "%s: beams times k must be at most %d, got %d beams and k = %d", who, kBeamProduct, beams, k);
 }
 
 }  // namespace mfqb
@@ -337,8 +352,8 @@ int mfqb_beam_select(const float* logits, int groups, int beams, int vocab, cons
         const int slices = beam_slices(vocab);
         launch_chained(beam_slice_kernel, dim3(slices, (unsigned)rows), dim3(kSliceThreads), 0, stream, logits, static_cast<const int*>(done), vocab, k, slices, wide,
                        w.sums, w.keys);
-        // Beams merged at once: as many as find room for their lists beside the results (at most 128 KB).
-        const size_t each = (size_t)slices * k * 8, results = (size_t)beams * k * 8;
+        // Beams merged at once: as many as find room for their lists beside the results.
+        const size_t each = (size_t)slices * k * 8, results = (size_t)beams * k * 16;
         const bool staged = results + each <= kMergeSmem;
         const int at_once = staged ? (int)std::min<size_t>({32, (size_t)beams, (kMergeSmem - results) / each}) : std::min(32, beams);
         const size_t smem = results + (staged ? at_once * each : 0);
@@ -346,11 +361,14 @@ int mfqb_beam_select(const float* logits, int groups, int beams, int vocab, cons
             int device = 0;
             MFQB_CUDA(cudaGetDevice(&device));
             static std::once_flag once[64];
-            std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMergeSmem)); });
+            std::call_once(once[device], [] {
+                for (auto* f : {beam_merge_kernel<1>, beam_merge_kernel<4>})
+                    MFQB_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMergeSmem));
+            });
         }
-        launch_chained(beam_merge_kernel, dim3(groups), dim3(1024), smem, stream, scores, static_cast<const int*>(done), eos, beams, k, slices, at_once, staged,
-                       static_cast<const SliceSum*>(w.sums), static_cast<const unsigned long long*>(w.keys), out_scores, static_cast<int*>(out_rows),
-                       static_cast<int*>(out_tokens));
+        launch_chained(slices <= 32 ? beam_merge_kernel<1> : beam_merge_kernel<4>, dim3(groups), dim3(1024), smem, stream, scores, static_cast<const int*>(done), eos,
+                       beams, k, slices, at_once, staged, static_cast<const SliceSum*>(w.sums), static_cast<const unsigned long long*>(w.keys), out_scores,
+                       static_cast<int*>(out_rows), static_cast<int*>(out_tokens));
     });
 }
 
