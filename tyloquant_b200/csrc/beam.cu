@@ -104,16 +104,17 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     float part = 0.f;
     if (top > -INFINITY && top < INFINITY && bound > -INFINITY) {
         // exp(x - top), the exponent in two terms (log2(e) in one float32 is off by 2^-26); NaN where there is a NaN
-        float sum[2] = {0.f, 0.f};
+        uint64_t sum = 0ull;
+        const uint64_t minus_top = pair_f32(-top, -top), hi = pair_f32(1.44269502f, 1.44269502f), lo = pair_f32(1.9259629e-8f, 1.9259629e-8f);
 #pragma unroll
-        for (int j = 0; j < kSliceEach; ++j) {
-            const float d = x[j] - top;
-            float e;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, 1.9259629e-8f, d * 1.44269502f)));
-            sum[j & 1] += e;
-            take |= (unsigned)(x[j] >= bound) << j;
+        for (int j = 0; j < kSliceEach; j += 2) {
+            const uint64_t d = add_f32x2(pair_f32(x[j], x[j + 1]), minus_top);
+            const float2 e = split_f32(fma_f32x2(d, lo, fma_f32x2(d, hi, 0ull)));
+            sum = add_f32x2(sum, pair_f32(exp2_approx(e.x), exp2_approx(e.y)));
+            take |= (unsigned)(x[j] >= bound) << j | (unsigned)(x[j + 1] >= bound) << (j + 1);
         }
-        part = sum[0] + sum[1];
+        const float2 both = split_f32(sum);
+        part = both.x + both.y;
     } else {   // the same for what is out of the ordinary; a NaN counts as minus infinity among the candidates
 #pragma unroll
         for (int j = 0; j < kSliceEach; ++j) {

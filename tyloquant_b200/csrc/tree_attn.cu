@@ -188,11 +188,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t* r, uint32_t* q) {
     asm volatile("" : MFQB_P8(q, 0), MFQB_P8(q, 8));
     asm volatile("" : MFQB_P8(q, 16), MFQB_P8(q, 24));
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -209,26 +204,6 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* a, uint32_t pa, uint64_t* b
     return warp_wait(a, pa) && warp_wait(b, pb);
 }
 
-__device__ __forceinline__ uint64_t pair_f32(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 split_f32(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // exp2(scale s + mc) of 16 scores, rounded to bf16 into p; their sums are added to l, their maxima to top where TOP.
 template <bool TOP>
 __device__ __forceinline__ void exp16(const uint32_t* s, uint64_t scale, uint64_t mc, uint64_t (&l)[2], float (&top)[2], uint32_t* p) {
