@@ -142,7 +142,9 @@ for _name, (_res, _args) in _SIGNATURES.items():
 
 from . import _fast  # noqa: E402  (built together with the library)
 
-_fast.bind(*(C.cast(getattr(lib, _name), C.c_void_p).value for _name in ("mfqb_mul_mat", "mfqb_moe_topk", "mfqb_moe_ffn")))
+_fast.bind(*(C.cast(getattr(lib, _name), C.c_void_p).value for _name in (
+    "mfqb_mul_mat", "mfqb_moe_topk", "mfqb_moe_ffn", "mfqb_cache_extend", "mfqb_cache_fork", "mfqb_tree_masks", "mfqb_cache_write", "mfqb_tree_attention",
+    "mfqb_tree_accept", "mfqb_beam_select")))
 
 
 def check(status: int) -> None:

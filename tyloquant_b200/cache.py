@@ -8,7 +8,9 @@ captured into a CUDA graph."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
+from . import _fast
 from ._capi import CacheView, check, lib
 from .linear import _torch
 
@@ -16,29 +18,23 @@ HEAD_DIM = 128
 MAX_NODES = 64
 
 
-def _need(t, dtype, shape, device, what):
-    """`t` as a contiguous tensor; raises unless it has this type, shape and device."""
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what} must be a {str(dtype).replace('torch.', '')} tensor {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    return t if t.is_contiguous() else t.contiguous()
+def _need(t, dtype, shape, device: int, what: str):
+    """`t` as a contiguous tensor; raises unless it has this type and shape and is on this GPU."""
+    if t.dtype is dtype and t.get_device() == device and t.shape == shape:
+        return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{what} must be a {str(dtype).replace('torch.', '')} tensor {list(shape)} on cuda:{device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-class _On:
-    """Makes a device current for the scope where it is not, and gives its current stream."""
-
-    def __init__(self, index: int):
-        torch = _torch()
-        self.index, self.prev = index, torch._C._cuda_getDevice()
-
-    def __enter__(self) -> int:
-        torch = _torch()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.prev != self.index:
-            _torch().cuda.set_device(self.prev)
+def _call(fn, device: int, *args) -> None:
+    """One library call on the current stream of a device, which is made current where it is not."""
+    cuda = _torch()._C
+    if cuda._cuda_getDevice() == device:
+        status = fn(*args, cuda._cuda_getCurrentRawStream(device))
+    else:
+        with _torch().cuda.device(device):
+            status = fn(*args, cuda._cuda_getCurrentRawStream(device))
+    if status:
+        check(status)
 
 
 def rope_frequencies(theta: float = 500000.0, device="cuda"):
@@ -54,10 +50,10 @@ def tree_masks(parents):
     torch = _torch()
     if parents.dim() != 2 or not parents.is_cuda:
         raise ValueError("parents must be an int32 CUDA tensor [rows, nodes]")
-    p = _need(parents, torch.int32, parents.shape, parents.device, "parents")
+    dev = parents.get_device()
+    p = _need(parents, torch.int32, parents.shape, dev, "parents")
     masks, depths = p.new_empty(p.shape, dtype=torch.int64), torch.empty_like(p)
-    with _On(p.get_device()) as s:
-        check(lib.mfqb_tree_masks(p.data_ptr(), p.shape[0], p.shape[1], masks.data_ptr(), depths.data_ptr(), s))
+    _call(_fast.tree_masks, dev, p.data_ptr(), p.shape[0], p.shape[1], masks.data_ptr(), depths.data_ptr())
     return masks, depths
 
 
@@ -75,15 +71,15 @@ class PagedCache:
         rows, width = table.shape
         for t, dtype, shape, what in ((k, torch.bfloat16, k.shape, "k"), (v, torch.bfloat16, k.shape, "v"), (table, torch.int32, (rows, width), "table"),
                                       (lens, torch.int32, (rows,), "lens"), (refs, torch.int32, (pages,), "refs")):
-            if _need(t, dtype, shape, k.device, what) is not t:
+            if _need(t, dtype, shape, k.get_device(), what) is not t:
                 raise ValueError(f"{what} must be contiguous")
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.layers, self.pages, self.kv_heads, self.page, self.rows, self.width = layers, pages, heads, page, rows, width
         self.device = k.get_device()
         self._view = CacheView(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), layers, heads, page, pages, rows, width)
-        self._ref = C.byref(self._view)
+        self._ptr = C.addressof(self._view)
         size = C.c_uint64()
-        check(lib.mfqb_cache_fork_work(self._ref, C.byref(size)))   # refuses a shape that the library does not take
+        check(lib.mfqb_cache_fork_work(C.byref(self._view), C.byref(size)))   # refuses a shape that the library does not take
         self._fork_work = size.value
         self._attend_work = {}
 
@@ -98,7 +94,7 @@ class PagedCache:
                    torch.zeros(pages, dtype=torch.int32, device=d))
 
     def _int32(self, t, shape, what):
-        return _need(t, _torch().int32, shape, self.k.device, what)
+        return _need(t, _torch().int32, shape, self.device, what)
 
     def extend(self, tokens):
         """Reserves pages for ``tokens[r]`` more tokens of every sequence (int32 [rows], or one number for all).  Returns int32 [1] on the
@@ -108,8 +104,7 @@ class PagedCache:
             tokens = torch.full((self.rows,), tokens, dtype=torch.int32, device=self.k.device)
         t = self._int32(tokens, (self.rows,), "tokens")
         status = self.lens.new_empty(1)
-        with _On(self.device) as s:
-            check(lib.mfqb_cache_extend(self._ref, t.data_ptr(), status.data_ptr(), s))
+        _call(_fast.cache_extend, self.device, self._ptr, t.data_ptr(), status.data_ptr())
         return status
 
     def fork(self, parents):
@@ -119,8 +114,7 @@ class PagedCache:
         p = self._int32(parents, (self.rows,), "parents")
         status = self.lens.new_empty(1)
         work = self.lens.new_empty(self._fork_work // 4)
-        with _On(self.device) as s:
-            check(lib.mfqb_cache_fork(self._ref, p.data_ptr(), status.data_ptr(), work.data_ptr(), self._fork_work, s))
+        _call(_fast.cache_fork, self.device, self._ptr, p.data_ptr(), status.data_ptr(), work.data_ptr(), self._fork_work)
         return status
 
     def write(self, layer: int, qkv, depths, freqs):
@@ -131,12 +125,11 @@ class PagedCache:
         if qkv.dim() != 3 or qkv.shape[0] != self.rows or qkv.shape[2] % HEAD_DIM or qkv.shape[2] // HEAD_DIM <= 2 * self.kv_heads:
             raise ValueError(f"qkv must be [{self.rows}, nodes, (q_heads + {2 * self.kv_heads}) * 128], got {list(qkv.shape)}")
         nodes, hq = qkv.shape[1], qkv.shape[2] // HEAD_DIM - 2 * self.kv_heads
-        x = _need(qkv, torch.float32, qkv.shape, self.k.device, "qkv")
+        x = _need(qkv, torch.float32, qkv.shape, self.device, "qkv")
         d = self._int32(depths, (self.rows, nodes), "depths")
-        f = _need(freqs, torch.float64, (HEAD_DIM // 2,), self.k.device, "freqs")
+        f = _need(freqs, torch.float64, (HEAD_DIM // 2,), self.device, "freqs")
         q = x.new_empty((self.rows, nodes, hq, HEAD_DIM), dtype=torch.bfloat16)
-        with _On(self.device) as s:
-            check(lib.mfqb_cache_write(self._ref, layer, x.data_ptr(), hq, nodes, d.data_ptr(), f.data_ptr(), q.data_ptr(), s))
+        _call(_fast.cache_write, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, d.data_ptr(), f.data_ptr(), q.data_ptr())
         return q
 
     def attend(self, layer: int, q, masks, scale: float | None = None, out=None):
@@ -147,21 +140,20 @@ class PagedCache:
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != HEAD_DIM:
             raise ValueError(f"q must be [{self.rows}, nodes, q_heads, 128], got {list(q.shape)}")
         _, nodes, hq, _ = q.shape
-        x = _need(q, torch.bfloat16, q.shape, self.k.device, "q")
-        m = _need(masks, torch.int64, (self.rows, nodes), self.k.device, "masks")
+        x = _need(q, torch.bfloat16, q.shape, self.device, "q")
+        m = _need(masks, torch.int64, (self.rows, nodes), self.device, "masks")
         if out is None:
             out = torch.empty_like(x)
-        elif _need(out, torch.bfloat16, q.shape, self.k.device, "out") is not out:
+        elif _need(out, torch.bfloat16, q.shape, self.device, "out") is not out:
             raise ValueError("out must be contiguous")
         size = self._attend_work.get((hq, nodes))
         if size is None:
             n = C.c_uint64()
-            check(lib.mfqb_tree_attention_work(self._ref, hq, nodes, C.byref(n)))
+            check(lib.mfqb_tree_attention_work(C.byref(self._view), hq, nodes, C.byref(n)))
             size = self._attend_work[(hq, nodes)] = (n.value + 15) // 16 * 16
         work = x.new_empty(size // 2)
-        with _On(self.device) as s:
-            check(lib.mfqb_tree_attention(self._ref, layer, x.data_ptr(), hq, nodes, m.data_ptr(), HEAD_DIM ** -0.5 if scale is None else scale,
-                                          out.data_ptr(), work.data_ptr(), size, s))
+        _call(_fast.tree_attention, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, m.data_ptr(), HEAD_DIM ** -0.5 if scale is None else scale,
+              out.data_ptr(), work.data_ptr(), size)
         return out
 
     def accept(self, ids, parents, targets, lens_out=None):
@@ -178,10 +170,16 @@ class PagedCache:
         elif self._int32(lens_out, (self.rows,), "lens_out") is not lens_out:
             raise ValueError("lens_out must be contiguous")
         count, token, path = self.lens.new_empty(self.rows), self.lens.new_empty(self.rows), self.lens.new_empty((self.rows, nodes))
-        with _On(self.device) as s:
-            check(lib.mfqb_tree_accept(self._ref, i.data_ptr(), p.data_ptr(), t.data_ptr(), nodes, count.data_ptr(), token.data_ptr(), path.data_ptr(),
-                                       lens_out.data_ptr(), s))
+        _call(_fast.tree_accept, self.device, self._ptr, i.data_ptr(), p.data_ptr(), t.data_ptr(), nodes, count.data_ptr(), token.data_ptr(), path.data_ptr(),
+              lens_out.data_ptr())
         return count, token, path, lens_out
+
+
+@functools.lru_cache(maxsize=64)
+def _beam_work(groups: int, beams: int, vocab: int, k: int) -> int:
+    n = C.c_uint64()
+    check(lib.mfqb_beam_select_work(groups, beams, vocab, k, C.byref(n)))
+    return (n.value + 15) // 16 * 16
 
 
 def beam_select(logits, scores, k: int, done=None, eos: int = -1):
@@ -193,15 +191,13 @@ def beam_select(logits, scores, k: int, done=None, eos: int = -1):
     if logits.dim() != 3 or not logits.is_cuda:
         raise ValueError("logits must be a float32 CUDA tensor [groups, beams, vocab]")
     g, w, vocab = logits.shape
-    z = _need(logits, torch.float32, logits.shape, logits.device, "logits")
-    sc = _need(scores, torch.float32, (g, w), z.device, "scores")
-    dn = None if done is None else _need(done, torch.int32, (g, w), z.device, "done")
-    n = C.c_uint64()
-    check(lib.mfqb_beam_select_work(g, w, vocab, k, C.byref(n)))
-    size = (n.value + 15) // 16 * 16
+    dev = logits.get_device()
+    z = _need(logits, torch.float32, logits.shape, dev, "logits")
+    sc = _need(scores, torch.float32, (g, w), dev, "scores")
+    dn = None if done is None else _need(done, torch.int32, (g, w), dev, "done")
+    size = _beam_work(g, w, vocab, k)
     work = z.new_empty(size // 4)
     out, rows, tokens = z.new_empty((g, k)), z.new_empty((g, k), dtype=torch.int32), z.new_empty((g, k), dtype=torch.int32)
-    with _On(z.get_device()) as s:
-        check(lib.mfqb_beam_select(z.data_ptr(), g, w, vocab, sc.data_ptr(), None if dn is None else dn.data_ptr(), eos, k, out.data_ptr(), rows.data_ptr(),
-                                   tokens.data_ptr(), work.data_ptr(), size, s))
+    _call(_fast.beam_select, dev, z.data_ptr(), g, w, vocab, sc.data_ptr(), None if dn is None else dn.data_ptr(), eos, k, out.data_ptr(), rows.data_ptr(),
+          tokens.data_ptr(), work.data_ptr(), size)
     return out, rows, tokens
