@@ -77,11 +77,15 @@ __global__ void __launch_bounds__(1024) extend_kernel(mfqb_cache c, const int* _
     __shared__ int total;
     if (r == 1023) total = upto;
     __syncthreads();
-    // Pages in rounds of 1024.  The first pass only counts, so that nothing has changed when the pool turns out too small.
+    // Up to 1024 pages come from one search; more are counted first, so that nothing has changed when the pool turns out too small.
     int have = 0;
-    for (int base = 0; base < c.pages && have < total; base += 1024) {
-        const int p = base + r;
-        have += __syncthreads_count(p < c.pages && c.refs[p] <= 0);
+    if (total > 1024) {
+        for (int base = 0; base < c.pages && have < total; base += 1024) {
+            const int p = base + r;
+            have += __syncthreads_count(p < c.pages && c.refs[p] <= 0);
+        }
+    } else if (total) {
+        have = find_free(c.refs, nullptr, c.pages, total, list, warp_sums);
     }
     if (have < total || lack_table) {
         if (r == 0) *status = (int)min(lack_table + max(0, total - have), 0x7FFFFFFFull);
@@ -90,7 +94,7 @@ __global__ void __launch_bounds__(1024) extend_kernel(mfqb_cache c, const int* _
     if (r == 0) *status = 0;
     int next = first, left = need, at = upto - need;   // this thread's next entry, and the rank of the page it waits for
     for (int done = 0; done < total; done += 1024) {
-        const int n = find_free(c.refs, nullptr, c.pages, min(1024, total - done), list, warp_sums);
+        const int n = total > 1024 ? find_free(c.refs, nullptr, c.pages, min(1024, total - done), list, warp_sums) : total;
         __syncthreads();
         while (left > 0 && at < done + n) {
             while ((unsigned)row[next] < (unsigned)c.pages) ++next;
@@ -126,12 +130,20 @@ static uint64_t fork_work_bytes(const mfqb_cache& c) {
     return 16 + 16ull * c.rows + 4ull * ((c.pages + 3) / 4 * 4) + 4ull * c.rows * c.width;
 }
 
+constexpr int kForkSmall = 8 * 1024;   // pages and table entries together that find room in shared memory
+
 // One CTA: the new table and the change of the counts are made beside the old ones and put in place at the end, when it is known
-// that the pages suffice.  Counts change by integer atomics, whose order does not matter.
-__global__ void __launch_bounds__(1024) fork_plan_kernel(mfqb_cache c, const int* __restrict__ parents, int* __restrict__ status, ForkWork w) {
+// that the pages suffice.  Counts change by integer atomics, whose order does not matter.  Bound by its chain of dependent trips, not by their
+// size: where both fit they are in shared memory.
+__global__ void __launch_bounds__(1024) fork_plan_kernel(mfqb_cache c, const int* __restrict__ parents, int* __restrict__ status, ForkWork w, bool small) {
     chained_wait();
     __shared__ int warp_sums[32], list[1024], s_len[kCacheRows], s_last[kCacheRows], total;
+    extern __shared__ int s_small[];
     const int r = threadIdx.x, bits = __ffs(c.page) - 1;
+    if (small) {
+        w.delta = s_small;
+        w.table = s_small + c.pages;
+    }
     int parent = -1, len = 0;
     bool bad = false;
     if (r < c.rows) {
@@ -350,40 +362,49 @@ __global__ void __launch_bounds__(32) accept_walk_kernel(mfqb_cache c, const int
     }
 }
 
-// CTA (layer and head, sequence): every slot of the branch is read into registers before the first one is written, since a slot that
-// one node leaves is another one's place.
+// CTA (some layers' heads, sequence): 64 rows at a time, which are the branch's nodes in as many heads as that makes.  Every row is read into
+// registers before the first one is written, since a slot that one node leaves is another one's place.  (A CTA for each head of each
+// layer spent its time on the chain from the count to the rows: 16 branches of 13 nodes in 128 heads 11.0 us with the walk in place of 8.4.)
 __global__ void __launch_bounds__(256) accept_move_kernel(mfqb_cache c, int nodes, const int* __restrict__ count, const int* __restrict__ path,
                                                           const int* __restrict__ lens_out) {
     chained_wait();
-    const int r = blockIdx.y, n = count[r], t = threadIdx.x;
+    const int r = blockIdx.y, n = count[r], t = threadIdx.x, heads = c.layers * c.kv_heads;
     if (n < 2) return;
-    const int layer = blockIdx.x / c.kv_heads, head = blockIdx.x % c.kv_heads;
+    const int each = kTreeNodes / n;   // heads at a time
     const int64_t len = lens_out[r] - n, cap = (int64_t)c.width * c.page;
-    auto slot = [&](int64_t p) -> int64_t {   // offset of a position in 16-byte pieces, -1 where there is no page
-        const int page = p < cap ? c.table[(int64_t)r * c.width + p / c.page] : -1;
-        if ((unsigned)page >= (unsigned)c.pages) return -1;
-        return ((((int64_t)layer * c.pages + page) * c.kv_heads + head) * c.page + (p & (c.page - 1))) * 16;
-    };
-    uint4 kv[4][2];
-    int64_t to[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {   // 16 threads a node, 16 nodes a round
-        const int at = 16 * i + (t >> 4), from = at < n ? path[(int64_t)r * nodes + at] : at;
-        to[i] = -1;
-        if (from == at) continue;
-        const int64_t src = slot(len + from);
-        if (src < 0) continue;
-        to[i] = slot(len + at);
-        kv[i][0] = static_cast<const uint4*>(c.k)[src + (t & 15)];
-        kv[i][1] = static_cast<const uint4*>(c.v)[src + (t & 15)];
+    __shared__ int64_t s_from[kTreeNodes], s_to[kTreeNodes];   // rows of the branch in 16-byte pieces, for head 0 of layer 0; -1: stays
+    if (t < n) {
+        auto slot = [&](int64_t p) -> int64_t {   // -1 where there is no page
+            const int page = p < cap ? c.table[(int64_t)r * c.width + p / c.page] : -1;
+            return (unsigned)page < (unsigned)c.pages ? ((int64_t)page * c.kv_heads * c.page + (p & (c.page - 1))) * 16 : -1;
+        };
+        const int from = path[(int64_t)r * nodes + t];
+        s_to[t] = slot(len + t);
+        s_from[t] = from == t || s_to[t] < 0 ? -1 : slot(len + from);
     }
     __syncthreads();
+    for (int64_t h0 = (int64_t)blockIdx.x * each; h0 < heads; h0 += (int64_t)gridDim.x * each) {
+        uint4 kv[4][2];
+        int64_t to[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (to[i] >= 0) {
-            static_cast<uint4*>(c.k)[to[i] + (t & 15)] = kv[i][0];
-            static_cast<uint4*>(c.v)[to[i] + (t & 15)] = kv[i][1];
+        for (int i = 0; i < 4; ++i) {   // 16 threads a row, 16 rows a round
+            const int x = 16 * i + (t >> 4), h = x / n, node = x - h * n, head = (int)h0 + h;
+            to[i] = -1;
+            if (h >= each || head >= heads || s_from[node] < 0) continue;
+            const int layer = head / c.kv_heads;
+            const int64_t at = ((int64_t)layer * c.pages * c.kv_heads + (head - layer * c.kv_heads)) * c.page * 16 + (t & 15);
+            to[i] = s_to[node] + at;
+            kv[i][0] = static_cast<const uint4*>(c.k)[s_from[node] + at];
+            kv[i][1] = static_cast<const uint4*>(c.v)[s_from[node] + at];
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (to[i] >= 0) {
+                static_cast<uint4*>(c.k)[to[i]] = kv[i][0];
+                static_cast<uint4*>(c.v)[to[i]] = kv[i][1];
+            }
+    }
 }
 
 }  // namespace mfqb
@@ -416,7 +437,9 @@ int mfqb_cache_fork(const mfqb_cache* c, const int32_t* parents, int32_t* status
         if (((uintptr_t)work & 15) || work_bytes < fork_work_bytes(*c))
             fail(MFQB_ERR_ARG, "mfqb_cache_fork: work must be 16-byte aligned and hold %llu bytes, got %llu", (unsigned long long)fork_work_bytes(*c), (unsigned long long)work_bytes);
         const ForkWork w = fork_work(*c, work);
-        launch_chained(fork_plan_kernel, dim3(1), dim3(1024), 0, stream, *c, parents, status, w);
+        const int64_t ints = (int64_t)c->pages + (int64_t)c->rows * c->width;
+        const bool small = ints <= kForkSmall;   // with the kernel's other arrays below the 48 KB that need no attribute
+        launch_chained(fork_plan_kernel, dim3(1), dim3(1024), small ? (size_t)ints * 4 : 0, stream, *c, parents, status, w, small);
         const int64_t most = (int64_t)c->rows * c->layers * c->kv_heads * 2;   // stretches, if every sequence got a copy
         launch_chained(fork_copy_kernel, dim3((unsigned)std::min<int64_t>(most, 148 * 8)), dim3(256), 0, stream, *c, w);
     });
@@ -455,7 +478,9 @@ int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* par
         if (!ids || !parents || !targets || !count || !token || !path || !lens_out) fail(MFQB_ERR_ARG, "mfqb_tree_accept: null argument");
         if ((int64_t)c->layers * c->kv_heads > (1ll << 30)) fail(MFQB_ERR_UNSUPPORTED, "mfqb_tree_accept: too many layers x heads");
         launch_chained(accept_walk_kernel, dim3(c->rows), dim3(32), 0, stream, *c, ids, parents, targets, nodes, count, token, path, lens_out);
-        launch_chained(accept_move_kernel, dim3((unsigned)(c->layers * c->kv_heads), c->rows), dim3(256), 0, stream, *c, nodes,
+        // enough CTAs for the SMs, at least one head each (how many nodes a branch has is known on the device alone)
+        const int per_row = std::min(c->layers * c->kv_heads, std::max(1, 148 * 5 / c->rows));
+        launch_chained(accept_move_kernel, dim3((unsigned)per_row, c->rows), dim3(256), 0, stream, *c, nodes,
                        static_cast<const int*>(count), static_cast<const int*>(path), static_cast<const int*>(lens_out));
     });
 }
