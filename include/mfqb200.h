@@ -397,7 +397,7 @@ typedef struct mfqb_decoder mfqb_decoder;
 typedef struct mfqb_decoder_config {
     int hidden, n_q_heads, n_kv_heads, head_dim; /* head_dim must be 128; hidden = n_q_heads * 128 */
     int ffn, vocab, layers;
-    int max_ctx, max_batch;
+    int max_ctx, max_batch; /* max_ctx 0: no cache of its own, see mfqb_decoder_set_cache */
     float rope_theta, rms_eps;
 } mfqb_decoder_config;
 int mfqb_decoder_create(const mfqb_decoder_config* cfg, int rank, int world, mfqb_comm* comm, int device,
@@ -429,6 +429,29 @@ int mfqb_decoder_read_cache(const mfqb_decoder* d, int layer, int row, int which
                             mfqb_stream_t stream);
 /* The logits of the last mfqb_decoder_step, this rank's vocabulary rows: out [rows, shard rows] float32. */
 int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_stream_t stream);
+/* Keys and values in pages (mfqb_cache, below): the decoder's passes run over this cache instead of its own, a row per sequence; the
+ * memory stays the caller's and must outlive them.  Null: its own cache again.  A decoder that only ever uses pages is created with
+ * max_ctx 0 and allocates no cache.  One rank only.  Allocates what a pass needs and waits for the device.
+ *
+ * mfqb_decoder_step over pages takes batch = rows and advances lens by one; one more token per sequence must have been reserved
+ * (mfqb_cache_extend).  Queries are rounded to bf16 there (the step over the decoder's own cache keeps them in float32).
+ *
+ * mfqb_decoder_verify runs all nodes of a drafted tree per sequence (ids, parents: device int32 [rows][nodes], see mfqb_tree_masks) in one
+ * pass: their keys and values go behind lens (reserve `nodes` tokens), targets [rows][nodes] are the model's own greedy tokens, lens
+ * stays.  mfqb_tree_accept keeps the branch that agrees.  A chain of nodes whose parents are the nodes before them is a piece of a prompt.
+ * rows * nodes <= max_batch.
+ *
+ * mfqb_decoder_beam_step: the sequences are groups of `beams` beams (ids_in [rows]); reserves a token each, runs the model, selects the
+ * best `beams` continuations of every group by scores [rows] + log softmax and forks the cache.  In place: scores, done (int32 [rows]); out:
+ * ids_out (the beams' new tokens), parents_out (the sequences they go on from), status [2]: of mfqb_cache_extend and of mfqb_cache_fork,
+ * to be looked at before the results are used: where one is not 0, pages were missing, and scores, done, lengths and tokens are as
+ * before the step, which can be done again.  A first step from one sequence per group starts the other beams' scores at minus
+ * infinity.  One call with as many beams must come before a stream capture. */
+struct mfqb_cache;
+int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
+int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream);
+int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, float* scores, int32_t* done, int eos, int32_t* ids_out,
+                           int32_t* parents_out, int32_t* status, mfqb_stream_t stream);
 int mfqb_decoder_free(mfqb_decoder* d);
 
 /* ---------------------------------------------------------------------------------

@@ -93,6 +93,9 @@ _SIGNATURES = {
     "mfqb_decoder_layer": (_i, [_vp, _i, _vp, _i, _vp, _vp]),
     "mfqb_decoder_read_cache": (_i, [_vp, _i, _i, _i, _i, _vp, _vp]),
     "mfqb_decoder_read_logits": (_i, [_vp, _i, _vp, _vp]),
+    "mfqb_decoder_set_cache": (_i, [_vp, _P(CacheView)]),
+    "mfqb_decoder_verify": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
+    "mfqb_decoder_beam_step": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
     "mfqb_decoder_free": (_i, [_vp]),
     "mfqb_cache_extend": (_i, [_P(CacheView), _vp, _vp, _vp]),
     "mfqb_cache_fork_work": (_i, [_P(CacheView), _P(_u64)]),

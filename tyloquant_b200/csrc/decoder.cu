@@ -20,7 +20,7 @@
 
 #include <cmath>
 
-#include "cuda_util.h"
+#include "paged.h"
 #include "rows_mma.h"
 #include "tile_tc.h"
 
@@ -28,8 +28,6 @@ namespace mfqb {
 
 const NintDevB& weight_device_layout(const mfqb_weight* w);
 void reserve_fewer_rows(const mfqb_weight* w, int m, bool glu, cudaStream_t s);
-
-constexpr int kHeadDim = 128;
 
 // Every kernel of the step is launched with the programmatic-dependent-launch attribute: it becomes
 // resident while its predecessor still runs, and waits here until that one has completed.
@@ -560,6 +558,40 @@ __global__ void add_one_kernel(int* p, int n) {
     if (i < n) p[i] += 1;
 }
 
+// Between the selection and the fork: the step's token counts where its page could be had; else no sequence moves.
+__global__ void __launch_bounds__(1024) beam_move_kernel(const int* __restrict__ status, const int* __restrict__ parents, int rows, int* __restrict__ lens, int* __restrict__ moves) {
+    dep_wait();
+    const int r = threadIdx.x;
+    if (r >= rows) return;
+    const bool ok = status[0] == 0;
+    moves[r] = ok ? parents[r] : r;
+    if (ok) lens[r] += 1;
+}
+// The chosen beams become the sequences' state: scores, tokens, and done where the beam that goes on was done or has now ended.  Where pages
+// were missing everything is as before the step, which can be done again.
+__global__ void __launch_bounds__(1024) beam_take_kernel(const int* __restrict__ status, const float* __restrict__ best, const int* __restrict__ tokens, int rows, int eos,
+                                                         const int* ids_in, int* __restrict__ lens, float* __restrict__ scores, int* done, int* ids, int* __restrict__ parents) {
+    dep_wait();
+    const int r = threadIdx.x;
+    const bool reserved = status[0] == 0, ok = reserved && status[1] == 0;
+    bool over = true;
+    if (r < rows && ok) {
+        const int p = parents[r];   // -1: fewer candidates than beams
+        over = p < 0 || done[p] || tokens[r] == eos;
+    }
+    __syncthreads();
+    if (r >= rows) return;
+    if (ok) {
+        done[r] = over;
+        scores[r] = best[r];
+        ids[r] = max(tokens[r], 0);
+    } else {
+        ids[r] = ids_in[r];
+        parents[r] = r;
+        if (reserved) lens[r] -= 1;
+    }
+}
+
 }  // namespace mfqb
 
 using namespace mfqb;
@@ -582,6 +614,14 @@ struct mfqb_decoder {
     std::vector<DecoderLayer> layers;
     const mfqb_weight* lm_head = nullptr;
     const void* embedding = nullptr;   // bf16 [vocab, H] on the device, borrowed
+    // Keys and values in pages (mfqb_decoder_set_cache): the step's rows are the nodes of the cache's sequences
+    bool paged = false;
+    mfqb_cache cache{};
+    int nodes = 1;                          // of the forward pass that is being queued
+    const uint64_t* node_masks = nullptr;   // its masks and depths
+    const int32_t* node_depths = nullptr;
+    uint64_t attn_work_bytes = 0;
+    DevBuf q16, freqs, masks, depths, single_masks, single_depths, attn_work, beam_work, beam_scores, beam_tokens, beam_moves, fork_work, one_each;
     DevBuf gamma_final;
     // workspaces
     DevBuf h, h2, xn, qkv, attn, attn_count, inv_freq, rope_table, proj, proj_sum, act, logits, part, best_val, best_idx, part_val, part_idx, gathered, gathered_sum, pos;
@@ -639,27 +679,13 @@ static void mul_mat(const mfqb_weight* w, const void* x, int m, void* y, cudaStr
     if (rc != MFQB_OK) throw Error(rc, mfqb_last_error());
 }
 
-// One transformer block on the residual stream d->h for `rows` sequences; `delta` is the previous
-// block's (already rank-summed) FFN output still to be added, and on return `*delta_out` is this
-// block's: the add is fused into the next RMSNorm.
-static const float* layer_forward(mfqb_decoder* d, int li, int rows, const float* delta, cudaStream_t s) {
-    DecoderLayer& L = d->layers[li];
-    const int H = d->cfg.hidden;
+static void check(int rc) {
+    if (rc != MFQB_OK) throw Error(rc, mfqb_last_error());
+}
+
+// Attention of a step over the decoder's own cache.
+static void attend_own(mfqb_decoder* d, DecoderLayer& L, int rows, cudaStream_t s) {
     const int G = d->cfg.n_q_heads / d->cfg.n_kv_heads;
-    // One row: the residual add and the normalisation run inside the products that consume them (h + delta goes to
-    // h2, h2 + attention output back to h).  Batches: a normalisation kernel, then the batched product.
-    bool fused = rows == 1 && d->fused_norm;
-    if (fused) {
-        const int rc = mfqb_mul_mat_rmsnorm(L.qkv, static_cast<const float*>(d->h.p), delta, static_cast<const float*>(L.gamma_attn.p), d->cfg.rms_eps,
-                                            static_cast<float*>(d->h2.p), d->qkv.p, MFQB_F32, 0, s);
-        if (rc == MFQB_ERR_UNSUPPORTED) d->fused_norm = fused = false;   // weights this form does not take: the two-kernel form from here on
-        else if (rc != MFQB_OK) throw Error(rc, mfqb_last_error());
-    }
-    if (!fused && !norm_mul_mat(d, L.qkv, delta, L.gamma_attn.p, rows, d->qkv.p, MFQB_F32, false, s)) {
-        launch_dep(add_rmsnorm_kernel, dim3(rows), dim3(1024), s, static_cast<float*>(d->h.p), delta, static_cast<const float*>(L.gamma_attn.p),
-                   static_cast<__nv_bfloat16*>(d->xn.p), H, d->cfg.rms_eps);
-        mul_mat(L.qkv, d->xn.p, rows, d->qkv.p, s);
-    }
     const int nsplit = attn_splits(d, rows, d->cfg.max_ctx);
     const dim3 agrid(nsplit, d->nkv, rows);
     auto attn = [&](auto kernel) {
@@ -675,6 +701,36 @@ static const float* layer_forward(mfqb_decoder* d, int li, int rows, const float
         case 8: attn(attn_decode_kernel<8>); break;
         default: fail(MFQB_ERR_UNSUPPORTED, "query heads per KV head must be 1, 2, 4 or 8, got %d", G);
     }
+}
+
+// Rotary embedding, cache write and attention of the nodes over the attached pages.
+static void attend_pages(mfqb_decoder* d, int li, cudaStream_t s) {
+    check(mfqb_cache_write(&d->cache, li, static_cast<const float*>(d->qkv.p), d->nq, d->nodes, d->node_depths, static_cast<const double*>(d->freqs.p), d->q16.p, s));
+    check(mfqb_tree_attention(&d->cache, li, d->q16.p, d->nq, d->nodes, d->node_masks, 0.08838834764831845f, d->attn.p, d->attn_work.p, d->attn_work_bytes, s));
+}
+
+// One transformer block on the residual stream d->h for `rows` sequences; `delta` is the previous
+// block's (already rank-summed) FFN output still to be added, and on return `*delta_out` is this
+// block's: the add is fused into the next RMSNorm.
+static const float* layer_forward(mfqb_decoder* d, int li, int rows, const float* delta, cudaStream_t s) {
+    DecoderLayer& L = d->layers[li];
+    const int H = d->cfg.hidden;
+    // One row: the residual add and the normalisation run inside the products that consume them (h + delta goes to
+    // h2, h2 + attention output back to h).  Batches: a normalisation kernel, then the batched product.
+    bool fused = rows == 1 && d->fused_norm;
+    if (fused) {
+        const int rc = mfqb_mul_mat_rmsnorm(L.qkv, static_cast<const float*>(d->h.p), delta, static_cast<const float*>(L.gamma_attn.p), d->cfg.rms_eps,
+                                            static_cast<float*>(d->h2.p), d->qkv.p, MFQB_F32, 0, s);
+        if (rc == MFQB_ERR_UNSUPPORTED) d->fused_norm = fused = false;   // weights this form does not take: the two-kernel form from here on
+        else if (rc != MFQB_OK) throw Error(rc, mfqb_last_error());
+    }
+    if (!fused && !norm_mul_mat(d, L.qkv, delta, L.gamma_attn.p, rows, d->qkv.p, MFQB_F32, false, s)) {
+        launch_dep(add_rmsnorm_kernel, dim3(rows), dim3(1024), s, static_cast<float*>(d->h.p), delta, static_cast<const float*>(L.gamma_attn.p),
+                   static_cast<__nv_bfloat16*>(d->xn.p), H, d->cfg.rms_eps);
+        mul_mat(L.qkv, d->xn.p, rows, d->qkv.p, s);
+    }
+    if (d->paged) attend_pages(d, li, s);
+    else attend_own(d, L, rows, s);
     // output projection: row-parallel under tensor parallelism
     const float* o_out;
     if (d->world > 1 && rows == 1) {
@@ -705,6 +761,49 @@ static const float* layer_forward(mfqb_decoder* d, int li, int rows, const float
     return rank_sum(d, static_cast<const float*>(d->proj.p), static_cast<float*>(d->proj_sum.p), (size_t)rows * H, s);
 }
 
+static void check_ready(const mfqb_decoder* d, int rows, const char* who) {
+    if (rows < 1 || rows > d->cfg.max_batch) fail(MFQB_ERR_ARG, "%s: %d rows outside [1, %d]", who, rows, d->cfg.max_batch);
+    if (!d->lm_head || !d->embedding) fail(MFQB_ERR_ARG, "%s: head weights are not set", who);
+    for (const auto& L : d->layers)
+        if (!L.qkv) fail(MFQB_ERR_ARG, "%s: a layer has no weights", who);
+    if (!d->paged && d->cfg.max_ctx < 1) fail(MFQB_ERR_ARG, "%s: the decoder has no cache of its own (max_ctx 0) and none is attached", who);
+}
+// The next pass has one node per sequence.
+static void single_nodes(mfqb_decoder* d) {
+    d->nodes = 1;
+    d->node_masks = static_cast<const uint64_t*>(d->single_masks.p);
+    d->node_depths = static_cast<const int32_t*>(d->single_depths.p);
+}
+// Embedding, blocks and head: the logits of `rows` rows.
+static void forward_logits(mfqb_decoder* d, const int32_t* ids, int rows, cudaStream_t s) {
+    const int H = d->cfg.hidden;
+    launch_dep(embed_rows_kernel, dim3(rows), dim3(1024), s, static_cast<const int*>(ids), static_cast<const __nv_bfloat16*>(d->embedding),
+               static_cast<float*>(d->h.p), H, d->cfg.vocab);
+    if (!d->paged) launch_rope_table(d, rows, s);
+    const float* delta = nullptr;
+    for (int li = 0; li < d->cfg.layers; ++li) delta = layer_forward(d, li, rows, delta, s);
+    bool fused_head = rows == 1 && d->fused_norm;
+    if (fused_head) {
+        const int rc = mfqb_mul_mat_rmsnorm(d->lm_head, static_cast<const float*>(d->h.p), delta, static_cast<const float*>(d->gamma_final.p),
+                                            d->cfg.rms_eps, nullptr, d->logits.p, MFQB_F32, 0, s);
+        if (rc == MFQB_ERR_UNSUPPORTED) fused_head = false;
+        else check(rc);
+    }
+    if (!fused_head && !norm_mul_mat(d, d->lm_head, delta, d->gamma_final.p, rows, d->logits.p, MFQB_F32, false, s)) {
+        launch_dep(add_rmsnorm_kernel, dim3(rows), dim3(1024), s, static_cast<float*>(d->h.p), delta, static_cast<const float*>(d->gamma_final.p),
+                   static_cast<__nv_bfloat16*>(d->xn.p), H, d->cfg.rms_eps);
+        mul_mat(d->lm_head, d->xn.p, rows, d->logits.p, s);
+    }
+}
+// And the largest of each row's, this rank's vocabulary: best_val, best_idx.
+static void forward_argmax(mfqb_decoder* d, const int32_t* ids, int rows, cudaStream_t s) {
+    forward_logits(d, ids, rows, s);
+    launch_dep(argmax_slices_kernel, dim3(kArgmaxSlices, rows), dim3(256), s, static_cast<const float*>(d->logits.p), d->vshard,
+               static_cast<float*>(d->part_val.p), static_cast<int*>(d->part_idx.p));
+    launch_dep(argmax_merge_kernel, dim3(rows), dim3(32), s, static_cast<const float*>(d->part_val.p), static_cast<const int*>(d->part_idx.p),
+               d->vbase, static_cast<float*>(d->best_val.p), static_cast<int*>(d->best_idx.p));
+}
+
 extern "C" {
 #pragma GCC visibility push(default)
 
@@ -714,7 +813,7 @@ int mfqb_decoder_create(const mfqb_decoder_config* cfg, int rank, int world, mfq
         if (world < 1 || rank < 0 || rank >= world) fail(MFQB_ERR_ARG, "mfqb_decoder_create: rank %d / world %d", rank, world);
         if (world > 1 && !comm) fail(MFQB_ERR_ARG, "mfqb_decoder_create: tensor parallelism needs a communicator");
         if (cfg->head_dim != kHeadDim) fail(MFQB_ERR_UNSUPPORTED, "head_dim must be %d", kHeadDim);
-        if (cfg->n_q_heads % cfg->n_kv_heads || cfg->n_kv_heads % world || cfg->ffn % world || cfg->layers < 1 || cfg->max_batch < 1 ||
+        if (cfg->n_q_heads % cfg->n_kv_heads || cfg->n_kv_heads % world || cfg->ffn % world || cfg->layers < 1 || cfg->max_batch < 1 || cfg->max_ctx < 0 ||
             cfg->hidden != cfg->n_q_heads * kHeadDim || cfg->hidden % 8 || (cfg->ffn / world) % 16)
             fail(MFQB_ERR_ARG, "mfqb_decoder_create: head counts, FFN width and hidden size must divide over %d ranks (hidden = heads x 128)", world);
         auto d = std::make_unique<mfqb_decoder>();
@@ -755,7 +854,7 @@ int mfqb_decoder_create(const mfqb_decoder_config* cfg, int rank, int world, mfq
             d->inv_freq.alloc(sizeof(freq));
             MFQB_CUDA(cudaMemcpy(d->inv_freq.p, freq, sizeof(freq), cudaMemcpyHostToDevice));
         }
-        {   // resident CTAs per SM of the attention kernel this model uses
+        if (cfg->max_ctx > 0) {   // resident CTAs per SM of the attention kernel this model uses
             int per_sm = 0;
             cudaError_t e = cudaErrorInvalidValue;
             switch (cfg->n_q_heads / cfg->n_kv_heads) {
@@ -780,14 +879,16 @@ int mfqb_decoder_create(const mfqb_decoder_config* cfg, int rank, int world, mfq
             MFQB_CUDA(e);
             d->attn_per_sm = std::max(1, per_sm);
         }
-        d->attn_count.alloc(B * d->nkv * 4);
-        MFQB_CUDA(cudaMemset(d->attn_count.p, 0, B * d->nkv * 4));
+        if (cfg->max_ctx > 0) {
+            d->attn_count.alloc(B * d->nkv * 4);
+            MFQB_CUDA(cudaMemset(d->attn_count.p, 0, B * d->nkv * 4));
+            d->part.alloc(B * d->nq * kMaxSplits * kPartStride * 4);
+        }
         d->attn.alloc(B * d->nq * kHeadDim * 2);
         d->proj.alloc(B * H * 4);
         d->proj_sum.alloc(B * H * 4);
         d->act.alloc(B * d->f * 2);
         d->logits.alloc(B * std::max(d->vshard, 1) * 4);
-        d->part.alloc(B * d->nq * kMaxSplits * kPartStride * 4);
         d->rope_table.alloc(B * 64 * sizeof(float2));
         d->best_val.alloc(B * 4);
         d->part_val.alloc(B * kArgmaxSlices * 4);
@@ -860,34 +961,12 @@ int mfqb_decoder_fill_cache(mfqb_decoder* d, int ctx_len, unsigned seed, mfqb_st
 int mfqb_decoder_step(mfqb_decoder* d, const int32_t* ids_in, int batch, int32_t* ids_out, mfqb_stream_t stream) {
     return guarded([&] {
         if (!d || !ids_in || !ids_out) fail(MFQB_ERR_ARG, "mfqb_decoder_step: null argument");
-        if (batch < 1 || batch > d->cfg.max_batch) fail(MFQB_ERR_ARG, "mfqb_decoder_step: batch %d outside [1, %d]", batch, d->cfg.max_batch);
-        if (!d->lm_head || !d->embedding) fail(MFQB_ERR_ARG, "mfqb_decoder_step: head weights are not set");
-        for (const auto& L : d->layers)
-            if (!L.qkv) fail(MFQB_ERR_ARG, "mfqb_decoder_step: a layer has no weights");
+        check_ready(d, batch, "mfqb_decoder_step");
+        if (d->paged && batch != d->cache.rows) fail(MFQB_ERR_ARG, "mfqb_decoder_step: the cache has %d sequences, got a batch of %d", d->cache.rows, batch);
         DeviceGuard guard(d->device);
         cudaStream_t s = stream;
-        const int H = d->cfg.hidden;
-        launch_dep(embed_rows_kernel, dim3(batch), dim3(1024), s, static_cast<const int*>(ids_in), static_cast<const __nv_bfloat16*>(d->embedding),
-                   static_cast<float*>(d->h.p), H, d->cfg.vocab);
-        launch_rope_table(d, batch, s);
-        const float* delta = nullptr;
-        for (int li = 0; li < d->cfg.layers; ++li) delta = layer_forward(d, li, batch, delta, s);
-        bool fused_head = batch == 1 && d->fused_norm;
-        if (fused_head) {
-            const int rc = mfqb_mul_mat_rmsnorm(d->lm_head, static_cast<const float*>(d->h.p), delta, static_cast<const float*>(d->gamma_final.p),
-                                                d->cfg.rms_eps, nullptr, d->logits.p, MFQB_F32, 0, s);
-            if (rc == MFQB_ERR_UNSUPPORTED) fused_head = false;
-            else if (rc != MFQB_OK) throw Error(rc, mfqb_last_error());
-        }
-        if (!fused_head && !norm_mul_mat(d, d->lm_head, delta, d->gamma_final.p, batch, d->logits.p, MFQB_F32, false, s)) {
-            launch_dep(add_rmsnorm_kernel, dim3(batch), dim3(1024), s, static_cast<float*>(d->h.p), delta, static_cast<const float*>(d->gamma_final.p),
-                       static_cast<__nv_bfloat16*>(d->xn.p), H, d->cfg.rms_eps);
-            mul_mat(d->lm_head, d->xn.p, batch, d->logits.p, s);
-        }
-        launch_dep(argmax_slices_kernel, dim3(kArgmaxSlices, batch), dim3(256), s, static_cast<const float*>(d->logits.p), d->vshard,
-                   static_cast<float*>(d->part_val.p), static_cast<int*>(d->part_idx.p));
-        launch_dep(argmax_merge_kernel, dim3(batch), dim3(32), s, static_cast<const float*>(d->part_val.p), static_cast<const int*>(d->part_idx.p),
-                   d->vbase, static_cast<float*>(d->best_val.p), static_cast<int*>(d->best_idx.p));
+        single_nodes(d);
+        forward_argmax(d, ids_in, batch, s);
         if (d->world == 1) {
             MFQB_CUDA(cudaMemcpyAsync(ids_out, d->best_idx.p, (size_t)batch * 4, cudaMemcpyDeviceToDevice, s));
         } else {
@@ -897,7 +976,109 @@ int mfqb_decoder_step(mfqb_decoder* d, const int32_t* ids_in, int batch, int32_t
             const float* g = rank_sum(d, static_cast<const float*>(d->gathered.p), static_cast<float*>(d->gathered_sum.p), (size_t)n, s);
             launch_dep(argmax_pick_kernel, dim3((batch + 127) / 128), dim3(128), s, g, d->world, batch, static_cast<int*>(ids_out));
         }
-        launch_dep(add_one_kernel, dim3((batch + 127) / 128), dim3(128), s, static_cast<int*>(d->pos.p), batch);
+        launch_dep(add_one_kernel, dim3((batch + 127) / 128), dim3(128), s, d->paged ? d->cache.lens : static_cast<int*>(d->pos.p), batch);
+    });
+}
+
+int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
+    return guarded([&] {
+        if (!d) fail(MFQB_ERR_ARG, "mfqb_decoder_set_cache: null decoder");
+        if (!cache) {
+            d->paged = false;
+            return;
+        }
+        check_cache(cache, "mfqb_decoder_set_cache");
+        if (d->world > 1) fail(MFQB_ERR_UNSUPPORTED, "mfqb_decoder_set_cache: pages are not built for tensor parallelism");
+        if (cache->layers != d->cfg.layers || cache->kv_heads != d->nkv)
+            fail(MFQB_ERR_ARG, "mfqb_decoder_set_cache: the decoder has %d layers of %d KV heads, the cache %d of %d", d->cfg.layers, d->nkv, cache->layers, cache->kv_heads);
+        if (cache->rows > d->cfg.max_batch) fail(MFQB_ERR_ARG, "mfqb_decoder_set_cache: %d sequences, the decoder takes %d rows", cache->rows, d->cfg.max_batch);
+        DeviceGuard guard(d->device);
+        for (const void* p : {cache->k, cache->v, (void*)cache->table, (void*)cache->lens, (void*)cache->refs}) {
+            cudaPointerAttributes at{};
+            MFQB_CUDA(cudaPointerGetAttributes(&at, p));
+            if (at.type != cudaMemoryTypeDevice || at.device != d->device) fail(MFQB_ERR_ARG, "mfqb_decoder_set_cache: the cache must be memory of device %d", d->device);
+        }
+        // Everything that a pass over this cache needs, so that none of its calls allocates.
+        const size_t B = d->cfg.max_batch, rows = cache->rows;
+        uint64_t most = 0, bytes = 0;
+        for (int nodes = 1; nodes <= kTreeNodes && nodes * rows <= B && (int64_t)nodes <= (int64_t)cache->width * cache->page; ++nodes) {
+            check(mfqb_tree_attention_work(cache, d->nq, nodes, &bytes));
+            most = std::max(most, bytes);
+        }
+        uint64_t fork_bytes = 0;
+        check(mfqb_cache_fork_work(cache, &fork_bytes));
+        double freqs[kHeadDim / 2];
+        for (int i = 0; i < kHeadDim / 2; ++i) freqs[i] = std::pow((double)d->cfg.rope_theta, -2.0 * i / kHeadDim);
+        std::vector<uint64_t> one(rows, 1);
+        std::vector<int32_t> zero(rows, 0), ones(rows, 1);
+        MFQB_CUDA(cudaDeviceSynchronize());   // passes over the cache before may still use the buffers
+        d->paged = false;
+        d->q16.alloc(B * d->nq * kHeadDim * 2);
+        d->masks.alloc(B * 8);
+        d->depths.alloc(B * 4);
+        d->attn_work.alloc(most);
+        d->attn_work_bytes = most;
+        d->fork_work.alloc(fork_bytes);
+        d->beam_scores.alloc(rows * 4);
+        d->beam_tokens.alloc(rows * 4);
+        d->beam_moves.alloc(rows * 4);
+        d->beam_work.release();
+        d->freqs.upload(freqs, sizeof(freqs));
+        d->single_masks.upload(one.data(), rows * 8);
+        d->single_depths.upload(zero.data(), rows * 4);
+        d->one_each.upload(ones.data(), rows * 4);
+        d->cache = *cache;
+        d->paged = true;
+    });
+}
+
+int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream) {
+    return guarded([&] {
+        if (!d || !ids || !parents || !targets) fail(MFQB_ERR_ARG, "mfqb_decoder_verify: null argument");
+        if (!d->paged) fail(MFQB_ERR_ARG, "mfqb_decoder_verify: needs a cache (mfqb_decoder_set_cache)");
+        check_nodes(&d->cache, nodes, "mfqb_decoder_verify");
+        const int rows = d->cache.rows * nodes;
+        check_ready(d, rows, "mfqb_decoder_verify");
+        DeviceGuard guard(d->device);
+        check(mfqb_tree_masks(parents, d->cache.rows, nodes, static_cast<uint64_t*>(d->masks.p), static_cast<int32_t*>(d->depths.p), stream));
+        d->nodes = nodes;
+        d->node_masks = static_cast<const uint64_t*>(d->masks.p);
+        d->node_depths = static_cast<const int32_t*>(d->depths.p);
+        forward_argmax(d, ids, rows, stream);
+        MFQB_CUDA(cudaMemcpyAsync(targets, d->best_idx.p, (size_t)rows * 4, cudaMemcpyDeviceToDevice, stream));
+    });
+}
+
+int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, float* scores, int32_t* done, int eos, int32_t* ids_out, int32_t* parents_out,
+                           int32_t* status, mfqb_stream_t stream) {
+    return guarded([&] {
+        if (!d || !ids_in || !scores || !done || !ids_out || !parents_out || !status) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: null argument");
+        if (!d->paged) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: needs a cache (mfqb_decoder_set_cache)");
+        const int rows = d->cache.rows;
+        if (beams < 1 || rows % beams) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: %d sequences do not make groups of %d beams", rows, beams);
+        check_ready(d, rows, "mfqb_decoder_beam_step");
+        DeviceGuard guard(d->device);
+        cudaStream_t s = stream;
+        uint64_t bytes = 0;
+        check(mfqb_beam_select_work(rows / beams, beams, d->vshard, beams, &bytes));
+        if (d->beam_work.bytes < bytes) {
+            cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+            MFQB_CUDA(cudaStreamIsCapturing(s, &capturing));
+            if (capturing != cudaStreamCaptureStatusNone) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: one call with this many beams must come before a stream capture");
+            MFQB_CUDA(cudaStreamSynchronize(s));
+            d->beam_work.alloc(bytes);
+        }
+        check(mfqb_cache_extend(&d->cache, static_cast<const int32_t*>(d->one_each.p), status, s));
+        single_nodes(d);
+        forward_logits(d, ids_in, rows, s);
+        check(mfqb_beam_select(static_cast<const float*>(d->logits.p), rows / beams, beams, d->vshard, scores, done, eos, beams, static_cast<float*>(d->beam_scores.p),
+                               parents_out, static_cast<int32_t*>(d->beam_tokens.p), d->beam_work.p, d->beam_work.bytes, s));
+        launch_dep(beam_move_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const int*>(parents_out), rows, d->cache.lens,
+                   static_cast<int*>(d->beam_moves.p));
+        check(mfqb_cache_fork(&d->cache, static_cast<const int32_t*>(d->beam_moves.p), status + 1, d->fork_work.p, d->fork_work.bytes, s));
+        launch_dep(beam_take_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const float*>(d->beam_scores.p),
+                   static_cast<const int*>(d->beam_tokens.p), rows, eos, static_cast<const int*>(ids_in), d->cache.lens, scores, static_cast<int*>(done),
+                   static_cast<int*>(ids_out), static_cast<int*>(parents_out));
     });
 }
 
@@ -909,8 +1090,11 @@ int mfqb_decoder_layer(mfqb_decoder* d, int layer, const float* h_in, int rows, 
             fail(MFQB_ERR_ARG, "mfqb_decoder_layer: bad argument");
         DeviceGuard guard(d->device);
         const size_t bytes = (size_t)rows * d->cfg.hidden * 4;
+        if (d->paged && rows != d->cache.rows) fail(MFQB_ERR_ARG, "mfqb_decoder_layer: the cache has %d sequences, got %d rows", d->cache.rows, rows);
+        if (!d->paged && d->cfg.max_ctx < 1) fail(MFQB_ERR_ARG, "mfqb_decoder_layer: the decoder has no cache of its own (max_ctx 0) and none is attached");
         MFQB_CUDA(cudaMemcpyAsync(d->h.p, h_in, bytes, cudaMemcpyDeviceToDevice, stream));
-        launch_rope_table(d, rows, stream);
+        single_nodes(d);
+        if (!d->paged) launch_rope_table(d, rows, stream);
         const float* delta = layer_forward(d, layer, rows, nullptr, stream);
         // fold the FFN output in with a norm whose bf16 output is discarded
         launch_dep(add_rmsnorm_kernel, dim3(rows), dim3(1024), stream, static_cast<float*>(d->h.p), delta, static_cast<const float*>(d->gamma_final.p),

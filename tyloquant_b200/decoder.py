@@ -21,6 +21,7 @@ class Decoder:
         self.rank, self.world, self.device = rank, world, device
         self._comm = comm
         self._keep = []   # the weights are borrowed by the native object: keep them alive here
+        self._cache = None
         self._h = C.c_void_p()
         check(lib.mfqb_decoder_create(C.byref(self.cfg), rank, world, comm._h if comm is not None else None, device, C.byref(self._h)))
 
@@ -73,6 +74,46 @@ class Decoder:
         out = torch.empty((rows, n.value), dtype=torch.float32, device=f"cuda:{self.device}")
         check(lib.mfqb_decoder_read_logits(self._h, rows, out.data_ptr(), _stream_ptr(self.device)))
         return out
+
+    def set_cache(self, cache) -> None:
+        """Runs over a :class:`PagedCache` from here on (``None``: over the decoder's own cache again); a row per sequence.  ``max_ctx=0`` at
+        creation leaves the decoder without a cache of its own."""
+        check(lib.mfqb_decoder_set_cache(self._h, None if cache is None else C.byref(cache._view)))
+        self._cache = cache   # borrowed by the native object
+
+    def _rows(self, t, shape, dtype, what):
+        from .cache import _need
+        if self._cache is None:
+            raise ValueError("the decoder runs over its own cache: set_cache first")
+        return _need(t, dtype, shape, self.device, what)
+
+    def verify(self, ids, parents):
+        """The drafted trees of all sequences in one pass (``ids``, ``parents`` int32 [rows, nodes], see ``tree_masks``): returns the model's own
+        greedy token at every node.  Reserve ``nodes`` tokens first (``cache.extend``); ``cache.accept`` keeps the branch that agrees."""
+        torch = _torch()
+        if ids.dim() != 2:
+            raise ValueError("ids must be an int32 tensor [rows, nodes]")
+        rows = self._cache.rows if self._cache is not None else 0
+        shape = (rows, ids.shape[1])
+        i, p = self._rows(ids, shape, torch.int32, "ids"), self._rows(parents, shape, torch.int32, "parents")
+        out = torch.empty_like(i)
+        check(lib.mfqb_decoder_verify(self._h, i.data_ptr(), p.data_ptr(), ids.shape[1], out.data_ptr(), _stream_ptr(self.device)))
+        return out
+
+    def beam_step(self, ids, scores, done, beams: int, eos: int):
+        """One step of beam search over groups of ``beams`` sequences: ``ids`` int32 [rows], ``scores`` float32 and ``done`` int32 [rows], which are
+        changed in place, like the cache.  Returns (tokens [rows], the sequences they go on from [rows], status [2]: of the
+        cache's extend and fork)."""
+        torch = _torch()
+        rows = self._cache.rows if self._cache is not None else 0
+        i = self._rows(ids, (rows,), torch.int32, "ids")
+        for t, dtype, what in ((scores, torch.float32, "scores"), (done, torch.int32, "done")):
+            if self._rows(t, (rows,), dtype, what) is not t:
+                raise ValueError(f"{what} must be contiguous")
+        tokens, parents, status = torch.empty_like(i), torch.empty_like(i), i.new_empty(2)
+        check(lib.mfqb_decoder_beam_step(self._h, i.data_ptr(), beams, scores.data_ptr(), done.data_ptr(), eos, tokens.data_ptr(), parents.data_ptr(),
+                                         status.data_ptr(), _stream_ptr(self.device)))
+        return tokens, parents, status
 
     def free(self) -> None:
         if self._h:
