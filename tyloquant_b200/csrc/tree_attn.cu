@@ -30,6 +30,7 @@ constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
 constexpr int tree_ctas(int ns) { return ns == 2 ? kTreeSms : 2 * kTreeSms; }
 constexpr int tree_ring(int ns) { return ns == 2 ? 5 : 2; }   // tiles
 constexpr int tree_threads(int ns) { return 64 + 128 * ns; }
+constexpr int kTreeWhole = 256;                       // positions
 constexpr int kTreeStart = 2;                         // what starting and ending a stretch takes, in tiles
 
 struct TreeArgs {
@@ -44,6 +45,7 @@ struct TreeArgs {
     int64_t* before;              // [rows + 1]: units of one item of each sequence before a sequence; their sum
     int* error;
     int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of 128 rows a stream; tile_rows: rows of a part, at most that
+    bool whole;                   // an item is one unit
     unsigned group_inv;           // ceil(65536 / group): row / group = row * group_inv >> 16 for rows below 1024, groups up to 16
     float scale_log2;
     __device__ __forceinline__ int node_of(int row_of_q) const { return (int)((unsigned)row_of_q * group_inv >> 16); }
@@ -57,7 +59,7 @@ struct TreeArgs {
 // Tiles of sequence r (at least one: a sequence has a node), its length and end.
 struct TreeSeq {
     int len, end, tiles;
-    __device__ __forceinline__ int units() const { return tiles + kTreeStart; }
+    int units;   // of an item: its tiles and its start, or 1 where items are not split (TreeArgs::whole)
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
     const int cap = a.width * a.page;   // at most 2^30
@@ -65,6 +67,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
     s.len = min(max(__ldcg(a.lens + r), 0), cap);
     s.end = min(s.len + a.nodes, cap);
     s.tiles = (s.end + kTile - 1) / kTile;
+    s.units = a.whole ? 1 : s.tiles + kTreeStart;
     return s;
 }
 struct TreeShared {
@@ -92,15 +95,15 @@ struct TreeWalk {
         left = sh.last - sh.first;
         if (left > 0) {
             seq = tree_seq(a, r);
-            item = (int)(sh.item_off / seq.units());
-            const int u0 = (int)(sh.item_off % seq.units());
+            item = (int)(sh.item_off / seq.units);
+            const int u0 = (int)(sh.item_off % seq.units);
             left += u0;   // as if the item's start were the CTA's too
-            stretch(max(u0 - kTreeStart, 0));
+            stretch(a, max(u0 - kTreeStart, 0));
         }
     }
     __device__ __forceinline__ void next(const TreeArgs& a) {
-        left -= seq.units();
-        if (left <= kTreeStart) {
+        left -= seq.units;
+        if (left <= (a.whole ? 0 : kTreeStart)) {
             left = 0;
             return;
         }
@@ -108,13 +111,13 @@ struct TreeWalk {
             item = 0;
             seq = tree_seq(a, ++r);
         }
-        stretch(0);
+        stretch(a, 0);
     }
 
 private:
-    __device__ __forceinline__ void stretch(int first) {
+    __device__ __forceinline__ void stretch(const TreeArgs& a, int first) {
         t0 = first;
-        t1 = (int)min((int64_t)seq.tiles, left - kTreeStart);
+        t1 = a.whole ? seq.tiles : (int)min((int64_t)seq.tiles, left - kTreeStart);
         if (t1 <= t0) left = 0;   // nothing but units of the start
     }
 };
@@ -226,7 +229,7 @@ __device__ __noinline__ void clean_values(TreeShared& sh, unsigned char* tile, T
     unsigned char* piece = tile + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;
     const int r0 = 2 * quarter + (lane >> 4);
     if (good != 0xFFu || (end & 15))
-        for (int r = r0; r < ((end + 15) & ~15); r += 8)
+        for (int r = r0 + (good == 0xFFu ? end & ~15 : 0); r < ((end + 15) & ~15); r += 8)
             if (r >= end || !((good >> (r >> 4)) & 1u)) *reinterpret_cast<uint4*>(piece + r * 128) = make_uint4(0u, 0u, 0u, 0u);
     for (int r = first + r0; r < end; r += 8) {
         if (!((good >> (r >> 4)) & 1u)) continue;
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
         int64_t mine = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            units_of[j] = kEach * tid + j < a.rows ? tree_seq(a, kEach * tid + j).units() : 0;
+            units_of[j] = kEach * tid + j < a.rows ? tree_seq(a, kEach * tid + j).units : 0;
             mine += units_of[j];
         }
         int64_t upto = mine;
@@ -662,7 +665,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             const float2 sum = joint(row_l);
             // What this copy's values are multiplied by: its maximum against the joint one, the sum where the row is complete.
             const float x = sh.ml[st][lane_l].x, e = x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
-            const float f = !complete ? e : sum.y == 0.f ? 0.f : e / sum.y;
+            const float f = !complete ? e : sum.y == 0.f ? 0.f : __fdividef(e, sum.y);
             const int64_t slot = ((int64_t)blockIdx.x * 2 + (stretch > 0)) * a.tile_rows + st * kTile;
             const int rows_here = min(kSpan, m_rows - tile0);   // may be 0 or less (NS = 2)
             auto take = [&](int c, uint32_t* o) {   // 32 columns of this thread's row; zero where it saw nothing (its O may be NaN then)
@@ -719,13 +722,17 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                     if (!ok) break;
                     if (busy) {
 #pragma unroll 1
-                        for (int c = 0; c < wide; c += 32) {
-                            uint32_t o[32];
-                            take(c0 + c, o);
+                        for (int c = 0; c < wide; c += 64) {
+                            uint32_t o[64];
+                            tmem_ld32(col_o + c0 + c, o);
+                            tmem_ld32(col_o + c0 + c + 32, o + 32);
+                            tmem_wait_ld(o, o + 32);
                             if (live)
 #pragma unroll
-                                for (int k = 0; k < 32; k += 4)
-                                    *place(row_l, copy, (c + k) >> 2) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+                                for (int k = 0; k < 64; k += 4)
+                                    *place(row_l, copy, (c + k) >> 2) = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                                               : make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f,
+                                                                                             __uint_as_float(o[k + 2]) * f, __uint_as_float(o[k + 3]) * f);
                             __syncwarp();
                         }
                     }
@@ -780,7 +787,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     const TreeSeq seq = tree_seq(a, r);
     const int span = streams * kTile, rt = row / span, row_l = row - rt * span;
     const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
-    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units(), c0 = (s0 + kTreeStart) / quota, c1 = (s0 + seq.units() - 1) / quota;
+    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units, c0 = (s0 + kTreeStart) / quota, c1 = (s0 + seq.units - 1) / quota;
     if (c0 == c1) return;
     auto slot = [&](int64_t c) { return (c * 2 + (s0 > c * quota ? 1 : 0)) * a.tile_rows + row_l; };
     float m = -INFINITY;
@@ -870,7 +877,7 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.group = q_heads / c.kv_heads;
     a.nodes = nodes;
     a.group_inv = (65536u + a.group - 1) / a.group;
-    const int ns = tree_streams(c, q_heads, nodes), m_rows = nodes * a.group, ctas = tree_ctas(ns);
+    const int ns = tree_streams(c, q_heads, nodes), m_rows = nodes * a.group;
     a.row_tiles = (m_rows + ns * kTile - 1) / (ns * kTile);
     a.tile_rows = std::min(ns * kTile, m_rows);
     a.part = static_cast<float*>(work);
@@ -886,7 +893,12 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
         for (auto* k : {tree_attn_kernel<1, 1>, tree_attn_kernel<1, 2>, tree_attn_kernel<1, 4>})
             MFQB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(1)));
     });
+    // Tables of up to kTreeWhole positions: an item is not split, and there is nothing to merge (one token at context 100: 8.2 us a pass in place of 9.4).
+    a.whole = (int64_t)c.width * c.page <= kTreeWhole;
+    const int64_t most = (int64_t)c.rows * c.kv_heads * a.row_tiles * (a.whole ? 1 : ((int64_t)c.width * c.page + kTile - 1) / kTile);   // tiles there can be
+    const int ctas = (int)std::min<int64_t>(tree_ctas(ns), most);
     launch_chained(kernel, dim3(ctas), dim3(tree_threads(ns)), tree_smem(ns), s, a, kmap, vmap);
+    if (a.whole) return;
     const int64_t rows = (int64_t)c.rows * c.kv_heads * m_rows;   // at most 1024 x 1024 x 1024
     launch_chained(tree_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a, ctas, ns, (int)rows);
 }
