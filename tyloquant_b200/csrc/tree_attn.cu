@@ -42,7 +42,7 @@ struct TreeArgs {
     __nv_bfloat16* out;
     float* part;                  // [CTA][first, last][rows of a tile][128], then their (maximum, sum)
     float2* part_ml;
-    int64_t* before;              // [rows + 1]: units of one item of each sequence before a sequence; their sum
+    int64_t* before;              // [rows + 1]: units of one item of each sequence before a sequence; the units of a CTA
     int* error;
     int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of 128 rows a stream; tile_rows: rows of a part, at most that
     bool whole;                   // an item is one unit
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             }
             begin = end;
         }
-        if (blockIdx.x == 0 && tid == 0) a.before[a.rows] = total;
+        if (blockIdx.x == 0 && tid == 0) a.before[a.rows] = quota;
         __syncthreads();
     }
     TreeWalk w;
@@ -777,23 +777,32 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
     }
 }
 
-// Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context.
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int ctas, int streams, int rows) {
+// Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context, eight loads at a
+// time, with a running maximum (a pass for the maximum before it was one more trip to memory of the four that the kernel consists of).
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int streams, int rows) {
     chained_wait();
     const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5), m_rows = a.nodes * a.group, per_seq = a.kv_heads * m_rows;
+    // What all rows ask for comes through one thread a CTA and sequence: a trip of every warp to the same few lines of the L2 cache was 11 of 24 us
+    // for 700 CTAs.  (A line of the L1 cache could be that of the call before.)
+    __shared__ int64_t s_before[8], s_quota;
+    __shared__ TreeSeq s_seq[8];
+    const int r0 = blockIdx.x * 8 / per_seq, r = min(warp, rows - 1) / per_seq;
+    if (threadIdx.x < 8 && r0 + (int)threadIdx.x < a.rows && (int64_t)(r0 + threadIdx.x) * per_seq < (int64_t)blockIdx.x * 8 + 8) {
+        s_before[threadIdx.x] = __ldcg(a.before + r0 + threadIdx.x);
+        s_seq[threadIdx.x] = tree_seq(a, r0 + threadIdx.x);
+    }
+    if (threadIdx.x == 32) s_quota = __ldcg(a.before + a.rows);
+    __syncthreads();
     if (warp >= rows) return;
-    const int r = warp / per_seq, local = warp - r * per_seq, kvh = local / m_rows, row = local - kvh * m_rows;
-    const int64_t before = __ldcg(a.before + r), total = __ldcg(a.before + a.rows);
-    const TreeSeq seq = tree_seq(a, r);
+    const int local = warp - r * per_seq, kvh = local / m_rows, row = local - kvh * m_rows;
+    const int64_t before = s_before[r - r0], quota = s_quota;
+    const TreeSeq seq = s_seq[r - r0];
     const int span = streams * kTile, rt = row / span, row_l = row - rt * span;
-    const int64_t items = (int64_t)a.kv_heads * a.row_tiles, quota = (total * items + ctas - 1) / ctas;
+    const int64_t items = (int64_t)a.kv_heads * a.row_tiles;
     const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units, c0 = (s0 + kTreeStart) / quota, c1 = (s0 + seq.units - 1) / quota;
     if (c0 == c1) return;
     auto slot = [&](int64_t c) { return (c * 2 + (s0 > c * quota ? 1 : 0)) * a.tile_rows + row_l; };
-    float m = -INFINITY;
-    for (int64_t c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, __ldcg(&a.part_ml[slot(c)]).x);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f;
+    float m = -INFINITY, l = 0.f, none = 0.f;   // none: of parts without a maximum, which count only among themselves
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int64_t c = c0; c <= c1; c += 8) {
         float2 ml[8];
@@ -805,14 +814,27 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
                 ml[u] = __ldcg(&a.part_ml[at]);
                 o[u] = __ldcg(reinterpret_cast<const float4*>(a.part + at * kHeadDim) + lane);
             }
+        float high = m;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (c + u <= c1 && (ml[u].x > -INFINITY || m == -INFINITY)) {
-                const float f = m == -INFINITY ? 1.f : exp2_approx(ml[u].x - m);
+            if (c + u <= c1) high = fmaxf(high, ml[u].x);
+        const float corr = m == -INFINITY ? 0.f : exp2_approx(m - high);
+        m = high;
+        l *= corr;
+        acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (c + u <= c1) {
+                if (ml[u].x == -INFINITY) {
+                    none += ml[u].y;
+                    continue;
+                }
+                const float f = exp2_approx(ml[u].x - m);
                 l += ml[u].y * f;
                 acc.x += o[u].x * f; acc.y += o[u].y * f; acc.z += o[u].z * f; acc.w += o[u].w * f;
             }
     }
+    if (m == -INFINITY) l = none;
     const float inv = 1.f / l;
     if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
     else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
@@ -900,7 +922,7 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     launch_chained(kernel, dim3(ctas), dim3(tree_threads(ns)), tree_smem(ns), s, a, kmap, vmap);
     if (a.whole) return;
     const int64_t rows = (int64_t)c.rows * c.kv_heads * m_rows;   // at most 1024 x 1024 x 1024
-    launch_chained(tree_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a, ctas, ns, (int)rows);
+    launch_chained(tree_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a, ns, (int)rows);
 }
 
 }  // namespace mfqb
