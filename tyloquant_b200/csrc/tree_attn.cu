@@ -56,6 +56,11 @@ struct TreeArgs {
     }
 };
 
+// a / b of numbers that are not negative; mostly they fit 32 bits, and a 64-bit division is some hundred instructions.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // Tiles of sequence r (at least one: a sequence has a node), its length and end.
 struct TreeSeq {
     int len, end, tiles;
@@ -95,8 +100,8 @@ struct TreeWalk {
         left = sh.last - sh.first;
         if (left > 0) {
             seq = tree_seq(a, r);
-            item = (int)(sh.item_off / seq.units);
-            const int u0 = (int)(sh.item_off % seq.units);
+            item = (int)quotient(sh.item_off, seq.units);
+            const int u0 = (int)(sh.item_off - (int64_t)item * seq.units);
             left += u0;   // as if the item's start were the CTA's too
             stretch(a, max(u0 - kTreeStart, 0));
         }
@@ -326,12 +331,12 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             if (w < warp) upto += sh.scan[w];
             total += sh.scan[w];
         }
-        const int64_t items = (int64_t)a.kv_heads * a.row_tiles, units = total * items, quota = (units + gridDim.x - 1) / gridDim.x;
+        const int64_t items = (int64_t)a.kv_heads * a.row_tiles, units = total * items, quota = quotient(units + gridDim.x - 1, gridDim.x);
         const int64_t first = (int64_t)blockIdx.x * quota, last = min(units, first + quota);
         int64_t begin = (upto - mine) * items;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            if (blockIdx.x == 0 && kEach * tid + j < a.rows) a.before[kEach * tid + j] = begin / items;   // for tree_merge_kernel
+            if (blockIdx.x == 0 && kEach * tid + j < a.rows) a.before[kEach * tid + j] = quotient(begin, items);   // for tree_merge_kernel
             const int64_t end = begin + units_of[j] * items;
             if (first < last && begin <= first && first < end) {
                 sh.row0 = kEach * tid + j;
@@ -799,32 +804,34 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     const TreeSeq seq = s_seq[r - r0];
     const int span = streams * kTile, rt = row / span, row_l = row - rt * span;
     const int64_t items = (int64_t)a.kv_heads * a.row_tiles;
-    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units, c0 = (s0 + kTreeStart) / quota, c1 = (s0 + seq.units - 1) / quota;
+    const int64_t s0 = before * items + (int64_t)(kvh * a.row_tiles + rt) * seq.units, c0 = quotient(s0 + kTreeStart, quota), c1 = quotient(s0 + seq.units - 1, quota);
     if (c0 == c1) return;
-    auto slot = [&](int64_t c) { return (c * 2 + (s0 > c * quota ? 1 : 0)) * a.tile_rows + row_l; };
+    // The item is its first CTA's second stretch unless it begins that CTA, and every later CTA's first.  At most 296 CTAs with two stretches of 256 rows.
+    const int first = (int)c0, last = (int)c1, shift = s0 > c0 * quota ? 1 : 0;
+    auto slot = [&](int c) { return (c * 2 + (c == first ? shift : 0)) * a.tile_rows + row_l; };
     float m = -INFINITY, l = 0.f, none = 0.f;   // none: of parts without a maximum, which count only among themselves
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t c = c0; c <= c1; c += 8) {
+    for (int c = first; c <= last; c += 8) {
         float2 ml[8];
         float4 o[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (c + u <= c1) {
-                const int64_t at = slot(c + u);
+            if (c + u <= last) {
+                const int at = slot(c + u);
                 ml[u] = __ldcg(&a.part_ml[at]);
                 o[u] = __ldcg(reinterpret_cast<const float4*>(a.part + at * kHeadDim) + lane);
             }
         float high = m;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (c + u <= c1) high = fmaxf(high, ml[u].x);
+            if (c + u <= last) high = fmaxf(high, ml[u].x);
         const float corr = m == -INFINITY ? 0.f : exp2_approx(m - high);
         m = high;
         l *= corr;
         acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (c + u <= c1) {
+            if (c + u <= last) {
                 if (ml[u].x == -INFINITY) {
                     none += ml[u].y;
                     continue;
