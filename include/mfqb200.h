@@ -431,7 +431,8 @@ int mfqb_decoder_read_cache(const mfqb_decoder* d, int layer, int row, int which
 int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_stream_t stream);
 /* Keys and values in pages (mfqb_cache, below): the decoder's passes run over this cache instead of its own, a row per sequence; the
  * memory stays the caller's and must outlive them.  Null: its own cache again.  A decoder that only ever uses pages is created with
- * max_ctx 0 and allocates no cache.  One rank only.  Allocates what a pass needs and waits for the device.
+ * max_ctx 0 and allocates no cache.  One rank only.  Allocates what a pass needs (not during a stream capture); graphs captured over
+ * another cache before stay valid.
  *
  * mfqb_decoder_step over pages takes batch = rows and advances lens by one; one more token per sequence must have been reserved
  * (mfqb_cache_extend).  Queries are rounded to bf16 there (the step over the decoder's own cache keeps them in float32).
@@ -469,7 +470,9 @@ int mfqb_decoder_free(mfqb_decoder* d);
  *
  * Pages are written only at positions from lens on, and mfqb_cache_fork leaves every page that is partly filled to one
  * sequence, so pages that sequences share are never written.  Calls on one cache must be ordered by their streams; calls on
- * different caches share nothing.  No call allocates memory, none waits for the device: all can be captured.
+ * different caches share nothing.  No call allocates device memory, none waits for the device: all can be captured, after a first
+ * call of each kind outside a capture (the driver loads a kernel's code at its first launch; the *_work calls ready the device).
+ * Waits inside the attention kernel are bounded: see mfqb_device_status.  Other holders than the table's entries hold whole pages.
  * --------------------------------------------------------------------------------- */
 typedef struct mfqb_cache {
     void* k;
@@ -508,7 +511,8 @@ int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_hea
 
 /* Attention of the nodes over the cache: q, out bf16 [rows][nodes][q_heads][128].  Node i of sequence r sees the positions below
  * lens[r] and those nodes j (at position lens[r] + j) whose bit is set in masks[r][i]; out = softmax(scale * q.k) v over what it sees,
- * zeros where it sees nothing.  What a node does not see has no effect on it, an infinity or NaN neither.  Scores, maxima and sums
+ * zeros where it sees nothing.  What a node does not see has no effect on it, an infinity or NaN neither; an infinite value that it
+ * sees makes that dimension infinity or NaN.  Scores, maxima and sums
  * are float32, probabilities are rounded to bf16 once.  scale: positive and finite.
  * work: device memory of mfqb_tree_attention_work bytes, 16-byte aligned. */
 int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes);

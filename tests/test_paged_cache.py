@@ -64,6 +64,9 @@ def test_arguments_that_are_refused():
     _says(1, "aligned", lib.mfqb_cache_write(v, 0, A + 4, 4, 1, A, A, A, None))
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         _says(1, "scale", lib.mfqb_tree_attention(v, 0, A, 4, 1, A, scale, A, A, 1 << 40, None))
+    _says(1, "aligned", lib.mfqb_tree_attention(v, 0, A, 4, 1, A + 4, 1.0, A, A, 1 << 40, None))
+    _says(1, "aligned", lib.mfqb_cache_write(v, 0, A, 4, 1, A, A + 4, A, None))
+    _says(1, "aligned", lib.mfqb_tree_masks(A, 3, 4, A + 4, A, None))
     assert lib.mfqb_tree_attention_work(v, 4, 1, C.byref(n)) == 0
     _says(1, "work must", lib.mfqb_tree_attention(v, 0, A, 4, 1, A, 1.0, A, A, n.value - 1, None))
 

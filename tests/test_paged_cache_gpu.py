@@ -50,14 +50,16 @@ def _random_trees(rng, rows, nodes):
     return np.array([[-1] + [int(rng.integers(max(0, i - 8), i)) for i in range(1, nodes)] for _ in range(rows)])
 
 
-def _check_attend(st, q, masks, scale=128 ** -0.5, layer=0, cache=None):
+def _check_attend(st, q, masks, scale=128 ** -0.5, layer=0, cache=None, same=True):
     q = _bf(q).float().numpy()
     cache = cache or _cache(st)
     got = cache.attend(layer, _bf(q).to(DEV), _u64(masks), scale=scale).float().cpu().numpy()
     want, weight = R.attend(st, layer, q, masks, scale)
     fine = np.isfinite(want)
-    assert np.array_equal(np.isnan(got), np.isnan(want)), "NaN in other places"
-    assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)].astype(np.float32))
+    assert np.array_equal(np.isfinite(got), fine)
+    if same:
+        assert np.array_equal(np.isnan(got), np.isnan(want)), "NaN in other places"
+        assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)].astype(np.float32))
     bound = 2.0 ** -8 * np.abs(want) + (2.0 ** -7 + 2.0 ** -12) * weight
     off = np.abs(got[fine] - want[fine])
     assert (off <= bound[fine]).all(), (off - bound[fine]).max()
@@ -106,6 +108,49 @@ def test_attention_of_many_sequences():
     st = _round_state(R.state(rng, lens, extra=3, page=16, kv_heads=2))
     masks, _ = R.masks_depths(_random_trees(rng, 70, 3))
     _check_attend(st, rng.standard_normal((70, 3, 4, 128)), masks)
+
+
+@pytest.mark.parametrize("hq,hk,nodes", [(16, 1, 64), (16, 1, 9), (8, 1, 17), (32, 8, 64), (3, 1, 43), (3, 1, 11), (3, 1, 22)])
+def test_attention_by_rows(hq, hk, nodes):
+    """Around 32, 64, 128 and 256 rows of a kv head, up to 1024; contexts that are split, and tables of up to 256 positions, which are not."""
+    rng = np.random.default_rng(hq * nodes)
+    for lens, width in (([700, 3, 257], None), ([192 - nodes // 2, 0, 100], 4)):
+        st = _round_state(R.state(rng, lens, extra=nodes, page=64, kv_heads=hk, width=width))
+        masks, _ = R.masks_depths(_random_trees(rng, 3, nodes))
+        _check_attend(st, 2.0 * rng.standard_normal((3, nodes, hq, 128)), masks)
+
+
+@pytest.mark.parametrize("value,which", [(np.nan, "k"), (np.nan, "v"), (np.inf, "k"), (-np.inf, "k"), (np.inf, "v")])
+def test_what_is_seen_counts(value, which):
+    """Infinities and NaN in the context, in one part of a split one, and scores that are all minus infinity.  (An infinite value is infinity or
+    NaN in its dimension: a part that does not hold it multiplies it by zero.)"""
+    rng = np.random.default_rng(30)
+    st = _round_state(R.state(rng, [900, 40, 1], extra=2, page=64, kv_heads=2))
+    for r, t in ((0, 333), (1, 7), (2, 0)):
+        st[which][0, st["table"][r, t // 64], :, t % 64, 5] = value
+    q = rng.standard_normal((3, 2, 4, 128))
+    q[..., 5] = 1.0   # an infinite key's score has its sign
+    masks = np.array([[1, 3], [1, 3], [0, 0]], np.uint64)   # the third sequence sees its one token alone
+    _check_attend(st, q, masks, same=which == "k")
+
+
+def test_caches_on_two_streams():
+    rng = np.random.default_rng(31)
+    sts = [_round_state(R.state(rng, lens, extra=20, page=32, kv_heads=2)) for lens in ([3000, 10, 500], [90, 2000, 1])]
+    masks, _ = R.masks_depths(_random_trees(rng, 3, 20))
+    caches, m = [_cache(st) for st in sts], _u64(masks)
+    qs = [_bf(rng.standard_normal((3, 20, 8, 128))).to(DEV) for _ in sts]
+    want = [c.attend(0, q, m).clone() for c, q in zip(caches, qs)]
+    streams = [torch.cuda.Stream() for _ in sts]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(caches[i].attend(0, qs[i], m))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
 
 
 def test_rising_scores_and_scales():

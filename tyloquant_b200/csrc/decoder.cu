@@ -621,6 +621,7 @@ struct mfqb_decoder {
     const uint64_t* node_masks = nullptr;   // its masks and depths
     const int32_t* node_depths = nullptr;
     uint64_t attn_work_bytes = 0;
+    std::vector<DevBuf> retired;   // buffers that a larger cache outgrew: graphs captured before still use them
     DevBuf q16, freqs, masks, depths, single_masks, single_depths, attn_work, beam_work, beam_scores, beam_tokens, beam_moves, fork_work, one_each;
     DevBuf gamma_final;
     // workspaces
@@ -761,6 +762,13 @@ static const float* layer_forward(mfqb_decoder* d, int li, int rows, const float
     return rank_sum(d, static_cast<const float*>(d->proj.p), static_cast<float*>(d->proj_sum.p), (size_t)rows * H, s);
 }
 
+// Makes a buffer at least this large; true if it is a new one.  The one it had stays allocated.
+static bool room(mfqb_decoder* d, DevBuf& buf, size_t bytes) {
+    if (buf.bytes >= bytes) return false;
+    d->retired.emplace_back(std::move(buf));
+    buf.alloc(bytes);
+    return true;
+}
 static void check_ready(const mfqb_decoder* d, int rows, const char* who) {
     if (rows < 1 || rows > d->cfg.max_batch) fail(MFQB_ERR_ARG, "%s: %d rows outside [1, %d]", who, rows, d->cfg.max_batch);
     if (!d->lm_head || !d->embedding) fail(MFQB_ERR_ARG, "%s: head weights are not set", who);
@@ -1011,22 +1019,20 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
         for (int i = 0; i < kHeadDim / 2; ++i) freqs[i] = std::pow((double)d->cfg.rope_theta, -2.0 * i / kHeadDim);
         std::vector<uint64_t> one(rows, 1);
         std::vector<int32_t> zero(rows, 0), ones(rows, 1);
-        MFQB_CUDA(cudaDeviceSynchronize());   // passes over the cache before may still use the buffers
         d->paged = false;
-        d->q16.alloc(B * d->nq * kHeadDim * 2);
-        d->masks.alloc(B * 8);
-        d->depths.alloc(B * 4);
-        d->attn_work.alloc(most);
-        d->attn_work_bytes = most;
-        d->fork_work.alloc(fork_bytes);
-        d->beam_scores.alloc(rows * 4);
-        d->beam_tokens.alloc(rows * 4);
-        d->beam_moves.alloc(rows * 4);
-        d->beam_work.release();
-        d->freqs.upload(freqs, sizeof(freqs));
-        d->single_masks.upload(one.data(), rows * 8);
-        d->single_depths.upload(zero.data(), rows * 4);
-        d->one_each.upload(ones.data(), rows * 4);
+        room(d, d->q16, B * d->nq * kHeadDim * 2);
+        room(d, d->masks, B * 8);
+        room(d, d->depths, B * 4);
+        room(d, d->attn_work, most);
+        d->attn_work_bytes = d->attn_work.bytes;
+        room(d, d->fork_work, fork_bytes);
+        room(d, d->beam_scores, rows * 4);
+        room(d, d->beam_tokens, rows * 4);
+        room(d, d->beam_moves, rows * 4);
+        if (room(d, d->freqs, sizeof(freqs))) MFQB_CUDA(cudaMemcpy(d->freqs.p, freqs, sizeof(freqs), cudaMemcpyHostToDevice));
+        if (room(d, d->single_masks, rows * 8)) MFQB_CUDA(cudaMemcpy(d->single_masks.p, one.data(), rows * 8, cudaMemcpyHostToDevice));
+        if (room(d, d->single_depths, rows * 4)) MFQB_CUDA(cudaMemcpy(d->single_depths.p, zero.data(), rows * 4, cudaMemcpyHostToDevice));
+        if (room(d, d->one_each, rows * 4)) MFQB_CUDA(cudaMemcpy(d->one_each.p, ones.data(), rows * 4, cudaMemcpyHostToDevice));
         d->cache = *cache;
         d->paged = true;
     });
@@ -1065,8 +1071,7 @@ int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, fl
             cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
             MFQB_CUDA(cudaStreamIsCapturing(s, &capturing));
             if (capturing != cudaStreamCaptureStatusNone) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: one call with this many beams must come before a stream capture");
-            MFQB_CUDA(cudaStreamSynchronize(s));
-            d->beam_work.alloc(bytes);
+            room(d, d->beam_work, bytes);
         }
         check(mfqb_cache_extend(&d->cache, static_cast<const int32_t*>(d->one_each.p), status, s));
         single_nodes(d);

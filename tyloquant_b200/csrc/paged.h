@@ -6,6 +6,15 @@
 
 namespace mfqb {
 
+int* device_status_word(int device);
+// What the attention needs of a device beside its arguments, the status word of its bounded waits, is allocated here and not at the first call,
+// which may be in a stream capture.  Without a device there is nothing to ready.
+inline void ready_device() {
+    int device = 0;
+    if (cudaGetDevice(&device) == cudaSuccess) device_status_word(device);
+    else cudaGetLastError();
+}
+
 constexpr int kHeadDim = 128;
 constexpr int kTreeNodes = 64;    // nodes of a drafted tree: one bit of a mask each
 constexpr int kCacheRows = 1024;  // sequences of a cache: one thread each in the kernels that give out pages

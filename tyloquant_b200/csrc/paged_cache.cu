@@ -426,6 +426,7 @@ int mfqb_cache_fork_work(const mfqb_cache* c, uint64_t* bytes) {
     return guarded([&] {
         check_cache(c, "mfqb_cache_fork_work");
         if (!bytes) fail(MFQB_ERR_ARG, "mfqb_cache_fork_work: null argument");
+        ready_device();
         *bytes = fork_work_bytes(*c);
     });
 }
@@ -449,6 +450,7 @@ int mfqb_tree_masks(const int32_t* parents, int rows, int nodes, uint64_t* masks
     return guarded([&] {
         if (!parents || !masks || !depths) fail(MFQB_ERR_ARG, "mfqb_tree_masks: null argument");
         if (rows < 1 || rows > kCacheRows) fail(MFQB_ERR_UNSUPPORTED, "mfqb_tree_masks: 1 to %d sequences, got %d", kCacheRows, rows);
+        if ((uintptr_t)masks & 7) fail(MFQB_ERR_ARG, "mfqb_tree_masks: masks must be 8-byte aligned");
         if (nodes < 1 || nodes > kTreeNodes) fail(MFQB_ERR_UNSUPPORTED, "mfqb_tree_masks: 1 to %d nodes per sequence, got %d", kTreeNodes, nodes);
         launch_chained(tree_masks_kernel, dim3(rows), dim3(32), 0, stream, parents, nodes, reinterpret_cast<unsigned long long*>(masks), depths);
     });
@@ -461,6 +463,7 @@ int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_hea
         check_nodes(c, nodes, "mfqb_cache_write");
         if (!qkv || !depths || !freqs || !q_out) fail(MFQB_ERR_ARG, "mfqb_cache_write: null argument");
         if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 15)) fail(MFQB_ERR_ARG, "mfqb_cache_write: qkv and q_out must be 16-byte aligned");
+        if ((uintptr_t)freqs & 7) fail(MFQB_ERR_ARG, "mfqb_cache_write: freqs must be 8-byte aligned");
         if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "mfqb_cache_write: layer %d of %d", layer, c->layers);
         if (q_heads < 1 || q_heads > 16384) fail(MFQB_ERR_ARG, "mfqb_cache_write: bad number of query heads %d", q_heads);
         // one CTA per token once there are CTAs for every SM, else its heads spread over more of them

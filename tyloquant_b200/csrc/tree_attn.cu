@@ -22,8 +22,6 @@
 
 namespace mfqb {
 
-int* device_status_word(int device);
-
 constexpr int kTreeSms = 148;
 constexpr int kTile = 128;                           // rows of Q, positions of a tile
 constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
@@ -945,6 +943,7 @@ int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64
         check_nodes(c, nodes, "mfqb_tree_attention_work");
         check_heads(c, q_heads, "mfqb_tree_attention_work");
         if (!bytes) fail(MFQB_ERR_ARG, "mfqb_tree_attention_work: null argument");
+        ready_device();
         *bytes = tree_attention_work_bytes(*c, q_heads, nodes);
     });
 }
@@ -957,6 +956,7 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
         check_heads(c, q_heads, "mfqb_tree_attention");
         if (!q || !masks || !out || !work) fail(MFQB_ERR_ARG, "mfqb_tree_attention: null argument");
         if (((uintptr_t)q & 15) || ((uintptr_t)out & 15)) fail(MFQB_ERR_ARG, "mfqb_tree_attention: q and out must be 16-byte aligned");
+        if ((uintptr_t)masks & 7) fail(MFQB_ERR_ARG, "mfqb_tree_attention: masks must be 8-byte aligned");
         if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "mfqb_tree_attention: layer %d of %d", layer, c->layers);
         if (!(scale > 0.f) || scale > 1e30f) fail(MFQB_ERR_ARG, "mfqb_tree_attention: scale must be positive and finite");
         if (((uintptr_t)work & 15) || work_bytes < tree_attention_work_bytes(*c, q_heads, nodes))
