@@ -39,8 +39,8 @@ constexpr int kListMax = 1024;   // candidates of a slice that are ranked by cou
 // and a candidate's place is the number of larger ones in it.  The bound costs a warp two sorts by shuffles; the k-th largest of all 256
 // maxima, found by counting, took as long as everything else.  Where too many elements are equal for the list, the best key is taken
 // k times.  128 rows of 128256 (115 of them read): 73 us in all with counting.
-__global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const float* __restrict__ logits, const int* __restrict__ done, int vocab, int k, int slices,
-                                                                      bool wide, SliceSum* __restrict__ sums, unsigned long long* __restrict__ keys) {
+__global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const float* logits, const int* done, int vocab, int k, int slices, bool wide, SliceSum* sums,
+                                                                      unsigned long long* keys) {
     chained_wait();
     __shared__ __align__(16) float s_x[kSlice];   // only where the list is too short
     unsigned long long* s_list = reinterpret_cast<unsigned long long*>(s_x);
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     __shared__ int s_count;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slice = blockIdx.x;
     const int64_t row = blockIdx.y;
-    if (done && done[row]) return;
+    if (done && __ldcg(done + row)) return;
     const int base = slice * kSlice;
     const float* src = logits + row * vocab + base;
     const int n = min(kSlice, vocab - base);
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
 #pragma unroll 1
         for (unsigned left = take; left && at < kListMax; left &= left - 1, ++at) {   // read again: few, and a loop over registers would have to be unrolled
             const int j = __ffs(left) - 1, i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
-            s_list[at] = beam_key(__ldg(src + i), (unsigned)(base + i));
+            s_list[at] = beam_key(__ldcg(src + i), (unsigned)(base + i));
         }
     }
     __syncthreads();
@@ -238,9 +238,8 @@ __device__ __forceinline__ int merge_lists(int lane, int k, Get get, Put put) {
 // into the group's.  The lists come into shared memory first where they fit (staged): every one of the k rounds waits for the entry behind
 // the one that it takes.
 template <int NL>
-__global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restrict__ scores, const int* __restrict__ done, int eos, int beams, int k, int slices, int at_once,
-                                                          bool staged, const SliceSum* __restrict__ sums, const unsigned long long* __restrict__ keys,
-                                                          float* __restrict__ out_scores, int* __restrict__ out_rows, int* __restrict__ out_tokens) {
+__global__ void __launch_bounds__(1024) beam_merge_kernel(const float* scores, const int* done, int eos, int beams, int k, int slices, int at_once, bool staged,
+                                                          const SliceSum* sums, const unsigned long long* keys, float* out_scores, int* out_rows, int* out_tokens) {
     chained_wait();
     extern __shared__ unsigned long long s_best[];   // the beams' results [beams][k]: keys, then scores; then [at_once][slices][k] where staged
     unsigned long long* s_value = s_best + beams * k;
@@ -249,8 +248,8 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restric
     if (warp < at_once) {
         for (int b = warp; b < beams; b += at_once) {
             const int64_t row = (int64_t)group * beams + b;
-            const bool over = done && done[row];
-            const double score = scores[row];
+            const bool over = done && __ldcg(done + row);
+            const double score = __ldcg(scores + row);
             if (lane == 0) s_done[b] = over;
             if (over) {
                 if (lane == 0) s_value[b * k] = order_f64(score);
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(const float* __restric
             if (staged) {
                 unsigned long long* dst = s_value + (size_t)beams * k + (size_t)warp * slices * k;
 #pragma unroll 4
-                for (int i = lane; i < slices * k; i += 32) dst[i] = src[i];
+                for (int i = lane; i < slices * k; i += 32) dst[i] = __ldcg(src + i);
                 mine = dst;
             }
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

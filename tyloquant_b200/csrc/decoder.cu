@@ -559,7 +559,7 @@ __global__ void add_one_kernel(int* p, int n) {
 }
 
 // Between the selection and the fork: the step's token counts where its page could be had; else no sequence moves.
-__global__ void __launch_bounds__(1024) beam_move_kernel(const int* __restrict__ status, const int* __restrict__ parents, int rows, int* __restrict__ lens, int* __restrict__ moves) {
+__global__ void __launch_bounds__(1024) beam_move_kernel(const int* status, const int* parents, int rows, int* lens, int* moves) {
     dep_wait();
     const int r = threadIdx.x;
     if (r >= rows) return;
@@ -569,8 +569,8 @@ __global__ void __launch_bounds__(1024) beam_move_kernel(const int* __restrict__
 }
 // The chosen beams become the sequences' state: scores, tokens, and done where the beam that goes on was done or has now ended.  Where pages
 // were missing everything is as before the step, which can be done again.
-__global__ void __launch_bounds__(1024) beam_take_kernel(const int* __restrict__ status, const float* __restrict__ best, const int* __restrict__ tokens, int rows, int eos,
-                                                         const int* ids_in, int* __restrict__ lens, float* __restrict__ scores, int* done, int* ids, int* __restrict__ parents) {
+__global__ void __launch_bounds__(1024) beam_take_kernel(const int* status, const float* best, const int* tokens, int rows, int eos, const int* ids_in, int* lens,
+                                                         float* scores, int* done, int* ids, int* parents) {
     dep_wait();
     const int r = threadIdx.x;
     const bool reserved = status[0] == 0, ok = reserved && status[1] == 0;

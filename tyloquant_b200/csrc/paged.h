@@ -54,6 +54,8 @@ void launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem
 }
 
 #if defined(__CUDACC__)
+// The kernels here start while the one before them runs, so what that one writes is not constant for their lifetime: they read it after this
+// wait, from the L2 cache (__ldcg) or by loads that the compiler may not take for constant (no const __restrict__).
 __device__ __forceinline__ void chained_wait() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
