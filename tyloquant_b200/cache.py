@@ -79,8 +79,9 @@ class PagedCache:
         self._view = CacheView(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), layers, heads, page, pages, rows, width)
         self._ptr = C.addressof(self._view)
         size = C.c_uint64()
-        check(lib.mfqb_cache_fork_work(C.byref(self._view), C.byref(size)))   # refuses a shape that the library does not take
-        self._fork_work = size.value
+        with torch.cuda.device(self.device):
+            check(lib.mfqb_cache_fork_work(C.byref(self._view), C.byref(size)))   # refuses a shape that the library does not take
+        self._fork_work = lens.new_empty((size.value + 3) // 4)   # calls on one cache are in order: they can share it
         self._attend_work = {}
 
     @classmethod
@@ -113,8 +114,8 @@ class PagedCache:
         pages were missing, or -1 for an entry outside [-1, rows); where it is not 0 nothing has changed."""
         p = self._int32(parents, (self.rows,), "parents")
         status = self.lens.new_empty(1)
-        work = self.lens.new_empty(self._fork_work // 4)
-        _call(_fast.cache_fork, self.device, self._ptr, p.data_ptr(), status.data_ptr(), work.data_ptr(), self._fork_work)
+        work = self._fork_work
+        _call(_fast.cache_fork, self.device, self._ptr, p.data_ptr(), status.data_ptr(), work.data_ptr(), work.numel() * 4)
         return status
 
     def write(self, layer: int, qkv, depths, freqs):
@@ -149,7 +150,8 @@ class PagedCache:
         size = self._attend_work.get((hq, nodes))
         if size is None:
             n = C.c_uint64()
-            check(lib.mfqb_tree_attention_work(C.byref(self._view), hq, nodes, C.byref(n)))
+            with torch.cuda.device(self.device):
+                check(lib.mfqb_tree_attention_work(C.byref(self._view), hq, nodes, C.byref(n)))
             size = self._attend_work[(hq, nodes)] = (n.value + 15) // 16 * 16
         work = x.new_empty(size // 2)
         _call(_fast.tree_attention, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, m.data_ptr(), HEAD_DIM ** -0.5 if scale is None else scale,
