@@ -784,16 +784,19 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
     }
 }
 
-// Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context, eight loads at a
-// time, with a running maximum (a pass for the maximum before it was one more trip to memory of the four that the kernel consists of).
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int streams, int rows) {
+constexpr int kMergeParts = 16, kMergeWarps = 4;   // parts in flight for a row, rows of a CTA
+
+// Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context, with a running
+// maximum.  Sixteen parts at a time are on their way, by asynchronous copies: with loads into registers eight were, and the 28 parts of a long
+// sequence's rows took 6 us of the ragged batch's 26.5.
+__global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __grid_constant__ TreeArgs a, int streams, int rows) {
     chained_wait();
-    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5), m_rows = a.nodes * a.group, per_seq = a.kv_heads * m_rows;
-    // What all rows ask for comes through one thread a CTA and sequence (the ragged batch 27.8 us a pass with a trip of every warp, 27.0 with this).
-    __shared__ int64_t s_before[8], s_quota;
-    __shared__ TreeSeq s_seq[8];
-    const int r0 = blockIdx.x * 8 / per_seq, r = min(warp, rows - 1) / per_seq;
-    if (threadIdx.x < 8 && r0 + (int)threadIdx.x < a.rows && (int64_t)(r0 + threadIdx.x) * per_seq < (int64_t)blockIdx.x * 8 + 8) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warp = blockIdx.x * kMergeWarps + wid, m_rows = a.nodes * a.group, per_seq = a.kv_heads * m_rows;
+    __shared__ float4 s_part[kMergeWarps][kMergeParts][32];
+    __shared__ int64_t s_before[kMergeWarps], s_quota;   // what all rows ask for comes through one thread a CTA and sequence
+    __shared__ TreeSeq s_seq[kMergeWarps];
+    const int r0 = blockIdx.x * kMergeWarps / per_seq, r = min(warp, rows - 1) / per_seq;
+    if (threadIdx.x < kMergeWarps && (int64_t)(r0 + threadIdx.x) * per_seq < min((int64_t)blockIdx.x * kMergeWarps + kMergeWarps, (int64_t)rows)) {
         s_before[threadIdx.x] = __ldcg(a.before + r0 + threadIdx.x);
         s_seq[threadIdx.x] = tree_seq(a, r0 + threadIdx.x);
     }
@@ -812,35 +815,31 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     auto slot = [&](int c) { return (c * 2 + (c == first ? shift : 0)) * a.tile_rows + row_l; };
     float m = -INFINITY, l = 0.f, none = 0.f;   // none: of parts without a maximum, which count only among themselves
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = first; c <= last; c += 8) {
-        float2 ml[8];
-        float4 o[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (c + u <= last) {
-                const int at = slot(c + u);
-                ml[u] = __ldcg(&a.part_ml[at]);
-                o[u] = __ldcg(reinterpret_cast<const float4*>(a.part + at * kHeadDim) + lane);
-            }
-        float high = m;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (c + u <= last) high = fmaxf(high, ml[u].x);
-        const float corr = m == -INFINITY ? 0.f : exp2_approx(m - high);
+    for (int c = first; c <= last; c += kMergeParts) {
+        const int n = min(kMergeParts, last - c + 1);
+        for (int u = 0; u < n; ++u)   // a lane reads what it has copied itself
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&s_part[wid][u][lane])), "l"(a.part + (int64_t)slot(c + u) * kHeadDim + 4 * lane) : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const float2 ml = lane < n ? __ldcg(&a.part_ml[slot(c + lane)]) : make_float2(-INFINITY, 0.f);
+        float high = ml.x;
+        for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        high = fmaxf(high, m);
+        const float corr = m == -INFINITY ? 0.f : exp2_approx(m - high), f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - high);
         m = high;
-        l *= corr;
+        float sum = ml.x == -INFINITY ? 0.f : ml.y * f, empty = ml.x == -INFINITY ? ml.y : 0.f;
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            empty += __shfl_xor_sync(0xffffffffu, empty, o);
+        }
+        l = l * corr + sum;
+        none += empty;
         acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (c + u <= last) {
-                if (ml[u].x == -INFINITY) {
-                    none += ml[u].y;
-                    continue;
-                }
-                const float f = exp2_approx(ml[u].x - m);
-                l += ml[u].y * f;
-                acc.x += o[u].x * f; acc.y += o[u].y * f; acc.z += o[u].z * f; acc.w += o[u].w * f;
-            }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int u = 0; u < n; ++u) {
+            const float g = __shfl_sync(0xffffffffu, f, u);
+            const float4 o = s_part[wid][u][lane];
+            acc.x += o.x * g; acc.y += o.y * g; acc.z += o.z * g; acc.w += o.w * g;
+        }
     }
     if (m == -INFINITY) l = none;
     const float inv = 1.f / l;
@@ -930,7 +929,7 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     launch_chained(kernel, dim3(ctas), dim3(tree_threads(ns)), tree_smem(ns), s, a, kmap, vmap);
     if (a.whole) return;
     const int64_t rows = (int64_t)c.rows * c.kv_heads * m_rows;   // at most 1024 x 1024 x 1024
-    launch_chained(tree_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a, ns, (int)rows);
+    launch_chained(tree_merge_kernel, dim3((unsigned)((rows + kMergeWarps - 1) / kMergeWarps)), dim3(32 * kMergeWarps), 0, s, a, ns, (int)rows);
 }
 
 }  // namespace mfqb
