@@ -29,15 +29,23 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
 
+// Float32 values in the order of unsigned numbers, for values that are no NaN.
+__device__ __forceinline__ unsigned order_f32(float v) {
+    const unsigned b = __float_as_uint(v);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_order_f32(unsigned o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
+
 constexpr int kListMax = 1024;   // candidates of a slice that are ranked by counting
 
 // CTA (slice, row).  A thread keeps its 32 logits in registers: element (j * 256 + thread) * 4 + e of the slice whatever the row's
 // alignment, so that equal rows have equal sums to the last bit and ties between beams are ties.
 //
 // Candidates are the elements that reach a bound which at least k of them do: the j-th largest thread maximum of a warp, j = ceil(k / c), in the
-// c-th best of the eight warps, for the best of c = 8, 4, 2, 1 (some 30 candidates for k = 16; with c = 8 alone some 100).  They go into a list,
-// and a candidate's place is the number of larger ones in it.  The bound costs a warp two sorts by shuffles; the k-th largest of all 256
-// maxima, found by counting, took as long as everything else.  Where too many elements are equal for the list, the best key is taken
+// c-th best of the eight warps, for the better of c = 8 and 4 (some 35 candidates for k = 16; with c = 8 alone some 100).  They go into a list,
+// and a candidate's place is the number of larger ones in it.  The j-th largest is found by j rounds of a warp's maximum up to k = 32, by a
+// sort beyond (a sort for k = 16 was a quarter of a CTA's time); the k-th largest of all 256 maxima, found by counting, took as long as
+// everything else.  Where too many elements are equal for the list, the best key is taken
 // k times.  128 rows of 128256 (115 of them read): 73 us in all with counting.
 __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const float* logits, const int* done, int vocab, int k, int slices, bool wide, SliceSum* sums,
                                                                       unsigned long long* keys) {
@@ -45,7 +53,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     __shared__ __align__(16) float s_x[kSlice];   // only where the list is too short
     unsigned long long* s_list = reinterpret_cast<unsigned long long*>(s_x);
     __shared__ unsigned long long s_round[2][8];
-    __shared__ float s_top[8], s_low[32];
+    __shared__ float s_top[8], s_low[16];
     __shared__ double s_sum[8];
     __shared__ int s_count;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slice = blockIdx.x;
@@ -72,34 +80,54 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kSliceEach; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
-    // values of `size` neighbouring lanes in descending order
-    auto sort = [&](float v, int width) {
+    // the warp's largest thread maximum, its ceil(k / 8)-th and its ceil(k / 4)-th
+    const int j8 = (k + 7) / 8, j4 = (k + 3) / 4;
+    float high, low8, low4;
+    if (j4 <= 8) {
+        unsigned mine = order_f32(top), best = 0u, first = 0u, eighth = 0u;
+        for (int j = 1; j <= j4; ++j) {   // lanes that are equal leave together: the value found is at most the j-th
+            best = __reduce_max_sync(0xffffffffu, mine);
+            if (j == 1) first = best;
+            if (j == j8) eighth = best;
+            if (mine == best) mine = 0u;
+        }
+        high = from_order_f32(first);
+        low8 = eighth ? from_order_f32(eighth) : -INFINITY;   // 0: no lane was left
+        low4 = best ? from_order_f32(best) : -INFINITY;
+    } else {
+        float v = top;   // in descending order
 #pragma unroll
         for (int size = 2; size <= 32; size <<= 1)
-            if (size <= width)
 #pragma unroll
-                for (int o = size >> 1; o > 0; o >>= 1) {
-                    const float u = __shfl_xor_sync(0xffffffffu, v, o);
-                    v = ((lane & o) == 0) == ((lane & size & (width - 1)) == 0) ? fmaxf(v, u) : fminf(v, u);
-                }
-        return v;
-    };
-    const float sorted = sort(top, 32);
-    if (lane == 0) s_top[warp] = sorted;
-#pragma unroll
-    for (int o = 0; o < 4; ++o) {
-        const int c = 8 >> o, j = (k + c - 1) / c;
-        const float v = __shfl_sync(0xffffffffu, sorted, min(j, 32) - 1);
-        if (lane == 0) s_low[o * 8 + warp] = j <= 32 ? v : -INFINITY;
+            for (int o = size >> 1; o > 0; o >>= 1) {
+                const float u = __shfl_xor_sync(0xffffffffu, v, o);
+                v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, u) : fminf(v, u);
+            }
+        high = __shfl_sync(0xffffffffu, v, 0);
+        low8 = __shfl_sync(0xffffffffu, v, j8 - 1);
+        low4 = __shfl_sync(0xffffffffu, v, j4 - 1);
+    }
+    if (lane == 0) {
+        s_top[warp] = high;
+        s_low[warp] = low8;
+        s_low[8 + warp] = low4;
     }
     __syncthreads();
-    top = s_top[0];
+    float bound;
+    {   // the least of the warps' first value, the fourth of their second
+        const float mine = s_low[8 + (lane & 7)];
+        float least = s_low[0];
+        int above = 0;
+        top = s_top[0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, s_top[w]);
-    float bound = sort(s_low[lane], 8);   // lane 8 o + i: the i-th best warp of choice o
-    bound = (lane & 7) == (8 >> (lane >> 3)) - 1 ? bound : -INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+        for (int w = 0; w < 8; ++w) {
+            const float v = s_low[8 + w];
+            top = fmaxf(top, s_top[w]);
+            least = fminf(least, s_low[w]);
+            above += v > mine || (v == mine && w < (lane & 7));
+        }
+        bound = fmaxf(least, __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, above == 3)) - 1));
+    }
     unsigned take = 0;
     float part = 0.f;
     if (top > -INFINITY && top < INFINITY && bound > -INFINITY) {
@@ -145,12 +173,15 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     const int have = s_count;
     unsigned long long* out = keys + (row * slices + slice) * k;
     if (have <= kListMax) {
-        for (int i = t; i < have; i += kSliceThreads) {
-            const unsigned long long key = s_list[i];
+        for (int i0 = 0; i0 < have; i0 += kSliceThreads / 4) {   // four threads a candidate
+            const int i = i0 + (t >> 2);
+            const unsigned long long key = i < have ? s_list[i] : 0ull;
             int rank = 0;
 #pragma unroll 4
-            for (int j = 0; j < have; ++j) rank += s_list[j] > key;
-            if (rank < k) out[rank] = key;
+            for (int j = t & 3; j < have; j += 4) rank += s_list[j] > key;
+            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+            rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+            if ((t & 3) == 0 && i < have && rank < k) out[rank] = key;
         }
         for (int i = have + t; i < k; i += kSliceThreads) out[i] = 0ull;   // a short slice
         return;
