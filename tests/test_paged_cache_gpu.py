@@ -239,6 +239,40 @@ def test_offsets_past_32_bits():
     _check_attend(small, rng.standard_normal((1, 4, 8, 128)), masks, cache=cache)
 
 
+def test_writes_and_moves_past_32_bits():
+    """The same pool sizes for what writes: cache write, accepted branch and fork on the last pages of a pool of more than 2^32 bytes."""
+    layers, pages, page, hk, hq = 2, 9000, 256, 2, 4
+    k = torch.zeros(layers, pages, hk, page, 128, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    assert k.numel() * 2 > 1 << 31 and k.numel() > 1 << 30
+    last = pages - 1
+    refs = torch.ones(pages, dtype=torch.int32, device=DEV)
+    refs[last - 1] = 0
+    cache = PagedCache(k, v, _i32([[last, -1], [-1, -1]]), _i32([10, 0]), refs)
+    rng = np.random.default_rng(40)
+    small = {"k": np.zeros((layers, 2, hk, page, 128), np.float32), "v": np.zeros((layers, 2, hk, page, 128), np.float32), "table": np.array([[1, -1], [-1, -1]], np.int32),
+             "lens": np.array([10, 0], np.int32), "refs": np.array([0, 1], np.int32)}
+    depths = np.array([[0, 1, 1, 2, 2]] * 2)
+    freqs = rope_frequencies(device=DEV)
+    for layer in range(layers):
+        qkv = rng.standard_normal((2, 5, (hq + 2 * hk) * 128)).astype(np.float32)
+        cache.write(layer, torch.from_numpy(qkv).to(DEV), _i32(depths), freqs)
+        R.write(small, layer, qkv, depths, freqs.cpu().numpy(), hq)
+    two = lambda pool: pool[:, last - 1:].float().cpu().numpy()   # the last two pages
+    for got, want in ((two(k), small["k"]), (two(v), small["v"])):
+        assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 12 * 2.0 ** -20).all()
+    small["k"], small["v"] = two(k), two(v)
+    parents, ids, targets = np.array([[-1, 0, 0, 2, 3]] * 2), np.array([[0, 7, 1, 1, 1]] * 2), np.ones((2, 5))
+    cache.accept(_i32(ids), _i32(parents), _i32(targets), lens_out=cache.lens)
+    small["lens"] = R.accept(small, ids, parents, targets)[3]
+    assert np.array_equal(two(k), small["k"]) and np.array_equal(two(v), small["v"])
+    cache.lens[1] = small["lens"][1] = 0
+    assert int(cache.fork(_i32([0, 0]))) == R.fork(small, [0, 0]) == 0
+    assert cache.table.tolist() == [[last, -1], [last - 1, -1]] and cache.lens.tolist() == [14, 14]
+    assert np.array_equal(two(k), small["k"]) and np.array_equal(two(v), small["v"])
+    assert not k[:, :last - 1].any() and not v[:, :last - 1].any()
+
+
 @pytest.mark.parametrize("rows,nodes,hq,hk", [(1, 1, 4, 2), (3, 5, 8, 1), (2, 64, 6, 2), (20, 9, 32, 8)])
 def test_write(rows, nodes, hq, hk):
     rng = np.random.default_rng(nodes)

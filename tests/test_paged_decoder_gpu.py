@@ -102,6 +102,26 @@ def test_a_prompt_in_one_pass_agrees_with_steps():
     dec.free()
 
 
+@pytest.mark.parametrize("heads,kv", [(6, 2), (8, 1), (16, 1), (2, 2)])
+def test_head_groups_that_the_own_cache_does_not_take_too(heads, kv):
+    """Three and sixteen query heads per KV head, over pages alone: a prompt in one pass against steps."""
+    rows, n = 2, 20
+    ids = _i32(np.random.default_rng(heads).integers(0, 1000, (rows, n)))
+    dec = D.random_decoder(hidden=heads * 128, n_q_heads=heads, n_kv_heads=kv, ffn=512, vocab=1000, layers=1, max_ctx=0, max_batch=rows * n, seed=5, distinct_layers=1)[0]
+    caches = [PagedCache.empty(layers=1, kv_heads=kv, page=16, pages=8, rows=rows, width=4) for _ in range(2)]
+    dec.set_cache(caches[0])
+    want = []
+    for i in range(n):
+        assert int(caches[0].extend(1)) == 0
+        dec.step(ids[:, i].contiguous())
+        want.append(dec.read_logits(rows))
+    dec.set_cache(caches[1])
+    got = _prompt(dec, caches[1], ids)
+    for i in range(n):
+        assert rel_l2(got[:, i].cpu().numpy(), want[i].cpu().numpy()) <= 1e-2, i
+    dec.free()
+
+
 def test_drafted_trees_give_what_single_steps_give():
     """Every node's logits are those of a decoder that has taken the tokens above it one by one; the accepted branch leaves the cache as if
     it had been decoded."""
@@ -246,8 +266,10 @@ def test_beams_that_end_and_pages_that_run_out():
 
 
 def test_a_captured_beam_step_replays():
+    """Bit for bit, with 4-bit weights throughout: two to four rows of 6-bit weights take a kernel whose sums differ in the last bit from call to
+    call."""
     beams = 4
-    dec = _decoder(16)
+    dec = _decoder(16, ffn_profile=(4, 24, 6))
     caches, outs = [], []
     prompt = _i32(np.random.default_rng(4).integers(0, 1000, (4, 4)))
     for captured in (False, True):
