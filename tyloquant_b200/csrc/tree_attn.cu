@@ -840,6 +840,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __gr
             const float4 o = s_part[wid][u][lane];
             acc.x += o.x * g; acc.y += o.y * g; acc.z += o.z * g; acc.w += o.w * g;
         }
+        __syncwarp();   // the parts have been read before the next come in their place
     }
     if (m == -INFINITY) l = none;
     const float inv = 1.f / l;
