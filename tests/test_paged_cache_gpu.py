@@ -500,6 +500,30 @@ def test_rows_with_few_live_tokens():
         _check_beams(logits, np.array([[0.0, -1.0], [-2.0, 0.0]], np.float32), 20)
 
 
+@pytest.mark.parametrize("k", [1, 16, 64, 128])
+@pytest.mark.parametrize("masked", [float("-inf"), float(torch.finfo(torch.float32).min), -1e4])
+def test_rows_that_a_mask_has_left_little_of(masked, k):
+    """One value for what is masked: with few others, with others in every slice; slices that begin with something below it or a NaN; its
+    count around a list's length; all of a slice's first tokens live, which fill the selection or not."""
+    rng = np.random.default_rng(22)
+    logits = np.full((4, 2, 20003), masked, np.float32)
+    logits[0, 0, rng.permutation(20003)[:5]] = 1.0
+    at = rng.permutation(20003)[:700]
+    logits[0, 1, at] = rng.standard_normal(700).astype(np.float32)
+    below = -np.inf if masked > -np.inf else np.nan
+    logits[1, 0, [0, 1, 8192, 8300, 16384]] = below
+    logits[1, 0, 9000:9003] = 2.0
+    logits[1, 1, :200] = below
+    logits[1, 1, 300:] = below
+    logits[2, 0, 1030:8192] = below
+    logits[2, 0, 8192 + 1020:] = below
+    logits[2, 1] = rng.standard_normal(20003).astype(np.float32)
+    logits[2, 1, ::2] = masked
+    logits[3, 0, :100] = rng.standard_normal(100).astype(np.float32)
+    logits[3, 1, 60:8192] = 3.0
+    _check_beams(logits, -rng.random((4, 2)).astype(np.float32), k, exact_ids=False)
+
+
 def test_equal_candidates_go_to_the_lower_beam_and_token():
     """Equal beams on rows of every alignment, equal logits, a row of one value, more equal logits than a thread holds."""
     for vocab in (997, 1000, 20001):

@@ -168,10 +168,11 @@ class PagedCache:
         nodes = ids.shape[1]
         i, p, t = (self._int32(x, (self.rows, nodes), what) for x, what in ((ids, "ids"), (parents, "parents"), (targets, "targets")))
         if lens_out is None:
-            lens_out = self.lens.new_empty(self.rows)
+            lens_out = _torch().empty_like(self.lens)
         elif self._int32(lens_out, (self.rows,), "lens_out") is not lens_out:
             raise ValueError("lens_out must be contiguous")
-        count, token, path = self.lens.new_empty(self.rows), self.lens.new_empty(self.rows), self.lens.new_empty((self.rows, nodes))
+        torch = _torch()
+        count, token, path = torch.empty_like(self.lens), torch.empty_like(self.lens), torch.empty_like(i)
         _call(_fast.tree_accept, self.device, self._ptr, i.data_ptr(), p.data_ptr(), t.data_ptr(), nodes, count.data_ptr(), token.data_ptr(), path.data_ptr(),
               lens_out.data_ptr())
         return count, token, path, lens_out
@@ -199,7 +200,8 @@ def beam_select(logits, scores, k: int, done=None, eos: int = -1):
     dn = None if done is None else _need(done, torch.int32, (g, w), dev, "done")
     size = _beam_work(g, w, vocab, k)
     work = z.new_empty(size // 4)
-    out, rows, tokens = z.new_empty((g, k)), z.new_empty((g, k), dtype=torch.int32), z.new_empty((g, k), dtype=torch.int32)
+    out, rows = z.new_empty((g, k)), z.new_empty((g, k), dtype=torch.int32)
+    tokens = torch.empty_like(rows)
     _call(_fast.beam_select, dev, z.data_ptr(), g, w, vocab, sc.data_ptr(), None if dn is None else dn.data_ptr(), eos, k, out.data_ptr(), rows.data_ptr(),
           tokens.data_ptr(), work.data_ptr(), size)
     return out, rows, tokens

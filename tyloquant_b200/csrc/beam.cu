@@ -37,6 +37,7 @@ __device__ __forceinline__ unsigned order_f32(float v) {
 __device__ __forceinline__ float from_order_f32(unsigned o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
 
 constexpr int kListMax = 1024;   // candidates of a slice that are ranked by counting
+constexpr int kThreadMost = 8;   // of a thread's 32
 
 // CTA (slice, row).  A thread keeps its 32 logits in registers: element (j * 256 + thread) * 4 + e of the slice whatever the row's
 // alignment, so that equal rows have equal sums to the last bit and ties between beams are ties.
@@ -45,17 +46,19 @@ constexpr int kListMax = 1024;   // candidates of a slice that are ranked by cou
 // c-th best of the eight warps, for the better of c = 8 and 4 (some 35 candidates for k = 16; with c = 8 alone some 100).  They go into a list,
 // and a candidate's place is the number of larger ones in it.  The j-th largest is found by j rounds of a warp's maximum up to k = 32, by a
 // sort beyond (a sort for k = 16 was a quarter of a CTA's time); the k-th largest of all 256 maxima, found by counting, took as long as
-// everything else.  Where too many elements are equal for the list, the best key is taken
-// k times.  128 rows of 128256 (115 of them read): 73 us in all with counting.
+// everything else.  Where too many elements reach the bound for the list (most of
+// the slice is masked) a second list leaves out equal ones that cannot be among the best, or, where that does not help, the k-th largest is found by
+// bisection, bit by bit of its value, then of its place.
+//
+// 16 groups of 8 beams, 128256 tokens, k = 16: 17 us of 24 (73 in all with counting); all but 100 tokens masked: 64 in all (k = 64: 87), and 200 (627) where
+// a short list meant k rounds of the largest.
 __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const float* logits, const int* done, int vocab, int k, int slices, bool wide, SliceSum* sums,
                                                                       unsigned long long* keys) {
     chained_wait();
-    __shared__ __align__(16) float s_x[kSlice];   // only where the list is too short
-    unsigned long long* s_list = reinterpret_cast<unsigned long long*>(s_x);
-    __shared__ unsigned long long s_round[2][8];
+    __shared__ unsigned long long s_list[kListMax];
     __shared__ float s_top[8], s_low[16];
     __shared__ double s_sum[8];
-    __shared__ int s_count;
+    __shared__ int s_count, s_part[2][8];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slice = blockIdx.x;
     const int64_t row = blockIdx.y;
     if (done && __ldcg(done + row)) return;
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     }
     unsigned take = 0;
     float part = 0.f;
-    if (top > -INFINITY && top < INFINITY && bound > -INFINITY) {
+    if (top > -INFINITY && top < INFINITY && (bound > -INFINITY || n == kSlice)) {
         // exp(x - top), the exponent in two terms (log2(e) in one float32 is off by 2^-26); NaN where there is a NaN
         uint64_t sum = 0ull;
         const uint64_t minus_top = pair_f32(-top, -top), hi = pair_f32(1.44269502f, 1.44269502f), lo = pair_f32(1.9259629e-8f, 1.9259629e-8f);
@@ -143,6 +146,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
         }
         const float2 both = split_f32(sum);
         part = both.x + both.y;
+        if (bound == -INFINITY) take = 0xFFFFFFFFu;   // a NaN too, as minus infinity
     } else {   // the same for what is out of the ordinary; a NaN counts as minus infinity among the candidates
 #pragma unroll
         for (int j = 0; j < kSliceEach; ++j) {
@@ -157,7 +161,9 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
     if (take) {
-        int at = atomicAdd(&s_count, __popc(take));   // the order in the list does not matter
+        // The order in the list does not matter.  Many of one thread's mean a slice with many equal ones: no list of these.
+        int at = atomicAdd(&s_count, __popc(take) > kThreadMost ? kListMax + 1 : __popc(take));
+        if (__popc(take) > kThreadMost) at = kListMax;
 #pragma unroll 1
         for (unsigned left = take; left && at < kListMax; left &= left - 1, ++at) {   // read again: few, and a loop over registers would have to be unrolled
             const int j = __ffs(left) - 1, i = ((j >> 2) * kSliceThreads + t) * 4 + (j & 3);
@@ -170,51 +176,79 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const floa
         for (int w = 1; w < 8; ++w) sum += s_sum[w];
         sums[row * slices + slice] = SliceSum{sum, top, 0.f};
     }
-    const int have = s_count;
-    unsigned long long* out = keys + (row * slices + slice) * k;
-    if (have <= kListMax) {
-        for (int i0 = 0; i0 < have; i0 += kSliceThreads / 4) {   // four threads a candidate
-            const int i = i0 + (t >> 2);
-            const unsigned long long key = i < have ? s_list[i] : 0ull;
-            int rank = 0;
-#pragma unroll 4
-            for (int j = t & 3; j < have; j += 4) rank += s_list[j] > key;
-            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-            rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-            if ((t & 3) == 0 && i < have && rank < k) out[rank] = key;
-        }
-        for (int i = have + t; i < k; i += kSliceThreads) out[i] = 0ull;   // a short slice
-        return;
-    }
-    // Too many: rounds of the largest key, the logits in shared memory (a loop over registers would have to be unrolled).
-    __syncthreads();   // the list is done with
+    int have = s_count;
+    if (have > kListMax) {
+        auto place_of = [&](int j) { return ((j >> 2) * kSliceThreads + t) * 4 + (j & 3); };
+        int counts = 0;
+        auto count_all = [&](int c) {   // over the CTA
+            c = __reduce_add_sync(0xffffffffu, c);
+            int* part_of = s_part[counts++ & 1];
+            if (lane == 0) part_of[warp] = c;
+            __syncthreads();
+            int all = 0;
 #pragma unroll
-    for (int j = 0; j < kSliceEach; ++j) s_x[j * kSliceThreads + t] = x[j];
-    unsigned long long best = 0ull;
-    int from = 0;
-    bool look = true;
-    for (int i = 0; i < k; ++i) {
-        if (look) {   // this thread's best one of what is left
-            best = 0ull;
+            for (int w = 0; w < 8; ++w) all += part_of[w];
+            return all;
+        };
+        unsigned o[kSliceEach];   // the candidates in the order of unsigned numbers, else 0
+        const unsigned least_o = order_f32(bound + 0.f);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < kSliceEach; ++j) {
+            const int i = place_of(j);
+            const float y = i < n ? __ldcg(src + i) : -INFINITY;
+            o[j] = i < n && (y >= bound || bound == -INFINITY) ? order_f32(y == y ? y + 0.f : -INFINITY) : 0u;
+            c += o[j] > least_o || i < min(k, n);
+            if (i < min(k, n) && !o[j]) c += kSlice;
+        }
+        // The usual case: what is masked has one value, and the bound is that.  Where the slice's first k elements reach it, no other that equals
+        // it is among the k best.
+        const int few = count_all(c);
+        unsigned least = least_o;
+        int upto = k - 1;   // taken: what is above `least`, and what equals it up to this place
+        if (few > kListMax) {
+            least = 0u;   // the k-th largest
 #pragma unroll 1
-            for (unsigned left = take; left; left &= left - 1) {
-                const int j = __ffs(left) - 1;
-                const unsigned long long key = beam_key(s_x[j * kSliceThreads + t], (unsigned)(base + ((j >> 2) * kSliceThreads + t) * 4 + (j & 3)));
-                if (key > best) { best = key; from = j; }
+            for (unsigned bit = 1u << 31; bit; bit >>= 1) {
+                c = 0;
+#pragma unroll
+                for (int j = 0; j < kSliceEach; ++j) c += o[j] >= (least | bit);
+                if (count_all(c) >= k) least |= bit;
+            }
+            c = 0;
+#pragma unroll
+            for (int j = 0; j < kSliceEach; ++j) c += o[j] > least;
+            const int equal = k - count_all(c);   // of the elements that equal it, the first so many
+            upto = 0;
+#pragma unroll 1
+            for (int bit = kSlice / 2; bit; bit >>= 1) {
+                c = 0;
+#pragma unroll
+                for (int j = 0; j < kSliceEach; ++j) c += o[j] == least && place_of(j) < (upto | bit);
+                if (count_all(c) < equal) upto |= bit;
             }
         }
-        unsigned long long all = best;
-        for (int o = 16; o > 0; o >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
-        if (lane == 0) s_round[i & 1][warp] = all;
+        if (t == 0) s_count = 0;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) all = max(all, s_round[i & 1][w]);
-        look = all && best == all;   // keys differ, so one thread at most
-        if (look) {
-            take &= ~(1u << from);
-            out[i] = all;
-        }
+        for (int j = 0; j < kSliceEach; ++j)
+            if (o[j] > least || (o[j] == least && place_of(j) <= upto))
+                s_list[atomicAdd(&s_count, 1)] = (unsigned long long)o[j] << 32 | (0xFFFFFFFFu - (unsigned)(base + place_of(j)));
+        __syncthreads();
+        have = s_count;
     }
+    unsigned long long* out = keys + (row * slices + slice) * k;
+    for (int i0 = 0; i0 < have; i0 += kSliceThreads / 4) {   // four threads a candidate
+        const int i = i0 + (t >> 2);
+        const unsigned long long key = i < have ? s_list[i] : 0ull;
+        int rank = 0;
+#pragma unroll 4
+        for (int j = t & 3; j < have; j += 4) rank += s_list[j] > key;
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if ((t & 3) == 0 && i < have && rank < k) out[rank] = key;
+    }
+    for (int i = have + t; i < k; i += kSliceThreads) out[i] = 0ull;   // a short slice
 }
 
 // The largest of 32 pairs (high, low word), the same in all lanes.
