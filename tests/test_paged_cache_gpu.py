@@ -524,6 +524,19 @@ def test_rows_that_a_mask_has_left_little_of(masked, k):
     _check_beams(logits, -rng.random((4, 2)).astype(np.float32), k, exact_ids=False)
 
 
+@pytest.mark.parametrize("k", [1, 7, 33, 128])
+def test_the_best_all_in_one_thread(k):
+    """A slice whose largest logits a single thread holds, one whose first tokens are the largest, in rising and falling order."""
+    rng = np.random.default_rng(23)
+    logits = rng.standard_normal((2, 2, 8192 + 900)).astype(np.float32)
+    mine = (np.arange(8)[:, None] * 1024 + 4 * 37 + np.arange(4)).ravel()
+    logits[0, 0, mine] += 20.0
+    logits[0, 1, mine[:9]] = 20.0
+    logits[1, 0] = np.sort(logits[1, 0])[::-1]
+    logits[1, 1] = np.sort(logits[1, 1])
+    _check_beams(logits, -rng.random((2, 2)).astype(np.float32), k, exact_ids=False)
+
+
 def test_equal_candidates_go_to_the_lower_beam_and_token():
     """Equal beams on rows of every alignment, equal logits, a row of one value, more equal logits than a thread holds."""
     for vocab in (997, 1000, 20001):
