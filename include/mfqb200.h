@@ -522,8 +522,8 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
 /* Keeps the branch of every tree that the model agrees with: from the root on, the lowest child whose drafted token ids[r][child] is
  * the model's own targets[r][node] (device int32 [rows][nodes]).  Keys and values of the branch move together in all layers, to
  * slots lens[r] .. lens[r] + count[r] - 1.  Per sequence (device int32): count, the branch's nodes with the root; token, the target of
- * its last node; path [rows][nodes], the nodes, -1 behind them; lens_out = lens + count (it may be lens itself).  An unused row has
- * count 0, token -1 and keeps its length. */
+ * its last node; path [rows][nodes], the nodes, -1 behind them; lens_out = lens + count (it may be lens itself; no
+ * other output may overlap an input).  An unused row has count 0, token -1 and keeps its length. */
 int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count,
                      int32_t* token, int32_t* path, int32_t* lens_out, mfqb_stream_t stream);
 

@@ -165,13 +165,13 @@ class PagedCache:
         are given as ``lens_out``."""
         if ids.dim() != 2:
             raise ValueError(f"ids must be an int32 tensor [{self.rows}, nodes]")
-        nodes = ids.shape[1]
-        i, p, t = (self._int32(x, (self.rows, nodes), what) for x, what in ((ids, "ids"), (parents, "parents"), (targets, "targets")))
+        torch, nodes = _torch(), ids.shape[1]
+        shape = (self.rows, nodes)
+        i, p, t = self._int32(ids, shape, "ids"), self._int32(parents, shape, "parents"), self._int32(targets, shape, "targets")
         if lens_out is None:
-            lens_out = _torch().empty_like(self.lens)
+            lens_out = torch.empty_like(self.lens)
         elif self._int32(lens_out, (self.rows,), "lens_out") is not lens_out:
             raise ValueError("lens_out must be contiguous")
-        torch = _torch()
         count, token, path = torch.empty_like(self.lens), torch.empty_like(self.lens), torch.empty_like(i)
         _call(_fast.tree_accept, self.device, self._ptr, i.data_ptr(), p.data_ptr(), t.data_ptr(), nodes, count.data_ptr(), token.data_ptr(), path.data_ptr(),
               lens_out.data_ptr())

@@ -325,60 +325,62 @@ __global__ void __launch_bounds__(256) cache_write_kernel(mfqb_cache c, int laye
     }
 }
 
-// A warp per sequence walks its tree, two nodes a lane.
-__global__ void __launch_bounds__(32) accept_walk_kernel(mfqb_cache c, const int* ids, const int* parents, const int* targets, int nodes, int* count, int* token,
-                                                         int* path, int* lens_out) {
+// CTA (some layers' heads, sequence): its first warp walks the tree, two nodes a lane, the first CTA of a sequence leaves the results, and all move
+// the branch's rows, 64 at a time, which are its nodes in as many heads as that makes.  Every row is read into registers before the first one is
+// written, since a slot that one node leaves is another one's place.  A chain from the lengths to the rows: one tree of 8 nodes 4.2 us, 16 of 48
+// with branches of 13 in 128 heads 8.9 (a launch for the walk and one for the rows: 5.0 and 9.0; with a CTA for each head of each layer 11).
+__global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* ids, const int* parents, const int* targets, int nodes, int* count, int* token,
+                                                     int* path, int* lens_out) {
     chained_wait();
-    const int r = blockIdx.x, lane = threadIdx.x;
-    const int64_t base = (int64_t)r * nodes;
-    int id[2], up[2], to[2], mine[2] = {-1, -1};
+    __shared__ int s_path[kTreeNodes], s_n, s_token;
+    __shared__ int64_t s_from[kTreeNodes], s_to[kTreeNodes];   // rows of the branch in 16-byte pieces, for head 0 of layer 0; -1: stays
+    const int r = blockIdx.y, t = threadIdx.x, lane = t & 31, heads = c.layers * c.kv_heads;
+    const int64_t base = (int64_t)r * nodes, cap = (int64_t)c.width * c.page, len = min(max((int64_t)c.lens[r], (int64_t)0), cap);
+    if (t < 32) {
+        int id[2], up[2], to[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int j = lane + 32 * h;
-        const bool in = j < nodes;
-        id[h] = in ? __ldcg(ids + base + j) : 0;
-        up[h] = in ? __ldcg(parents + base + j) : -2;
-        to[h] = in ? __ldcg(targets + base + j) : 0;
-    }
-    const int64_t len = min(max((int64_t)c.lens[r], (int64_t)0), (int64_t)c.width * c.page);
-    int cur = 0, n = 0, want = -1;
-    if (__shfl_sync(0xffffffffu, up[0], 0) == -1) {
-        for (;;) {
-            if (lane == (n & 31)) mine[n >> 5] = cur;
-            ++n;
-            want = __shfl_sync(0xffffffffu, cur < 32 ? to[0] : to[1], cur & 31);
-            const unsigned lo = __ballot_sync(0xffffffffu, lane > cur && up[0] == cur && id[0] == want);
-            const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 > cur && up[1] == cur && id[1] == want);
-            if (!(lo | hi)) break;
-            cur = lo ? __ffs(lo) - 1 : __ffs(hi) + 31;
+        for (int h = 0; h < 2; ++h) {
+            const int j = lane + 32 * h;
+            const bool in = j < nodes;
+            id[h] = in ? __ldcg(ids + base + j) : 0;
+            up[h] = in ? __ldcg(parents + base + j) : -2;
+            to[h] = in ? __ldcg(targets + base + j) : 0;
+        }
+        int cur = 0, n = 0, want = -1;
+        if (__shfl_sync(0xffffffffu, up[0], 0) == -1) {
+            for (;;) {
+                if (lane == 0) s_path[n] = cur;
+                ++n;
+                want = __shfl_sync(0xffffffffu, cur < 32 ? to[0] : to[1], cur & 31);
+                const unsigned lo = __ballot_sync(0xffffffffu, lane > cur && up[0] == cur && id[0] == want);
+                const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 > cur && up[1] == cur && id[1] == want);
+                if (!(lo | hi)) break;
+                cur = lo ? __ffs(lo) - 1 : __ffs(hi) + 31;
+            }
+        }
+        if (lane == 0) {
+            s_n = n;
+            s_token = want;
         }
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (lane + 32 * h < nodes) path[base + lane + 32 * h] = mine[h];
-    if (lane == 0) {
-        count[r] = n;
-        token[r] = want;
-        lens_out[r] = (int)len + n;
+    __syncthreads();
+    const int n = s_n;
+    if (blockIdx.x == 0) {
+        if (t < nodes) path[base + t] = t < n ? s_path[t] : -1;
+        if (t == 0) {
+            count[r] = n;
+            token[r] = s_token;
+            if (lens_out) lens_out[r] = (int)len + n;
+        }
     }
-}
-
-// CTA (some layers' heads, sequence): 64 rows at a time, which are the branch's nodes in as many heads as that makes.  Every row is read into
-// registers before the first one is written, since a slot that one node leaves is another one's place.  (A CTA for each head of each
-// layer spent its time on the chain from the count to the rows: 16 branches of 13 nodes in 128 heads 11.0 us with the walk in place of 8.4.)
-__global__ void __launch_bounds__(256) accept_move_kernel(mfqb_cache c, int nodes, const int* count, const int* path, const int* lens_out) {
-    chained_wait();
-    const int r = blockIdx.y, n = __ldcg(count + r), t = threadIdx.x, heads = c.layers * c.kv_heads;
     if (n < 2) return;
     const int each = kTreeNodes / n;   // heads at a time
-    const int64_t len = __ldcg(lens_out + r) - n, cap = (int64_t)c.width * c.page;
-    __shared__ int64_t s_from[kTreeNodes], s_to[kTreeNodes];   // rows of the branch in 16-byte pieces, for head 0 of layer 0; -1: stays
     if (t < n) {
         auto slot = [&](int64_t p) -> int64_t {   // -1 where there is no page
             const int page = p < cap ? c.table[(int64_t)r * c.width + p / c.page] : -1;
             return (unsigned)page < (unsigned)c.pages ? ((int64_t)page * c.kv_heads * c.page + (p & (c.page - 1))) * 16 : -1;
         };
-        const int from = __ldcg(path + (int64_t)r * nodes + t);
+        const int from = s_path[t];
         s_to[t] = slot(len + t);
         s_from[t] = from == t || s_to[t] < 0 ? -1 : slot(len + from);
     }
@@ -405,6 +407,16 @@ __global__ void __launch_bounds__(256) accept_move_kernel(mfqb_cache c, int node
                 static_cast<uint4*>(c.v)[to[i]] = kv[i][1];
             }
     }
+}
+
+// The new lengths, where they take the place of the old ones, which all of accept_kernel's CTAs read.
+__global__ void __launch_bounds__(1024) accept_lens_kernel(mfqb_cache c, const int* count, int* lens_out) {
+    chained_wait();
+    const int r = threadIdx.x;
+    int len = 0;
+    if (r < c.rows) len = (int)min(max((int64_t)c.lens[r], (int64_t)0), (int64_t)c.width * c.page) + __ldcg(count + r);
+    __syncthreads();
+    if (r < c.rows) lens_out[r] = len;
 }
 
 }  // namespace mfqb
@@ -480,11 +492,12 @@ int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* par
         check_nodes(c, nodes, "mfqb_tree_accept");
         if (!ids || !parents || !targets || !count || !token || !path || !lens_out) fail(MFQB_ERR_ARG, "mfqb_tree_accept: null argument");
         if ((int64_t)c->layers * c->kv_heads > (1ll << 30)) fail(MFQB_ERR_UNSUPPORTED, "mfqb_tree_accept: too many layers x heads");
-        launch_chained(accept_walk_kernel, dim3(c->rows), dim3(32), 0, stream, *c, ids, parents, targets, nodes, count, token, path, lens_out);
         // enough CTAs for the SMs, at least one head each (how many nodes a branch has is known on the device alone)
         const int per_row = std::min(c->layers * c->kv_heads, std::max(1, 148 * 5 / c->rows));
-        launch_chained(accept_move_kernel, dim3((unsigned)per_row, c->rows), dim3(256), 0, stream, *c, nodes,
-                       static_cast<const int*>(count), static_cast<const int*>(path), static_cast<const int*>(lens_out));
+        const bool in_place = lens_out < c->lens + c->rows && c->lens < lens_out + c->rows;
+        launch_chained(accept_kernel, dim3((unsigned)per_row, c->rows), dim3(256), 0, stream, *c, ids, parents, targets, nodes, count, token, path,
+                       in_place ? nullptr : lens_out);
+        if (in_place) launch_chained(accept_lens_kernel, dim3(1), dim3(1024), 0, stream, *c, static_cast<const int*>(count), lens_out);
     });
 }
 
