@@ -431,8 +431,8 @@ int mfqb_decoder_read_cache(const mfqb_decoder* d, int layer, int row, int which
 int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_stream_t stream);
 /* Keys and values in pages (mfqb_cache, below): the decoder's passes run over this cache instead of its own, a row per sequence; the
  * memory stays the caller's and must outlive them.  Null: its own cache again.  A decoder that only ever uses pages is created with
- * max_ctx 0 and allocates no cache.  One rank only.  Allocates what a pass needs (not during a stream capture); graphs captured over
- * another cache before stay valid.
+ * max_ctx 0 and allocates no cache.  One rank only.  Allocates what a pass needs (not during a stream capture; where there is no
+ * memory for it, no pages are attached any more); graphs captured over another cache before stay valid.
  *
  * mfqb_decoder_step over pages takes batch = rows and advances lens by one; one more token per sequence must have been reserved
  * (mfqb_cache_extend).  Queries are rounded to bf16 there (the step over the decoder's own cache keeps them in float32).
