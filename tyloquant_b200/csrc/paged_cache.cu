@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(1024) fork_plan_kernel(mfqb_cache c, const int
         const int p = list[upto - 1];
         w.table[(int64_t)r * c.width + at] = p;
         w.copies[upto - 1] = ForkCopy{last, p, fill, 0};
-        w.delta[p] += 1;
+        w.delta[p] = (int)(1u - (unsigned)c.refs[p]);   // one holder, whatever a free page's count was
     }
     if (r == 0) {
         *status = 0;
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(1024) fork_plan_kernel(mfqb_cache c, const int
     __syncthreads();
     for (int e = r; e < entries; e += 1024) c.table[e] = w.table[e];
     for (int p = r; p < c.pages; p += 1024)
-        if (const int d = w.delta[p]) c.refs[p] += d;
+        if (const int d = w.delta[p]) c.refs[p] = (int)((unsigned)c.refs[p] + (unsigned)d);
 }
 
 // Copies of the filled part of a page: (copy, layer, head, keys or values) is one contiguous stretch of tokens * 256 bytes.  Bound by memory: 32
