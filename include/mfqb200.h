@@ -442,8 +442,9 @@ int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_s
  * stays.  mfqb_tree_accept keeps the branch that agrees.  A chain of nodes whose parents are the nodes before them is a piece of a prompt.
  * rows * nodes <= max_batch.
  *
- * mfqb_decoder_beam_step: the sequences are groups of `beams` beams (ids_in [rows]); reserves a token each, runs the model, selects the
- * best `beams` continuations of every group by scores [rows] + log softmax and forks the cache.  In place: scores, done (int32 [rows]); out:
+ * mfqb_decoder_beam_step: the sequences are groups of `beams` beams (ids_in [rows]); reserves a token for every beam that is not done, runs the
+ * model, selects the best `beams` continuations of every group by scores [rows] + log softmax and forks the cache.  A beam that is done keeps
+ * its score, its length and its pages (the token that ended it is not written), and takes no others.  In place: scores, done (int32 [rows]); out:
  * ids_out (the beams' new tokens), parents_out (the sequences they go on from), status [2]: of mfqb_cache_extend and of mfqb_cache_fork,
  * to be looked at before the results are used: where one is not 0, pages were missing, and scores, done, lengths and tokens are as
  * before the step, which can be done again.  A first step from one sequence per group starts the other beams' scores at minus

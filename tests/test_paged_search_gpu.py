@@ -1,0 +1,115 @@
+"""Beam search over pages: beams that have ended, steps that cannot be made, a search against beams run on their own."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+import paged_reference as R  # noqa: E402
+from test_nint_gpu import rel_l2  # noqa: E402
+from test_paged_decoder_gpu import DEV, _cache, _chain, _decoder, _i32, _prompt  # noqa: E402
+
+BITWISE = dict(ffn_profile=(4, 24, 6))   # no kernel whose sums differ in the last bit from call to call
+
+
+def _state(cache, *more):
+    return [x.clone() for x in (cache.k, cache.v, cache.table, cache.lens, cache.refs, *more)]
+
+
+def _restore(cache, saved, *more):
+    for x, y in zip((cache.k, cache.v, cache.table, cache.lens, cache.refs, *more), saved):
+        x.copy_(y)
+
+
+def _counts(cache):
+    return torch.bincount(cache.table[cache.table >= 0], minlength=cache.pages).int()
+
+
+def test_a_group_that_has_ended_takes_no_pages():
+    """A finished group at the end of its table, beside a living one that takes the last pages of the pool: its lengths, pages and scores stay,
+    and the living group goes on as it does beside a group that has room."""
+    dec = _decoder(64, **BITWISE)
+    got = []
+    for width, pages, length in ((2, 7, 32), (4, 40, 32)):
+        cache = _cache(4, pages=pages, width=width)
+        dec.set_cache(cache)
+        _prompt(dec, cache, _i32(np.random.default_rng(6).integers(0, 1000, (4, 12))))
+        assert int(cache.extend(_i32([length - 12] * 2 + [0, 0]))) == 0
+        cache.lens[:2] = length          # the first group's tables are full where they are two wide
+        assert int(cache.extend(_i32([0, 0, 4, 4]))) == 0
+        scores, done, tokens = torch.tensor([-3.0, -4.0, 0.0, -0.5], device=DEV), _i32([1, 1, 0, 0]), _i32([9, 9, 1, 2])
+        table, k, v = cache.table[:2].clone(), cache.k.clone(), cache.v.clone()
+        mine = table[:, :2].reshape(-1).long()
+        steps = []
+        for step in range(8):
+            tokens, parents, status = dec.beam_step(tokens, scores, done, 2, eos=-1)
+            if width == 2 and step == 4:
+                # past its first page the living group needs a page a beam and has one: that, and nothing else, stops it
+                assert int((cache.refs == 0).sum()) <= 1
+            if status.tolist() != [0, 0]:
+                break
+            steps.append((tokens[2:].tolist(), parents[2:].tolist(), scores[2:].tolist()))
+            assert cache.lens.tolist() == [length] * 2 + [12 + step + 1] * 2
+            assert scores[:2].tolist() == [-3.0, -4.0] and done.tolist() == [1, 1, 0, 0]
+            assert tokens[:2].tolist() == [0, 0] and parents[:2].tolist() == [0, 1]   # eos -1 is handed on as token 0
+            assert torch.equal(cache.table[:2, :2], table[:, :2]) and torch.equal(cache.k[:, mine], k[:, mine]) and torch.equal(cache.v[:, mine], v[:, mine])
+        got.append(steps)
+    assert len(got[0]) >= 4 and len(got[1]) == 8
+    for a, b in zip(*got):
+        assert a[0] == b[0] and a[1] == b[1] and np.allclose(a[2], b[2], atol=0.05)
+    dec.free()
+
+
+def test_a_beam_that_ends_stays_as_it_is():
+    """The token that a step selects first is made the end: that beam is done from then on, with its score, its length and that token, as long as it is
+    among the best; a captured step does the same."""
+    beams = 3
+    dec = _decoder(64, **BITWISE)
+    cache = _cache(2 * beams, pages=80)
+    dec.set_cache(cache)
+    _prompt(dec, cache, _i32(np.random.default_rng(7).integers(0, 1000, (2 * beams, 9))))
+    scores, done, tokens = torch.tensor([0.0, -9.0, -9.5] * 2, device=DEV), _i32([0] * 6), _i32([1, 2, 3, 4, 5, 6])
+    saved = _state(cache, scores, done)
+    dry, dry_from, _ = dec.beam_step(tokens, scores, done, beams, eos=-1)
+    dry_scores = scores.clone()
+    assert not done.any()
+    eos = int(dry[0])
+    _restore(cache, saved, scores, done)
+    tokens, parents, status = dec.beam_step(tokens, scores, done, beams, eos=eos)
+    assert torch.equal(tokens, dry) and torch.equal(parents, dry_from) and torch.equal(scores, dry_scores) and status.tolist() == [0, 0]
+    assert torch.equal(done, (dry == eos).int()) and int(done[0]) == 1
+    assert cache.lens.tolist() == [10] * 6   # the last token of each beam before this step
+    graph, stayed = None, 0
+    for step in range(12):
+        old_scores, old_done, old_lens = scores.tolist(), done.tolist(), cache.lens.tolist()
+        old_pages = [cache.table[r, :-(-n // 16)].tolist() for r, n in enumerate(old_lens)]
+        if step == 6:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                tokens, parents, status = dec.beam_step(tokens_in := tokens, scores, done, beams, eos=eos)
+        if graph is not None:
+            if step > 6:
+                tokens_in.copy_(tokens)
+            graph.replay()
+        else:
+            tokens, parents, status = dec.beam_step(tokens, scores, done, beams, eos=eos)
+        assert status.tolist() == [0, 0]
+        for r, p in enumerate(parents.tolist()):
+            assert r // beams == p // beams
+            if old_done[p]:
+                stayed += 1
+                assert int(done[r]) == 1 and int(tokens[r]) == eos and float(scores[r]) == old_scores[p] and int(cache.lens[r]) == old_lens[p]
+                n = old_lens[p] // 16   # whole pages are the same ones
+                assert cache.table[r, :n].tolist() == old_pages[p][:n]
+            else:
+                assert int(done[r]) == int(int(tokens[r]) == eos) and float(scores[r]) < old_scores[p] and int(cache.lens[r]) == old_lens[p] + 1
+        assert parents[:beams].tolist().count(0) >= 1 or not old_done[0]   # the best beam, done, is never lost
+        assert torch.equal(cache.refs, _counts(cache))
+        # what is held is what the lengths need
+        assert [(row >= 0).sum().item() for row in cache.table] == [-(-n // 16) for n in cache.lens.tolist()]
+    assert stayed >= 12
+    dec.free()
+
+

@@ -558,14 +558,26 @@ __global__ void add_one_kernel(int* p, int n) {
     if (i < n) p[i] += 1;
 }
 
-// Between the selection and the fork: the step's token counts where its page could be had; else no sequence moves.
-__global__ void __launch_bounds__(1024) beam_move_kernel(const int* status, const int* parents, int rows, int* lens, int* moves) {
+// Before a beam step: a beam that is done needs its score alone.  No token is reserved for it, its keys and values are behind the end of its
+// table, where there is no page, and it reads no context.
+__global__ void __launch_bounds__(1024) beam_begin_kernel(const int* done, const int* lens, int rows, int capacity, int* tokens, int* write_lens, int* read_lens) {
+    dep_wait();
+    const int r = threadIdx.x;
+    if (r >= rows) return;
+    const bool over = __ldcg(done + r) != 0;
+    const int len = __ldcg(lens + r);
+    tokens[r] = over ? 0 : 1;
+    write_lens[r] = over ? capacity : len;
+    read_lens[r] = over ? 0 : len;
+}
+// Between the selection and the fork: the step's tokens count where their pages could be had; else no sequence moves.
+__global__ void __launch_bounds__(1024) beam_move_kernel(const int* status, const int* done, const int* parents, int rows, int* lens, int* moves) {
     dep_wait();
     const int r = threadIdx.x;
     if (r >= rows) return;
     const bool ok = status[0] == 0;
     moves[r] = ok ? parents[r] : r;
-    if (ok) lens[r] += 1;
+    if (ok && !done[r]) lens[r] += 1;
 }
 // The chosen beams become the sequences' state: scores, tokens, and done where the beam that goes on was done or has now ended.  Where pages
 // were missing everything is as before the step, which can be done again.
@@ -588,7 +600,7 @@ __global__ void __launch_bounds__(1024) beam_take_kernel(const int* status, cons
     } else {
         ids[r] = ids_in[r];
         parents[r] = r;
-        if (reserved) lens[r] -= 1;
+        if (reserved && !done[r]) lens[r] -= 1;
     }
 }
 
@@ -617,12 +629,13 @@ struct mfqb_decoder {
     // Keys and values in pages (mfqb_decoder_set_cache): the step's rows are the nodes of the cache's sequences
     bool paged = false;
     mfqb_cache cache{};
-    int nodes = 1;                          // of the forward pass that is being queued
-    const uint64_t* node_masks = nullptr;   // its masks and depths
+    mfqb_cache write_to{}, read_from{};     // the same with the lengths that the forward pass which is being queued goes by
+    int nodes = 1;                          // of that pass
+    const uint64_t* node_masks = nullptr;   // masks and depths
     const int32_t* node_depths = nullptr;
     uint64_t attn_work_bytes = 0;
     std::vector<DevBuf> retired;   // buffers that a larger cache outgrew: graphs captured before still use them
-    DevBuf q16, freqs, masks, depths, single_masks, single_depths, attn_work, beam_work, beam_scores, beam_tokens, beam_moves, fork_work, one_each;
+    DevBuf q16, freqs, masks, depths, single_masks, single_depths, attn_work, beam_work, beam_scores, beam_tokens, beam_moves, beam_counts, fork_work;
     DevBuf gamma_final;
     // workspaces
     DevBuf h, h2, xn, qkv, attn, attn_count, inv_freq, rope_table, proj, proj_sum, act, logits, part, best_val, best_idx, part_val, part_idx, gathered, gathered_sum, pos;
@@ -706,8 +719,8 @@ static void attend_own(mfqb_decoder* d, DecoderLayer& L, int rows, cudaStream_t 
 
 // Rotary embedding, cache write and attention of the nodes over the attached pages.
 static void attend_pages(mfqb_decoder* d, int li, cudaStream_t s) {
-    check(mfqb_cache_write(&d->cache, li, static_cast<const float*>(d->qkv.p), d->nq, d->nodes, d->node_depths, static_cast<const double*>(d->freqs.p), d->q16.p, s));
-    check(mfqb_tree_attention(&d->cache, li, d->q16.p, d->nq, d->nodes, d->node_masks, 0.08838834764831845f, d->attn.p, d->attn_work.p, d->attn_work_bytes, s));
+    check(mfqb_cache_write(&d->write_to, li, static_cast<const float*>(d->qkv.p), d->nq, d->nodes, d->node_depths, static_cast<const double*>(d->freqs.p), d->q16.p, s));
+    check(mfqb_tree_attention(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, 0.08838834764831845f, d->attn.p, d->attn_work.p, d->attn_work_bytes, s));
 }
 
 // One transformer block on the residual stream d->h for `rows` sequences; `delta` is the previous
@@ -776,9 +789,10 @@ static void check_ready(const mfqb_decoder* d, int rows, const char* who) {
         if (!L.qkv) fail(MFQB_ERR_ARG, "%s: a layer has no weights", who);
     if (!d->paged && d->cfg.max_ctx < 1) fail(MFQB_ERR_ARG, "%s: the decoder has no cache of its own (max_ctx 0) and none is attached", who);
 }
-// The next pass has one node per sequence.
+// The next pass has one node per sequence, at the cache's own lengths.
 static void single_nodes(mfqb_decoder* d) {
     d->nodes = 1;
+    d->write_to = d->read_from = d->cache;
     d->node_masks = static_cast<const uint64_t*>(d->single_masks.p);
     d->node_depths = static_cast<const int32_t*>(d->single_depths.p);
 }
@@ -1018,7 +1032,7 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
         double freqs[kHeadDim / 2];
         for (int i = 0; i < kHeadDim / 2; ++i) freqs[i] = std::pow((double)d->cfg.rope_theta, -2.0 * i / kHeadDim);
         std::vector<uint64_t> one(rows, 1);
-        std::vector<int32_t> zero(rows, 0), ones(rows, 1);
+        std::vector<int32_t> zero(rows, 0);
         d->paged = false;
         room(d, d->q16, B * d->nq * kHeadDim * 2);
         room(d, d->masks, B * 8);
@@ -1029,10 +1043,10 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
         room(d, d->beam_scores, rows * 4);
         room(d, d->beam_tokens, rows * 4);
         room(d, d->beam_moves, rows * 4);
+        room(d, d->beam_counts, rows * 12);
         if (room(d, d->freqs, sizeof(freqs))) MFQB_CUDA(cudaMemcpy(d->freqs.p, freqs, sizeof(freqs), cudaMemcpyHostToDevice));
         if (room(d, d->single_masks, rows * 8)) MFQB_CUDA(cudaMemcpy(d->single_masks.p, one.data(), rows * 8, cudaMemcpyHostToDevice));
         if (room(d, d->single_depths, rows * 4)) MFQB_CUDA(cudaMemcpy(d->single_depths.p, zero.data(), rows * 4, cudaMemcpyHostToDevice));
-        if (room(d, d->one_each, rows * 4)) MFQB_CUDA(cudaMemcpy(d->one_each.p, ones.data(), rows * 4, cudaMemcpyHostToDevice));
         d->cache = *cache;
         d->paged = true;
     });
@@ -1048,6 +1062,7 @@ int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* pare
         DeviceGuard guard(d->device);
         check(mfqb_tree_masks(parents, d->cache.rows, nodes, static_cast<uint64_t*>(d->masks.p), static_cast<int32_t*>(d->depths.p), stream));
         d->nodes = nodes;
+        d->write_to = d->read_from = d->cache;
         d->node_masks = static_cast<const uint64_t*>(d->masks.p);
         d->node_depths = static_cast<const int32_t*>(d->depths.p);
         forward_argmax(d, ids, rows, stream);
@@ -1073,13 +1088,18 @@ int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, fl
             if (capturing != cudaStreamCaptureStatusNone) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: one call with this many beams must come before a stream capture");
             room(d, d->beam_work, bytes);
         }
-        check(mfqb_cache_extend(&d->cache, static_cast<const int32_t*>(d->one_each.p), status, s));
+        int* counts = static_cast<int*>(d->beam_counts.p);   // tokens to reserve, lengths to write at, lengths to read
+        launch_dep(beam_begin_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(done), static_cast<const int*>(d->cache.lens), rows,
+                   d->cache.width * d->cache.page, counts, counts + rows, counts + 2 * rows);
+        check(mfqb_cache_extend(&d->cache, counts, status, s));
         single_nodes(d);
+        d->write_to.lens = counts + rows;
+        d->read_from.lens = counts + 2 * rows;
         forward_logits(d, ids_in, rows, s);
         check(mfqb_beam_select(static_cast<const float*>(d->logits.p), rows / beams, beams, d->vshard, scores, done, eos, beams, static_cast<float*>(d->beam_scores.p),
                                parents_out, static_cast<int32_t*>(d->beam_tokens.p), d->beam_work.p, d->beam_work.bytes, s));
-        launch_dep(beam_move_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const int*>(parents_out), rows, d->cache.lens,
-                   static_cast<int*>(d->beam_moves.p));
+        launch_dep(beam_move_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const int*>(done), static_cast<const int*>(parents_out), rows,
+                   d->cache.lens, static_cast<int*>(d->beam_moves.p));
         check(mfqb_cache_fork(&d->cache, static_cast<const int32_t*>(d->beam_moves.p), status + 1, d->fork_work.p, d->fork_work.bytes, s));
         launch_dep(beam_take_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const float*>(d->beam_scores.p),
                    static_cast<const int*>(d->beam_tokens.p), rows, eos, static_cast<const int*>(ids_in), d->cache.lens, scores, static_cast<int*>(done),
