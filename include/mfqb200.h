@@ -447,8 +447,9 @@ int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_s
  * its score, its length and its pages (the token that ended it is not written), and takes no others.  In place: scores, done (int32 [rows]); out:
  * ids_out (the beams' new tokens), parents_out (the sequences they go on from), status [2]: of mfqb_cache_extend and of mfqb_cache_fork,
  * to be looked at before the results are used: where one is not 0, pages were missing, and scores, done, lengths and tokens are as
- * before the step, which can be done again.  A first step from one sequence per group starts the other beams' scores at minus
- * infinity.  One call with as many beams must come before a stream capture. */
+ * before the step, which can be done again; reserved pages stay reserved, the step's own too where it was the fork that lacked some.  (A step
+ * that is made gives back what was reserved behind the lengths, as every fork does.)  A first step from one sequence per group starts
+ * the other beams' scores at minus infinity.  One call with as many beams must come before a stream capture. */
 struct mfqb_cache;
 int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
 int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream);

@@ -27,6 +27,50 @@ def _counts(cache):
     return torch.bincount(cache.table[cache.table >= 0], minlength=cache.pages).int()
 
 
+def test_a_step_that_lacks_pages_changes_nothing():
+    """Neither lengths nor pages that the caller has reserved behind them: the step is done again when there is room."""
+    dec = _decoder(64)
+    cache = _cache(2, pages=6, width=5)
+    dec.set_cache(cache)
+    _prompt(dec, cache, _i32(np.random.default_rng(5).integers(0, 1000, (2, 16))))
+    assert int(cache.extend(_i32([40, 0]))) == 0   # three more pages for the first sequence; the second needs one
+    cache.refs[cache.refs == 0] = 1                # and somebody else holds the last
+    scores, done, tokens = torch.tensor([-1.0, -2.0], device=DEV), _i32([0, 0]), _i32([3, 4])
+    before = _state(cache, scores, done)
+    got, parents, status = dec.beam_step(tokens, scores, done, 2, eos=-1)
+    assert status.tolist() == [1, 0] and got.tolist() == [3, 4] and parents.tolist() == [0, 1]
+    for x, y in zip((cache.table, cache.lens, cache.refs, scores, done), before[2:]):
+        assert torch.equal(x, y)
+    cache.refs[(cache.refs == 1) & (_counts(cache) == 0)] = 0
+    got, parents, status = dec.beam_step(tokens, scores, done, 2, eos=-1)
+    assert status.tolist() == [0, 0] and cache.lens.tolist() == [17, 17]
+    assert torch.equal(cache.refs, _counts(cache))
+    dec.free()
+
+
+def test_a_fork_that_lacks_pages_changes_nothing():
+    """Both beams go on from the first, the pages of the second are held elsewhere too: there is none for the copy."""
+    dec = _decoder(64)
+    cache = _cache(4, pages=8, width=4)
+    dec.set_cache(cache)
+    _prompt(dec, cache, _i32(np.random.default_rng(5).integers(0, 1000, (4, 16))))
+    assert int(cache.extend(4)) == 0   # two pages each, none is left
+    cache.lens.copy_(_i32([20, 31, 19, 20]))
+    cache.refs[cache.table[1, :2].long()] += 1
+    scores, done, tokens = torch.tensor([0.0, -1e4, -2.0, -3.0], device=DEV), _i32([0, 0, 1, 1]), _i32([3, 4, 5, 6])
+    before = _state(cache, scores, done)
+    for _ in range(2):
+        got, parents, status = dec.beam_step(tokens, scores, done, 2, eos=-1)
+        assert status.tolist() == [0, 1] and got.tolist() == [3, 4, 5, 6] and parents.tolist() == [0, 1, 2, 3]
+        for x, y in zip((cache.table, cache.lens, cache.refs, scores, done), before[2:]):
+            assert torch.equal(x, y)
+    cache.refs[cache.table[1, :2].long()] -= 1   # its other holder lets go
+    got, parents, status = dec.beam_step(tokens, scores, done, 2, eos=-1)
+    assert status.tolist() == [0, 0] and parents.tolist() == [0, 0, 2, 3] and cache.lens.tolist() == [21, 21, 19, 20]
+    assert torch.equal(cache.refs, _counts(cache))
+    dec.free()
+
+
 def test_a_group_that_has_ended_takes_no_pages():
     """A finished group at the end of its table, beside a living one that takes the last pages of the pool: its lengths, pages and scores stay,
     and the living group goes on as it does beside a group that has room."""

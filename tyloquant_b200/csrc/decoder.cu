@@ -570,18 +570,19 @@ __global__ void __launch_bounds__(1024) beam_begin_kernel(const int* done, const
     write_lens[r] = over ? capacity : len;
     read_lens[r] = over ? 0 : len;
 }
-// Between the selection and the fork: the step's tokens count where their pages could be had; else no sequence moves.
+// Between the selection and the fork: the step's tokens count where their pages could be had; else the fork is one that changes nothing (parents
+// that are no sequences).
 __global__ void __launch_bounds__(1024) beam_move_kernel(const int* status, const int* done, const int* parents, int rows, int* lens, int* moves) {
     dep_wait();
     const int r = threadIdx.x;
     if (r >= rows) return;
     const bool ok = status[0] == 0;
-    moves[r] = ok ? parents[r] : r;
+    moves[r] = ok ? parents[r] : -2;
     if (ok && !done[r]) lens[r] += 1;
 }
 // The chosen beams become the sequences' state: scores, tokens, and done where the beam that goes on was done or has now ended.  Where pages
 // were missing everything is as before the step, which can be done again.
-__global__ void __launch_bounds__(1024) beam_take_kernel(const int* status, const float* best, const int* tokens, int rows, int eos, const int* ids_in, int* lens,
+__global__ void __launch_bounds__(1024) beam_take_kernel(int* status, const float* best, const int* tokens, int rows, int eos, const int* ids_in, int* lens,
                                                          float* scores, int* done, int* ids, int* parents) {
     dep_wait();
     const int r = threadIdx.x;
@@ -592,6 +593,7 @@ __global__ void __launch_bounds__(1024) beam_take_kernel(const int* status, cons
         over = p < 0 || done[p] || tokens[r] == eos;
     }
     __syncthreads();
+    if (r == 0 && !reserved) status[1] = 0;   // there was no fork that could lack pages
     if (r >= rows) return;
     if (ok) {
         done[r] = over;
@@ -1101,7 +1103,7 @@ int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, fl
         launch_dep(beam_move_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const int*>(done), static_cast<const int*>(parents_out), rows,
                    d->cache.lens, static_cast<int*>(d->beam_moves.p));
         check(mfqb_cache_fork(&d->cache, static_cast<const int32_t*>(d->beam_moves.p), status + 1, d->fork_work.p, d->fork_work.bytes, s));
-        launch_dep(beam_take_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(status), static_cast<const float*>(d->beam_scores.p),
+        launch_dep(beam_take_kernel, dim3(1), dim3(1024), s, static_cast<int*>(status), static_cast<const float*>(d->beam_scores.p),
                    static_cast<const int*>(d->beam_tokens.p), rows, eos, static_cast<const int*>(ids_in), d->cache.lens, scores, static_cast<int*>(done),
                    static_cast<int*>(ids_out), static_cast<int*>(parents_out));
     });
