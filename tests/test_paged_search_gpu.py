@@ -157,3 +157,22 @@ def test_a_beam_that_ends_stays_as_it_is():
     dec.free()
 
 
+def test_tokens_that_go_round_in_place():
+    """The tokens that one step writes are the next one's input, with nothing between the two; against steps that are waited for."""
+    beams, runs = 4, []
+    dec = _decoder(64, **BITWISE)
+    for wait in (True, False):
+        cache = _cache(beams, pages=40)
+        dec.set_cache(cache)
+        _prompt(dec, cache, _i32(np.random.default_rng(8).integers(0, 1000, (beams, 5))))
+        scores, done, tokens = torch.zeros(beams, device=DEV), _i32([0] * beams), _i32([1, 2, 3, 4])
+        history = []
+        for _ in range(30):
+            tokens, parents, _ = dec.beam_step(tokens, scores, done, beams, eos=-1)
+            if wait:
+                torch.cuda.synchronize()
+                tokens = tokens.clone()
+            history.append((tokens, parents))
+        runs.append((torch.stack([torch.stack(h) for h in history]), scores, cache.k))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    dec.free()

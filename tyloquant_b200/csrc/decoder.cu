@@ -506,11 +506,12 @@ __global__ void argmax_pack_kernel(const float* __restrict__ val, const int* __r
     out[i] = w == rank ? (f ? (float)idx[r] : val[r]) : 0.f;
 }
 
-// Embedding rows: h[r, :] = table[ids[r], :] (bf16 table) as float32.
-__global__ void embed_rows_kernel(const int* __restrict__ ids, const __nv_bfloat16* __restrict__ table, float* __restrict__ h, int H, int vocab) {
+// Embedding rows: h[r, :] = table[ids[r], :] (bf16 table) as float32.  The tokens may be the output of a beam step that still runs when this kernel
+// starts: they are read behind the wait and from the L2 cache, not as constants.
+__global__ void embed_rows_kernel(const int* ids, const __nv_bfloat16* __restrict__ table, float* __restrict__ h, int H, int vocab) {
     dep_wait();
     const int r = blockIdx.x;
-    const int id = min(max(ids[r], 0), vocab - 1);
+    const int id = min(max(__ldcg(ids + r), 0), vocab - 1);
     const uint2* src = reinterpret_cast<const uint2*>(table + (size_t)id * H);   // H is a multiple of 8: four bf16 per load
     float4* dst = reinterpret_cast<float4*>(h + (size_t)r * H);
     for (int i = threadIdx.x; i < (H >> 2); i += blockDim.x) {
