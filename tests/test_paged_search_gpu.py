@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 
 import paged_reference as R  # noqa: E402
 from test_nint_gpu import rel_l2  # noqa: E402
-from test_paged_decoder_gpu import DEV, _cache, _chain, _decoder, _i32, _prompt  # noqa: E402
+from test_paged_decoder_gpu import DEV, _cache, _chain, _decoder, _i32, _prompt, _sequence  # noqa: E402
 
 BITWISE = dict(ffn_profile=(4, 24, 6))   # no kernel whose sums differ in the last bit from call to call
 
@@ -175,4 +175,73 @@ def test_tokens_that_go_round_in_place():
             history.append((tokens, parents))
         runs.append((torch.stack([torch.stack(h) for h in history]), scores, cache.k))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+    dec.free()
+
+
+def test_one_beam_is_the_greedy_step():
+    dec = _decoder(64, **BITWISE)
+    caches = [_cache(1), _cache(1)]
+    prompt = _i32(np.random.default_rng(9).integers(0, 1000, (1, 7)))
+    for c in caches:
+        dec.set_cache(c)
+        _prompt(dec, c, prompt)
+    token = [_i32([11]), _i32([11])]
+    scores, done = torch.zeros(1, device=DEV), _i32([0])
+    for _ in range(20):
+        dec.set_cache(caches[0])
+        assert int(caches[0].extend(1)) == 0
+        token[0] = dec.step(token[0])
+        dec.set_cache(caches[1])
+        token[1], parents, status = dec.beam_step(token[1], scores, done, 1, eos=-1)
+        assert torch.equal(token[0], token[1]) and parents.tolist() == [0] and status.tolist() == [0, 0]
+    assert caches[0].lens.tolist() == caches[1].lens.tolist() == [27]
+    dec.free()
+
+
+def test_every_step_of_a_search():
+    """Rows, tokens and scores of each step are those that 64 bits select from the step's own logits; the logits of every beam, and at the end its keys
+    and values token by token, are those of its tokens run on their own."""
+    beams, steps = 4, 10
+    dec = _decoder(96)
+    prompt = _i32(np.random.default_rng(100).integers(0, 1000, (1, 18)))
+    cache = _cache(beams, pages=30)
+    dec.set_cache(cache)
+    ids, chain = prompt.repeat(beams, 1), _chain(beams, 17)
+    chain[1:] = -2   # one sequence has the prompt, up to its last token
+    assert int(cache.extend(_i32([17] + [0] * (beams - 1)))) == 0
+    dec.verify(ids[:, :17].contiguous(), chain)
+    cache.accept(ids[:, :17].contiguous(), chain, torch.cat([ids[:, 1:17], ids[:, :1]], 1).contiguous(), lens_out=cache.lens)
+    assert int(cache.fork(_i32([0] * beams))) == 0
+    scores = torch.tensor([0.0] + [-np.inf] * (beams - 1), dtype=torch.float32, device=DEV)
+    done, tokens, history, moved = _i32([0] * beams), prompt[:, -1].repeat(beams).contiguous(), [[]] * beams, 0
+    logits, asked = [], []
+    for _ in range(steps):
+        before = scores.cpu().numpy().copy()
+        tokens, parents, status = dec.beam_step(tokens, scores, done, beams, eos=-1)
+        assert status.tolist() == [0, 0]
+        z = dec.read_logits(beams)
+        logits.append(z.cpu().numpy())
+        asked.append(history)
+        cand = R.beam_candidates(logits[-1][None], before[None], None, -1, beams)[0][:beams]
+        assert [(p, t) for _, p, t in cand] == list(zip(parents.tolist(), tokens.tolist()))
+        # a float32 rounding, and the log of a sum of float32 exponentials with 2^-21 each
+        assert all(abs(s - c[0]) <= 2.0 ** -24 * abs(c[0]) + 2.0 ** -20 for s, c in zip(scores.tolist(), cand))
+        moved += parents.tolist() != list(range(beams))
+        history = [history[p] + [t] for p, t in zip(parents.tolist(), tokens.tolist())]
+    assert moved >= 3 and torch.equal(cache.refs, _counts(cache))
+    held = [(history[r], _sequence(cache, r, "k"), _sequence(cache, r, "v")) for r in range(beams)]
+    for z, beams_then in zip(logits, asked):
+        for b, toks in enumerate(beams_then):
+            alone = _cache(1)
+            dec.set_cache(alone)
+            want = _prompt(dec, alone, torch.cat([prompt, _i32([toks])], 1).contiguous() if toks else prompt)[0, -1]
+            assert rel_l2(z[b], want.cpu().numpy()) <= 1e-2, (b, toks)
+    for toks, k, v in held:   # the last token is not in the cache yet
+        alone = _cache(1)
+        dec.set_cache(alone)
+        _prompt(dec, alone, torch.cat([prompt, _i32([toks[:-1]])], 1).contiguous())
+        for got, which in ((k, "k"), (v, "v")):
+            want = _sequence(alone, 0, which)
+            assert got.shape == want.shape
+            assert all(rel_l2(got[layer, t], want[layer, t]) <= 1e-2 for layer in range(got.shape[0]) for t in range(got.shape[1]))
     dec.free()
