@@ -472,9 +472,10 @@ int mfqb_decoder_free(mfqb_decoder* d);
  *
  * Pages are written only at positions from lens on, and mfqb_cache_fork leaves every page that is partly filled to one
  * sequence, so pages that sequences share are never written.  Calls on one cache must be ordered by their streams; calls on
- * different caches share nothing.  No call allocates device memory, none waits for the device: all can be captured, after a first
- * call of each kind outside a capture (the driver loads a kernel's code at its first launch; the *_work calls ready the device).
- * Waits inside the attention kernel are bounded: see mfqb_device_status.  Other holders than the table's entries hold whole pages.
+ * different caches share nothing.  An output overlaps no input and no other output unless its call says so.  No call allocates
+ * device memory, none waits for the device: all can be captured, after a first call of each kind outside a capture (the driver
+ * loads a kernel's code at its first launch; the *_work calls ready the device).  Waits inside the attention kernel are
+ * bounded: see mfqb_device_status.  Other holders than the table's entries hold whole pages.
  * --------------------------------------------------------------------------------- */
 typedef struct mfqb_cache {
     void* k;

@@ -36,6 +36,11 @@ inline void check_nodes(const mfqb_cache* c, int nodes, const char* who) {
     if ((int64_t)nodes > (int64_t)c->width * c->page) fail(MFQB_ERR_ARG, "%s: %d nodes do not fit a table of %d pages of %d", who, nodes, c->width, c->page);
 }
 
+inline void check_apart(const void* out, uint64_t out_bytes, const void* in, uint64_t in_bytes, const char* who, const char* what) {
+    const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
+    if (o < i + in_bytes && i < o + out_bytes) fail(MFQB_ERR_ARG, "%s: %s overlap", who, what);
+}
+
 // Launched with the programmatic-dependent-launch attribute: the kernel becomes resident while its predecessor runs and waits
 // (after_predecessor) until that one has completed.
 template <typename... KArgs, typename... Args>

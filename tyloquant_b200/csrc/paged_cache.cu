@@ -478,6 +478,8 @@ int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_hea
         if ((uintptr_t)freqs & 7) fail(MFQB_ERR_ARG, "mfqb_cache_write: freqs must be 8-byte aligned");
         if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "mfqb_cache_write: layer %d of %d", layer, c->layers);
         if (q_heads < 1 || q_heads > 16384) fail(MFQB_ERR_ARG, "mfqb_cache_write: bad number of query heads %d", q_heads);
+        const uint64_t tokens = (uint64_t)c->rows * nodes;   // a head's queries are written elsewhere than they are read, while other CTAs read
+        check_apart(q_out, 256 * tokens * q_heads, qkv, 512 * tokens * (q_heads + 2 * c->kv_heads), "mfqb_cache_write", "qkv and q_out");
         // one CTA per token once there are CTAs for every SM, else its heads spread over more of them
         const int parts = c->rows * nodes >= 148 ? 1 : (q_heads + 2 * c->kv_heads + 15) / 16;
         launch_chained(cache_write_kernel, dim3(parts, nodes, c->rows), dim3(256), 0, stream, *c, layer, qkv, q_heads, nodes, depths, freqs,

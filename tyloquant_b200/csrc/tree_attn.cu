@@ -965,6 +965,9 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
         if (((uintptr_t)work & 15) || work_bytes < tree_attention_work_bytes(*c, q_heads, nodes))
             fail(MFQB_ERR_ARG, "mfqb_tree_attention: work must be 16-byte aligned and hold %llu bytes, got %llu",
                  (unsigned long long)tree_attention_work_bytes(*c, q_heads, nodes), (unsigned long long)work_bytes);
+        // add_bad_nodes reads the queries of rows that have been written
+        const uint64_t bytes = 256ull * c->rows * nodes * q_heads;
+        check_apart(out, bytes, q, bytes, "mfqb_tree_attention", "q and out");
         launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, work, stream);
     });
 }
