@@ -119,3 +119,14 @@ def test_a_captured_verification_replays():
             assert (want[2] >= 2).all()
     assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].table, caches[1].table)
     dec.free()
+
+
+def test_tensors_of_a_cache_are_not_exchanged():
+    """The library holds their addresses: another tensor under the same name would not be what the calls work on."""
+    cache = _cache(2)
+    for name in ("k", "v", "table", "lens", "refs"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, getattr(cache, name).clone())
+    lens = cache.lens
+    cache.lens += 3   # in place: the same tensor
+    assert cache.lens is lens and cache.lens.tolist() == [3, 3]

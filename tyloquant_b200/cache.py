@@ -59,7 +59,15 @@ def tree_masks(parents):
 
 class PagedCache:
     """Keys and values ``k``, ``v`` bf16 [layers, pages, kv_heads, page, 128], ``table`` int32 [rows, width], ``lens`` int32 [rows],
-    ``refs`` int32 [pages], all contiguous on one device; the tensors stay the caller's and are changed in place."""
+    ``refs`` int32 [pages], all contiguous on one device; the tensors stay the caller's and are changed in place, never exchanged.
+
+    The object holds a workspace beside them: like them it has to live as long as calls on it are under way on other streams
+    than that it was made on, and as long as a graph that has captured its calls is replayed."""
+
+    def __setattr__(self, name, value):
+        if name in ("k", "v", "table", "lens", "refs") and getattr(self, name, value) is not value:
+            raise AttributeError(f"{name} of a cache is not exchanged, the library holds its address: change it in place")
+        object.__setattr__(self, name, value)
 
     def __init__(self, k, v, table, lens, refs):
         torch = _torch()
