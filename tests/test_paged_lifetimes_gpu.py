@@ -130,3 +130,29 @@ def test_tensors_of_a_cache_are_not_exchanged():
     lens = cache.lens
     cache.lens += 3   # in place: the same tensor
     assert cache.lens is lens and cache.lens.tolist() == [3, 3]
+
+
+def test_tokens_with_a_stride():
+    """A column of a matrix is a batch of tokens like any other; outputs that a step cannot fill are refused."""
+    dec = _decoder(8, max_ctx=40, **BITWISE)
+    ids = _i32(np.random.default_rng(5).integers(0, 1000, (3, 8)))
+    for paged in (False, True):
+        got = []
+        for contiguous in (True, False):
+            if paged:
+                cache = _cache(3)
+                dec.set_cache(cache)
+                assert int(cache.extend(8)) == 0
+            else:
+                dec.fill_cache(0)
+            run = []
+            for i in range(8):
+                dec.step(ids[:, i].contiguous() if contiguous else ids[:, i])
+                run.append(dec.read_logits(3))
+            got.append(torch.stack(run))
+        assert torch.equal(*got)
+    out = torch.empty(3, 2, dtype=torch.int32, device=DEV)
+    for bad in (out[:, 0], out[:2, 0].contiguous(), torch.empty(3, dtype=torch.int64, device=DEV), torch.empty(3, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="ids_out"):
+            dec.step(ids[:, 0], bad)
+    dec.free()

@@ -46,9 +46,13 @@ class Decoder:
 
     def step(self, ids_in, ids_out=None):
         torch = _torch()
-        if ids_in.dtype != torch.int32 or not ids_in.is_cuda:
-            raise ValueError("ids_in must be an int32 CUDA tensor [batch]")
-        ids_out = torch.empty_like(ids_in) if ids_out is None else ids_out
+        if ids_in.dtype != torch.int32 or ids_in.get_device() != self.device:
+            raise ValueError(f"ids_in must be an int32 tensor [batch] on cuda:{self.device}")
+        ids_in = ids_in.contiguous()
+        if ids_out is None:
+            ids_out = torch.empty_like(ids_in)
+        elif ids_out.dtype != torch.int32 or ids_out.get_device() != self.device or ids_out.numel() < ids_in.numel() or not ids_out.is_contiguous():
+            raise ValueError(f"ids_out must be a contiguous int32 tensor with room for {ids_in.numel()} tokens on cuda:{self.device}")
         check(lib.mfqb_decoder_step(self._h, ids_in.data_ptr(), ids_in.numel(), ids_out.data_ptr(), _stream_ptr(self.device)))
         return ids_out
 
