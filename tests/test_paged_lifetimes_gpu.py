@@ -80,6 +80,24 @@ def test_passes_on_a_side_stream():
     dec.free()
 
 
+def test_a_cache_attached_and_run_at_once_on_a_side_stream():
+    """Nothing between the attachment, whose constants are copied from the host, and the first pass on a stream that waits for no other."""
+    tokens, runs = _i32([1, 2, 3]), []
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side):
+        dec = _decoder(8, **BITWISE)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            cache = _cache(3)
+            cache.extend(5)
+            dec.set_cache(cache)
+            steps = [dec.step(tokens) for _ in range(5)]
+            runs.append((torch.stack(steps), dec.read_logits(3), cache.k, cache.v))
+        torch.cuda.synchronize()
+        dec.free()
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 def test_a_captured_verification_replays():
     dec = _decoder(2 * 64, **BITWISE)
     rng = np.random.default_rng(4)

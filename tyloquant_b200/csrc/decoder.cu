@@ -1047,9 +1047,17 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
         room(d, d->beam_tokens, rows * 4);
         room(d, d->beam_moves, rows * 4);
         room(d, d->beam_counts, rows * 12);
-        if (room(d, d->freqs, sizeof(freqs))) MFQB_CUDA(cudaMemcpy(d->freqs.p, freqs, sizeof(freqs), cudaMemcpyHostToDevice));
-        if (room(d, d->single_masks, rows * 8)) MFQB_CUDA(cudaMemcpy(d->single_masks.p, one.data(), rows * 8, cudaMemcpyHostToDevice));
-        if (room(d, d->single_depths, rows * 4)) MFQB_CUDA(cudaMemcpy(d->single_depths.p, zero.data(), rows * 4, cudaMemcpyHostToDevice));
+        bool copied = false;
+        auto constant = [&](DevBuf& buf, const void* from, size_t bytes) {
+            if (!room(d, buf, bytes)) return;
+            MFQB_CUDA(cudaMemcpy(buf.p, from, bytes, cudaMemcpyHostToDevice));
+            copied = true;
+        };
+        constant(d->freqs, freqs, sizeof(freqs));
+        constant(d->single_masks, one.data(), rows * 8);
+        constant(d->single_depths, zero.data(), rows * 4);
+        // A copy from pageable memory returns when it has been read, not when it has arrived, and the next pass may run on a stream that does not wait.
+        if (copied) MFQB_CUDA(cudaStreamSynchronize(nullptr));
         d->cache = *cache;
         d->paged = true;
     });

@@ -81,7 +81,8 @@ class Decoder:
 
     def set_cache(self, cache) -> None:
         """Runs over a :class:`PagedCache` from here on (``None``: over the decoder's own cache again); a row per sequence.  ``max_ctx=0`` at
-        creation leaves the decoder without a cache of its own."""
+        creation leaves the decoder without a cache of its own.  The decoder keeps the cache alive while it is attached; a graph that was
+        captured over it needs it as long as it is replayed."""
         check(lib.mfqb_decoder_set_cache(self._h, None if cache is None else C.byref(cache._view)))
         self._cache = cache   # borrowed by the native object
 
