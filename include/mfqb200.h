@@ -533,7 +533,9 @@ int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* par
 /* Beam selection: logits float32 [groups][beams][vocab], scores float32 [groups][beams].  The k best candidates of every group by
  * scores + log softmax(logits), largest first, into out_scores float32 [groups][k], out_rows int32 (group * beams + beam: what
  * mfqb_cache_fork takes) and out_tokens int32.  Candidates of one beam are ordered by logit, equal ones by token; candidates of
- * different beams by score (log sums and scores are compared in 64 bits), equal ones by beam.  A NaN counts as minus infinity.
+ * different beams by score (log sums and scores are compared in 64 bits), equal ones by beam.  A NaN ranks as minus infinity.  A beam
+ * with a NaN or plus infinity among its logits, or with nothing above minus infinity, has no log sum: all its candidates, finite logits
+ * too, have the score minus infinity (a token that is masked out is minus infinity, not NaN).
  * A beam with a non-zero entry in done (int32 [groups][beams], may be null) has one candidate: the token eos at its own score.
  * Where a group has fewer than k candidates the rest is row -1, token -1, score minus infinity.  beams <= 128, k <= min(128, vocab),
  * beams * k <= 8192, vocab <= 1048576.  work: device memory of mfqb_beam_select_work bytes, 16-byte aligned. */

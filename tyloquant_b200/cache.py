@@ -197,7 +197,8 @@ def beam_select(logits, scores, k: int, done=None, eos: int = -1):
     """The ``k`` best continuations of every group by ``scores + log_softmax(logits)``, largest first: ``logits`` float32 [groups, beams, vocab],
     ``scores`` float32 [groups, beams], ``done`` int32 [groups, beams] (a beam with a non-zero entry goes on as itself with token
     ``eos``).  Returns (scores float32 [groups, k], rows int32 [groups, k] = group * beams + beam, tokens int32 [groups, k]);
-    equal candidates: the lower beam, then the larger logit, then the lower token."""
+    equal candidates: the lower beam, then the larger logit, then the lower token.  A NaN or plus infinity among a beam's logits makes all
+    its candidates' scores minus infinity; what is masked out is minus infinity."""
     torch = _torch()
     if logits.dim() != 3 or not logits.is_cuda:
         raise ValueError("logits must be a float32 CUDA tensor [groups, beams, vocab]")
