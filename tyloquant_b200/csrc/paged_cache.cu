@@ -135,7 +135,8 @@ constexpr int kForkSmall = 8 * 1024;   // pages and table entries together that 
 
 // One CTA: the new table and the change of the counts are made beside the old ones and put in place at the end, when it is known
 // that the pages suffice.  Counts change by integer atomics, whose order does not matter.  Bound by its chain of dependent trips, not by their
-// size: where both fit they are in shared memory.
+// size: where both fit they are in shared memory.  With the copies of 32 pages in two layers, 64 sequences at context 4090 on pages of 64: 11.7 us over
+// a pool of 1200 pages, 13.3 over 5000, 17.0 over 20000.
 __global__ void __launch_bounds__(1024) fork_plan_kernel(mfqb_cache c, const int* parents, int* status, ForkWork w, bool small) {
     chained_wait();
     __shared__ int warp_sums[32], list[1024], s_len[kCacheRows], s_last[kCacheRows], total;
@@ -277,7 +278,8 @@ __global__ void __launch_bounds__(32) tree_masks_kernel(const int* parents, int 
 
 // CTA (heads of one sixteenth, node, sequence): 16 threads per head, four pairs (j, j + 64) a thread.  The angle is formed and reduced
 // to [-pi, pi] in 64 bits (a float32 product is off by 2e-3 radians at position 32768), its sine and cosine are taken once per
-// CTA.  Bound by memory: six bytes per value (64 nodes of 16 sequences, 32 + 2 x 8 heads: 7.0 us, 5.4 TB/s).
+// CTA.  Queries are rounded to bf16 once, the type in which the attention's first product takes them.  Bound by memory: six bytes per value (64
+// nodes of 16 sequences, 32 + 2 x 8 heads: 7.1 us, 5.3 TB/s).
 __global__ void __launch_bounds__(256) cache_write_kernel(mfqb_cache c, int layer, const float* qkv, int hq, int nodes, const int* depths, const double* freqs,
                                                           __nv_bfloat16* q_out) {
     chained_wait();
@@ -328,7 +330,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(mfqb_cache c, int laye
 // CTA (some layers' heads, sequence): its first warp walks the tree, two nodes a lane, the first CTA of a sequence leaves the results, and all move
 // the branch's rows, 64 at a time, which are its nodes in as many heads as that makes.  Every row is read into registers before the first one is
 // written, since a slot that one node leaves is another one's place.  A chain from the lengths to the rows: one tree of 8 nodes 4.2 us, 16 of 48
-// with branches of 13 in 128 heads 8.9 (a launch for the walk and one for the rows: 5.0 and 9.0; with a CTA for each head of each layer 11).
+// with branches of 13 in 128 heads 8.6 (a launch for the walk and one for the rows: 5.0 and 9.0; with a CTA for each head of each layer 11).  Lengths
+// that change in place are a second launch, 0.7 and 1.1 us more.
 __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* ids, const int* parents, const int* targets, int nodes, int* count, int* token,
                                                      int* path, int* lens_out) {
     chained_wait();
