@@ -157,6 +157,26 @@ def test_a_beam_that_ends_stays_as_it_is():
     dec.free()
 
 
+def test_every_row_has_a_beam_to_go_on_from():
+    """Scores of minus infinity and NaN, beams that are done: a group never has fewer candidates than beams."""
+    beams = 3
+    dec = _decoder(64, **BITWISE)
+    cache = _cache(3 * beams, pages=80)
+    dec.set_cache(cache)
+    _prompt(dec, cache, _i32(np.random.default_rng(10).integers(0, 1000, (3 * beams, 5))))
+    scores = torch.tensor([-np.inf] * 3 + [np.nan, -np.inf, -1.0] + [-np.inf, np.nan, -2.0], dtype=torch.float32, device=DEV)
+    done, tokens = _i32([0, 0, 0, 0, 1, 1, 1, 1, 1]), _i32(list(range(9)))
+    for _ in range(4):
+        tokens, parents, status = dec.beam_step(tokens, scores, done, beams, eos=-1)
+        assert status.tolist() == [0, 0]
+        assert [p // beams for p in parents.tolist()] == [r // beams for r in range(9)] and not torch.isnan(scores).any()
+        assert done[:3].tolist() == [0] * 3 and done[6:].tolist() == [1] * 3 and int(done[3]) == 1
+        assert float(scores[3]) == -1.0 and float(scores[6]) == -2.0 and (scores[:3] == -np.inf).all()
+        assert torch.equal(cache.refs, _counts(cache))
+    assert cache.lens[:3].tolist() == [9] * 3 and cache.lens[6:].tolist() == [5] * 3
+    dec.free()
+
+
 def test_tokens_that_go_round_in_place():
     """The tokens that one step writes are the next one's input, with nothing between the two; against steps that are waited for."""
     beams, runs = 4, []

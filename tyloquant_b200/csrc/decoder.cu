@@ -590,8 +590,8 @@ __global__ void __launch_bounds__(1024) beam_take_kernel(int* status, const floa
     const bool reserved = status[0] == 0, ok = reserved && status[1] == 0;
     bool over = true;
     if (r < rows && ok) {
-        const int p = parents[r];   // -1: fewer candidates than beams
-        over = p < 0 || done[p] || tokens[r] == eos;
+        // every row has a beam that it goes on from: a living one has as many candidates as there are beams, one that is done has itself
+        over = done[parents[r]] || tokens[r] == eos;
     }
     __syncthreads();
     if (r == 0 && !reserved) status[1] = 0;   // there was no fork that could lack pages
