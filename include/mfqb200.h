@@ -34,6 +34,8 @@ enum {
 };
 
 enum { MFQB_F32 = 0, MFQB_BF16 = 1 }; /* element types of activations / outputs */
+enum { MFQB_F16 = 2 };                /* of the logits of mfqb_token_logprobs alone */
+enum { MFQB_ROPE_HALVES = 0, MFQB_ROPE_INTERLEAVED = 1 }; /* which dims of a head turn together: mfqb_cache_write_rope */
 
 enum { MFQB_FAMILY_NINT = 1, MFQB_FAMILY_NVQ = 2 };
 
@@ -512,6 +514,13 @@ int mfqb_tree_masks(const int32_t* parents, int rows, int nodes, uint64_t* masks
 int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_heads, int nodes, const int32_t* depths, const double* freqs,
                      void* q_out, mfqb_stream_t stream);
 
+/* mfqb_cache_write in other conventions: the first 2 * pairs dims of every query and key head turn (freqs: device float64 [pairs], 1 to 64), those
+ * behind them pass.  layout MFQB_ROPE_HALVES: dims j and j + pairs turn together; MFQB_ROPE_INTERLEAVED: dims 2j and 2j + 1.  What has turned is
+ * multiplied by factor (positive, finite; 1 unless positions are scaled for longer contexts with a correction of the scores).  qkv is float32 or
+ * bf16 (qkv_dtype). */
+int mfqb_cache_write_rope(const mfqb_cache* c, int layer, const void* qkv, int qkv_dtype, int q_heads, int nodes, const int32_t* depths, const double* freqs, int pairs,
+                          int layout, float factor, void* q_out, mfqb_stream_t stream);
+
 /* Attention of the nodes over the cache: q, out bf16 [rows][nodes][q_heads][128].  Node i of sequence r sees the positions below
  * lens[r] and those nodes j (at position lens[r] + j) whose bit is set in masks[r][i]; out = softmax(scale * q.k) v over what it sees,
  * zeros where it sees nothing.  What a node does not see has no effect on it, an infinity or NaN neither; an infinite value that it
@@ -521,6 +530,37 @@ int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_hea
 int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes);
 int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out,
                         void* work, uint64_t work_bytes, mfqb_stream_t stream);
+
+/* The same attention, which also adds up how much every position was looked at: weights float32 [layers][rows][kv_heads][width * page], of which the
+ * call changes the layer's.  With p(i, h, t) the probability that node i's query head h gives position t, kv head g of sequence r
+ * gets the sum over the nodes and over its query heads: added at positions t < lens[r], written over what was there at lens[r] <= t <
+ * lens[r] + nodes (what the nodes' slots held is of tokens that are gone).  All else stays.  Probabilities are float32 here.  A position without a page
+ * gets nothing (a node's: 0), nor does one whose score is minus infinity; a NaN or plus infinity among the scores of a row makes NaN of the weights
+ * of all else that it sees.  Each sum is made in one order: a call repeats bit for bit.  out is the same as of
+ * mfqb_tree_attention.  weights overlaps neither q, out nor work.  mfqb_tree_accept and mfqb_cache_fork move keys and values alone, not the weights.
+ * work: device memory of mfqb_tree_attention_weigh_work bytes, 16-byte aligned (with the scores of up to 64 query rows of a kv head, where
+ * they take at most 512 MB). */
+int mfqb_tree_attention_weigh_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes);
+int mfqb_tree_attention_weigh(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights,
+                              void* work, uint64_t work_bytes, mfqb_stream_t stream);
+
+/* Eviction by weight: sequence r of n = lens[r] tokens is cut to k = keep[r] (device int32 [rows]) where 0 <= k < n; a negative entry, or
+ * one that is not below n, leaves it.  Its last R = min(recent, k) positions stay, and of the older ones, for every kv head of
+ * every layer by itself, the k - R with the largest weights (float32 [layers][rows][kv_heads][width * page], as above; a NaN ranks as minus infinity;
+ * equal ones: the lower slot).  Of those, what lies in slots below k - R stays in its slot; the others go in ascending order to the
+ * slots that this leaves free there, in ascending order; slot n - R + i goes to k - R + i.  Keys, values and weights move together; what
+ * lies behind k is left as it was.  So the latest positions stay in order at the end, the older ones do not, and attention does not
+ * ask for their order: keys keep the rotation of the positions that they had.  The next tokens go on from those positions when dropped
+ * is added to their depths in mfqb_cache_write.
+ *
+ * lens becomes k, pages behind it go back.  A page below it that has other holders too (refs above 1 before the call) is exchanged for a
+ * free one, the lowest to the first (sequences, then entries, in order), among those that were free before the call; what other sequences see
+ * does not change.  A position without a page has nothing to move, and its weight moves alone.
+ * dropped: int32 [rows], n - k or 0.  status (device int32 [1]): 0, or how many pages were missing: then nothing has changed and
+ * dropped is 0.  work: device memory of mfqb_cache_evict_work bytes, 16-byte aligned. */
+int mfqb_cache_evict_work(const mfqb_cache* c, uint64_t* bytes);
+int mfqb_cache_evict(const mfqb_cache* c, float* weights, const int32_t* keep, int recent, int32_t* dropped, int32_t* status, void* work, uint64_t work_bytes,
+                     mfqb_stream_t stream);
 
 /* Keeps the branch of every tree that the model agrees with: from the root on, the lowest child whose drafted token ids[r][child] is
  * the model's own targets[r][node] (device int32 [rows][nodes]).  Keys and values of the branch move together in all layers, to
@@ -542,6 +582,16 @@ int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* par
 int mfqb_beam_select_work(int groups, int beams, int vocab, int k, uint64_t* bytes);
 int mfqb_beam_select(const float* logits, int groups, int beams, int vocab, const float* scores, const int32_t* done, int eos, int k,
                      float* out_scores, int32_t* out_rows, int32_t* out_tokens, void* work, uint64_t work_bytes, mfqb_stream_t stream);
+
+/* Log probabilities of given tokens: logits [rows][vocab] (dtype MFQB_F32, MFQB_BF16 or MFQB_F16; row_stride values from row to row, at least vocab), tokens
+ * int32 [rows].  Per row: logprob float32, log softmax(logits)[token]; entropy float32, of softmax(logits), in nats; rank int32, 1 + the number
+ * of tokens before it (by logit, equal ones by number); and the `top` best tokens, best first in the same order: top_logprobs float32 [rows][top],
+ * top_tokens int32 [rows][top].  A token outside [0, vocab) stands for none (padding): logprob 0, rank 0, the rest as for any row.  Masked
+ * tokens are minus infinity.  A row with a NaN or plus infinity, or with nothing above minus infinity, has no log sum: logprob (of a token),
+ * entropy and top_logprobs are NaN, top_tokens -1, rank 0.  Sums are float32.  top <= min(32, vocab), vocab <= 1048576.  Nothing is allocated
+ * and no work memory needed; the first call of each type comes before a stream capture. */
+int mfqb_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride, const int32_t* tokens, int top, float* logprob, float* entropy,
+                        int32_t* rank, float* top_logprobs, int32_t* top_tokens, mfqb_stream_t stream);
 
 /* ---------------------------------------------------------------------------------
  * Host-side self-check of the device layout (no GPU): packs the blob into the device

@@ -13,7 +13,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libmfqb200.so")
 
 OK, ERR_ARG, ERR_FORMAT, ERR_UNSUPPORTED, ERR_CUDA, ERR_IO, ERR_TIMEOUT = range(7)
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2
+ROPE_HALVES, ROPE_INTERLEAVED = 0, 1
 FAMILY_NINT, FAMILY_NVQ = 1, 2
 
 
@@ -102,6 +103,12 @@ _SIGNATURES = {
     "mfqb_cache_fork": (_i, [_P(CacheView), _vp, _vp, _vp, _u64, _vp]),
     "mfqb_tree_masks": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
     "mfqb_cache_write": (_i, [_P(CacheView), _i, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "mfqb_cache_write_rope": (_i, [_P(CacheView), _i, _vp, _i, _i, _i, _vp, _vp, _i, _i, C.c_float, _vp, _vp]),
+    "mfqb_cache_evict_work": (_i, [_P(CacheView), _P(_u64)]),
+    "mfqb_cache_evict": (_i, [_P(CacheView), _vp, _vp, _i, _vp, _vp, _vp, _u64, _vp]),
+    "mfqb_tree_attention_weigh_work": (_i, [_P(CacheView), _i, _i, _P(_u64)]),
+    "mfqb_tree_attention_weigh": (_i, [_P(CacheView), _i, _vp, _i, _i, _vp, C.c_float, _vp, _vp, _vp, _u64, _vp]),
+    "mfqb_token_logprobs": (_i, [_vp, _i, _i, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mfqb_tree_attention_work": (_i, [_P(CacheView), _i, _i, _P(_u64)]),
     "mfqb_tree_attention": (_i, [_P(CacheView), _i, _vp, _i, _i, _vp, C.c_float, _vp, _vp, _u64, _vp]),
     "mfqb_tree_accept": (_i, [_P(CacheView), _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
@@ -147,7 +154,7 @@ from . import _fast  # noqa: E402  (built together with the library)
 
 _fast.bind(*(C.cast(getattr(lib, _name), C.c_void_p).value for _name in (
     "mfqb_mul_mat", "mfqb_moe_topk", "mfqb_moe_ffn", "mfqb_cache_extend", "mfqb_cache_fork", "mfqb_tree_masks", "mfqb_cache_write", "mfqb_tree_attention",
-    "mfqb_tree_accept", "mfqb_beam_select")))
+    "mfqb_tree_accept", "mfqb_beam_select", "mfqb_cache_write_rope", "mfqb_tree_attention_weigh", "mfqb_cache_evict", "mfqb_token_logprobs")))
 
 
 def check(status: int) -> None:

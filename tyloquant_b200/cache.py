@@ -1,5 +1,5 @@
 """A key/value cache in pages that sequences share, and the operators of a decoder over it: writing a step's keys and values, attention
-of drafted tokens, keeping the accepted branch, forking sequences; and the selection of beams.  torch only provides device
+of drafted tokens, keeping the accepted branch, forking sequences, evicting what attention has looked at least; and the selection of beams.  torch only provides device
 memory and streams.
 
 All calls are asynchronous on the current stream of the cache's device, allocate nothing outside torch's allocator and can be
@@ -9,9 +9,10 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 
 from . import _fast
-from ._capi import CacheView, check, lib
+from ._capi import BF16, F32, ROPE_HALVES, ROPE_INTERLEAVED, CacheView, check, lib
 from .linear import _torch
 
 HEAD_DIM = 128
@@ -37,10 +38,52 @@ def _call(fn, device: int, *args) -> None:
         check(status)
 
 
-def rope_frequencies(theta: float = 500000.0, device="cuda"):
-    """float64 [64]: theta^(-2j/128), what ``PagedCache.write`` takes."""
+_LAYOUTS = {"halves": ROPE_HALVES, "interleaved": ROPE_INTERLEAVED}
+
+
+def rope_frequencies(theta: float = 500000.0, device="cuda", *, dims: int = HEAD_DIM, scaling: str | None = None, factor: float = 1.0, original: int | None = None,
+                     low: float = 1.0, high: float | None = None):
+    """float64 [dims / 2]: theta^(-2j / dims), what ``PagedCache.write`` takes; ``dims`` of a head turn.  ``scaling`` for contexts ``factor`` times
+    as long as the ``original`` one that a model was trained on:
+
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"bands"``: frequencies that turn more than ``high`` (4) times over the original context are kept, those that turn less than ``low``
+      (1) times are divided by ``factor``, the ones between are mixed, linearly in the number of turns;
+    * ``"yarn"``: the same ends (``high`` 32, ``low`` 1), mixed linearly in j between the dims at which they lie; goes with a factor on the
+      rotated values, :func:`rope_yarn_factor`."""
     torch = _torch()
-    return float(theta) ** (-torch.arange(HEAD_DIM // 2, dtype=torch.float64, device=device) * 2 / HEAD_DIM)
+    if dims < 2 or dims > HEAD_DIM or dims % 2:
+        raise ValueError(f"dims must be even, 2 to {HEAD_DIM}, got {dims}")
+    j = torch.arange(dims // 2, dtype=torch.float64, device=device)
+    f = float(theta) ** (-j * 2 / dims)
+    if scaling is None:
+        return f
+    if not factor >= 1.0 or math.isinf(factor):
+        raise ValueError(f"factor must be a number from 1 on, got {factor}")
+    if scaling == "linear":
+        return f / factor
+    if scaling not in ("bands", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'bands' or 'yarn', got {scaling!r}")
+    if original is None or original < 1:
+        raise ValueError(f"{scaling!r} needs the original context length")
+    high = high if high is not None else 4.0 if scaling == "bands" else 32.0
+    if not 0 < low < high:
+        raise ValueError(f"low must be above 0 and below high, got {low} and {high}")
+    if scaling == "bands":
+        keep = ((original * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)   # turns over the original context
+    else:
+        def at(turns):   # the j at which a frequency turns so many times
+            return dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        first, last = max(math.floor(at(high)), 0), min(math.ceil(at(low)), dims - 1)
+        keep = 1 - ((j - first) / max(last - first, 1e-3)).clamp(0, 1)
+    return f * keep + f / factor * (1 - keep)
+
+
+def rope_yarn_factor(factor: float) -> float:
+    """0.1 ln(factor) + 1: what rotated queries and keys are multiplied by under ``scaling="yarn"``."""
+    if not factor >= 1.0 or math.isinf(factor):
+        raise ValueError(f"factor must be a number from 1 on, got {factor}")
+    return 0.1 * math.log(factor) + 1.0
 
 
 def tree_masks(parents):
@@ -91,6 +134,7 @@ class PagedCache:
             check(lib.mfqb_cache_fork_work(C.byref(self._view), C.byref(size)))   # refuses a shape that the library does not take
         self._fork_work = lens.new_empty((size.value + 3) // 4)   # calls on one cache are in order: they can share it
         self._attend_work = {}
+        self._evict_work = None
 
     @classmethod
     def empty(cls, *, layers: int, kv_heads: int, page: int, pages: int, rows: int, width: int, device: int = 0):
@@ -126,25 +170,39 @@ class PagedCache:
         _call(_fast.cache_fork, self.device, self._ptr, p.data_ptr(), status.data_ptr(), work.data_ptr(), work.numel() * 4)
         return status
 
-    def write(self, layer: int, qkv, depths, freqs):
-        """Rotary embedding and cache write of the nodes of every sequence: ``qkv`` float32 [rows, nodes, (q_heads + 2 kv_heads) * 128], positions
-        ``lens + depths`` (int32 [rows, nodes]), ``freqs`` float64 [64].  Keys and values of node i go to slot lens + i; returns the
-        rotated queries, bf16 [rows, nodes, q_heads, 128]."""
+    def write(self, layer: int, qkv, depths, freqs, layout: str = "halves", factor: float = 1.0):
+        """Rotary embedding and cache write of the nodes of every sequence: ``qkv`` float32 or bfloat16 [rows, nodes, (q_heads + 2 kv_heads) * 128], positions
+        ``lens + depths`` (int32 [rows, nodes]), ``freqs`` float64 [pairs] (``rope_frequencies``): the first 2 * pairs dims of a head turn, those behind
+        them pass.  ``layout``: dims j and j + pairs turn together ("halves") or dims 2j and 2j + 1 ("interleaved"); what has turned is multiplied by
+        ``factor``.  Keys and values of node i go to slot lens + i; returns the rotated queries, bf16 [rows, nodes, q_heads, 128].  Of a sequence
+        that has been cut (``evict``) the depths count from its length: add what has been dropped."""
         torch = _torch()
         if qkv.dim() != 3 or qkv.shape[0] != self.rows or qkv.shape[2] % HEAD_DIM or qkv.shape[2] // HEAD_DIM <= 2 * self.kv_heads:
             raise ValueError(f"qkv must be [{self.rows}, nodes, (q_heads + {2 * self.kv_heads}) * 128], got {list(qkv.shape)}")
         nodes, hq = qkv.shape[1], qkv.shape[2] // HEAD_DIM - 2 * self.kv_heads
-        x = _need(qkv, torch.float32, qkv.shape, self.device, "qkv")
+        dtype = torch.bfloat16 if qkv.dtype is torch.bfloat16 else torch.float32
+        x = _need(qkv, dtype, qkv.shape, self.device, "qkv")
         d = self._int32(depths, (self.rows, nodes), "depths")
-        f = _need(freqs, torch.float64, (HEAD_DIM // 2,), self.device, "freqs")
+        pairs = freqs.shape[0] if freqs.dim() == 1 and 1 <= freqs.shape[0] <= HEAD_DIM // 2 else HEAD_DIM // 2
+        f = _need(freqs, torch.float64, (pairs,), self.device, "freqs")
+        if layout not in _LAYOUTS:
+            raise ValueError(f"layout must be 'halves' or 'interleaved', got {layout!r}")
         q = x.new_empty((self.rows, nodes, hq, HEAD_DIM), dtype=torch.bfloat16)
-        _call(_fast.cache_write, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, d.data_ptr(), f.data_ptr(), q.data_ptr())
+        if dtype is torch.float32 and pairs == HEAD_DIM // 2 and layout == "halves" and factor == 1.0:
+            _call(_fast.cache_write, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, d.data_ptr(), f.data_ptr(), q.data_ptr())
+        else:
+            _call(_fast.cache_write_rope, self.device, self._ptr, layer, x.data_ptr(), BF16 if dtype is torch.bfloat16 else F32, hq, nodes, d.data_ptr(), f.data_ptr(),
+                  pairs, _LAYOUTS[layout], factor, q.data_ptr())
         return q
 
-    def attend(self, layer: int, q, masks, scale: float | None = None, out=None):
+    def attend(self, layer: int, q, masks, scale: float | None = None, out=None, weights=None):
         """Attention of the nodes over the cache: ``q`` bf16 [rows, nodes, q_heads, 128], ``masks`` int64 [rows, nodes] (``tree_masks``); node i sees
         the positions below its sequence's length and the nodes whose bits are set.  Returns bf16 like ``q``; zeros where a node sees
-        nothing.  ``scale`` is 1 / sqrt(128) unless given."""
+        nothing.  ``scale`` is 1 / sqrt(128) unless given.
+
+        ``weights`` (``new_weights``), changed in place: for every kv head of the layer, the probabilities that the nodes and the head's queries
+        give to a position are added to its entry; the nodes' own entries, at positions from ``lens`` on, are set.  ``accept`` and ``fork`` move keys
+        and values alone: entries of a branch, or of sequences that go on from others, are the caller's to move."""
         torch = _torch()
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != HEAD_DIM:
             raise ValueError(f"q must be [{self.rows}, nodes, q_heads, 128], got {list(q.shape)}")
@@ -155,16 +213,54 @@ class PagedCache:
             out = torch.empty_like(x)
         elif _need(out, torch.bfloat16, q.shape, self.device, "out") is not out:
             raise ValueError("out must be contiguous")
-        size = self._attend_work.get((hq, nodes))
+        weigh = weights is not None
+        if weigh:
+            self._weights(weights)
+        size = self._attend_work.get((hq, nodes, weigh))
         if size is None:
             n = C.c_uint64()
             with torch.cuda.device(self.device):
-                check(lib.mfqb_tree_attention_work(C.byref(self._view), hq, nodes, C.byref(n)))
-            size = self._attend_work[(hq, nodes)] = (n.value + 15) // 16 * 16
+                check((lib.mfqb_tree_attention_weigh_work if weigh else lib.mfqb_tree_attention_work)(C.byref(self._view), hq, nodes, C.byref(n)))
+            size = self._attend_work[(hq, nodes, weigh)] = (n.value + 15) // 16 * 16
         work = x.new_empty(size // 2)
-        _call(_fast.tree_attention, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, m.data_ptr(), HEAD_DIM ** -0.5 if scale is None else scale,
-              out.data_ptr(), work.data_ptr(), size)
+        scale = HEAD_DIM ** -0.5 if scale is None else scale
+        if weigh:
+            _call(_fast.tree_attention_weigh, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, m.data_ptr(), scale, out.data_ptr(), weights.data_ptr(),
+                  work.data_ptr(), size)
+        else:
+            _call(_fast.tree_attention, self.device, self._ptr, layer, x.data_ptr(), hq, nodes, m.data_ptr(), scale, out.data_ptr(), work.data_ptr(), size)
         return out
+
+    def new_weights(self):
+        """Zeros, float32 [layers, rows, kv_heads, width * page]: what ``attend`` adds to and ``evict`` goes by."""
+        torch = _torch()
+        return torch.zeros((self.layers, self.rows, self.kv_heads, self.width * self.page), dtype=torch.float32, device=self.k.device)
+
+    def _weights(self, t):
+        if _need(t, _torch().float32, (self.layers, self.rows, self.kv_heads, self.width * self.page), self.device, "weights") is not t:
+            raise ValueError("weights must be contiguous")
+
+    def evict(self, weights, keep, recent: int = 0):
+        """Cuts every sequence that is longer than ``keep`` (int32 [rows], or one number for all; a negative entry leaves its sequence alone) to that
+        length: the last ``recent`` positions stay and, for every kv head of every layer by itself, the older ones with the largest ``weights``
+        (equal ones: the lower slot).  The latest stay in order at the end; of the older ones those within the new length keep their slots, the others
+        fill the slots that are free.  ``weights`` (float32, as of ``new_weights``) move along; pages that become free go back, and what other sequences
+        see of shared pages stays.  Returns (dropped int32 [rows], what to add to ``write``'s depths from here on; status int32 [1]: 0, or
+        how many pages were missing: then nothing has changed)."""
+        torch = _torch()
+        self._weights(weights)
+        if isinstance(keep, int):
+            keep = torch.full((self.rows,), keep, dtype=torch.int32, device=self.k.device)
+        k = self._int32(keep, (self.rows,), "keep")
+        if self._evict_work is None:
+            n = C.c_uint64()
+            with torch.cuda.device(self.device):
+                check(lib.mfqb_cache_evict_work(C.byref(self._view), C.byref(n)))
+            self._evict_work = (n.value + 15) // 16 * 16
+        dropped, status = torch.empty_like(self.lens), self.lens.new_empty(1)
+        work = self.lens.new_empty(self._evict_work // 4)
+        _call(_fast.cache_evict, self.device, self._ptr, weights.data_ptr(), k.data_ptr(), recent, dropped.data_ptr(), status.data_ptr(), work.data_ptr(), self._evict_work)
+        return dropped, status
 
     def accept(self, ids, parents, targets, lens_out=None):
         """Keeps the branch of every tree that the model agrees with: from the root on the lowest child whose drafted token ``ids`` is the model's

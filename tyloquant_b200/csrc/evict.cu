@@ -1,0 +1,338 @@
+// Eviction from a paged cache: every head of every layer keeps the positions with the largest weights and the latest ones; their keys and
+// values close up, and the pages behind them go back.
+#include <mutex>
+
+#include "select.cuh"
+
+namespace mfqb {
+
+constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictStep = 4 * kEvictThreads;          // slots that are looked at together
+constexpr int kEvictCached = 48 * 1024;                // positions whose keys fit shared memory
+
+struct EvictRow {
+    int len, keep;   // keep -1: the sequence stays as it is
+    int swapped;     // some of its first pages have been exchanged for others
+    int pad;
+};
+struct EvictWork {
+    EvictRow* row;   // [rows]
+    int* old;        // [rows][width]: the table as it was
+    int* rank;       // [rows][width]: which of the new pages an entry gets, -1 none
+    int* free;       // [pages]
+};
+static EvictWork evict_work(const mfqb_cache& c, void* work) {
+    const int64_t entries = (int64_t)c.rows * c.width;
+    EvictWork w;
+    w.row = static_cast<EvictRow*>(work);
+    w.old = reinterpret_cast<int*>(w.row + c.rows);
+    w.rank = w.old + entries;
+    w.free = w.rank + entries;
+    return w;
+}
+static uint64_t evict_work_bytes(const mfqb_cache& c) { return 16ull * c.rows + 8ull * c.rows * c.width + 4ull * c.pages; }
+
+// One CTA.  Which entries change is settled from the counts as they were: a page that two sequences have is exchanged in both, so that no
+// page is written that another one still reads from, and the new pages are among those that were free before.
+__global__ void __launch_bounds__(1024) evict_plan_kernel(mfqb_cache c, const int* keep, int* dropped, int* status, EvictWork w) {
+    chained_wait();
+    __shared__ int sums[33], s_keep[kCacheRows], s_swapped[kCacheRows];
+    const int r = threadIdx.x;
+    const int64_t cap = (int64_t)c.width * c.page;
+    int len = 0, to = -1;
+    if (r < c.rows) {
+        len = (int)min(max((int64_t)c.lens[r], (int64_t)0), cap);
+        to = __ldcg(keep + r);
+        if (to >= len) to = -1;
+        to = max(to, -1);
+    }
+    s_keep[r] = to;
+    s_swapped[r] = 0;
+    __syncthreads();
+    auto valid = [&](int p) { return (unsigned)p < (unsigned)c.pages; };
+    const int entries = c.rows * c.width;
+    int need = 0;
+    for (int base = 0; base < entries; base += 1024) {
+        const int e = base + r;
+        int swap = 0, row = 0;
+        if (e < entries) {
+            row = e / c.width;
+            const int p = c.table[e];
+            w.old[e] = p;
+            swap = (int64_t)(e - row * c.width) * c.page < s_keep[row] && valid(p) && c.refs[p] > 1;
+        }
+        const int upto = block_scan<1024>(swap, sums);
+        if (e < entries) w.rank[e] = swap ? need + upto - 1 : -1;
+        if (swap) s_swapped[row] = 1;
+        __syncthreads();
+        need += sums[32];
+    }
+    int have = 0;
+    if (need > 0) {   // the lowest free pages, in order
+        for (int base = 0; base < c.pages && have < need; base += 1024) {
+            const int p = base + r;
+            const int is = p < c.pages && c.refs[p] <= 0;
+            const int upto = block_scan<1024>(is, sums);
+            if (is && have + upto <= need) w.free[have + upto - 1] = p;
+            __syncthreads();
+            have += sums[32];
+        }
+        have = min(have, need);
+    }
+    const bool go = have == need;
+    if (r == 0) *status = need - have;
+    if (r < c.rows) {
+        if (!go) to = -1;
+        w.row[r] = EvictRow{len, to, s_swapped[r], 0};
+        dropped[r] = to < 0 ? 0 : len - to;
+        if (to >= 0) c.lens[r] = to;
+    }
+    __syncthreads();
+    if (!go) return;
+    for (int e = r; e < entries; e += 1024) {
+        const int row = e / c.width, k = s_keep[row];
+        if (k < 0) continue;
+        const int p = w.old[e], at = w.rank[e];
+        if ((int64_t)(e - row * c.width) * c.page >= k) {
+            c.table[e] = -1;
+            if (valid(p)) atomicSub(c.refs + p, 1);
+        } else if (at >= 0) {
+            const int fresh = w.free[at];
+            c.table[e] = fresh;
+            c.refs[fresh] = 1;   // whatever a free page's count was
+            atomicSub(c.refs + p, 1);
+        }
+    }
+}
+
+struct EvictShared {
+    CutShared cut;
+    int holes[kEvictStep], movers[kEvictStep];
+};
+
+// A cluster per head of a layer of a sequence.  Each of its CTAs finds the cut and the same lists of free slots and of rows to move, and moves its
+// share; the latest rows follow when all others have moved.  Rows are read before a slot that holds one is written: the others go to
+// slots below the new length's older part, where none of them lies, and the latest ones in ascending order.
+template <bool CACHED>
+__global__ void __launch_bounds__(kEvictThreads) evict_kernel(mfqb_cache c, float* weights, int recent_most, EvictWork w) {
+    extern __shared__ unsigned s_keys[];
+    __shared__ EvictShared sh;
+    chained_wait();
+    unsigned part, parts;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
+    const int64_t unit = blockIdx.x / parts, layer = unit / ((int64_t)c.rows * c.kv_heads);
+    const int left = (int)(unit - layer * c.rows * c.kv_heads), r = left / c.kv_heads, head = left - r * c.kv_heads, tid = threadIdx.x;
+    const EvictRow row = w.row[r];
+    if (row.keep < 0) return;   // the whole cluster
+    const int n = row.len, k = row.keep, recent = min(recent_most, k), older = n - recent, b = k - recent;   // of `older` slots b stay, the first b of the new ones
+    const int bits = __ffs(c.page) - 1, low = c.page - 1;
+    const int *old_table = w.old + (int64_t)r * c.width, *table = c.table + (int64_t)r * c.width;
+    float* wt = weights + unit * c.width * c.page;
+    const int64_t base = (layer * c.pages * c.kv_heads + head) * c.page;   // row of page 0
+    auto at = [&](const int* t, int slot) -> int64_t {                      // row of a slot in the pools, -1 without a page
+        const int p = t[slot >> bits];
+        return (unsigned)p < (unsigned)c.pages ? base + (int64_t)p * c.kv_heads * c.page + (slot & low) : -1;
+    };
+    uint4 *kp = static_cast<uint4*>(c.k), *vp = static_cast<uint4*>(c.v);
+    auto key = [&](int i) { return CACHED ? s_keys[i] : ordered_f32(wt[i]); };
+
+    auto sync_all = [&]() {
+        if (parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else __syncthreads();
+    };
+    if (b > 0) {
+        if (CACHED) {
+            for (int i = tid; i < older; i += kEvictThreads) s_keys[i] = ordered_f32(wt[i]);
+            sync_all();   // no CTA moves weights that another one has not read
+        }
+        const Cut cut = select_cut<kEvictThreads>(b, sh.cut, [&](auto f) {
+            for (int i = tid; i < older; i += kEvictThreads) f(key(i));
+        });
+        // Walks slots [slot, end) in steps until it has found some that `take` wants (stay: is the slot kept?), in ascending order.
+        struct Walk {
+            int slot, end, ties, n, used;
+        };
+        auto fill = [&](Walk& x, int* list, auto take) {
+            x.n = x.used = 0;
+            while (x.n == 0 && x.slot < x.end) {
+                const int i0 = x.slot + 4 * tid;
+                unsigned o[4];
+                int equal = 0, mine = x.ties, want = 0;
+                bool t[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[e] = i0 + e < x.end ? key(i0 + e) : 0u;
+                    equal += o[e] == cut.key;
+                }
+                if (cut.ties) {
+                    const int upto = block_scan<kEvictThreads>(equal, sh.cut.sums);
+                    __syncthreads();
+                    mine += upto - equal;
+                    x.ties += sh.cut.sums[kEvictWarps];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool tie = o[e] == cut.key, stays = o[e] > cut.key || (tie && mine < cut.ties);
+                    mine += tie;
+                    t[e] = i0 + e < x.end && take(stays, i0 + e);
+                    want += t[e];
+                }
+                int to = block_scan<kEvictThreads>(want, sh.cut.sums) - want;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (t[e]) list[to++] = i0 + e;
+                __syncthreads();
+                x.n = sh.cut.sums[kEvictWarps];
+                x.slot = min(x.end, x.slot + kEvictStep);
+            }
+        };
+        // Moves `count` rows, 16 threads each; the CTAs of the cluster take them in turns.
+        constexpr int kTeams = kEvictThreads / 16;
+        auto move = [&](const int* from, const int* to, int count) {
+            const int lane = tid & 15;
+            for (int i0 = (int)part * kTeams + (tid >> 4); i0 < count; i0 += (int)parts * kTeams * 4) {
+                int64_t src[4], dst[4];
+                uint4 a[4], v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int i = i0 + u * (int)parts * kTeams;
+                    src[u] = i < count ? at(old_table, from[i]) : -1;
+                    dst[u] = src[u] >= 0 ? at(table, to[i]) : -1;
+                    if (dst[u] >= 0) {
+                        a[u] = kp[src[u] * 16 + lane];
+                        v[u] = vp[src[u] * 16 + lane];
+                    }
+                    if (i < count && lane == 0 && from[i] != to[i]) wt[to[i]] = wt[from[i]];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (dst[u] >= 0) {
+                        kp[dst[u] * 16 + lane] = a[u];
+                        vp[dst[u] * 16 + lane] = v[u];
+                    }
+            }
+        };
+        if (row.swapped) {   // what stays in its slot on a page that has been exchanged
+            Walk x = {0, b, 0, 0, 0};
+            for (;;) {
+                fill(x, sh.holes, [&](bool stays, int slot) { return stays && old_table[slot >> bits] != table[slot >> bits]; });
+                if (x.n == 0) break;
+                move(sh.holes, sh.holes, x.n);
+                __syncthreads();
+            }
+        }
+        Walk hole = {0, b, 0, 0, 0}, mover = {b, older, 0, 0, 0};
+        if (cut.ties) {
+            int equal = 0;
+            for (int i = tid; i < b; i += kEvictThreads) equal += key(i) == cut.key;
+            block_scan<kEvictThreads>(equal, sh.cut.sums);
+            __syncthreads();
+            mover.ties = sh.cut.sums[kEvictWarps];
+            __syncthreads();
+        }
+        for (;;) {
+            if (hole.used == hole.n) fill(hole, sh.holes, [](bool stays, int) { return !stays; });
+            if (hole.n == 0) break;
+            if (mover.used == mover.n) fill(mover, sh.movers, [](bool stays, int) { return stays; });
+            const int count = min(hole.n - hole.used, mover.n - mover.used);   // as many rows move as there are free slots
+            if (count <= 0) break;
+            move(sh.movers + mover.used, sh.holes + hole.used, count);
+            hole.used += count;
+            mover.used += count;
+            __syncthreads();
+        }
+    }
+    sync_all();
+    // The latest rows: a CTA reads a batch before it writes any of it, and later ones lie behind all that has been written.
+    if (part == 0) {
+        constexpr int kTeams = kEvictThreads / 16, kBatch = 4 * kTeams;
+        const int lane = tid & 15, team = tid >> 4;
+        for (int i0 = 0; i0 < recent; i0 += kBatch) {
+            int64_t dst[4];
+            uint4 a[4], v[4];
+            float f[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * kTeams + team;
+                const int64_t src = i < recent ? at(old_table, older + i) : -1;
+                dst[u] = src >= 0 ? at(table, b + i) : -1;
+                if (dst[u] >= 0) {
+                    a[u] = kp[src * 16 + lane];
+                    v[u] = vp[src * 16 + lane];
+                }
+                f[u] = i < recent ? wt[older + i] : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * kTeams + team;
+                if (dst[u] >= 0) {
+                    kp[dst[u] * 16 + lane] = a[u];
+                    vp[dst[u] * 16 + lane] = v[u];
+                }
+                if (i < recent && lane == 0) wt[b + i] = f[u];
+            }
+        }
+    }
+}
+
+static void launch_evict(const mfqb_cache& c, float* weights, const int* keep, int recent, int* dropped, int* status, EvictWork w, cudaStream_t s) {
+    int device = 0;
+    MFQB_CUDA(cudaGetDevice(&device));
+    static std::once_flag once[64];
+    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(evict_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictCached * 4)); });
+    launch_chained(evict_plan_kernel, dim3(1), dim3(1024), 0, s, c, keep, dropped, status, w);
+    const int64_t cap = (int64_t)c.width * c.page, units = (int64_t)c.layers * c.rows * c.kv_heads;
+    const bool cached = cap <= kEvictCached;
+    // Keys that are read from the weights themselves may not be read by one CTA while another one moves weights.
+    int parts = 1;
+    while (cached && parts < 8 && units * parts < 2 * 148) parts *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * parts));
+    cfg.blockDim = dim3(kEvictThreads);
+    cfg.dynamicSmemBytes = cached ? (size_t)cap * 4 : 0;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    MFQB_CUDA(cudaLaunchKernelEx(&cfg, cached ? evict_kernel<true> : evict_kernel<false>, c, weights, recent, w));
+}
+
+}  // namespace mfqb
+
+using namespace mfqb;
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+int mfqb_cache_evict_work(const mfqb_cache* c, uint64_t* bytes) {
+    return guarded([&] {
+        check_cache(c, "mfqb_cache_evict_work");
+        if (!bytes) fail(MFQB_ERR_ARG, "mfqb_cache_evict_work: null argument");
+        ready_device();
+        *bytes = evict_work_bytes(*c);
+    });
+}
+
+int mfqb_cache_evict(const mfqb_cache* c, float* weights, const int32_t* keep, int recent, int32_t* dropped, int32_t* status, void* work, uint64_t work_bytes,
+                     mfqb_stream_t stream) {
+    return guarded([&] {
+        check_cache(c, "mfqb_cache_evict");
+        if (!weights || !keep || !dropped || !status || !work) fail(MFQB_ERR_ARG, "mfqb_cache_evict: null argument");
+        if (recent < 0) fail(MFQB_ERR_ARG, "mfqb_cache_evict: the number of latest positions must not be negative, got %d", recent);
+        if ((int64_t)c->layers * c->rows * c->kv_heads > (1ll << 27)) fail(MFQB_ERR_UNSUPPORTED, "mfqb_cache_evict: too many layers x sequences x heads");
+        if (((uintptr_t)work & 15) || work_bytes < evict_work_bytes(*c))
+            fail(MFQB_ERR_ARG, "mfqb_cache_evict: work must be 16-byte aligned and hold %llu bytes, got %llu", (unsigned long long)evict_work_bytes(*c),
+                 (unsigned long long)work_bytes);
+        launch_evict(*c, weights, keep, recent, dropped, status, evict_work(*c, work), stream);
+    });
+}
+
+#pragma GCC visibility pop
+}  // extern "C"

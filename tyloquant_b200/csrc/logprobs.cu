@@ -1,0 +1,418 @@
+// Log probabilities of given tokens, with entropy, rank and the best alternatives: one pass over the logits.
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "select.cuh"
+#include "tc05.cuh"
+
+namespace mfqb {
+
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4;
+constexpr int kLpVocab = 1 << 20;
+
+struct LogprobArgs {
+    const char* logits;
+    int64_t stride;   // bytes
+    const int* tokens;
+    int vocab, top;
+    float *logprob, *entropy, *top_logprobs;
+    int *rank, *top_tokens;
+};
+
+// Sums of some of a row's logits: exp(z - top), the same times (z - top) log2(e), and how many come before the given token.
+struct LogprobSum {
+    float top, sum, moment;
+    int before;
+};
+struct LogprobShared {
+    CutShared cut;
+    LogprobSum warp[kLpWarps], all;
+    float group[kLpGroups], bound;
+    int hot[kLpThreads], hots, count, best_n, total;
+    unsigned long long list[kLpList], best[kLpTop], merged[kLpTop];
+};
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLpLowest = -3.402823466e38f, kLpNone = -200.f;   // 2^-200 is 0 in float32
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long lp_key(float z, int token) { return (unsigned long long)ordered_f32(z) << 32 | (0xFFFFFFFFu - (unsigned)token); }
+
+// 16 bytes of logits as float32.
+template <typename T>
+struct LpVec;
+template <>
+struct LpVec<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void widen(const uint4& v, float* z) {
+        z[0] = __uint_as_float(v.x); z[1] = __uint_as_float(v.y); z[2] = __uint_as_float(v.z); z[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint32_t lowest() { return 0xFF800000u; }
+};
+template <>
+struct LpVec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void widen(const uint4& v, float* z) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            z[2 * i] = __uint_as_float(w[i] << 16);
+            z[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+template <>
+struct LpVec<__half> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void widen(const uint4& v, float* z) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            z[2 * i] = f.x;
+            z[2 * i + 1] = f.y;
+        }
+    }
+};
+__device__ __forceinline__ float lp_float(float x) { return x; }
+__device__ __forceinline__ float lp_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float lp_float(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ LogprobSum lp_join(LogprobSum a, LogprobSum b) {
+    LogprobSum r;
+    r.top = fmaxf(a.top, b.top);
+    const float da = fmaxf((a.top - r.top) * kLog2e, kLpNone), db = fmaxf((b.top - r.top) * kLog2e, kLpNone);
+    const float fa = exp2_approx(da), fb = exp2_approx(db);
+    r.sum = a.sum * fa + b.sum * fb;
+    r.moment = (a.moment + da * a.sum) * fa + (b.moment + db * b.sum) * fb;
+    r.before = a.before + b.before;
+    return r;
+}
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared variable in another CTA of the cluster, and a load from there.
+__device__ __forceinline__ uint32_t remote_smem(const void* p, unsigned rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t remote_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// A cluster per row, a slice of the row per CTA.  A thread takes every 512th vector of 16 bytes and keeps a running maximum with its sums.  The k
+// best: a bound that at least k logits reach comes from the maxima of 64 groups of threads (the k-th largest of them), and only the
+// vectors of threads whose own maximum reaches it are read again, a warp for each of those threads.  Where too many logits reach the
+// bound (equal ones, or all in a few threads' vectors) the cut is searched by counting instead.
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+    constexpr int kN = LpVec<T>::kN;
+    __shared__ LogprobShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned rank = cluster_rank(), ctas = cluster_size();
+    const int64_t row = blockIdx.x / ctas;
+    chained_wait();
+    const T* z = reinterpret_cast<const T*>(a.logits + row * a.stride);
+    // Vectors start at 16-byte boundaries; vector v holds logits v * kN - skew ..; those outside the row count as minus infinity.
+    const int skew = (int)(((uintptr_t)z & 15) / sizeof(T)), vectors = (skew + a.vocab + kN - 1) / kN;
+    const int first = (int)((int64_t)vectors * rank / ctas), last = (int)((int64_t)vectors * (rank + 1) / ctas);
+    auto load = [&](int v, float* x) {
+        const int at = v * kN - skew;
+        if (at >= 0 && at + kN <= a.vocab) {
+            LpVec<T>::widen(__ldcg(reinterpret_cast<const uint4*>(z + at)), x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kN; ++e) x[e] = at + e >= 0 && at + e < a.vocab ? lp_float(z[at + e]) : -INFINITY;
+        }
+    };
+    const int token = __ldcg(a.tokens + row);
+    const bool there = (unsigned)token < (unsigned)a.vocab;
+    // A logit comes before the token's own if it is larger, or equal with a lower number.
+    const float zt = there ? lp_float(z[token]) + 0.f : INFINITY;
+    const float above = unordered_f32(ordered_f32(zt) + 1u);
+    LogprobSum s = {kLpLowest, 0.f, 0.f, 0};
+    float most = -INFINITY;
+    for (int v0 = first + tid; v0 < last; v0 += kLpThreads * kLpBatch) {
+        float x[kLpBatch][kN];
+#pragma unroll
+        for (int u = 0; u < kLpBatch; ++u) {
+            if (v0 + u * kLpThreads < last) {
+                load(v0 + u * kLpThreads, x[u]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kN; ++e) x[u][e] = -INFINITY;
+            }
+        }
+        float high = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kLpBatch; ++u)
+#pragma unroll
+            for (int e = 0; e < kN; ++e) high = fmaxf(high, x[u][e]);
+        most = fmaxf(most, high);
+        if (high > s.top) {
+            const float d = fmaxf((s.top - high) * kLog2e, kLpNone), f = exp2_approx(d);
+            s.moment = (s.moment + d * s.sum) * f;
+            s.sum *= f;
+            s.top = high;
+        }
+#pragma unroll
+        for (int u = 0; u < kLpBatch; ++u) {
+            const int at = (v0 + u * kLpThreads) * kN - skew;
+            if (v0 + u * kLpThreads >= last) break;
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+                const float d = max_nan((x[u][e] - s.top) * kLog2e, kLpNone), p = exp2_approx(d);
+                s.sum += p;
+                s.moment += p * d;
+                s.before += x[u][e] >= (at + e < token ? zt : above);
+            }
+        }
+    }
+    if (first + tid == 0 && first < last && there && zt == -INFINITY) s.before -= skew;   // minus infinities that are not the row's
+    // ---- the CTA's sums
+    LogprobSum joint = s;
+    for (int o = 16; o > 0; o >>= 1) {
+        LogprobSum other;
+        other.top = __shfl_xor_sync(0xffffffffu, joint.top, o);
+        other.sum = __shfl_xor_sync(0xffffffffu, joint.sum, o);
+        other.moment = __shfl_xor_sync(0xffffffffu, joint.moment, o);
+        other.before = __shfl_xor_sync(0xffffffffu, joint.before, o);
+        joint = lp_join(joint, other);
+    }
+    if (lane == 0) sh.warp[warp] = joint;
+    if (a.top > 0) {
+        float group = most;   // eight threads
+        for (int o = 4; o > 0; o >>= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+        if ((lane & 7) == 0) sh.group[tid >> 3] = group;
+        if (tid == 0) sh.hots = sh.count = 0;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        LogprobSum x = sh.warp[lane & (kLpWarps - 1)];
+        for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+            LogprobSum other;
+            other.top = __shfl_xor_sync(0xffffffffu, x.top, o);
+            other.sum = __shfl_xor_sync(0xffffffffu, x.sum, o);
+            other.moment = __shfl_xor_sync(0xffffffffu, x.moment, o);
+            other.before = __shfl_xor_sync(0xffffffffu, x.before, o);
+            x = lp_join(x, other);
+        }
+        if (lane == 0) sh.all = x;
+    }
+    if (a.top > 0) {
+        // ---- the bound: the group maxima in order, equal ones by group
+        if (tid < kLpGroups) {
+            const float g = sh.group[tid];
+            int larger = 0;
+            for (int j = 0; j < kLpGroups; ++j) larger += sh.group[j] > g || (sh.group[j] == g && j < tid);
+            if (larger == a.top - 1) sh.bound = g;
+        }
+        __syncthreads();
+        const float bound = sh.bound;
+        if (first + tid < last && most >= bound) sh.hot[atomicAdd(&sh.hots, 1)] = tid;
+        __syncthreads();
+        const int hots = sh.hots;
+        for (int h = warp; h < hots; h += kLpWarps) {
+            for (int v = first + sh.hot[h] + lane * kLpThreads; v < last; v += 32 * kLpThreads) {
+                float x[kN];
+                load(v, x);
+                const int at = v * kN - skew;
+#pragma unroll
+                for (int e = 0; e < kN; ++e)
+                    if (x[e] >= bound && at + e >= 0 && at + e < a.vocab) {
+                        const int i = atomicAdd(&sh.count, 1);
+                        if (i < kLpList) sh.list[i] = lp_key(x[e], at + e);
+                    }
+            }
+        }
+        __syncthreads();
+        int n = sh.count;
+        if (n > kLpList) {
+            auto each = [&](auto f) {
+                for (int v = first + tid; v < last; v += kLpThreads) {
+                    float x[kN];
+                    load(v, x);
+                    const int at = v * kN - skew;
+#pragma unroll
+                    for (int e = 0; e < kN; ++e)
+                        if (at + e >= 0 && at + e < a.vocab) f(ordered_f32(x[e]));
+                }
+            };
+            const Cut cut = select_cut<kLpThreads>(a.top, sh.cut, each);
+            __syncthreads();
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            int ties = 0;   // of the vectors before
+            for (int v0 = first; v0 < last; v0 += kLpThreads) {
+                const int v = v0 + tid, at = v * kN - skew;
+                unsigned o[kN];
+                int equal = 0;
+                if (v < last) {
+                    float x[kN];
+                    load(v, x);
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) {
+                        const bool in = at + e >= 0 && at + e < a.vocab;
+                        o[e] = in ? ordered_f32(x[e]) : 0u;
+                        equal += o[e] == cut.key;
+                    }
+                }
+                int mine = ties;
+                if (ties < cut.ties) {   // the same in all threads
+                    const int upto = block_scan<kLpThreads>(equal, sh.cut.sums);
+                    __syncthreads();
+                    mine += upto - equal;
+                    ties += sh.cut.sums[kLpWarps];
+                }
+                if (v < last)
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) {
+                        const bool tie = o[e] == cut.key;
+                        if (o[e] > cut.key || (tie && mine < cut.ties)) {
+                            const int i = atomicAdd(&sh.count, 1);
+                            if (i < kLpList) sh.list[i] = (unsigned long long)o[e] << 32 | (0xFFFFFFFFu - (unsigned)(at + e));
+                        }
+                        mine += tie;
+                    }
+            }
+            __syncthreads();
+            n = min(sh.count, kLpList);
+        }
+        // ---- the list in order: every key counts those above it
+        const int keep = min(n, a.top);
+        for (int i = tid; i < n; i += kLpThreads) {
+            const unsigned long long key = sh.list[i];
+            int larger = 0;
+            for (int j = 0; j < n; ++j) larger += sh.list[j] > key;
+            if (larger < keep) sh.best[larger] = key;
+        }
+        if (tid == 0) sh.best_n = keep;
+    }
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
+    if (rank == 0) {
+        LogprobSum x = sh.all;
+        for (unsigned c = 1; c < ctas; ++c) {   // all threads the same
+            const uint32_t at = remote_smem(&sh.all, c);
+            const LogprobSum other = {__uint_as_float(remote_u32(at)), __uint_as_float(remote_u32(at + 4)), __uint_as_float(remote_u32(at + 8)), (int)remote_u32(at + 12)};
+            x = lp_join(x, other);
+        }
+        // a NaN, plus infinity, or nothing above minus infinity leaves no log sum
+        const bool good = x.sum > 0.f && x.sum < INFINITY && x.top < INFINITY;
+        const float log_sum = logf(x.sum);
+        if (tid == 0) {
+            a.logprob[row] = !there ? 0.f : good ? (zt - x.top) - log_sum : NAN;
+            a.entropy[row] = good ? log_sum - x.moment / x.sum * kLn2 : NAN;
+            a.rank[row] = good && there ? x.before + 1 : 0;
+        }
+        if (a.top > 0) {
+            if (ctas > 1) {
+                // A thread per key of each list; lists are in order.
+                const int c = tid / kLpTop, i = tid % kLpTop;
+                if ((unsigned)c < ctas) {
+                    const int n = (int)remote_u32(remote_smem(&sh.best_n, c));
+                    if (i < n) {
+                        const unsigned long long key = remote_u64(remote_smem(&sh.best[i], c));
+                        int larger = i;
+                        for (unsigned d = 0; d < ctas; ++d) {
+                            if ((int)d == c) continue;
+                            int lo = 0, hi = (int)remote_u32(remote_smem(&sh.best_n, d));   // keys of list d above this one
+                            const uint32_t list = remote_smem(sh.best, d);
+                            while (lo < hi) {
+                                const int mid = (lo + hi) >> 1;
+                                if (remote_u64(list + mid * 8) > key) lo = mid + 1;
+                                else hi = mid;
+                            }
+                            larger += lo;
+                        }
+                        if (larger < a.top) sh.merged[larger] = key;
+                    }
+                }
+                __syncthreads();
+            }
+            if (tid < a.top) {
+                const unsigned long long key = ctas > 1 ? sh.merged[tid] : sh.best[tid];
+                a.top_logprobs[row * a.top + tid] = good ? (unordered_f32((unsigned)(key >> 32)) - x.top) - log_sum : NAN;
+                a.top_tokens[row * a.top + tid] = good ? (int)(0xFFFFFFFFu - (unsigned)key) : -1;
+            }
+        }
+    }
+    if (ctas > 1) cluster_sync();   // no CTA leaves while its lists are read
+}
+
+template <typename T>
+static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
+    int device = 0;
+    MFQB_CUDA(cudaGetDevice(&device));
+    static std::once_flag once[64];
+    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); });
+    // CTAs of a row: until there are two for every SM, as long as a slice has a batch of vectors for every thread.
+    int ctas = 1;
+    while (ctas < 16 && (int64_t)rows * ctas < 2 * 148 && a.vocab / (2 * ctas) >= kLpThreads * kLpBatch) ctas *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * ctas);
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    MFQB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a));
+}
+
+}  // namespace mfqb
+
+using namespace mfqb;
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+int mfqb_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride, const int32_t* tokens, int top, float* logprob, float* entropy,
+                        int32_t* rank, float* top_logprobs, int32_t* top_tokens, mfqb_stream_t stream) {
+    return guarded([&] {
+        if (!logits || !tokens || !logprob || !entropy || !rank) fail(MFQB_ERR_ARG, "mfqb_token_logprobs: null argument");
+        if (dtype != MFQB_F32 && dtype != MFQB_BF16 && dtype != MFQB_F16) fail(MFQB_ERR_ARG, "mfqb_token_logprobs: bad type of logits %d", dtype);
+        const int size = dtype == MFQB_F32 ? 4 : 2;
+        if ((uintptr_t)logits & (size - 1)) fail(MFQB_ERR_ARG, "mfqb_token_logprobs: logits must be aligned to their type");
+        if (rows < 1 || rows > (1 << 24)) fail(MFQB_ERR_ARG, "mfqb_token_logprobs: 1 to %d rows, got %d", 1 << 24, rows);
+        if (vocab < 1 || vocab > kLpVocab) fail(MFQB_ERR_UNSUPPORTED, "mfqb_token_logprobs: a vocabulary of 1 to %d tokens, got %d", kLpVocab, vocab);
+        if (row_stride < vocab && rows > 1) fail(MFQB_ERR_ARG, "mfqb_token_logprobs: rows of %d logits every %lld", vocab, (long long)row_stride);
+        if (top < 0 || top > kLpTop || top > vocab) fail(MFQB_ERR_UNSUPPORTED, "mfqb_token_logprobs: 0 to min(%d, vocab) alternatives, got %d", kLpTop, top);
+        if (top && (!top_logprobs || !top_tokens)) fail(MFQB_ERR_ARG, "mfqb_token_logprobs: null argument");
+        LogprobArgs a{static_cast<const char*>(logits), row_stride * size, tokens, vocab, top, logprob, entropy, top_logprobs, rank, top_tokens};
+        if (dtype == MFQB_F32) launch_logprobs<float>(a, rows, stream);
+        else if (dtype == MFQB_BF16) launch_logprobs<__nv_bfloat16>(a, rows, stream);
+        else launch_logprobs<__half>(a, rows, stream);
+    });
+}
+
+#pragma GCC visibility pop
+}  // extern "C"

@@ -327,6 +327,116 @@ __global__ void __launch_bounds__(256) cache_write_kernel(mfqb_cache c, int laye
     }
 }
 
+// Four of a head's values at dims d .., as float32.
+__device__ __forceinline__ float4 rope_load4(const float* p) { return __ldcg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ float4 rope_load4(const __nv_bfloat16* p) {
+    const uint2 v = __ldcg(reinterpret_cast<const uint2*>(p));
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ float rope_load(const float* p) { return __ldcg(p); }
+__device__ __forceinline__ float rope_load(const __nv_bfloat16* p) { return __bfloat162float(__ldcg(p)); }
+__device__ __forceinline__ uint2 rope_pack(float a, float b, float c, float d) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(a, b), hi = __floats2bfloat162_rn(c, d);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
+// How a thread's four pairs of a head lie: pairs (2j, 2j + 1); pairs (j, j + P) with P a multiple of four; with any P.
+enum RopeForm { kRopeNeighbours, kRopeHalves4, kRopeHalves };
+
+// cache_write_kernel's work for P <= 64 pairs, in other layouts and with a factor on what is turned.  Dims from 2P on pass, as pairs of neighbours: a head
+// has 64 pairs in all, of which thread t of 16 takes 4t .. 4t + 3 (kRopeHalves: t, t + 16, ..).
+template <typename T, RopeForm FORM>
+__global__ void __launch_bounds__(256) cache_rope_kernel(mfqb_cache c, int layer, const T* qkv, int hq, int nodes, const int* depths, const double* freqs, int pairs, float factor,
+                                                         __nv_bfloat16* q_out) {
+    chained_wait();
+    __shared__ float s_cos[64], s_sin[64];
+    const int node = blockIdx.y, r = blockIdx.z, t = threadIdx.x, heads = hq + 2 * c.kv_heads;
+    const int64_t cap = (int64_t)c.width * c.page;
+    const int64_t len = min(max((int64_t)c.lens[r], (int64_t)0), cap);
+    const int64_t item = (int64_t)r * nodes + node;
+    if (t < pairs) {
+        const double a = (double)(len + __ldcg(depths + item)) * __ldcg(freqs + t);
+        const double n = rint(a * 0.15915494309189533577);
+        float sn, cs;
+        sincosf((float)fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586477, a)), &sn, &cs);
+        s_cos[t] = cs * factor;
+        s_sin[t] = sn * factor;
+    }
+    __syncthreads();
+    const int64_t slot = len + node;
+    int page = -1;
+    if (slot < cap) page = c.table[(int64_t)r * c.width + slot / c.page];
+    const bool room = (unsigned)page < (unsigned)c.pages;
+    const int p0 = t & 15;
+    float cs[4], sn[4];
+    bool turn[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int j = FORM == kRopeHalves ? p0 + 16 * e : 4 * p0 + e;
+        turn[e] = j < pairs;
+        cs[e] = turn[e] ? s_cos[j] : 0.f;
+        sn[e] = turn[e] ? s_sin[j] : 0.f;
+    }
+    for (int h = blockIdx.x * 16 + (t >> 4); h < heads; h += gridDim.x * 16) {
+        const T* src = qkv + (item * heads + h) * kHeadDim;
+        __nv_bfloat16* dst;
+        if (h < hq) {
+            dst = q_out + (item * hq + h) * kHeadDim;
+        } else {
+            if (!room) continue;
+            const int kv = h < hq + c.kv_heads ? h - hq : h - hq - c.kv_heads;
+            dst = static_cast<__nv_bfloat16*>(h < hq + c.kv_heads ? c.k : c.v) +
+                  ((((int64_t)layer * c.pages + page) * c.kv_heads + kv) * c.page + (slot & (c.page - 1))) * kHeadDim;
+        }
+        const bool near = FORM == kRopeNeighbours || !turn[0];   // this thread's pairs are eight dims in a row (not asked in kRopeHalves)
+        float x[4], y[4];
+        if (FORM == kRopeHalves) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = p0 + 16 * e;
+                x[e] = rope_load(src + (turn[e] ? j : 2 * j));
+                y[e] = rope_load(src + (turn[e] ? j + pairs : 2 * j + 1));
+            }
+        } else {
+            const float4 u = rope_load4(src + (near ? 8 * p0 : 4 * p0)), v = rope_load4(src + (near ? 8 * p0 + 4 : 4 * p0 + pairs));
+            x[0] = u.x; x[1] = near ? u.z : u.y; x[2] = near ? v.x : u.z; x[3] = near ? v.z : u.w;
+            y[0] = near ? u.y : v.x; y[1] = near ? u.w : v.y; y[2] = near ? v.y : v.z; y[3] = v.w;
+        }
+        if (h < hq + c.kv_heads) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (turn[e]) {
+                    const float a = x[e], b = y[e];
+                    x[e] = a * cs[e] - b * sn[e];
+                    y[e] = b * cs[e] + a * sn[e];
+                }
+        }
+        if (FORM == kRopeHalves) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = p0 + 16 * e;
+                dst[turn[e] ? j : 2 * j] = __float2bfloat16_rn(x[e]);
+                dst[turn[e] ? j + pairs : 2 * j + 1] = __float2bfloat16_rn(y[e]);
+            }
+        } else if (near) {
+            const uint2 u = rope_pack(x[0], y[0], x[1], y[1]), v = rope_pack(x[2], y[2], x[3], y[3]);
+            *reinterpret_cast<uint4*>(dst + 8 * p0) = make_uint4(u.x, u.y, v.x, v.y);
+        } else {
+            *reinterpret_cast<uint2*>(dst + 4 * p0) = rope_pack(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint2*>(dst + 4 * p0 + pairs) = rope_pack(y[0], y[1], y[2], y[3]);
+        }
+    }
+}
+
+template <typename T>
+static void launch_cache_rope(const mfqb_cache& c, int layer, const void* qkv, int q_heads, int nodes, const int32_t* depths, const double* freqs, int pairs, int layout,
+                              float factor, void* q_out, cudaStream_t s) {
+    const int parts = c.rows * nodes >= 148 ? 1 : (q_heads + 2 * c.kv_heads + 15) / 16;
+    auto* kernel = layout == MFQB_ROPE_INTERLEAVED ? cache_rope_kernel<T, kRopeNeighbours> : pairs % 4 == 0 ? cache_rope_kernel<T, kRopeHalves4> : cache_rope_kernel<T, kRopeHalves>;
+    launch_chained(kernel, dim3(parts, nodes, c.rows), dim3(256), 0, s, c, layer, static_cast<const T*>(qkv), q_heads, nodes, depths, freqs, pairs, factor,
+                   static_cast<__nv_bfloat16*>(q_out));
+}
+
 // CTA (some layers' heads, sequence): its first warp walks the tree, two nodes a lane, the first CTA of a sequence leaves the results, and all move
 // the branch's rows, 64 at a time, which are its nodes in as many heads as that makes.  Every row is read into registers before the first one is
 // written, since a slot that one node leaves is another one's place.  A chain from the lengths to the rows: one tree of 8 nodes 4.2 us, 16 of 48
@@ -487,6 +597,28 @@ int mfqb_cache_write(const mfqb_cache* c, int layer, const float* qkv, int q_hea
         const int parts = c->rows * nodes >= 148 ? 1 : (q_heads + 2 * c->kv_heads + 15) / 16;
         launch_chained(cache_write_kernel, dim3(parts, nodes, c->rows), dim3(256), 0, stream, *c, layer, qkv, q_heads, nodes, depths, freqs,
                        static_cast<__nv_bfloat16*>(q_out));
+    });
+}
+
+int mfqb_cache_write_rope(const mfqb_cache* c, int layer, const void* qkv, int qkv_dtype, int q_heads, int nodes, const int32_t* depths, const double* freqs, int pairs,
+                          int layout, float factor, void* q_out, mfqb_stream_t stream) {
+    return guarded([&] {
+        const char* who = "mfqb_cache_write_rope";
+        check_cache(c, who);
+        check_nodes(c, nodes, who);
+        if (!qkv || !depths || !freqs || !q_out) fail(MFQB_ERR_ARG, "%s: null argument", who);
+        if (qkv_dtype != MFQB_F32 && qkv_dtype != MFQB_BF16) fail(MFQB_ERR_ARG, "%s: bad type of qkv %d", who, qkv_dtype);
+        if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 15)) fail(MFQB_ERR_ARG, "%s: qkv and q_out must be 16-byte aligned", who);
+        if ((uintptr_t)freqs & 7) fail(MFQB_ERR_ARG, "%s: freqs must be 8-byte aligned", who);
+        if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "%s: layer %d of %d", who, layer, c->layers);
+        if (q_heads < 1 || q_heads > 16384) fail(MFQB_ERR_ARG, "%s: bad number of query heads %d", who, q_heads);
+        if (pairs < 1 || pairs > kHeadDim / 2) fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to %d pairs of dims, got %d", who, kHeadDim / 2, pairs);
+        if (layout != MFQB_ROPE_HALVES && layout != MFQB_ROPE_INTERLEAVED) fail(MFQB_ERR_ARG, "%s: bad layout %d", who, layout);
+        if (!(factor > 0.f) || factor > 1e30f) fail(MFQB_ERR_ARG, "%s: factor must be positive and finite", who);
+        const uint64_t tokens = (uint64_t)c->rows * nodes, size = qkv_dtype == MFQB_F32 ? 4 : 2;
+        check_apart(q_out, 256 * tokens * q_heads, qkv, size * kHeadDim * tokens * (q_heads + 2 * c->kv_heads), who, "qkv and q_out");
+        if (qkv_dtype == MFQB_F32) launch_cache_rope<float>(*c, layer, qkv, q_heads, nodes, depths, freqs, pairs, layout, factor, q_out, stream);
+        else launch_cache_rope<__nv_bfloat16>(*c, layer, qkv, q_heads, nodes, depths, freqs, pairs, layout, factor, q_out, stream);
     });
 }
 

@@ -12,67 +12,15 @@
 // the 128-byte swizzle), one issues tcgen05.mma, four (or eight) do the softmax, a row a thread: S comes out of tensor memory, P goes back
 // into it as the A operand of the second product, O stays there.  O is multiplied by a correction only when a row's maximum has
 // grown by more than 2^8 (P then stays below 2^8, which bf16 holds as exactly as values below 1).
-#include <cuda.h>
-#include <cuda_bf16.h>
-
-#include <mutex>
-
-#include "paged.h"
-#include "tc05.cuh"
+#include "tree_attn.cuh"
 
 namespace mfqb {
 
-constexpr int kTreeSms = 148;
-constexpr int kTile = 128;                           // rows of Q, positions of a tile
-constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
 constexpr int tree_ctas(int ns) { return ns == 2 ? kTreeSms : 2 * kTreeSms; }
 constexpr int tree_ring(int ns) { return ns == 2 ? 5 : 2; }   // tiles
 constexpr int tree_threads(int ns) { return 64 + 128 * ns; }
 constexpr int kTreeWhole = 256;                       // positions
-constexpr int kTreeStart = 2;                         // what starting and ending a stretch takes, in tiles
 
-struct TreeArgs {
-    const int* table;
-    const int* lens;
-    const __nv_bfloat16* q;
-    const unsigned long long* masks;
-    const __nv_bfloat16 *k, *v;   // of the layer
-    __nv_bfloat16* out;
-    float* part;                  // [CTA][first, last][rows of a tile][128], then their (maximum, sum)
-    float2* part_ml;
-    int64_t* before;              // [rows + 1]: units of one item of each sequence before a sequence; the units of a CTA
-    int* error;
-    int rows, width, pages, page, kv_heads, hq, group, nodes, row_tiles, tile_rows;   // row_tiles: of 128 rows a stream; tile_rows: rows of a part, at most that
-    bool whole;                   // an item is one unit
-    unsigned group_inv;           // ceil(65536 / group): row / group = row * group_inv >> 16 for rows below 1024, groups up to 16
-    float scale_log2;
-    __device__ __forceinline__ int node_of(int row_of_q) const { return (int)((unsigned)row_of_q * group_inv >> 16); }
-    // element offset of a row of Q (or of the output) of sequence r and kv head kvh
-    __device__ __forceinline__ int64_t row_at(int r, int kvh, int row_of_q) const {
-        const int node = node_of(row_of_q);
-        return (((int64_t)r * nodes + node) * hq + kvh * group + row_of_q - node * group) * kHeadDim;
-    }
-};
-
-// a / b of numbers that are not negative; mostly they fit 32 bits, and a 64-bit division is some hundred instructions.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b;
-}
-
-// Tiles of sequence r (at least one: a sequence has a node), its length and end.
-struct TreeSeq {
-    int len, end, tiles;
-    int units;   // of an item: its tiles and its start, or 1 where items are not split (TreeArgs::whole)
-};
-__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int r) {
-    const int cap = a.width * a.page;   // at most 2^30
-    TreeSeq s;
-    s.len = min(max(__ldcg(a.lens + r), 0), cap);
-    s.end = min(s.len + a.nodes, cap);
-    s.tiles = (s.end + kTile - 1) / kTile;
-    s.units = a.whole ? 1 : s.tiles + kTreeStart;
-    return s;
-}
 struct TreeShared {
     uint64_t kv_full[5], kv_empty[5], q_full, s_full[2], p_full[2], o_done[2], drain, all, group[2];
     unsigned long long bad_nodes;   // nodes of the stretch whose values hold an infinity or NaN
@@ -125,91 +73,6 @@ private:
     }
 };
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-                 : "memory");
-}
-// D (+)= A B^T, both operands in shared memory.
-__device__ __forceinline__ void tc_mma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-// bf16 x bf16 -> f32; B with its K index running over rows of 128 bytes (values: position by position) where mn is set.
-constexpr uint32_t instr_desc_bf16(int m, int n, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-// Descriptor of a [positions][64 dims] half in 128-byte rows taken as B operand with the dims as its rows: eight positions 1024
-// bytes apart, the next 64 dims one half further.
-__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(kHalfBytes >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-#define MFQB_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
-#define MFQB_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
-// 32 lanes x 32 columns, a lane's columns in its registers; the load's values may be used after tmem_wait_ld.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : MFQB_R8(r, 0), MFQB_R8(r, 8), MFQB_R8(r, 16), MFQB_R8(r, 24)
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : MFQB_R8(r, 0), MFQB_R8(r, 8)
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-                 ::MFQB_W8(r, 0), MFQB_W8(r, 8), MFQB_W8(r, 16), MFQB_W8(r, 24), "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MFQB_W8(r, 0), MFQB_W8(r, 8), "r"(taddr)
-                 : "memory");
-}
-#define MFQB_P8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
-// Waits for this thread's loads.  The 32 registers of a load pass through it, so that no use of them can be moved before the wait.
-__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    asm volatile("" : MFQB_P8(r, 0), MFQB_P8(r, 8));
-    asm volatile("" : MFQB_P8(r, 16), MFQB_P8(r, 24));
-}
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    asm volatile("" : MFQB_P8(r, 0), MFQB_P8(r, 8));
-}
-__device__ __forceinline__ void tmem_wait_ld(uint32_t* r, uint32_t* q) {
-    tmem_wait_ld(r);
-    asm volatile("" : MFQB_P8(q, 0), MFQB_P8(q, 8));
-    asm volatile("" : MFQB_P8(q, 16), MFQB_P8(q, 24));
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ void warp_arrive(uint64_t* bar) {   // one arrival for what all lanes have done
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
-// Both of two barriers; the polls of barriers that are complete (the usual case of one of them) overlap.
-__device__ __forceinline__ bool warp_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
-    const bool da = mbar_test(a, pa), db = mbar_test(b, pb);
-    if (__all_sync(0xffffffffu, da && db)) return true;
-    return warp_wait(a, pa) && warp_wait(b, pb);
-}
-
 // exp2(scale s + mc) of 16 scores, rounded to bf16 into p; their sums are added to l, their maxima to top where TOP.
 // The one rounding of the probabilities: the tensor core takes them in the values' type, and a second bf16 term would be the second product
 // again and half of S's columns.  Against 64 bits the output is off by 0.0019 to 0.0023 of its size, where rounding it alone makes 0.0017.
@@ -256,6 +119,9 @@ __device__ __noinline__ void clean_values(TreeShared& sh, unsigned char* tile, T
     __syncwarp();
 }
 
+// What turns a row's scores into weights: exp2(scale' score - x) y.  Nothing seen: y = 0; no maximum above minus infinity: NaN.
+__device__ __forceinline__ float2 row_scale(float m, float l) { return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l); }
+
 // Rare: values of visible nodes that hold an infinity or NaN were taken out of the product (0 in their place, so that rows which do not see
 // the node keep clear of them); here they are added to the row's result, where the row sees them.
 template <typename T>
@@ -283,7 +149,8 @@ __device__ __noinline__ void add_bad_nodes(const TreeArgs& a, unsigned long long
 // One warp issues for both streams: with a warp each they fall into step, and the tensor core waits while both do softmax.
 // REP: up to 32 (64) rows stand in Q four times (twice), and a copy's warps take a quarter (a half) of every tile's positions: their
 // P is zero elsewhere.  A row's 128 exponentials in one thread are what a tile waits for otherwise.
-template <int NS, int REP>
+// WEIGH: leaves what the sums of the weights are made of, every row's maximum and sum and, for few rows, the scores.
+template <int NS, int REP, bool WEIGH>
 __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
                                                                                      const __grid_constant__ CUtensorMap vmap) {
     constexpr int kRing = tree_ring(NS);
@@ -571,6 +438,13 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                         for (int c = 0; c < kCols; c += 32) tmem_ld32(col_s + copy * kCols + c, s + c);
 #pragma unroll
                         for (int c = 0; c < kCols; c += 32) tmem_wait_ld(s + c);
+                        if constexpr (WEIGH) {
+                            if (a.scores && live) {
+                                uint4* to = reinterpret_cast<uint4*>(a.scores + (((int64_t)w.r * a.kv_heads + kvh) * m_rows + row) * a.score_stride + pos0 + copy * kCols);
+#pragma unroll
+                                for (int c = 0; c < kCols; c += 4) to[c / 4] = make_uint4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+                            }
+                        }
                         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int e = 0; e < kCols; e += 2) top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
@@ -765,6 +639,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             }
             if (live && copy == 0) {
                 if (!complete) a.part_ml[slot + row_l] = sum;
+                else if constexpr (WEIGH) a.row_ml[((int64_t)w.r * a.kv_heads + kvh) * m_rows + row] = row_scale(sum.x, sum.y);
                 if (bad) {
                     if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + a.row_at(w.r, kvh, row));
                     else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim);
@@ -845,33 +720,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __gr
         __syncwarp();   // the parts have been read before the next come in their place
     }
     if (m == -INFINITY) l = none;
+    if (a.row_ml && lane == 0) a.row_ml[((int64_t)r * a.kv_heads + kvh) * m_rows + row] = row_scale(m, l);
     const float inv = 1.f / l;
     if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
     else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(a.out + a.row_at(r, kvh, row) + 4 * lane) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-}
-
-// Keys or values of one layer as [page][head][position][128]: boxes of min(page, 128) positions x 64 dims with the 128-byte swizzle.
-static CUtensorMap page_map(const void* base, const mfqb_cache& c) {
-    typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static encode_fn encode = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess)
-            encode = reinterpret_cast<encode_fn>(p);
-    });
-    if (!encode) fail(MFQB_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-    CUtensorMap map;
-    const cuuint64_t dims[4] = {kHeadDim, (cuuint64_t)c.page, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
-    const cuuint64_t strides[3] = {256, (cuuint64_t)c.page * 256, (cuuint64_t)c.kv_heads * c.page * 256};
-    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(c.page, kTile), 1, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (rc != CUDA_SUCCESS) fail(MFQB_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)rc);
-    return map;
 }
 
 // Rows are paid for in steps, of which the last begin behind 128 and 256: 4 sequences at context 8192 over 8 kv heads take 47 us for 128 rows (32 nodes
@@ -884,13 +737,32 @@ static int64_t tree_parts(const mfqb_cache& c, int q_heads, int nodes) {   // ro
 static uint64_t tree_attention_work_bytes(const mfqb_cache& c, int q_heads, int nodes) {
     return (uint64_t)tree_parts(c, q_heads, nodes) * (kHeadDim * 4 + 8) + 8ull * (c.rows + 1);
 }
-static void check_heads(const mfqb_cache* c, int q_heads, const char* who) {
+static uint64_t weigh_work_bytes(const mfqb_cache& c, int q_heads, int nodes) {
+    return (tree_attention_work_bytes(c, q_heads, nodes) + 15) / 16 * 16 + tree_weigh_bytes(c, q_heads, nodes);
+}
+static void check_attention_shape(const mfqb_cache* c, int q_heads, int nodes, const char* who) {
+    check_cache(c, who);
+    check_nodes(c, nodes, who);
     if (q_heads < 1 || q_heads % c->kv_heads || q_heads / c->kv_heads > 16)
         fail(MFQB_ERR_UNSUPPORTED, "%s: 1 to 16 query heads per kv head, got %d over %d", who, q_heads, c->kv_heads);
 }
+static void check_attention(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, const void* out, const void* work,
+                            uint64_t work_bytes, uint64_t need, const char* who) {
+    if (!q || !masks || !out || !work) fail(MFQB_ERR_ARG, "%s: null argument", who);
+    if (((uintptr_t)q & 15) || ((uintptr_t)out & 15)) fail(MFQB_ERR_ARG, "%s: q and out must be 16-byte aligned", who);
+    if ((uintptr_t)masks & 7) fail(MFQB_ERR_ARG, "%s: masks must be 8-byte aligned", who);
+    if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "%s: layer %d of %d", who, layer, c->layers);
+    if (!(scale > 0.f) || scale > 1e30f) fail(MFQB_ERR_ARG, "%s: scale must be positive and finite", who);
+    if (((uintptr_t)work & 15) || work_bytes < need)
+        fail(MFQB_ERR_ARG, "%s: work must be 16-byte aligned and hold %llu bytes, got %llu", who, (unsigned long long)need, (unsigned long long)work_bytes);
+    // add_bad_nodes reads the queries of rows that have been written
+    const uint64_t bytes = 256ull * c->rows * nodes * q_heads;
+    check_apart(out, bytes, q, bytes, who, "q and out");
+}
 
-static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, void* work,
-                                  cudaStream_t s) {
+// weights (of all layers): added up behind the attention, where given.
+static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights,
+                                  void* work, cudaStream_t s) {
     int device = 0;
     MFQB_CUDA(cudaGetDevice(&device));
     const int64_t per_layer = (int64_t)c.pages * c.kv_heads * c.page * kHeadDim;
@@ -920,11 +792,20 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     a.scale_log2 = scale * 1.4426950408889634f;
     a.error = device_status_word(device);
     const CUtensorMap kmap = page_map(a.k, c), vmap = page_map(a.v, c);
-    auto* kernel = ns == 2 ? tree_attn_kernel<2, 1> : m_rows > 64 ? tree_attn_kernel<1, 1> : m_rows > 32 ? tree_attn_kernel<1, 2> : tree_attn_kernel<1, 4>;
+    if (weights) {
+        char* more = static_cast<char*>(work) + (tree_attention_work_bytes(c, q_heads, nodes) + 15) / 16 * 16;
+        a.score_stride = tree_score_stride(c, q_heads, nodes);
+        a.scores = a.score_stride ? reinterpret_cast<float*>(more) : nullptr;
+        a.row_ml = reinterpret_cast<float2*>(more + 4ull * c.rows * c.kv_heads * m_rows * a.score_stride);
+    }
+    auto* kernel = weights ? ns == 2 ? tree_attn_kernel<2, 1, true> : m_rows > 64 ? tree_attn_kernel<1, 1, true> : m_rows > 32 ? tree_attn_kernel<1, 2, true> : tree_attn_kernel<1, 4, true>
+                   : ns == 2 ? tree_attn_kernel<2, 1, false> : m_rows > 64 ? tree_attn_kernel<1, 1, false> : m_rows > 32 ? tree_attn_kernel<1, 2, false> : tree_attn_kernel<1, 4, false>;
     static std::once_flag once[64];
     std::call_once(once[device], [] {
-        MFQB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<2, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(2)));
-        for (auto* k : {tree_attn_kernel<1, 1>, tree_attn_kernel<1, 2>, tree_attn_kernel<1, 4>})
+        for (auto* k : {tree_attn_kernel<2, 1, false>, tree_attn_kernel<2, 1, true>})
+            MFQB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(2)));
+        for (auto* k : {tree_attn_kernel<1, 1, false>, tree_attn_kernel<1, 2, false>, tree_attn_kernel<1, 4, false>, tree_attn_kernel<1, 1, true>, tree_attn_kernel<1, 2, true>,
+                        tree_attn_kernel<1, 4, true>})
             MFQB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(1)));
     });
     // Tables of up to kTreeWhole positions: an item is not split, and there is nothing to merge (one token at context 100: 8.1 us a pass, 9.3 with a table of
@@ -933,9 +814,9 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     const int64_t most = (int64_t)c.rows * c.kv_heads * a.row_tiles * (a.whole ? 1 : ((int64_t)c.width * c.page + kTile - 1) / kTile);   // tiles there can be
     const int ctas = (int)std::min<int64_t>(tree_ctas(ns), most);
     launch_chained(kernel, dim3(ctas), dim3(tree_threads(ns)), tree_smem(ns), s, a, kmap, vmap);
-    if (a.whole) return;
     const int64_t rows = (int64_t)c.rows * c.kv_heads * m_rows;   // at most 1024 x 1024 x 1024
-    launch_chained(tree_merge_kernel, dim3((unsigned)((rows + kMergeWarps - 1) / kMergeWarps)), dim3(32 * kMergeWarps), 0, s, a, ns, (int)rows);
+    if (!a.whole) launch_chained(tree_merge_kernel, dim3((unsigned)((rows + kMergeWarps - 1) / kMergeWarps)), dim3(32 * kMergeWarps), 0, s, a, ns, (int)rows);
+    if (weights) launch_tree_weigh(c, a, weights + (int64_t)layer * c.rows * c.kv_heads * c.width * c.page, s);
 }
 
 }  // namespace mfqb
@@ -947,9 +828,7 @@ extern "C" {
 
 int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes) {
     return guarded([&] {
-        check_cache(c, "mfqb_tree_attention_work");
-        check_nodes(c, nodes, "mfqb_tree_attention_work");
-        check_heads(c, q_heads, "mfqb_tree_attention_work");
+        check_attention_shape(c, q_heads, nodes, "mfqb_tree_attention_work");
         if (!bytes) fail(MFQB_ERR_ARG, "mfqb_tree_attention_work: null argument");
         ready_device();
         *bytes = tree_attention_work_bytes(*c, q_heads, nodes);
@@ -959,21 +838,33 @@ int mfqb_tree_attention_work(const mfqb_cache* c, int q_heads, int nodes, uint64
 int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out,
                         void* work, uint64_t work_bytes, mfqb_stream_t stream) {
     return guarded([&] {
-        check_cache(c, "mfqb_tree_attention");
-        check_nodes(c, nodes, "mfqb_tree_attention");
-        check_heads(c, q_heads, "mfqb_tree_attention");
-        if (!q || !masks || !out || !work) fail(MFQB_ERR_ARG, "mfqb_tree_attention: null argument");
-        if (((uintptr_t)q & 15) || ((uintptr_t)out & 15)) fail(MFQB_ERR_ARG, "mfqb_tree_attention: q and out must be 16-byte aligned");
-        if ((uintptr_t)masks & 7) fail(MFQB_ERR_ARG, "mfqb_tree_attention: masks must be 8-byte aligned");
-        if (layer < 0 || layer >= c->layers) fail(MFQB_ERR_ARG, "mfqb_tree_attention: layer %d of %d", layer, c->layers);
-        if (!(scale > 0.f) || scale > 1e30f) fail(MFQB_ERR_ARG, "mfqb_tree_attention: scale must be positive and finite");
-        if (((uintptr_t)work & 15) || work_bytes < tree_attention_work_bytes(*c, q_heads, nodes))
-            fail(MFQB_ERR_ARG, "mfqb_tree_attention: work must be 16-byte aligned and hold %llu bytes, got %llu",
-                 (unsigned long long)tree_attention_work_bytes(*c, q_heads, nodes), (unsigned long long)work_bytes);
-        // add_bad_nodes reads the queries of rows that have been written
-        const uint64_t bytes = 256ull * c->rows * nodes * q_heads;
-        check_apart(out, bytes, q, bytes, "mfqb_tree_attention", "q and out");
-        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, work, stream);
+        check_attention_shape(c, q_heads, nodes, "mfqb_tree_attention");
+        check_attention(c, layer, q, q_heads, nodes, masks, scale, out, work, work_bytes, tree_attention_work_bytes(*c, q_heads, nodes), "mfqb_tree_attention");
+        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, nullptr, work, stream);
+    });
+}
+
+int mfqb_tree_attention_weigh_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes) {
+    return guarded([&] {
+        check_attention_shape(c, q_heads, nodes, "mfqb_tree_attention_weigh_work");
+        if (!bytes) fail(MFQB_ERR_ARG, "mfqb_tree_attention_weigh_work: null argument");
+        ready_device();
+        *bytes = weigh_work_bytes(*c, q_heads, nodes);
+    });
+}
+
+int mfqb_tree_attention_weigh(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights,
+                              void* work, uint64_t work_bytes, mfqb_stream_t stream) {
+    return guarded([&] {
+        const char* who = "mfqb_tree_attention_weigh";
+        check_attention_shape(c, q_heads, nodes, who);
+        check_attention(c, layer, q, q_heads, nodes, masks, scale, out, work, work_bytes, weigh_work_bytes(*c, q_heads, nodes), who);
+        if (!weights || ((uintptr_t)weights & 3)) fail(MFQB_ERR_ARG, "%s: weights must be float32 values on 4-byte boundaries", who);
+        const uint64_t bytes = 256ull * c->rows * nodes * q_heads, all = 4ull * c->layers * c->rows * c->kv_heads * c->width * c->page;
+        check_apart(weights, all, q, bytes, who, "q and weights");   // q is read again for the weights
+        check_apart(weights, all, out, bytes, who, "out and weights");
+        check_apart(weights, all, work, work_bytes, who, "work and weights");
+        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, weights, work, stream);
     });
 }
 

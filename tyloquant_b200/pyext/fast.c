@@ -19,6 +19,11 @@ typedef int (*attend_fn)(const void*, int, const void*, int, int, const void*, f
 typedef int (*accept_fn)(const void*, const void*, const void*, const void*, int, void*, void*, void*, void*, void*);
 typedef int (*beam_fn)(const void*, int, int, int, const void*, const void*, int, int, void*, void*, void*, void*, uint64_t, void*);
 
+typedef int (*rope_fn)(const void*, int, const void*, int, int, int, const void*, const void*, int, int, float, void*, void*);
+typedef int (*weigh_fn)(const void*, int, const void*, int, int, const void*, float, void*, void*, void*, uint64_t, void*);
+typedef int (*evict_fn)(const void*, void*, const void*, int, void*, void*, void*, uint64_t, void*);
+typedef int (*logprobs_fn)(const void*, int, int, int, int64_t, const void*, int, void*, void*, void*, void*, void*, void*);
+
 static mul_mat_fn p_mul_mat;
 static topk_fn p_topk;
 static ffn_fn p_ffn;
@@ -29,6 +34,10 @@ static write_fn p_write;
 static attend_fn p_attend;
 static accept_fn p_accept;
 static beam_fn p_beam;
+static rope_fn p_rope;
+static weigh_fn p_weigh;
+static evict_fn p_evict;
+static logprobs_fn p_logprobs;
 
 static void* address(PyObject* o) { return o == Py_None ? NULL : (void*)(uintptr_t)PyLong_AsUnsignedLongLong(o); }
 static int number(PyObject* o) {
@@ -44,7 +53,7 @@ static int arity(Py_ssize_t got, Py_ssize_t want) {
 
 static PyObject* bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
-    if (!arity(n, 10)) return NULL;
+    if (!arity(n, 14)) return NULL;
     p_mul_mat = (mul_mat_fn)address(a[0]);
     p_topk = (topk_fn)address(a[1]);
     p_ffn = (ffn_fn)address(a[2]);
@@ -55,6 +64,10 @@ static PyObject* bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     p_attend = (attend_fn)address(a[7]);
     p_accept = (accept_fn)address(a[8]);
     p_beam = (beam_fn)address(a[9]);
+    p_rope = (rope_fn)address(a[10]);
+    p_weigh = (weigh_fn)address(a[11]);
+    p_evict = (evict_fn)address(a[12]);
+    p_logprobs = (logprobs_fn)address(a[13]);
     if (PyErr_Occurred()) return NULL;
     Py_RETURN_NONE;
 }
@@ -245,6 +258,97 @@ static PyObject* beam_select(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(rc);
 }
+/* cache, layer, qkv, dtype, q_heads, nodes, depths, freqs, pairs, layout, factor, q_out, stream */
+static PyObject* cache_write_rope(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    (void)self;
+    if (!arity(n, 13)) return NULL;
+    void* c = address(a[0]);
+    const int l = number(a[1]);
+    void* x = address(a[2]);
+    const int dt = number(a[3]);
+    const int hq = number(a[4]);
+    const int nodes = number(a[5]);
+    void* d = address(a[6]);
+    void* f = address(a[7]);
+    const int pairs = number(a[8]);
+    const int layout = number(a[9]);
+    const float factor = (float)PyFloat_AsDouble(a[10]);
+    void* q = address(a[11]);
+    void* s = address(a[12]);
+    if (PyErr_Occurred()) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_rope(c, l, x, dt, hq, nodes, d, f, pairs, layout, factor, q, s);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+/* cache, layer, q, q_heads, nodes, masks, scale, out, weights, work, work_bytes, stream */
+static PyObject* tree_attention_weigh(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    (void)self;
+    if (!arity(n, 12)) return NULL;
+    void* c = address(a[0]);
+    const int l = number(a[1]);
+    void* q = address(a[2]);
+    const int hq = number(a[3]);
+    const int nodes = number(a[4]);
+    void* m = address(a[5]);
+    const float scale = (float)PyFloat_AsDouble(a[6]);
+    void* o = address(a[7]);
+    void* wt = address(a[8]);
+    void* w = address(a[9]);
+    const uint64_t wb = PyLong_AsUnsignedLongLong(a[10]);
+    void* s = address(a[11]);
+    if (PyErr_Occurred()) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_weigh(c, l, q, hq, nodes, m, scale, o, wt, w, wb, s);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+/* cache, weights, keep, recent, dropped, status, work, work_bytes, stream */
+static PyObject* cache_evict(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    (void)self;
+    if (!arity(n, 9)) return NULL;
+    void* c = address(a[0]);
+    void* wt = address(a[1]);
+    void* k = address(a[2]);
+    const int recent = number(a[3]);
+    void* d = address(a[4]);
+    void* st = address(a[5]);
+    void* w = address(a[6]);
+    const uint64_t wb = PyLong_AsUnsignedLongLong(a[7]);
+    void* s = address(a[8]);
+    if (PyErr_Occurred()) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_evict(c, wt, k, recent, d, st, w, wb, s);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+/* logits, dtype, rows, vocab, row_stride, tokens, top, logprob, entropy, rank, top_logprobs, top_tokens, stream */
+static PyObject* token_logprobs(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    (void)self;
+    if (!arity(n, 13)) return NULL;
+    void* z = address(a[0]);
+    const int dt = number(a[1]);
+    const int rows = number(a[2]);
+    const int vocab = number(a[3]);
+    const int64_t stride = PyLong_AsLongLong(a[4]);
+    void* t = address(a[5]);
+    const int top = number(a[6]);
+    void* lp = address(a[7]);
+    void* en = address(a[8]);
+    void* rk = address(a[9]);
+    void* tl = address(a[10]);
+    void* tt = address(a[11]);
+    void* s = address(a[12]);
+    if (PyErr_Occurred()) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_logprobs(z, dt, rows, vocab, stride, t, top, lp, en, rk, tl, tt, s);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
 
 static PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, "addresses of the entry points below, in their order"},
                                 {"mul_mat", (PyCFunction)(void (*)(void))mul_mat, METH_FASTCALL, "mfqb_mul_mat"},
@@ -257,6 +361,10 @@ static PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH
                                 {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, "mfqb_tree_attention"},
                                 {"tree_accept", (PyCFunction)(void (*)(void))tree_accept, METH_FASTCALL, "mfqb_tree_accept"},
                                 {"beam_select", (PyCFunction)(void (*)(void))beam_select, METH_FASTCALL, "mfqb_beam_select"},
+                                {"cache_write_rope", (PyCFunction)(void (*)(void))cache_write_rope, METH_FASTCALL, "mfqb_cache_write_rope"},
+                                {"tree_attention_weigh", (PyCFunction)(void (*)(void))tree_attention_weigh, METH_FASTCALL, "mfqb_tree_attention_weigh"},
+                                {"cache_evict", (PyCFunction)(void (*)(void))cache_evict, METH_FASTCALL, "mfqb_cache_evict"},
+                                {"token_logprobs", (PyCFunction)(void (*)(void))token_logprobs, METH_FASTCALL, "mfqb_token_logprobs"},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "Direct calls of the library's hot entry points.", -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__fast(void) { return PyModule_Create(&module); }
