@@ -1,13 +1,14 @@
 // Eviction from a paged cache: every head of every layer keeps the positions with the largest weights and the latest ones; their keys and
 // values close up, and the pages behind them go back.
 #include <mutex>
+#include <type_traits>
 
 #include "select.cuh"
 
 namespace mfqb {
 
-constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
-constexpr int kEvictStep = 4 * kEvictThreads;          // slots that are looked at together
+constexpr int kEvictThreads = 256, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictStep = 8 * kEvictThreads;          // slots that are looked at together, and room for as many as are found
 constexpr int kEvictCached = 48 * 1024;                // positions whose keys fit shared memory
 
 struct EvictRow {
@@ -105,116 +106,134 @@ __global__ void __launch_bounds__(1024) evict_plan_kernel(mfqb_cache c, const in
     }
 }
 
+template <typename Slot>
 struct EvictShared {
-    CutShared cut;
-    int holes[kEvictStep], movers[kEvictStep];
+    union {   // the search for the cut, then what is to be moved
+        CutShared cut;
+        struct {
+            Slot holes[kEvictStep], movers[kEvictStep];
+        };
+    };
+    int sums[kEvictWarps + 1];
 };
 
 // A cluster per head of a layer of a sequence.  Each of its CTAs finds the cut and the same lists of free slots and of rows to move, and moves its
 // share; the latest rows follow when all others have moved.  Rows are read before a slot that holds one is written: the others go to
 // slots below the new length's older part, where none of them lies, and the latest ones in ascending order.
 template <bool CACHED>
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(mfqb_cache c, float* weights, int recent_most, EvictWork w) {
-    extern __shared__ unsigned s_keys[];
-    __shared__ EvictShared sh;
+__global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(mfqb_cache c, float* weights, int recent_most, EvictWork w) {
+    extern __shared__ uint4 s_keys[];   // four slots each; 0, which no value has, behind the last one
+    using Slot = typename std::conditional<CACHED, unsigned short, int>::type;
+    static_assert(!CACHED || kEvictCached <= 65536, "a slot in 16 bits");
+    __shared__ EvictShared<Slot> sh;
     chained_wait();
     unsigned part, parts;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
-    const int64_t unit = blockIdx.x / parts, layer = unit / ((int64_t)c.rows * c.kv_heads);
-    const int left = (int)(unit - layer * c.rows * c.kv_heads), r = left / c.kv_heads, head = left - r * c.kv_heads, tid = threadIdx.x;
+    const int layer = blockIdx.z, r = blockIdx.y, head = blockIdx.x / parts, tid = threadIdx.x;
+    const int64_t unit = ((int64_t)layer * c.rows + r) * c.kv_heads + head;
     const EvictRow row = w.row[r];
     if (row.keep < 0) return;   // the whole cluster
     const int n = row.len, k = row.keep, recent = min(recent_most, k), older = n - recent, b = k - recent;   // of `older` slots b stay, the first b of the new ones
     const int bits = __ffs(c.page) - 1, low = c.page - 1;
     const int *old_table = w.old + (int64_t)r * c.width, *table = c.table + (int64_t)r * c.width;
     float* wt = weights + unit * c.width * c.page;
-    const int64_t base = (layer * c.pages * c.kv_heads + head) * c.page;   // row of page 0
-    auto at = [&](const int* t, int slot) -> int64_t {                      // row of a slot in the pools, -1 without a page
+    constexpr int kTeams = kEvictThreads / 16;   // a row is 16 threads'
+    const int lane = tid & 15, team = tid >> 4, stride = c.kv_heads * c.page;
+    uint4* const kp = static_cast<uint4*>(c.k) + ((int64_t)layer * c.pages * c.kv_heads + head) * c.page * 16 + lane;   // this thread's part of row 0 of page 0
+    uint4* const vp = static_cast<uint4*>(c.v) + ((int64_t)layer * c.pages * c.kv_heads + head) * c.page * 16 + lane;
+    auto at = [&](const int* t, int slot) -> int64_t {   // of a slot, -1 without a page
         const int p = t[slot >> bits];
-        return (unsigned)p < (unsigned)c.pages ? base + (int64_t)p * c.kv_heads * c.page + (slot & low) : -1;
+        return (unsigned)p < (unsigned)c.pages ? ((int64_t)p * stride + (slot & low)) * 16 : -1;
     };
-    uint4 *kp = static_cast<uint4*>(c.k), *vp = static_cast<uint4*>(c.v);
-    auto key = [&](int i) { return CACHED ? s_keys[i] : ordered_f32(wt[i]); };
-
+    auto read = [&](int i) {   // keys of slots 4i ..
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(wt) + i);
+        return make_uint4(ordered_f32(x.x), 4 * i + 1 < older ? ordered_f32(x.y) : 0u, 4 * i + 2 < older ? ordered_f32(x.z) : 0u, 4 * i + 3 < older ? ordered_f32(x.w) : 0u);
+    };
+    auto keys = [&](int i) { return CACHED ? s_keys[i] : read(i); };
     auto sync_all = [&]() {
         if (parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         else __syncthreads();
     };
     if (b > 0) {
-        if (CACHED) {
-            for (int i = tid; i < older; i += kEvictThreads) s_keys[i] = ordered_f32(wt[i]);
-            sync_all();   // no CTA moves weights that another one has not read
+        const int fours = (older + 3) / 4;
+        unsigned low = 0xFFFFFFFFu, high = 0u;
+#pragma unroll 2
+        for (int i = tid; i < fours; i += kEvictThreads) {
+            const uint4 k = read(i);
+            if (CACHED) s_keys[i] = k;
+            low = min(min(low, k.x - 1u), min(k.y - 1u, min(k.z - 1u, k.w - 1u)));   // less 1, so that none is the largest
+            high = max(max(high, k.x), max(k.y, max(k.z, k.w)));
         }
-        const Cut cut = select_cut<kEvictThreads>(b, sh.cut, [&](auto f) {
-            for (int i = tid; i < older; i += kEvictThreads) f(key(i));
-        });
-        // Walks slots [slot, end) in steps until it has found some that `take` wants (stay: is the slot kept?), in ascending order.
-        struct Walk {
-            int slot, end, ties, n, used;
-        };
-        auto fill = [&](Walk& x, int* list, auto take) {
-            x.n = x.used = 0;
-            while (x.n == 0 && x.slot < x.end) {
-                const int i0 = x.slot + 4 * tid;
-                unsigned o[4];
-                int equal = 0, mine = x.ties, want = 0;
-                bool t[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[e] = i0 + e < x.end ? key(i0 + e) : 0u;
-                    equal += o[e] == cut.key;
-                }
-                if (cut.ties) {
-                    const int upto = block_scan<kEvictThreads>(equal, sh.cut.sums);
-                    __syncthreads();
-                    mine += upto - equal;
-                    x.ties += sh.cut.sums[kEvictWarps];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool tie = o[e] == cut.key, stays = o[e] > cut.key || (tie && mine < cut.ties);
-                    mine += tie;
-                    t[e] = i0 + e < x.end && take(stays, i0 + e);
-                    want += t[e];
-                }
-                int to = block_scan<kEvictThreads>(want, sh.cut.sums) - want;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (t[e]) list[to++] = i0 + e;
-                __syncthreads();
-                x.n = sh.cut.sums[kEvictWarps];
-                x.slot = min(x.end, x.slot + kEvictStep);
+        if (low != 0xFFFFFFFFu) ++low;
+        if (CACHED) sync_all();   // no CTA moves weights that another one has not read
+        const Cut cut = select_cut<kEvictThreads>(b, low, high, older, sh.cut, [&](auto f) {
+#pragma unroll 2
+            for (int i = tid; i < fours; i += kEvictThreads) {
+                const uint4 k = keys(i);
+                f(k.x, 4 * i); f(k.y, 4 * i + 1); f(k.z, 4 * i + 2); f(k.w, 4 * i + 3);
             }
+        });
+        // Walks slots [slot, end) until it has found some that `take` wants (stays: is the slot kept?), in ascending order; a step whose finds have no room
+        // beside the ones before it is walked again.
+        struct Walk {
+            int slot, end, n, used;
+        };
+        auto fill = [&](Walk& x, Slot* list, auto take) {
+            x.n = x.used = 0;
+            while (x.slot < x.end) {
+                const int i0 = (x.slot & ~7) + 8 * tid;
+                unsigned found = 0;
+                if (i0 < x.end) {
+                    const uint4 k = keys(i0 >> 2), l = i0 + 4 < x.end ? keys((i0 >> 2) + 1) : make_uint4(0u, 0u, 0u, 0u);
+                    const unsigned o[8] = {k.x, k.y, k.z, k.w, l.x, l.y, l.z, l.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (i0 + e >= x.slot && i0 + e < x.end && take(cut.in(o[e], i0 + e), i0 + e)) found |= 1u << e;
+                }
+                const int want = __popc(found), upto = block_scan<kEvictThreads>(want, sh.sums);
+                __syncthreads();
+                const int more = sh.sums[kEvictWarps];
+                if (x.n + more > kEvictStep) break;
+                int to = x.n + upto - want;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((found >> e) & 1u) list[to++] = (Slot)(i0 + e);
+                x.n += more;
+                x.slot = min(x.end, (x.slot & ~7) + kEvictStep);
+            }
+            __syncthreads();
         };
         // Moves `count` rows, 16 threads each; the CTAs of the cluster take them in turns.
-        constexpr int kTeams = kEvictThreads / 16;
-        auto move = [&](const int* from, const int* to, int count) {
-            const int lane = tid & 15;
-            for (int i0 = (int)part * kTeams + (tid >> 4); i0 < count; i0 += (int)parts * kTeams * 4) {
-                int64_t src[4], dst[4];
+        auto move = [&](const Slot* from, const Slot* to, int count) {
+            for (int i0 = (int)part * kTeams + team; i0 < count; i0 += (int)parts * kTeams * 4) {
                 uint4 a[4], v[4];
+                unsigned there = 0;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int i = i0 + u * (int)parts * kTeams;
-                    src[u] = i < count ? at(old_table, from[i]) : -1;
-                    dst[u] = src[u] >= 0 ? at(table, to[i]) : -1;
-                    if (dst[u] >= 0) {
-                        a[u] = kp[src[u] * 16 + lane];
-                        v[u] = vp[src[u] * 16 + lane];
+                    if (i >= count) continue;
+                    const int64_t src = at(old_table, from[i]);
+                    if (src >= 0) {
+                        there |= 1u << u;
+                        a[u] = kp[src];
+                        v[u] = vp[src];
                     }
-                    if (i < count && lane == 0 && from[i] != to[i]) wt[to[i]] = wt[from[i]];
+                    if (lane == 0 && from[i] != to[i]) wt[to[i]] = wt[from[i]];
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (dst[u] >= 0) {
-                        kp[dst[u] * 16 + lane] = a[u];
-                        vp[dst[u] * 16 + lane] = v[u];
+                for (int u = 0; u < 4; ++u) {
+                    if (!((there >> u) & 1u)) continue;
+                    const int64_t dst = at(table, to[i0 + u * (int)parts * kTeams]);
+                    if (dst >= 0) {
+                        kp[dst] = a[u];
+                        vp[dst] = v[u];
                     }
+                }
             }
         };
         if (row.swapped) {   // what stays in its slot on a page that has been exchanged
-            Walk x = {0, b, 0, 0, 0};
+            Walk x = {0, b, 0, 0};
             for (;;) {
                 fill(x, sh.holes, [&](bool stays, int slot) { return stays && old_table[slot >> bits] != table[slot >> bits]; });
                 if (x.n == 0) break;
@@ -222,15 +241,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(mfqb_cache c, floa
                 __syncthreads();
             }
         }
-        Walk hole = {0, b, 0, 0, 0}, mover = {b, older, 0, 0, 0};
-        if (cut.ties) {
-            int equal = 0;
-            for (int i = tid; i < b; i += kEvictThreads) equal += key(i) == cut.key;
-            block_scan<kEvictThreads>(equal, sh.cut.sums);
-            __syncthreads();
-            mover.ties = sh.cut.sums[kEvictWarps];
-            __syncthreads();
-        }
+        Walk hole = {0, b, 0, 0}, mover = {b, older, 0, 0};
         for (;;) {
             if (hole.used == hole.n) fill(hole, sh.holes, [](bool stays, int) { return !stays; });
             if (hole.n == 0) break;
@@ -244,34 +255,40 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(mfqb_cache c, floa
         }
     }
     sync_all();
-    // The latest rows: a CTA reads a batch before it writes any of it, and later ones lie behind all that has been written.
-    if (part == 0) {
-        constexpr int kTeams = kEvictThreads / 16, kBatch = 4 * kTeams;
-        const int lane = tid & 15, team = tid >> 4;
-        for (int i0 = 0; i0 < recent; i0 += kBatch) {
-            int64_t dst[4];
+    // The latest rows: a CTA reads a batch before it writes any of it, and later ones lie behind all that has been written.  Where they are fewer than
+    // those that go, no place is another one's source, and the CTAs share them.
+    const bool apart = n - k >= recent;
+    if (apart || part == 0) {
+        constexpr int kBatch = 4 * kTeams;
+        for (int i0 = apart ? (int)part * kBatch : 0; i0 < recent; i0 += apart ? (int)parts * kBatch : kBatch) {
             uint4 a[4], v[4];
             float f[4];
+            unsigned there = 0;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int i = i0 + u * kTeams + team;
-                const int64_t src = i < recent ? at(old_table, older + i) : -1;
-                dst[u] = src >= 0 ? at(table, b + i) : -1;
-                if (dst[u] >= 0) {
-                    a[u] = kp[src * 16 + lane];
-                    v[u] = vp[src * 16 + lane];
+                if (i >= recent) continue;
+                const int64_t src = at(old_table, older + i);
+                if (src >= 0) {
+                    there |= 1u << u;
+                    a[u] = kp[src];
+                    v[u] = vp[src];
                 }
-                f[u] = i < recent ? wt[older + i] : 0.f;
+                f[u] = wt[older + i];
             }
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int i = i0 + u * kTeams + team;
-                if (dst[u] >= 0) {
-                    kp[dst[u] * 16 + lane] = a[u];
-                    vp[dst[u] * 16 + lane] = v[u];
+                if (i >= recent) continue;
+                if ((there >> u) & 1u) {
+                    const int64_t dst = at(table, b + i);
+                    if (dst >= 0) {
+                        kp[dst] = a[u];
+                        vp[dst] = v[u];
+                    }
                 }
-                if (i < recent && lane == 0) wt[b + i] = f[u];
+                if (lane == 0) wt[b + i] = f[u];
             }
         }
     }
@@ -289,7 +306,7 @@ static void launch_evict(const mfqb_cache& c, float* weights, const int* keep, i
     int parts = 1;
     while (cached && parts < 8 && units * parts < 2 * 148) parts *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * parts));
+    cfg.gridDim = dim3((unsigned)(c.kv_heads * parts), c.rows, c.layers);
     cfg.blockDim = dim3(kEvictThreads);
     cfg.dynamicSmemBytes = cached ? (size_t)cap * 4 : 0;
     cfg.stream = s;
@@ -325,8 +342,9 @@ int mfqb_cache_evict(const mfqb_cache* c, float* weights, const int32_t* keep, i
     return guarded([&] {
         check_cache(c, "mfqb_cache_evict");
         if (!weights || !keep || !dropped || !status || !work) fail(MFQB_ERR_ARG, "mfqb_cache_evict: null argument");
+        if ((uintptr_t)weights & 15) fail(MFQB_ERR_ARG, "mfqb_cache_evict: weights must be 16-byte aligned");
         if (recent < 0) fail(MFQB_ERR_ARG, "mfqb_cache_evict: the number of latest positions must not be negative, got %d", recent);
-        if ((int64_t)c->layers * c->rows * c->kv_heads > (1ll << 27)) fail(MFQB_ERR_UNSUPPORTED, "mfqb_cache_evict: too many layers x sequences x heads");
+        if (c->layers > 65535) fail(MFQB_ERR_UNSUPPORTED, "mfqb_cache_evict: at most 65535 layers, got %d", c->layers);
         if (((uintptr_t)work & 15) || work_bytes < evict_work_bytes(*c))
             fail(MFQB_ERR_ARG, "mfqb_cache_evict: work must be 16-byte aligned and hold %llu bytes, got %llu", (unsigned long long)evict_work_bytes(*c),
                  (unsigned long long)work_bytes);

@@ -8,7 +8,7 @@
 
 namespace mfqb {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4;
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4, kLpCtas = 16;
 constexpr int kLpVocab = 1 << 20;
 
 struct LogprobArgs {
@@ -20,7 +20,7 @@ struct LogprobArgs {
     int *rank, *top_tokens;
 };
 
-// Sums of some of a row's logits: exp(z - top), the same times (z - top) log2(e), and how many come before the given token.
+// Sums of some of a row's logits: exp(z - top), the same times z - top, and how many come before the given token.
 struct LogprobSum {
     float top, sum, moment;
     int before;
@@ -29,12 +29,12 @@ struct LogprobShared {
     CutShared cut;
     LogprobSum warp[kLpWarps], all;
     float group[kLpGroups], bound;
-    int hot[kLpThreads], hots, count, best_n, total;
-    unsigned long long list[kLpList], best[kLpTop], merged[kLpTop];
+    int hot[kLpThreads], hots, count;
+    unsigned long long list[kLpList], best[kLpTop], gathered[kLpCtas][kLpTop];   // 0: none
 };
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLpLowest = -3.402823466e38f, kLpNone = -200.f;   // 2^-200 is 0 in float32
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLpLowest = -3.402823466e38f, kLpNone = -150.f;   // exp(-150) is 0 in float32; its product with this too, where minus infinity's would be NaN
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
     float r;
@@ -52,11 +52,12 @@ struct LpVec<float> {
     static __device__ __forceinline__ void widen(const uint4& v, float* z) {
         z[0] = __uint_as_float(v.x); z[1] = __uint_as_float(v.y); z[2] = __uint_as_float(v.z); z[3] = __uint_as_float(v.w);
     }
-    static __device__ __forceinline__ uint32_t lowest() { return 0xFF800000u; }
+    static __device__ __forceinline__ float lowest() { return -INFINITY; }
 };
 template <>
 struct LpVec<__nv_bfloat16> {
     static constexpr int kN = 8;
+    static __device__ __forceinline__ __nv_bfloat16 lowest() { return __ushort_as_bfloat16(0xFF80); }
     static __device__ __forceinline__ void widen(const uint4& v, float* z) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -69,6 +70,7 @@ struct LpVec<__nv_bfloat16> {
 template <>
 struct LpVec<__half> {
     static constexpr int kN = 8;
+    static __device__ __forceinline__ __half lowest() { return __ushort_as_half(0xFC00); }
     static __device__ __forceinline__ void widen(const uint4& v, float* z) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -86,12 +88,21 @@ __device__ __forceinline__ float lp_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ LogprobSum lp_join(LogprobSum a, LogprobSum b) {
     LogprobSum r;
     r.top = fmaxf(a.top, b.top);
-    const float da = fmaxf((a.top - r.top) * kLog2e, kLpNone), db = fmaxf((b.top - r.top) * kLog2e, kLpNone);
-    const float fa = exp2_approx(da), fb = exp2_approx(db);
+    const float da = fmaxf(a.top - r.top, kLpNone), db = fmaxf(b.top - r.top, kLpNone);
+    const float fa = exp2_approx(da * kLog2e), fb = exp2_approx(db * kLog2e);
     r.sum = a.sum * fa + b.sum * fb;
     r.moment = (a.moment + da * a.sum) * fa + (b.moment + db * b.sum) * fb;
     r.before = a.before + b.before;
     return r;
+}
+
+__device__ __forceinline__ LogprobSum lp_shuffle_join(LogprobSum a, int o) {
+    LogprobSum b;
+    b.top = __shfl_xor_sync(0xffffffffu, a.top, o);
+    b.sum = __shfl_xor_sync(0xffffffffu, a.sum, o);
+    b.moment = __shfl_xor_sync(0xffffffffu, a.moment, o);
+    b.before = __shfl_xor_sync(0xffffffffu, a.before, o);
+    return lp_join(a, b);
 }
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -124,12 +135,12 @@ __device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
     return v;
 }
 
-// A cluster per row, a slice of the row per CTA.  A thread takes every 512th vector of 16 bytes and keeps a running maximum with its sums.  The k
+// A cluster per row, a slice of the row per CTA.  A thread takes every 256th vector of 16 bytes and keeps a running maximum with its sums.  The k
 // best: a bound that at least k logits reach comes from the maxima of 64 groups of threads (the k-th largest of them), and only the
 // vectors of threads whose own maximum reaches it are read again, a warp for each of those threads.  Where too many logits reach the
 // bound (equal ones, or all in a few threads' vectors) the cut is searched by counting instead.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int kN = LpVec<T>::kN;
     __shared__ LogprobShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -140,33 +151,43 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
     // Vectors start at 16-byte boundaries; vector v holds logits v * kN - skew ..; those outside the row count as minus infinity.
     const int skew = (int)(((uintptr_t)z & 15) / sizeof(T)), vectors = (skew + a.vocab + kN - 1) / kN;
     const int first = (int)((int64_t)vectors * rank / ctas), last = (int)((int64_t)vectors * (rank + 1) / ctas);
-    auto load = [&](int v, float* x) {
+    auto fetch = [&](int v) -> uint4 {
         const int at = v * kN - skew;
-        if (at >= 0 && at + kN <= a.vocab) {
-            LpVec<T>::widen(__ldcg(reinterpret_cast<const uint4*>(z + at)), x);
-        } else {
+        if (at >= 0 && at + kN <= a.vocab) return __ldcg(reinterpret_cast<const uint4*>(z + at));
+        alignas(16) T x[kN];
 #pragma unroll
-            for (int e = 0; e < kN; ++e) x[e] = at + e >= 0 && at + e < a.vocab ? lp_float(z[at + e]) : -INFINITY;
-        }
+        for (int e = 0; e < kN; ++e) x[e] = at + e >= 0 && at + e < a.vocab ? z[at + e] : LpVec<T>::lowest();
+        return *reinterpret_cast<const uint4*>(x);
     };
+    auto load = [&](int v, float* x) { LpVec<T>::widen(fetch(v), x); };
     const int token = __ldcg(a.tokens + row);
     const bool there = (unsigned)token < (unsigned)a.vocab;
     // A logit comes before the token's own if it is larger, or equal with a lower number.
     const float zt = there ? lp_float(z[token]) + 0.f : INFINITY;
     const float above = unordered_f32(ordered_f32(zt) + 1u);
     LogprobSum s = {kLpLowest, 0.f, 0.f, 0};
+    uint64_t sum = 0ull, moment = 0ull;   // of the even and the odd ones of a vector
     float most = -INFINITY;
+    uint4 next[kLpBatch];
+    auto ask = [&](int v0) {
+#pragma unroll
+        for (int u = 0; u < kLpBatch; ++u) {
+            if (v0 + u * kLpThreads < last) next[u] = fetch(v0 + u * kLpThreads);
+        }
+    };
+    ask(first + tid);
     for (int v0 = first + tid; v0 < last; v0 += kLpThreads * kLpBatch) {
         float x[kLpBatch][kN];
 #pragma unroll
         for (int u = 0; u < kLpBatch; ++u) {
             if (v0 + u * kLpThreads < last) {
-                load(v0 + u * kLpThreads, x[u]);
+                LpVec<T>::widen(next[u], x[u]);
             } else {
 #pragma unroll
                 for (int e = 0; e < kN; ++e) x[u][e] = -INFINITY;
             }
         }
+        ask(v0 + kLpThreads * kLpBatch);   // on its way while this one is worked on
         float high = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kLpBatch; ++u)
@@ -174,53 +195,55 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
             for (int e = 0; e < kN; ++e) high = fmaxf(high, x[u][e]);
         most = fmaxf(most, high);
         if (high > s.top) {
-            const float d = fmaxf((s.top - high) * kLog2e, kLpNone), f = exp2_approx(d);
-            s.moment = (s.moment + d * s.sum) * f;
-            s.sum *= f;
+            const float d = fmaxf(s.top - high, kLpNone), f = exp2_approx(d * kLog2e);
+            moment = fma_f32x2(fma_f32x2(pair_f32(d, d), sum, moment), pair_f32(f, f), 0ull);
+            sum = fma_f32x2(sum, pair_f32(f, f), 0ull);
             s.top = high;
         }
+        const uint64_t down = pair_f32(-s.top, -s.top);
 #pragma unroll
         for (int u = 0; u < kLpBatch; ++u) {
             const int at = (v0 + u * kLpThreads) * kN - skew;
             if (v0 + u * kLpThreads >= last) break;
 #pragma unroll
-            for (int e = 0; e < kN; ++e) {
-                const float d = max_nan((x[u][e] - s.top) * kLog2e, kLpNone), p = exp2_approx(d);
-                s.sum += p;
-                s.moment += p * d;
-                s.before += x[u][e] >= (at + e < token ? zt : above);
+            for (int e = 0; e < kN; e += 2) {
+                const float2 d = split_f32(add_f32x2(pair_f32(x[u][e], x[u][e + 1]), down));
+                const uint64_t dd = pair_f32(max_nan(d.x, kLpNone), max_nan(d.y, kLpNone));
+                const float2 y = split_f32(fma_f32x2(dd, pair_f32(kLog2e, kLog2e), 0ull));
+                const uint64_t p = pair_f32(exp2_approx(y.x), exp2_approx(y.y));
+                sum = add_f32x2(sum, p);
+                moment = fma_f32x2(p, dd, moment);
+            }
+            if (at + kN <= token || at > token) {
+                const float line = at > token ? above : zt;
+#pragma unroll
+                for (int e = 0; e < kN; ++e) s.before += x[u][e] >= line;
+            } else {
+#pragma unroll
+                for (int e = 0; e < kN; ++e) s.before += x[u][e] >= (at + e < token ? zt : above);
             }
         }
     }
     if (first + tid == 0 && first < last && there && zt == -INFINITY) s.before -= skew;   // minus infinities that are not the row's
+    {
+        const float2 x = split_f32(sum), y = split_f32(moment);
+        s.sum = x.x + x.y;
+        s.moment = y.x + y.y;
+    }
     // ---- the CTA's sums
     LogprobSum joint = s;
-    for (int o = 16; o > 0; o >>= 1) {
-        LogprobSum other;
-        other.top = __shfl_xor_sync(0xffffffffu, joint.top, o);
-        other.sum = __shfl_xor_sync(0xffffffffu, joint.sum, o);
-        other.moment = __shfl_xor_sync(0xffffffffu, joint.moment, o);
-        other.before = __shfl_xor_sync(0xffffffffu, joint.before, o);
-        joint = lp_join(joint, other);
-    }
+    for (int o = 16; o > 0; o >>= 1) joint = lp_shuffle_join(joint, o);
     if (lane == 0) sh.warp[warp] = joint;
     if (a.top > 0) {
-        float group = most;   // eight threads
-        for (int o = 4; o > 0; o >>= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
-        if ((lane & 7) == 0) sh.group[tid >> 3] = group;
+        float group = most;   // of neighbouring threads
+        for (int o = kLpThreads / kLpGroups / 2; o > 0; o >>= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+        if (tid % (kLpThreads / kLpGroups) == 0) sh.group[tid / (kLpThreads / kLpGroups)] = group;
         if (tid == 0) sh.hots = sh.count = 0;
     }
     __syncthreads();
     if (warp == 0) {
         LogprobSum x = sh.warp[lane & (kLpWarps - 1)];
-        for (int o = kLpWarps / 2; o > 0; o >>= 1) {
-            LogprobSum other;
-            other.top = __shfl_xor_sync(0xffffffffu, x.top, o);
-            other.sum = __shfl_xor_sync(0xffffffffu, x.sum, o);
-            other.moment = __shfl_xor_sync(0xffffffffu, x.moment, o);
-            other.before = __shfl_xor_sync(0xffffffffu, x.before, o);
-            x = lp_join(x, other);
-        }
+        for (int o = kLpWarps / 2; o > 0; o >>= 1) x = lp_shuffle_join(x, o);
         if (lane == 0) sh.all = x;
     }
     if (a.top > 0) {
@@ -259,48 +282,23 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
                     const int at = v * kN - skew;
 #pragma unroll
                     for (int e = 0; e < kN; ++e)
-                        if (at + e >= 0 && at + e < a.vocab) f(ordered_f32(x[e]));
+                        if (at + e >= 0 && at + e < a.vocab) f(ordered_f32(x[e]), at + e);
                 }
             };
-            const Cut cut = select_cut<kLpThreads>(a.top, sh.cut, each);
+            unsigned low = 0xFFFFFFFFu, high = 0u;
+            each([&](unsigned k, int) {
+                low = min(low, k);
+                high = max(high, k);
+            });
+            const Cut cut = select_cut<kLpThreads>(a.top, low, high, a.vocab, sh.cut, each);
             __syncthreads();
             if (tid == 0) sh.count = 0;
             __syncthreads();
-            int ties = 0;   // of the vectors before
-            for (int v0 = first; v0 < last; v0 += kLpThreads) {
-                const int v = v0 + tid, at = v * kN - skew;
-                unsigned o[kN];
-                int equal = 0;
-                if (v < last) {
-                    float x[kN];
-                    load(v, x);
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) {
-                        const bool in = at + e >= 0 && at + e < a.vocab;
-                        o[e] = in ? ordered_f32(x[e]) : 0u;
-                        equal += o[e] == cut.key;
-                    }
-                }
-                int mine = ties;
-                if (ties < cut.ties) {   // the same in all threads
-                    const int upto = block_scan<kLpThreads>(equal, sh.cut.sums);
-                    __syncthreads();
-                    mine += upto - equal;
-                    ties += sh.cut.sums[kLpWarps];
-                }
-                if (v < last)
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) {
-                        const bool tie = o[e] == cut.key;
-                        if (o[e] > cut.key || (tie && mine < cut.ties)) {
-                            const int i = atomicAdd(&sh.count, 1);
-                            if (i < kLpList) sh.list[i] = (unsigned long long)o[e] << 32 | (0xFFFFFFFFu - (unsigned)(at + e));
-                        }
-                        mine += tie;
-                    }
-            }
+            each([&](unsigned k, int token) {
+                if (cut.in(k, token)) sh.list[atomicAdd(&sh.count, 1)] = (unsigned long long)k << 32 | (0xFFFFFFFFu - (unsigned)token);   // a.top of them
+            });
             __syncthreads();
-            n = min(sh.count, kLpList);
+            n = sh.count;
         }
         // ---- the list in order: every key counts those above it
         const int keep = min(n, a.top);
@@ -310,55 +308,53 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
             for (int j = 0; j < n; ++j) larger += sh.list[j] > key;
             if (larger < keep) sh.best[larger] = key;
         }
-        if (tid == 0) sh.best_n = keep;
+        if (tid >= keep && tid < kLpTop) sh.best[tid] = 0ull;
     }
     if (ctas > 1) cluster_sync();
     else __syncthreads();
     if (rank == 0) {
         LogprobSum x = sh.all;
-        for (unsigned c = 1; c < ctas; ++c) {   // all threads the same
-            const uint32_t at = remote_smem(&sh.all, c);
-            const LogprobSum other = {__uint_as_float(remote_u32(at)), __uint_as_float(remote_u32(at + 4)), __uint_as_float(remote_u32(at + 8)), (int)remote_u32(at + 12)};
-            x = lp_join(x, other);
+        const unsigned long long* best = sh.best;
+        if (ctas > 1) {   // lane c has CTA c's sums, every warp the same; all lists are brought here at once
+            const uint32_t at = remote_smem(&sh.all, lane % ctas);
+            x = LogprobSum{__uint_as_float(remote_u32(at)), __uint_as_float(remote_u32(at + 4)), __uint_as_float(remote_u32(at + 8)), (int)remote_u32(at + 12)};
+            if (a.top > 0) {
+                for (int i = tid; i < (int)ctas * kLpTop; i += kLpThreads) sh.gathered[i / kLpTop][i % kLpTop] = remote_u64(remote_smem(&sh.best[i % kLpTop], i / kLpTop));
+                if (tid == 0) sh.count = 0;
+            }
+            for (int o = ctas / 2; o > 0; o >>= 1) x = lp_shuffle_join(x, o);
+            if (a.top > 0) {
+                __syncthreads();
+                // In order, the lists have at least `top` keys up to here; what lies below the smallest of these is not among the best.
+                unsigned long long line = sh.gathered[lane % ctas][(a.top + ctas - 1) / ctas - 1];
+                for (int o = ctas / 2; o > 0; o >>= 1) line = min(line, __shfl_xor_sync(0xffffffffu, line, o));
+                for (int i = tid; i < (int)ctas * kLpTop; i += kLpThreads) {
+                    const unsigned long long key = sh.gathered[i / kLpTop][i % kLpTop];
+                    if (key && key >= line) sh.list[atomicAdd(&sh.count, 1)] = key;   // at most 16 lists of 32
+                }
+                __syncthreads();
+                const int n = sh.count;
+                for (int i = tid; i < n; i += kLpThreads) {
+                    const unsigned long long key = sh.list[i];
+                    int larger = 0;
+                    for (int j = 0; j < n; ++j) larger += sh.list[j] > key;
+                    if (larger < a.top) sh.best[larger] = key;
+                }
+                __syncthreads();
+            }
         }
         // a NaN, plus infinity, or nothing above minus infinity leaves no log sum
         const bool good = x.sum > 0.f && x.sum < INFINITY && x.top < INFINITY;
         const float log_sum = logf(x.sum);
         if (tid == 0) {
             a.logprob[row] = !there ? 0.f : good ? (zt - x.top) - log_sum : NAN;
-            a.entropy[row] = good ? log_sum - x.moment / x.sum * kLn2 : NAN;
+            a.entropy[row] = good ? log_sum - x.moment / x.sum : NAN;
             a.rank[row] = good && there ? x.before + 1 : 0;
         }
-        if (a.top > 0) {
-            if (ctas > 1) {
-                // A thread per key of each list; lists are in order.
-                const int c = tid / kLpTop, i = tid % kLpTop;
-                if ((unsigned)c < ctas) {
-                    const int n = (int)remote_u32(remote_smem(&sh.best_n, c));
-                    if (i < n) {
-                        const unsigned long long key = remote_u64(remote_smem(&sh.best[i], c));
-                        int larger = i;
-                        for (unsigned d = 0; d < ctas; ++d) {
-                            if ((int)d == c) continue;
-                            int lo = 0, hi = (int)remote_u32(remote_smem(&sh.best_n, d));   // keys of list d above this one
-                            const uint32_t list = remote_smem(sh.best, d);
-                            while (lo < hi) {
-                                const int mid = (lo + hi) >> 1;
-                                if (remote_u64(list + mid * 8) > key) lo = mid + 1;
-                                else hi = mid;
-                            }
-                            larger += lo;
-                        }
-                        if (larger < a.top) sh.merged[larger] = key;
-                    }
-                }
-                __syncthreads();
-            }
-            if (tid < a.top) {
-                const unsigned long long key = ctas > 1 ? sh.merged[tid] : sh.best[tid];
-                a.top_logprobs[row * a.top + tid] = good ? (unordered_f32((unsigned)(key >> 32)) - x.top) - log_sum : NAN;
-                a.top_tokens[row * a.top + tid] = good ? (int)(0xFFFFFFFFu - (unsigned)key) : -1;
-            }
+        if (tid < a.top) {
+            const unsigned long long key = best[tid];
+            a.top_logprobs[row * a.top + tid] = good ? (unordered_f32((unsigned)(key >> 32)) - x.top) - log_sum : NAN;
+            a.top_tokens[row * a.top + tid] = good ? (int)(0xFFFFFFFFu - (unsigned)key) : -1;
         }
     }
     if (ctas > 1) cluster_sync();   // no CTA leaves while its lists are read
@@ -370,9 +366,9 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     MFQB_CUDA(cudaGetDevice(&device));
     static std::once_flag once[64];
     std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); });
-    // CTAs of a row: until there are two for every SM, as long as a slice has a batch of vectors for every thread.
+    // CTAs of a row: until there are four for every SM, as long as a slice has a batch of vectors for every thread.
     int ctas = 1;
-    while (ctas < 16 && (int64_t)rows * ctas < 2 * 148 && a.vocab / (2 * ctas) >= kLpThreads * kLpBatch) ctas *= 2;
+    while (ctas < kLpCtas && (int64_t)rows * ctas < 4 * 148 && a.vocab / (2 * ctas) >= kLpThreads * kLpBatch) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ctas);
     cfg.blockDim = dim3(kLpThreads);

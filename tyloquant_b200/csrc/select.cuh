@@ -32,56 +32,68 @@ __device__ __forceinline__ int block_scan(int v, int* sums) {
     return v + (warp ? __shfl_sync(0xffffffffu, before, warp - 1) : 0);
 }
 
-// What is in: keys above `key`, and the first `ties` of those that equal it.
+// What is in: keys above `key`, and of those that equal it the ones at places up to `last`.
 struct Cut {
     unsigned key;
-    int ties;
+    int last;
+    __device__ __forceinline__ bool in(unsigned k, int place) const { return k > key || (k == key && place <= last); }
 };
-constexpr int kCutBins = 2048;
+constexpr int kCutBins = 2048, kCutFew = 64;
 struct CutShared {
-    int bins[kCutBins], sums[33], at, left, inside;
-    unsigned low, high;
+    alignas(16) int bins[kCutBins];
+    alignas(16) unsigned long long few[kCutFew];
+    int sums[33], at, left, inside;
+    unsigned low[32], high[32];
+    Cut cut;
 };
 
-// The cut that lets `want` of the keys in (1 <= want <= how many there are).  each(f) calls f(key) for this thread's share of the keys, the same
-// ones every time.  Bins divide the range from the smallest to the largest key: float32 values that span orders of magnitude lie in
-// many of them (by the first bits of the keys they would meet in a few counters, whose additions wait for one another), and three rounds
-// of 11 bits are enough for any range; a round ends the search when all of its last bin is in.
+// The cut that lets `want` of the keys in, equal ones by place (1 <= want <= how many there are).  each(f) calls f(key, place) for this
+// thread's share of the keys, the same ones every time, at places 0 .. places - 1; a key 0 is none.  low and high are the smallest and the
+// largest of the thread's (all ones and 0 where there are none).  Bins divide the range from the smallest to the largest key: float32 values
+// that span orders of magnitude lie in many of them (by the first bits of the keys they would meet in a few counters, whose additions
+// wait for one another), and three rounds of 11 bits are enough for any range.  A round ends the search when all of its last bin is in, or
+// when that holds so few keys that they are better counted against each other.  The next one goes by what the keys of the bin span; where
+// they are equal, by their places.
 template <int THREADS, class Each>
-__device__ Cut select_cut(int want, CutShared& sh, Each each) {
-    static_assert(kCutBins % THREADS == 0, "bins of a thread");
-    constexpr int kOwn = kCutBins / THREADS;
-    unsigned low = 0xFFFFFFFFu, high = 0u;
-    each([&](unsigned k) {
-        low = min(low, k);
-        high = max(high, k);
-    });
+__device__ Cut select_cut(int want, unsigned low, unsigned high, int places, CutShared& sh, Each each) {
+    static_assert(kCutBins % (4 * THREADS) == 0 && kCutFew <= THREADS, "bins of a thread");
+    constexpr int kOwn = kCutBins / THREADS, kWarps = THREADS / 32;
+    const int lane = threadIdx.x & 31;
     low = __reduce_min_sync(0xffffffffu, low);
     high = __reduce_max_sync(0xffffffffu, high);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sh.low = 0xFFFFFFFFu;
-        sh.high = 0u;
+    if (lane == 0) {
+        sh.low[threadIdx.x >> 5] = low;
+        sh.high[threadIdx.x >> 5] = high;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-        atomicMin(&sh.low, low);
-        atomicMax(&sh.high, high);
-    }
-    __syncthreads();
-    unsigned base = sh.low, range = sh.high - sh.low;   // keys base .. base + range
+    unsigned base = __reduce_min_sync(0xffffffffu, sh.low[lane % kWarps]);
+    unsigned range = __reduce_max_sync(0xffffffffu, sh.high[lane % kWarps]) - base;   // keys base .. base + range
+    unsigned tied = 0;   // the key whose places are being sorted out, the first one the largest
     for (;;) {
         const int shift = max(0, 21 - __clz(range | 1u));   // range >> shift is below 2048
-        for (int b = threadIdx.x; b < kCutBins; b += THREADS) sh.bins[b] = 0;
-        __syncthreads();
-        each([&](unsigned k) {
-            if (k - base <= range) atomicAdd(&sh.bins[(k - base) >> shift], 1);
-        });
-        __syncthreads();
-        int own[kOwn], mine = 0;   // this thread's bins, from the last one down
+        int4* own_bins = reinterpret_cast<int4*>(sh.bins + kCutBins - kOwn * ((int)threadIdx.x + 1));   // from the last one down
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j) mine += own[j] = sh.bins[kCutBins - 1 - ((int)threadIdx.x * kOwn + j)];
-        int upto = block_scan<THREADS>(mine, sh.sums);
+        for (int j = 0; j < kOwn / 4; ++j) own_bins[j] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        if (!tied) {
+            each([&](unsigned k, int) {
+                if (k - base <= range) atomicAdd(&sh.bins[(k - base) >> shift], 1);
+            });
+        } else {
+            each([&](unsigned k, int place) {
+                const unsigned x = ~(unsigned)place - base;
+                if (k == tied && x <= range) atomicAdd(&sh.bins[x >> shift], 1);
+            });
+        }
+        __syncthreads();
+        int own[kOwn], mine = 0;
+#pragma unroll
+        for (int j = 0; j < kOwn / 4; ++j) {
+            const int4 x = own_bins[j];
+            own[kOwn - 4 * j - 1] = x.x; own[kOwn - 4 * j - 2] = x.y; own[kOwn - 4 * j - 3] = x.z; own[kOwn - 4 * j - 4] = x.w;
+            mine += x.x + x.y + x.z + x.w;
+        }
+        const int upto = block_scan<THREADS>(mine, sh.sums);
         if (upto >= want && upto - mine < want) {
             int before = upto - mine;
 #pragma unroll
@@ -98,10 +110,52 @@ __device__ Cut select_cut(int want, CutShared& sh, Each each) {
         want = sh.left;
         const int inside = sh.inside;
         base += (unsigned)sh.at << shift;
-        __syncthreads();
-        if (want == inside) return Cut{base - 1u, 0};   // no key of a value is 0
-        if (shift == 0) return Cut{base, want};
+        if (want == inside) return tied ? Cut{tied, (int)~base} : Cut{base - 1u, -1};   // no key of a value is 0
         range = (1u << shift) - 1u;
+        if (inside <= kCutFew) {
+            __syncthreads();
+            if (threadIdx.x == 0) sh.at = 0;
+            __syncthreads();
+            each([&](unsigned k, int place) {
+                if (tied ? k == tied && ~(unsigned)place - base <= range : k - base <= range)
+                    sh.few[atomicAdd(&sh.at, 1)] = (unsigned long long)k << 32 | ~(unsigned)place;
+            });
+            __syncthreads();
+            if ((int)threadIdx.x < inside) {
+                const unsigned long long x = sh.few[threadIdx.x];
+                int above = 0;
+#pragma unroll 4
+                for (int i = 0; i < inside; ++i) above += sh.few[i] > x;
+                if (above == want - 1) sh.cut = Cut{(unsigned)(x >> 32), (int)~(unsigned)x};
+            }
+            __syncthreads();
+            return sh.cut;
+        }
+        if (!tied) {   // what the bin's keys really span: equal ones are found so at once
+            low = 0xFFFFFFFFu;
+            high = 0u;
+            each([&](unsigned k, int) {
+                if (k - base <= range) {
+                    low = min(low, k);
+                    high = max(high, k);
+                }
+            });
+            low = __reduce_min_sync(0xffffffffu, low);
+            high = __reduce_max_sync(0xffffffffu, high);
+            if (lane == 0) {
+                sh.low[threadIdx.x >> 5] = low;
+                sh.high[threadIdx.x >> 5] = high;
+            }
+            __syncthreads();
+            base = __reduce_min_sync(0xffffffffu, sh.low[lane % kWarps]);
+            range = __reduce_max_sync(0xffffffffu, sh.high[lane % kWarps]) - base;
+            if (range == 0) {
+                tied = base;
+                base = ~(unsigned)(places - 1);
+                range = (unsigned)(places - 1);
+            }
+        }
+        __syncthreads();
     }
 }
 

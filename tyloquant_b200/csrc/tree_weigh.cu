@@ -55,11 +55,12 @@ __global__ void __launch_bounds__(128) weigh_scores_kernel(const __grid_constant
 struct WeighShared {
     uint64_t k_full[kWeighRing], k_empty[kWeighRing], q_full, s_full[2], s_empty[2], all;
     int64_t scan[kWeighThreads / 32], first, last, off;
-    int row0, failed, bad;
+    int row0, failed;
+    int bad;                         // the last head (its number in the CTA, from 1 on) with a row whose weights are no numbers
     uint32_t tmem;
     unsigned good[8];
     unsigned long long masks[kTreeNodes];
-    float2 ml[kWeighRows];
+    float4 ml[kWeighRows / 2];   // of two rows: minus their maxima, the factors
 };
 constexpr size_t kWeighSmem = (size_t)kWeighRing * kTileBytes + (size_t)kWeighRows * kHeadDim * 2 + sizeof(WeighShared);
 static_assert(kWeighSmem <= 227 * 1024, "shared memory of an SM");
@@ -214,7 +215,9 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
     } else {
         const int g = (warp - 2) >> 2, quarter = warp & 3, t = tid - 64;
         const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + g * kWeighRows;
+        const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
         uint32_t j = 0, alls = 0;
+        int items = 0;
         bool ok = true;
         auto all_sync = [&]() {
             warp_arrive(&sh.all);
@@ -224,76 +227,100 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
             if (w.fresh) {   // all tiles of the head before have been summed, and their products read the rows that change now
                 all_sync();
                 if (!ok) break;
-                const int c = t & 15;
-                for (int rr = t >> 4; rr < (rows + 15) / 16 * 16; rr += 16) {   // rows behind the last one repeat it
-                    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(a.q + a.row_at(w.r, w.kvh, min(row0 + rr, m_rows - 1))) + c);
-                    *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kQHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+                ++items;
+                const int c = t & 15, padded = (rows + 15) / 16 * 16;
+                for (int r0 = t >> 4; r0 < padded; r0 += 128) {   // rows behind the last one repeat it
+                    uint4 v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (r0 + 16 * u < padded) v[u] = __ldcg(reinterpret_cast<const uint4*>(a.q + a.row_at(w.r, w.kvh, min(row0 + r0 + 16 * u, m_rows - 1))) + c);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int rr = r0 + 16 * u;
+                        if (rr < padded) *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kQHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[u];
+                    }
                 }
-                if (t == 0) sh.bad = 0;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&sh.q_full);
-                if (t < rows) sh.ml[t] = __ldcg(a.row_ml + ((int64_t)w.r * a.kv_heads + w.kvh) * m_rows + row0 + t);
-                if (t < a.nodes) sh.masks[t] = __ldcg(a.masks + (int64_t)w.r * a.nodes + t);
-                all_sync();
-                if (!ok) break;
-                if (t < rows && !(fabsf(sh.ml[t].x) < INFINITY && sh.ml[t].y < INFINITY)) sh.bad = 1;   // NaN too
+                if (t < kWeighRows) {   // rows behind the last one have its maximum and count for nothing
+                    const float2 ml = __ldcg(a.row_ml + ((int64_t)w.r * a.kv_heads + w.kvh) * m_rows + min(row0 + t, row0 + rows - 1));
+                    float* to = reinterpret_cast<float*>(&sh.ml[t >> 1]) + (t & 1);
+                    to[0] = -ml.x;
+                    to[2] = t < rows ? ml.y : 0.f;
+                    if (t < rows && !(fabsf(ml.x) < INFINITY && ml.y < INFINITY)) sh.bad = items;   // NaN too
+                }
+                if (t < kTreeNodes) sh.masks[t] = t < a.nodes ? __ldcg(a.masks + (int64_t)w.r * a.nodes + t) : 0ull;
                 all_sync();
                 if (!ok) break;
             }
             if ((int)(j & 1u) != g) continue;
+            const int at = quarter * 32 + lane, pos = w.t * kTile + at, node = pos - w.seq.len;
+            float* to = weights + ((int64_t)w.r * a.kv_heads + w.kvh) * a.width * a.page + pos;
+            const bool adds = pos < w.seq.end && (node < 0 || row0 > 0);   // to what is there
+            const float before = adds ? *to : 0.f;
             ok = warp_wait(&sh.s_full[g], (j >> 1) & 1u);
             if (!ok) break;
             tc_fence_after_sync();
-            const int at = quarter * 32 + lane, pos = w.t * kTile + at;
             const unsigned good = sh.good[j & 7];
             const bool page = (good >> (at >> 4)) & 1u;
-            float sum = 0.f;
-            if (w.t * kTile + kTile <= w.seq.len && good == 0xFFu && !sh.bad) {
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+            uint64_t sum2[2] = {0ull, 0ull};
+            // Sixteen rows at a time, the next ones' scores on their way; columns behind the last row are products with it too.
+            auto rows_of = [&](auto each) {
+                const int chunks = (rows + 15) / 16;
+                uint32_t s[2][16];
+                tmem_ld16_async(col, s[0]);
 #pragma unroll 1
-                for (int c = 0; c < rows; c += 32) {
-                    uint32_t s[32];
-                    tmem_ld32(col + c, s);
-                    tmem_wait_ld(s);
-                    if (c + 32 <= rows) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float2 ml = sh.ml[c + e];
-                            part[e & 3] += exp2_approx(fmaf(__uint_as_float(s[e]), a.scale_log2, -ml.x)) * ml.y;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (c + e < rows) {
-                                const float2 ml = sh.ml[c + e];
-                                part[e & 3] += exp2_approx(fmaf(__uint_as_float(s[e]), a.scale_log2, -ml.x)) * ml.y;
-                            }
+                for (int c = 0; c < chunks; c += 2) {
+                    tmem_wait_ld16(s[0]);
+                    if (c + 1 < chunks) tmem_ld16_async(col + 16 * (c + 1), s[1]);
+                    each(16 * c, s[0]);
+                    if (c + 1 < chunks) {
+                        tmem_wait_ld16(s[1]);
+                        if (c + 2 < chunks) tmem_ld16_async(col + 16 * (c + 2), s[0]);
+                        each(16 * (c + 1), s[1]);
                     }
                 }
-                sum = (part[0] + part[1]) + (part[2] + part[3]);
+            };
+            if (w.t * kTile + kTile <= w.seq.len && good == 0xFFu && sh.bad != items) {
+                rows_of([&](int c, const uint32_t* s) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float4 ml = sh.ml[(c + e) >> 1];
+                        const float2 x = split_f32(fma_f32x2(pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, pair_f32(ml.x, ml.y)));
+                        sum2[(e >> 1) & 1] = fma_f32x2(pair_f32(exp2_approx(x.x), exp2_approx(x.y)), pair_f32(ml.z, ml.w), sum2[(e >> 1) & 1]);
+                    }
+                });
             } else {   // a row counts where it sees the position and its score is above minus infinity
-                const int node = pos - w.seq.len;
-#pragma unroll 1
-                for (int c = 0; c < rows; c += 32) {
-                    uint32_t s[32];
-                    tmem_ld32(col + c, s);
-                    tmem_wait_ld(s);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (c + e >= rows) continue;
-                        const float2 ml = sh.ml[c + e];
-                        const float x = __uint_as_float(s[e]);
-                        const bool sees = node < 0 || (node < a.nodes && ((sh.masks[a.node_of(row0 + c + e)] >> node) & 1ull));
-                        if (page && sees && x != -INFINITY) sum += exp2_approx(fmaf(x, a.scale_log2, -ml.x)) * ml.y;
-                    }
+                unsigned long long seen = ~0ull;   // by which nodes the position is
+                if (!page || node >= a.nodes) {
+                    seen = 0ull;
+                } else if (node >= 0) {
+                    seen = 0ull;
+                    for (int i = 0; i < a.nodes; ++i) seen |= ((sh.masks[i] >> node) & 1ull) << i;
                 }
+                rows_of([&](int c, const uint32_t* s) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float4 ml = sh.ml[(c + e) >> 1];
+                        float p[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const float x = __uint_as_float(s[e + u]);
+                            const bool on = ((seen >> a.node_of(min(row0 + c + e + u, m_rows - 1))) & 1ull) && x != -INFINITY && c + e + u < rows;
+                            p[u] = on ? exp2_approx(fmaf(x, a.scale_log2, u ? ml.y : ml.x)) * (u ? ml.w : ml.z) : 0.f;
+                        }
+                        sum2[(e >> 1) & 1] = add_f32x2(pair_f32(p[0], p[1]), sum2[(e >> 1) & 1]);
+                    }
+                });
             }
+            const float2 half = split_f32(add_f32x2(sum2[0], sum2[1]));
+            const float sum = half.x + half.y;
             tc_fence_before_sync();
             warp_arrive(&sh.s_empty[g]);
-            if (pos < w.seq.end) {
-                float* to = weights + ((int64_t)w.r * a.kv_heads + w.kvh) * a.width * a.page + pos;
-                if (pos >= w.seq.len && row0 == 0) *to = sum;
-                else if (page) *to += sum;
+            if (adds) {
+                if (page) *to = before + sum;
+            } else if (pos < w.seq.end) {
+                *to = sum;
             }
         }
         if (!ok) sh.failed = 1;
