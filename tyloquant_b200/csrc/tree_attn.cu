@@ -546,6 +546,14 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                 return make_float2(mc, l);
             };
             const float2 sum = joint(row_l);
+            if constexpr (WEIGH && REP > 1) {
+                if (a.whole && a.scores) {   // all of the item is here; the other stream's place in sh.ml is free
+                    if (live && copy == 0) sh.ml[1][row_l] = row_scale(sum.x, sum.y);
+                    group_sync();   // the scores of all rows too
+                    if (!ok) break;
+                    for (int pos = lane_l; pos < w.seq.end; pos += kTile) add_weights<1>(a, w.seq, w.r, kvh, sh.ml[1], m_rows, pos);
+                }
+            }
             // What this copy's values are multiplied by: its maximum against the joint one, the sum where the row is complete.
             const float x = sh.ml[st][lane_l].x, e = x == -INFINITY ? 0.f : exp2_approx(x - sum.x);
             const float f = !complete ? e : sum.y == 0.f ? 0.f : __fdividef(e, sum.y);
@@ -666,8 +674,50 @@ constexpr int kMergeParts = 16, kMergeWarps = 4;   // parts in flight for a row,
 // Rows whose positions were shared by several CTAs: a warp per output row adds the parts in the order of the context, with a running
 // maximum.  Sixteen parts at a time are on their way, by asynchronous copies: with loads into registers eight were, and the ragged batch (rows of
 // up to 28 parts) took 26.5 us in place of 25.
-__global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __grid_constant__ TreeArgs a, int streams, int rows) {
+// WEIGH: CTAs from `merges` on add up the weights from the scores that the attention has kept, (stretch of positions, kv head, sequence) each; they find
+// the rows' maxima and sums from the parts themselves, so that no further launch waits for the merge.
+template <bool WEIGH>
+__global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __grid_constant__ TreeArgs a, int streams, int rows, int merges, int stretches) {
     chained_wait();
+    if constexpr (WEIGH) {
+        if ((int)blockIdx.x >= merges) {
+            __shared__ float2 s_scale[kScoreRows];
+            const int at = blockIdx.x - merges, item = at / stretches, r = item / a.kv_heads, kvh = item - r * a.kv_heads, m_rows = a.nodes * a.group;
+            const int lane = threadIdx.x & 31;
+            const TreeSeq seq = tree_seq(a, r);
+            const int64_t quota = __ldcg(a.before + a.rows), s0 = __ldcg(a.before + r) * a.kv_heads + (int64_t)kvh * seq.units;
+            const int first = (int)quotient(s0 + kTreeStart, quota), last = (int)quotient(s0 + seq.units - 1, quota), shift = s0 > first * quota ? 1 : 0;
+            for (int row = threadIdx.x >> 5; row < m_rows; row += kMergeWarps) {
+                if (first == last) {
+                    if (lane == 0) s_scale[row] = __ldcg(a.row_ml + (int64_t)item * m_rows + row);
+                    continue;
+                }
+                float m = -INFINITY, l = 0.f, none = 0.f;
+                for (int c = first + lane; c <= last; c += 32) {
+                    const float2 ml = __ldcg(&a.part_ml[(int64_t)(c * 2 + (c == first ? shift : 0)) * a.tile_rows + row]);
+                    if (ml.x == -INFINITY) {
+                        none += ml.y;
+                    } else {
+                        const float high = fmaxf(m, ml.x);
+                        l = (m == -INFINITY ? 0.f : l * exp2_approx(m - high)) + ml.y * exp2_approx(ml.x - high);
+                        m = high;
+                    }
+                }
+                float high = m;
+                for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+                l = m == -INFINITY ? 0.f : l * exp2_approx(m - high);
+                for (int o = 16; o > 0; o >>= 1) {
+                    l += __shfl_xor_sync(0xffffffffu, l, o);
+                    none += __shfl_xor_sync(0xffffffffu, none, o);
+                }
+                if (lane == 0) s_scale[row] = row_scale(high, high == -INFINITY ? none : l);
+            }
+            __syncthreads();
+            for (int pos = ((at - item * stretches) * 32 * kMergeWarps + threadIdx.x) * 4; pos < seq.end; pos += stretches * 128 * kMergeWarps)
+                add_weights<4>(a, seq, r, kvh, s_scale, m_rows, pos);
+            return;
+        }
+    }
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warp = blockIdx.x * kMergeWarps + wid, m_rows = a.nodes * a.group, per_seq = a.kv_heads * m_rows;
     __shared__ float4 s_part[kMergeWarps][kMergeParts][32];
     __shared__ int64_t s_before[kMergeWarps], s_quota;   // what all rows ask for comes through one thread a CTA and sequence
@@ -794,6 +844,7 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     const CUtensorMap kmap = page_map(a.k, c), vmap = page_map(a.v, c);
     if (weights) {
         char* more = static_cast<char*>(work) + (tree_attention_work_bytes(c, q_heads, nodes) + 15) / 16 * 16;
+        a.weights = weights + (int64_t)layer * c.rows * c.kv_heads * c.width * c.page;
         a.score_stride = tree_score_stride(c, q_heads, nodes);
         a.scores = a.score_stride ? reinterpret_cast<float*>(more) : nullptr;
         a.row_ml = reinterpret_cast<float2*>(more + 4ull * c.rows * c.kv_heads * m_rows * a.score_stride);
@@ -815,8 +866,17 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     const int ctas = (int)std::min<int64_t>(tree_ctas(ns), most);
     launch_chained(kernel, dim3(ctas), dim3(tree_threads(ns)), tree_smem(ns), s, a, kmap, vmap);
     const int64_t rows = (int64_t)c.rows * c.kv_heads * m_rows;   // at most 1024 x 1024 x 1024
-    if (!a.whole) launch_chained(tree_merge_kernel, dim3((unsigned)((rows + kMergeWarps - 1) / kMergeWarps)), dim3(32 * kMergeWarps), 0, s, a, ns, (int)rows);
-    if (weights) launch_tree_weigh(c, a, weights + (int64_t)layer * c.rows * c.kv_heads * c.width * c.page, s);
+    if (!a.whole) {
+        const int merges = (int)((rows + kMergeWarps - 1) / kMergeWarps);
+        if (a.scores) {   // with as many CTAs as fill the SMs several times, none for positions that the table cannot hold
+            const int64_t items = (int64_t)c.rows * c.kv_heads;
+            const int stretches = (int)std::min(a.score_stride / kTile, std::max<int64_t>(1, 8 * kTreeSms / items));
+            launch_chained(tree_merge_kernel<true>, dim3((unsigned)(merges + items * stretches)), dim3(32 * kMergeWarps), 0, s, a, ns, (int)rows, merges, stretches);
+        } else {
+            launch_chained(tree_merge_kernel<false>, dim3((unsigned)merges), dim3(32 * kMergeWarps), 0, s, a, ns, (int)rows, merges, 0);
+        }
+    }
+    if (weights && !a.scores) launch_tree_weigh(c, a, s);
 }
 
 }  // namespace mfqb

@@ -13,6 +13,7 @@ namespace mfqb {
 constexpr int kTreeSms = 148;
 constexpr int kTile = 128;                           // rows of Q, positions of a tile
 constexpr int kTileBytes = kTile * kHeadDim * 2, kHalfBytes = kTileBytes / 2;
+constexpr int kScoreRows = 64;                       // up to so many rows the attention may keep its scores
 constexpr int kTreeStart = 2;                        // what starting and ending a stretch takes, in tiles
 
 struct TreeArgs {
@@ -31,6 +32,7 @@ struct TreeArgs {
     float2* row_ml;               // [rows][kv_heads][rows of Q]: maximum (in powers of two) and 1 / sum of every row, where weights are added up
     float* scores;                // [rows][kv_heads][rows of Q][score_stride]: raw scores, minus infinity where a row does not see, or null
     int64_t score_stride;
+    float* weights;               // of the layer: [rows][kv_heads][width * page], or null
     unsigned group_inv;           // ceil(65536 / group): row / group = row * group_inv >> 16 for rows below 1024, groups up to 16
     float scale_log2;
     __device__ __forceinline__ int node_of(int row_of_q) const { return (int)((unsigned)row_of_q * group_inv >> 16); }
@@ -169,9 +171,45 @@ inline CUtensorMap page_map(const void* base, const mfqb_cache& c) {
 }
 
 
-// The sums of the attention's weights (tree_weigh.cu), from row_ml and, where they were kept, the scores.
+// What a position of sequence r gets, from the scores that the attention has kept: exp2(scale' score - x) y of every row's (x, y), in their order, nothing
+// for a score of minus infinity.  Positions pos .. pos + N - 1 lie in one page.
+template <int N>
+__device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& seq, int r, int kvh, const float2* scale, int m_rows, int pos) {
+    const int64_t item = (int64_t)r * a.kv_heads + kvh;
+    const float* scores = a.scores + item * m_rows * a.score_stride + pos;
+    float* to = a.weights + item * a.width * a.page + pos;
+    const int page = __ldcg(a.table + (int64_t)r * a.width + pos / a.page);
+    const bool good = (unsigned)page < (unsigned)a.pages;
+    float before[N], sum[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        before[e] = pos + e < seq.len ? to[e] : 0.f;
+        sum[e] = 0.f;
+    }
+#pragma unroll 4
+    for (int row = 0; row < m_rows; ++row) {
+        const float2 ml = scale[row];
+        float v[N];
+        if constexpr (N == 4) {
+            const float4 s = __ldcg(reinterpret_cast<const float4*>(scores + row * a.score_stride));
+            v[0] = s.x; v[1] = s.y; v[2] = s.z; v[3] = s.w;
+        } else {
+            v[0] = __ldcg(scores + row * a.score_stride);
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += v[e] == -INFINITY ? 0.f : exp2_approx(fmaf(v[e], a.scale_log2, -ml.x)) * ml.y;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (pos + e >= seq.end) break;
+        if (pos + e >= seq.len) to[e] = good ? sum[e] : 0.f;   // a node's
+        else if (good) to[e] = before[e] + sum[e];
+    }
+}
+
+// The sums of the attention's weights where it has not kept its scores (tree_weigh.cu), from row_ml and the keys.
 uint64_t tree_weigh_bytes(const mfqb_cache& c, int q_heads, int nodes);
 int64_t tree_score_stride(const mfqb_cache& c, int q_heads, int nodes);   // 0 where scores are not kept
-void launch_tree_weigh(const mfqb_cache& c, const TreeArgs& a, float* weights, cudaStream_t s);
+void launch_tree_weigh(const mfqb_cache& c, const TreeArgs& a, cudaStream_t s);
 
 }  // namespace mfqb

@@ -7,10 +7,9 @@
 
 namespace mfqb {
 
-constexpr int kScoreRows = 64;                     // up to so many rows the attention may keep its scores
 constexpr uint64_t kScoreBytes = 512ull << 20;     // as long as they take at most this
 constexpr int kWeighRows = 256;                    // rows of a pass over the keys
-constexpr int kWeighRing = 4, kWeighThreads = 320;
+constexpr int kWeighRing = 4, kWeighGroups = 4, kWeighThreads = 64 + 128 * kWeighGroups;   // a loader, an issuer, groups of four warps that sum
 
 int64_t tree_score_stride(const mfqb_cache& c, int q_heads, int nodes) {
     const int64_t m_rows = (int64_t)nodes * (q_heads / c.kv_heads), stride = ((int64_t)c.width * c.page + kTile - 1) / kTile * kTile;
@@ -21,46 +20,16 @@ uint64_t tree_weigh_bytes(const mfqb_cache& c, int q_heads, int nodes) {
     return rows * 8 + 4 * rows * tree_score_stride(c, q_heads, nodes);
 }
 
-// From the scores that the attention has kept.  CTA (stretch of positions, kv head, sequence), four positions a thread.
-__global__ void __launch_bounds__(128) weigh_scores_kernel(const __grid_constant__ TreeArgs a, float* weights) {
-    chained_wait();
-    __shared__ float2 s_ml[kScoreRows];
-    const int kvh = blockIdx.y, r = blockIdx.z, m_rows = a.nodes * a.group;
-    const int64_t item = (int64_t)r * a.kv_heads + kvh;
-    if ((int)threadIdx.x < m_rows) s_ml[threadIdx.x] = __ldcg(a.row_ml + item * m_rows + threadIdx.x);
-    __syncthreads();
-    const TreeSeq seq = tree_seq(a, r);
-    const float* scores = a.scores + item * m_rows * a.score_stride;
-    float* to = weights + item * a.width * a.page;
-    for (int pos = (blockIdx.x * 128 + threadIdx.x) * 4; pos < seq.end; pos += gridDim.x * 512) {   // four positions lie in one page
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int row = 0; row < m_rows; ++row) {
-            const float2 ml = s_ml[row];
-            const float4 s = __ldcg(reinterpret_cast<const float4*>(scores + row * a.score_stride + pos));
-            const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += v[e] == -INFINITY ? 0.f : exp2_approx(fmaf(v[e], a.scale_log2, -ml.x)) * ml.y;
-        }
-        const int page = __ldcg(a.table + (int64_t)r * a.width + pos / a.page);
-        const bool good = (unsigned)page < (unsigned)a.pages;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (pos + e >= seq.end) break;
-            if (pos + e >= seq.len) to[pos + e] = good ? sum[e] : 0.f;
-            else if (good) to[pos + e] += sum[e];
-        }
-    }
-}
-
 struct WeighShared {
-    uint64_t k_full[kWeighRing], k_empty[kWeighRing], q_full, s_full[2], s_empty[2], all;
+    uint64_t k_full[kWeighRing], k_empty[kWeighRing], q_full, s_full[2], s_empty[2], all, half[4];
     int64_t scan[kWeighThreads / 32], first, last, off;
     int row0, failed;
     int bad;                         // the last head (its number in the CTA, from 1 on) with a row whose weights are no numbers
     uint32_t tmem;
     unsigned good[8];
-    unsigned long long masks[kTreeNodes];
-    float4 ml[kWeighRows / 2];   // of two rows: minus their maxima, the factors
+    unsigned long long seen_by[kTreeNodes];   // by which nodes a node is
+    float sum[4][kTile];         // of the rows' second half, of every fourth tile
+    float4 shift[kWeighRows / 4];   // of every row: - maximum - log2(sum), so that weight = exp2(scale' score + shift)
 };
 constexpr size_t kWeighSmem = (size_t)kWeighRing * kTileBytes + (size_t)kWeighRows * kHeadDim * 2 + sizeof(WeighShared);
 static_assert(kWeighSmem <= 227 * 1024, "shared memory of an SM");
@@ -92,9 +61,49 @@ struct WeighWalk {
     }
 };
 
+// A position that not every row sees, or (BAD) where weights of some rows are no numbers: a row counts where it sees the position and its score is
+// above minus infinity.
+template <bool BAD>
+__device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shift, uint32_t col, int row0, int rows, unsigned long long seen) {
+    const int m_rows = a.nodes * a.group;
+    uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll 1
+    for (int c = 0; c < rows; c += 16) {
+        uint32_t s[16];
+        tmem_ld16_async(col + c, s);
+        unsigned in = rows - c >= 16 ? 0xFFFFu : (1u << (rows - c)) - 1u;   // of these 16
+        if (seen != ~0ull) {
+            unsigned by = 0u;
+            const int n0 = a.node_of(row0 + c), n1 = a.node_of(min(row0 + c + 15, m_rows - 1));
+            for (int i = n0; i <= n1; ++i) {   // a node's rows, at most 16, follow each other
+                const int from = i * a.group - (row0 + c);
+                const unsigned run = (1u << a.group) - 1u;
+                if ((seen >> i) & 1ull) by |= from >= 0 ? run << from : run >> -from;
+            }
+            in &= by;
+        }
+        tmem_wait_ld16(s);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const float4 m = s_shift[(c + e) / 4];
+            const float shift[4] = {m.x, m.y, m.z, m.w};
+            float p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float x = __uint_as_float(s[e + u]);
+                p[u] = (in >> (e + u)) & 1u && (!BAD || x != -INFINITY) ? exp2_approx(fmaf(x, a.scale_log2, shift[u])) : 0.f;
+            }
+            sum2[0] = add_f32x2(sum2[0], pair_f32(p[0], p[1]));
+            sum2[1] = add_f32x2(sum2[1], pair_f32(p[2], p[3]));
+        }
+    }
+    const float2 two = split_f32(add_f32x2(sum2[0], sum2[1]));
+    return two.x + two.y;
+}
+
 // From the keys, by rows row0 .. row0 + rows of Q: S^T = K Q^T puts a position into each lane of tensor memory, so that the sum over the rows stays in
 // a thread.  One warp asks for the pages' keys, one issues tcgen05.mma, two groups of four warps take the tiles in turns.
-__global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap, float* weights, int row0, int rows) {
+__global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap, int row0, int rows) {
     extern __shared__ __align__(1024) unsigned char ring[];
     unsigned char* q_tile = ring + (size_t)kWeighRing * kTileBytes;   // two halves of 64 dims, kWeighRows rows of 128 bytes each
     constexpr int kQHalf = kWeighRows * 128;
@@ -106,9 +115,10 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
     }
     if (tid == 0) {
         for (int i = 0; i < kWeighRing; ++i) { mbar_init(&sh.k_full[i], 1); mbar_init(&sh.k_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.s_empty[i], 4); }
-        mbar_init(&sh.q_full, 8);
-        mbar_init(&sh.all, 8);
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.s_empty[i], 8); }
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.half[i], 4);
+        mbar_init(&sh.q_full, 4 * kWeighGroups);
+        mbar_init(&sh.all, 4 * kWeighGroups);
         sh.failed = sh.bad = 0;
         sh.first = sh.last = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -161,10 +171,21 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
         const int box = min(a.page, kTile), boxes = kTile / box;
         uint32_t j = 0;
         bool ok = true;
+        auto look = [&](const WeighWalk& x) {   // this lane's page of a tile
+            const int pos = x.t * kTile + lane * box;
+            return x.left > 0 && lane < boxes && pos < x.seq.end ? __ldcg(a.table + (int64_t)x.r * a.width + pos / a.page) : -1;
+        };
+        WeighWalk ahead = w;   // two tiles ahead: a look into the table takes as long as a tile
+        int pages[2];
+        pages[0] = look(ahead);
+        if (ahead.left > 0) ahead.next(a);
+        pages[1] = look(ahead);
         for (; w.left > 0; w.next(a), ++j) {
             const int pos = w.t * kTile + lane * box;
-            int page = -1;
-            if (lane < boxes && pos < w.seq.end) page = __ldcg(a.table + (int64_t)w.r * a.width + pos / a.page);
+            int page = pages[0];
+            if (ahead.left > 0) ahead.next(a);
+            pages[0] = pages[1];
+            pages[1] = look(ahead);
             if ((unsigned)page >= (unsigned)a.pages) page = -1;
             const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
             const uint32_t stage = j % kWeighRing;
@@ -189,14 +210,13 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
         for (uint32_t i = 1; i <= min(j, (uint32_t)kWeighRing); ++i)   // no copy outlives the CTA
             if (!warp_wait(&sh.k_full[(j - i) % kWeighRing], ((j - i) / kWeighRing) & 1u)) sh.failed = 1;
     } else if (warp == 1) {
-        const uint32_t idesc = __shfl_sync(0xffffffffu, instr_desc_bf16(kTile, (rows + 15) / 16 * 16, false), 0);
+        const uint32_t idesc = __shfl_sync(0xffffffffu, instr_desc_bf16(kTile, (rows + 31) / 32 * 32, false), 0);
         const uint32_t q_addr = smem_u32(q_tile), ring_addr = smem_u32(ring);
         uint32_t j = 0, items = 0;
         bool ok = true;
         for (; w.left > 0; w.next(a), ++j) {
             const uint32_t stage = j % kWeighRing, g = j & 1u;
-            ok = (!w.fresh || warp_wait(&sh.q_full, items & 1u)) && warp_wait(&sh.k_full[stage], (j / kWeighRing) & 1u) &&
-                 warp_wait(&sh.s_empty[g], ((j >> 1) & 1u) ^ 1u);
+            ok = (!w.fresh || warp_wait(&sh.q_full, items & 1u)) && warp_wait2(&sh.k_full[stage], (j / kWeighRing) & 1u, &sh.s_empty[g], ((j >> 1) & 1u) ^ 1u);
             if (!ok) break;
             items += w.fresh;
             tc_fence_after_sync();
@@ -213,9 +233,13 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
         }
         if (!ok) sh.failed = 1;
     } else {
-        const int g = (warp - 2) >> 2, quarter = warp & 3, t = tid - 64;
-        const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + g * kWeighRows;
+        // Two groups, g, for tiles in turns, of two halves, h, of the rows.
+        const int g = (warp - 2) >> 3, h = ((warp - 2) >> 2) & 1, quarter = warp & 3, t = tid - 64, at = quarter * 32 + lane;
+        const int first_row = h * ((rows + 63) / 64 * 32), some = h ? rows - first_row : min(rows, (rows + 63) / 64 * 32);   // this half; may be none of 32 rows or fewer
+        const float4* my_shift = sh.shift + first_row / 4;
+        const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + g * kWeighRows + first_row;
         const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
+        const unsigned long long every = a.nodes < 64 ? ~0ull << a.nodes : 0ull;   // nodes that there are not
         uint32_t j = 0, alls = 0;
         int items = 0;
         bool ok = true;
@@ -223,106 +247,108 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
             warp_arrive(&sh.all);
             ok = ok && warp_wait(&sh.all, alls++ & 1u);
         };
+        // A tile's sum waits for its second half until the group's next one.
+        float* due_to = nullptr;
+        float due_sum = 0.f;
+        int due = -1;   // the tile
+        auto put = [&]() {
+            if (due < 0) return;
+            ok = warp_wait(&sh.half[due & 3], (due >> 2) & 1);
+            if (ok && due_to) *due_to = due_sum + sh.sum[due & 3][at];
+        };
         for (; ok && w.left > 0; w.next(a), ++j) {
             if (w.fresh) {   // all tiles of the head before have been summed, and their products read the rows that change now
                 all_sync();
                 if (!ok) break;
                 ++items;
-                const int c = t & 15, padded = (rows + 15) / 16 * 16;
-                for (int r0 = t >> 4; r0 < padded; r0 += 128) {   // rows behind the last one repeat it
-                    uint4 v[8];
+                const int c = t & 15, padded = (rows + 31) / 32 * 32;
+                constexpr int kStep = 8 * kWeighGroups, kLoads = 4;   // rows of a step: 16 threads each
+#pragma unroll 1
+                for (int r0 = t >> 4; r0 < padded; r0 += kStep * kLoads) {   // rows behind the last one repeat it
+                    uint4 v[kLoads];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u)
-                        if (r0 + 16 * u < padded) v[u] = __ldcg(reinterpret_cast<const uint4*>(a.q + a.row_at(w.r, w.kvh, min(row0 + r0 + 16 * u, m_rows - 1))) + c);
+                    for (int u = 0; u < kLoads; ++u) {
+                        const int rr = r0 + kStep * u;
+                        if (rr < padded) v[u] = __ldcg(reinterpret_cast<const uint4*>(a.q + a.row_at(w.r, w.kvh, min(row0 + rr, m_rows - 1))) + c);
+                    }
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const int rr = r0 + 16 * u;
+                    for (int u = 0; u < kLoads; ++u) {
+                        const int rr = r0 + kStep * u;
                         if (rr < padded) *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kQHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[u];
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&sh.q_full);
-                if (t < kWeighRows) {   // rows behind the last one have its maximum and count for nothing
+                if (t < kWeighRows) {   // rows behind the last one count for nothing, nor do those that see nothing
                     const float2 ml = __ldcg(a.row_ml + ((int64_t)w.r * a.kv_heads + w.kvh) * m_rows + min(row0 + t, row0 + rows - 1));
-                    float* to = reinterpret_cast<float*>(&sh.ml[t >> 1]) + (t & 1);
-                    to[0] = -ml.x;
-                    to[2] = t < rows ? ml.y : 0.f;
-                    if (t < rows && !(fabsf(ml.x) < INFINITY && ml.y < INFINITY)) sh.bad = items;   // NaN too
+                    const float shift = t < rows ? log2f(ml.y) - ml.x : -INFINITY;
+                    reinterpret_cast<float*>(sh.shift)[t] = shift;
+                    if (!(shift < INFINITY)) sh.bad = items;   // NaN too
                 }
-                if (t < kTreeNodes) sh.masks[t] = t < a.nodes ? __ldcg(a.masks + (int64_t)w.r * a.nodes + t) : 0ull;
+                {   // a lane has two nodes' masks, a warp makes the bits of four nodes
+                    const unsigned long long* masks = a.masks + (int64_t)w.r * a.nodes;
+                    const unsigned long long lo = lane < a.nodes ? __ldcg(masks + lane) : 0ull, hi = lane + 32 < a.nodes ? __ldcg(masks + lane + 32) : 0ull;
+#pragma unroll
+                    for (int u = 0; u < kTreeNodes / (4 * kWeighGroups); ++u) {
+                        const int node = (warp - 2) * (kTreeNodes / (4 * kWeighGroups)) + u;
+                        const unsigned x = __ballot_sync(0xffffffffu, (lo >> node) & 1ull), y = __ballot_sync(0xffffffffu, (hi >> node) & 1ull);
+                        if (lane == 0) sh.seen_by[node] = (unsigned long long)y << 32 | x;
+                    }
+                }
                 all_sync();
                 if (!ok) break;
             }
             if ((int)(j & 1u) != g) continue;
-            const int at = quarter * 32 + lane, pos = w.t * kTile + at, node = pos - w.seq.len;
-            float* to = weights + ((int64_t)w.r * a.kv_heads + w.kvh) * a.width * a.page + pos;
-            const bool adds = pos < w.seq.end && (node < 0 || row0 > 0);   // to what is there
-            const float before = adds ? *to : 0.f;
+            const int pos = w.t * kTile + at, node = pos - w.seq.len;
+            float* to = a.weights + ((int64_t)w.r * a.kv_heads + w.kvh) * a.width * a.page + pos;
+            const bool adds = node < 0 || row0 > 0;   // to what is there
+            const float before = h == 0 && adds && pos < w.seq.end ? *to : 0.f;
             ok = warp_wait(&sh.s_full[g], (j >> 1) & 1u);
             if (!ok) break;
             tc_fence_after_sync();
             const unsigned good = sh.good[j & 7];
             const bool page = (good >> (at >> 4)) & 1u;
-            uint64_t sum2[2] = {0ull, 0ull};
-            // Sixteen rows at a time, the next ones' scores on their way; columns behind the last row are products with it too.
-            auto rows_of = [&](auto each) {
-                const int chunks = (rows + 15) / 16;
-                uint32_t s[2][16];
-                tmem_ld16_async(col, s[0]);
+            float sum = 0.f;   // columns behind the last row are products with it too
+            // What comes of a position behind the end or without a page is not used.
+            const unsigned long long seen = node < 0 || node >= a.nodes ? ~0ull : sh.seen_by[node] | every;
+            if (__all_sync(0xffffffffu, seen == ~0ull) && sh.bad != items) {   // every row sees all 32 positions
+                uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll 1
-                for (int c = 0; c < chunks; c += 2) {
-                    tmem_wait_ld16(s[0]);
-                    if (c + 1 < chunks) tmem_ld16_async(col + 16 * (c + 1), s[1]);
-                    each(16 * c, s[0]);
-                    if (c + 1 < chunks) {
-                        tmem_wait_ld16(s[1]);
-                        if (c + 2 < chunks) tmem_ld16_async(col + 16 * (c + 2), s[0]);
-                        each(16 * (c + 1), s[1]);
+                for (int c = 0; c < some; c += 32) {
+                    uint32_t s[32];
+                    tmem_ld32(col + c, s);
+                    tmem_wait_ld(s);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float4 m = my_shift[c / 4 + e];
+                        const float2 x = split_f32(fma_f32x2(pair_f32(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])), scale2, pair_f32(m.x, m.y)));
+                        const float2 y = split_f32(fma_f32x2(pair_f32(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])), scale2, pair_f32(m.z, m.w)));
+                        sum2[0] = add_f32x2(sum2[0], pair_f32(exp2_approx(x.x), exp2_approx(x.y)));
+                        sum2[1] = add_f32x2(sum2[1], pair_f32(exp2_approx(y.x), exp2_approx(y.y)));
                     }
                 }
-            };
-            if (w.t * kTile + kTile <= w.seq.len && good == 0xFFu && sh.bad != items) {
-                rows_of([&](int c, const uint32_t* s) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float4 ml = sh.ml[(c + e) >> 1];
-                        const float2 x = split_f32(fma_f32x2(pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, pair_f32(ml.x, ml.y)));
-                        sum2[(e >> 1) & 1] = fma_f32x2(pair_f32(exp2_approx(x.x), exp2_approx(x.y)), pair_f32(ml.z, ml.w), sum2[(e >> 1) & 1]);
-                    }
-                });
-            } else {   // a row counts where it sees the position and its score is above minus infinity
-                unsigned long long seen = ~0ull;   // by which nodes the position is
-                if (!page || node >= a.nodes) {
-                    seen = 0ull;
-                } else if (node >= 0) {
-                    seen = 0ull;
-                    for (int i = 0; i < a.nodes; ++i) seen |= ((sh.masks[i] >> node) & 1ull) << i;
-                }
-                rows_of([&](int c, const uint32_t* s) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float4 ml = sh.ml[(c + e) >> 1];
-                        float p[2];
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const float x = __uint_as_float(s[e + u]);
-                            const bool on = ((seen >> a.node_of(min(row0 + c + e + u, m_rows - 1))) & 1ull) && x != -INFINITY && c + e + u < rows;
-                            p[u] = on ? exp2_approx(fmaf(x, a.scale_log2, u ? ml.y : ml.x)) * (u ? ml.w : ml.z) : 0.f;
-                        }
-                        sum2[(e >> 1) & 1] = add_f32x2(pair_f32(p[0], p[1]), sum2[(e >> 1) & 1]);
-                    }
-                });
+                const float2 two = split_f32(add_f32x2(sum2[0], sum2[1]));
+                sum = two.x + two.y;
+            } else {
+                sum = sh.bad == items ? weigh_some<true>(a, my_shift, col, row0 + first_row, some, seen) : weigh_some<false>(a, my_shift, col, row0 + first_row, some, seen);
             }
-            const float2 half = split_f32(add_f32x2(sum2[0], sum2[1]));
-            const float sum = half.x + half.y;
+            if (!page) sum = 0.f;
             tc_fence_before_sync();
+            if (h) {   // the sum of four tiles before was read before this product was issued
+                sh.sum[j & 3][at] = sum;
+                warp_arrive(&sh.half[j & 3]);
+            } else {
+                put();
+                if (!ok) break;
+            }
             warp_arrive(&sh.s_empty[g]);
-            if (adds) {
-                if (page) *to = before + sum;
-            } else if (pos < w.seq.end) {
-                *to = sum;
+            if (h == 0) {
+                due_to = pos < w.seq.end && (page || !adds) ? to : nullptr;
+                due_sum = before + sum;
+                due = (int)j;
             }
         }
+        if (ok && h == 0) put();
         if (!ok) sh.failed = 1;
     }
     __syncwarp();
@@ -335,15 +361,9 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
     }
 }
 
-void launch_tree_weigh(const mfqb_cache& c, const TreeArgs& a, float* weights, cudaStream_t s) {
+void launch_tree_weigh(const mfqb_cache& c, const TreeArgs& a, cudaStream_t s) {
     const int m_rows = a.nodes * a.group;
     const int64_t cap = (int64_t)c.width * c.page, items = (int64_t)c.rows * c.kv_heads;
-    if (a.scores) {
-        // as many CTAs as fill the SMs several times, none for positions that the table cannot hold
-        const int64_t each = std::min((cap + 511) / 512, std::max<int64_t>(1, 8 * kTreeSms / items));
-        launch_chained(weigh_scores_kernel, dim3((unsigned)each, c.kv_heads, c.rows), dim3(128), 0, s, a, weights);
-        return;
-    }
     int device = 0;
     MFQB_CUDA(cudaGetDevice(&device));
     static std::once_flag once[64];
@@ -351,7 +371,7 @@ void launch_tree_weigh(const mfqb_cache& c, const TreeArgs& a, float* weights, c
     const CUtensorMap kmap = page_map(a.k, c);
     const unsigned ctas = (unsigned)std::min<int64_t>(kTreeSms, items * ((cap + kTile - 1) / kTile));
     for (int row0 = 0; row0 < m_rows; row0 += kWeighRows)
-        launch_chained(tree_weigh_kernel, dim3(ctas), dim3(kWeighThreads), kWeighSmem, s, a, kmap, weights, row0, std::min(kWeighRows, m_rows - row0));
+        launch_chained(tree_weigh_kernel, dim3(ctas), dim3(kWeighThreads), kWeighSmem, s, a, kmap, row0, std::min(kWeighRows, m_rows - row0));
 }
 
 }  // namespace mfqb
