@@ -454,6 +454,12 @@ int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_s
  * the other beams' scores at minus infinity.  One call with as many beams must come before a stream capture. */
 struct mfqb_cache;
 int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
+/* Passes over the attached pages that add up how much every position was looked at and go on behind evicted ones (mfqb_cache_evict): weights float32
+ * [layers][rows][kv_heads][width * page] of mfqb_tree_attention_weigh (null: none), dropped int32 [rows] (null: none), what has been
+ * evicted of every sequence so far, which is added to its positions.  Both are the caller's memory on the decoder's device and must outlive the
+ * passes; attaching a cache (mfqb_decoder_set_cache) takes them off again.  Allocates as mfqb_decoder_set_cache does.  Weights do not
+ * move with sequences: mfqb_decoder_beam_step is refused meanwhile. */
+int mfqb_decoder_set_weights(mfqb_decoder* d, float* weights, const int32_t* dropped);
 int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream);
 int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, float* scores, int32_t* done, int eos, int32_t* ids_out,
                            int32_t* parents_out, int32_t* status, mfqb_stream_t stream);

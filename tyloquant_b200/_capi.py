@@ -95,6 +95,7 @@ _SIGNATURES = {
     "mfqb_decoder_read_cache": (_i, [_vp, _i, _i, _i, _i, _vp, _vp]),
     "mfqb_decoder_read_logits": (_i, [_vp, _i, _vp, _vp]),
     "mfqb_decoder_set_cache": (_i, [_vp, _P(CacheView)]),
+    "mfqb_decoder_set_weights": (_i, [_vp, _vp, _vp]),
     "mfqb_decoder_verify": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
     "mfqb_decoder_beam_step": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
     "mfqb_decoder_free": (_i, [_vp]),

@@ -637,8 +637,10 @@ struct mfqb_decoder {
     const uint64_t* node_masks = nullptr;   // masks and depths
     const int32_t* node_depths = nullptr;
     uint64_t attn_work_bytes = 0;
+    float* weights = nullptr;               // mfqb_decoder_set_weights: of the cache's positions, and what has been dropped before them; the caller's
+    const int32_t* dropped = nullptr;
     std::vector<DevBuf> retired;   // buffers that a larger cache outgrew: graphs captured before still use them
-    DevBuf q16, freqs, masks, depths, single_masks, single_depths, attn_work, beam_work, beam_scores, beam_tokens, beam_moves, beam_counts, fork_work;
+    DevBuf q16, freqs, masks, depths, single_masks, single_depths, attn_work, beam_work, beam_scores, beam_tokens, beam_moves, beam_counts, fork_work, moved_depths;
     DevBuf gamma_final;
     // workspaces
     DevBuf h, h2, xn, qkv, attn, attn_count, inv_freq, rope_table, proj, proj_sum, act, logits, part, best_val, best_idx, part_val, part_idx, gathered, gathered_sum, pos;
@@ -723,7 +725,25 @@ static void attend_own(mfqb_decoder* d, DecoderLayer& L, int rows, cudaStream_t 
 // Rotary embedding, cache write and attention of the nodes over the attached pages.
 static void attend_pages(mfqb_decoder* d, int li, cudaStream_t s) {
     check(mfqb_cache_write(&d->write_to, li, static_cast<const float*>(d->qkv.p), d->nq, d->nodes, d->node_depths, static_cast<const double*>(d->freqs.p), d->q16.p, s));
-    check(mfqb_tree_attention(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, 0.08838834764831845f, d->attn.p, d->attn_work.p, d->attn_work_bytes, s));
+    const float scale = 0.08838834764831845f;
+    if (d->weights)
+        check(mfqb_tree_attention_weigh(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, scale, d->attn.p, d->weights, d->attn_work.p, d->attn_work_bytes, s));
+    else
+        check(mfqb_tree_attention(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, scale, d->attn.p, d->attn_work.p, d->attn_work_bytes, s));
+}
+
+// A pass's depths count from the lengths; where tokens have been evicted the positions are further on.
+__global__ void move_depths_kernel(const int* depths, const int* dropped, int nodes, int n, int* out) {
+    chained_wait();
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) out[i] = __ldcg(depths + i) + __ldcg(dropped + i / nodes);
+}
+static void move_depths(mfqb_decoder* d, cudaStream_t s) {
+    if (!d->dropped) return;
+    const int n = d->cache.rows * d->nodes;
+    launch_dep(move_depths_kernel, dim3((n + 127) / 128), dim3(128), s, static_cast<const int*>(d->node_depths), static_cast<const int*>(d->dropped), d->nodes, n,
+               static_cast<int*>(d->moved_depths.p));
+    d->node_depths = static_cast<const int32_t*>(d->moved_depths.p);
 }
 
 // One transformer block on the residual stream d->h for `rows` sequences; `delta` is the previous
@@ -793,11 +813,12 @@ static void check_ready(const mfqb_decoder* d, int rows, const char* who) {
     if (!d->paged && d->cfg.max_ctx < 1) fail(MFQB_ERR_ARG, "%s: the decoder has no cache of its own (max_ctx 0) and none is attached", who);
 }
 // The next pass has one node per sequence, at the cache's own lengths.
-static void single_nodes(mfqb_decoder* d) {
+static void single_nodes(mfqb_decoder* d, cudaStream_t s) {
     d->nodes = 1;
     d->write_to = d->read_from = d->cache;
     d->node_masks = static_cast<const uint64_t*>(d->single_masks.p);
     d->node_depths = static_cast<const int32_t*>(d->single_depths.p);
+    if (d->paged) move_depths(d, s);
 }
 // Embedding, blocks and head: the logits of `rows` rows.
 static void forward_logits(mfqb_decoder* d, const int32_t* ids, int rows, cudaStream_t s) {
@@ -990,7 +1011,7 @@ int mfqb_decoder_step(mfqb_decoder* d, const int32_t* ids_in, int batch, int32_t
         if (d->paged && batch != d->cache.rows) fail(MFQB_ERR_ARG, "mfqb_decoder_step: the cache has %d sequences, got a batch of %d", d->cache.rows, batch);
         DeviceGuard guard(d->device);
         cudaStream_t s = stream;
-        single_nodes(d);
+        single_nodes(d, s);
         forward_argmax(d, ids_in, batch, s);
         if (d->world == 1) {
             MFQB_CUDA(cudaMemcpyAsync(ids_out, d->best_idx.p, (size_t)batch * 4, cudaMemcpyDeviceToDevice, s));
@@ -1037,6 +1058,8 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
         std::vector<uint64_t> one(rows, 1);
         std::vector<int32_t> zero(rows, 0);
         d->paged = false;
+        d->weights = nullptr;
+        d->dropped = nullptr;
         room(d, d->q16, B * d->nq * kHeadDim * 2);
         room(d, d->masks, B * 8);
         room(d, d->depths, B * 4);
@@ -1063,6 +1086,36 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
     });
 }
 
+int mfqb_decoder_set_weights(mfqb_decoder* d, float* weights, const int32_t* dropped) {
+    return guarded([&] {
+        if (!d) fail(MFQB_ERR_ARG, "mfqb_decoder_set_weights: null decoder");
+        if (!d->paged) fail(MFQB_ERR_ARG, "mfqb_decoder_set_weights: needs a cache (mfqb_decoder_set_cache)");
+        if ((uintptr_t)weights & 15) fail(MFQB_ERR_ARG, "mfqb_decoder_set_weights: weights must be 16-byte aligned");
+        DeviceGuard guard(d->device);
+        for (const void* p : {(const void*)weights, (const void*)dropped}) {
+            if (!p) continue;
+            cudaPointerAttributes at{};
+            MFQB_CUDA(cudaPointerGetAttributes(&at, p));
+            if (at.type != cudaMemoryTypeDevice || at.device != d->device) fail(MFQB_ERR_ARG, "mfqb_decoder_set_weights: weights and dropped must be memory of device %d", d->device);
+        }
+        d->weights = nullptr;
+        d->dropped = nullptr;
+        if (weights) {
+            const size_t B = d->cfg.max_batch, rows = d->cache.rows;
+            uint64_t most = 0, bytes = 0;
+            for (int nodes = 1; nodes <= kTreeNodes && nodes * rows <= B && (int64_t)nodes <= (int64_t)d->cache.width * d->cache.page; ++nodes) {
+                check(mfqb_tree_attention_weigh_work(&d->cache, d->nq, nodes, &bytes));
+                most = std::max(most, bytes);
+            }
+            room(d, d->attn_work, most);
+            d->attn_work_bytes = d->attn_work.bytes;
+        }
+        if (dropped) room(d, d->moved_depths, (size_t)d->cfg.max_batch * 4);
+        d->weights = weights;
+        d->dropped = dropped;
+    });
+}
+
 int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream) {
     return guarded([&] {
         if (!d || !ids || !parents || !targets) fail(MFQB_ERR_ARG, "mfqb_decoder_verify: null argument");
@@ -1076,6 +1129,7 @@ int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* pare
         d->write_to = d->read_from = d->cache;
         d->node_masks = static_cast<const uint64_t*>(d->masks.p);
         d->node_depths = static_cast<const int32_t*>(d->depths.p);
+        move_depths(d, stream);
         forward_argmax(d, ids, rows, stream);
         MFQB_CUDA(cudaMemcpyAsync(targets, d->best_idx.p, (size_t)rows * 4, cudaMemcpyDeviceToDevice, stream));
     });
@@ -1087,6 +1141,7 @@ int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, fl
         if (!d || !ids_in || !scores || !done || !ids_out || !parents_out || !status) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: null argument");
         if (!d->paged) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: needs a cache (mfqb_decoder_set_cache)");
         const int rows = d->cache.rows;
+        if (d->weights || d->dropped) fail(MFQB_ERR_UNSUPPORTED, "mfqb_decoder_beam_step: weights are attached, which do not move with sequences");
         if (beams < 1 || rows % beams) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: %d sequences do not make groups of %d beams", rows, beams);
         check_ready(d, rows, "mfqb_decoder_beam_step");
         DeviceGuard guard(d->device);
@@ -1103,7 +1158,7 @@ int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, fl
         launch_dep(beam_begin_kernel, dim3(1), dim3(1024), s, static_cast<const int*>(done), static_cast<const int*>(d->cache.lens), rows,
                    d->cache.width * d->cache.page, counts, counts + rows, counts + 2 * rows);
         check(mfqb_cache_extend(&d->cache, counts, status, s));
-        single_nodes(d);
+        single_nodes(d, s);
         d->write_to.lens = counts + rows;
         d->read_from.lens = counts + 2 * rows;
         forward_logits(d, ids_in, rows, s);
@@ -1129,7 +1184,7 @@ int mfqb_decoder_layer(mfqb_decoder* d, int layer, const float* h_in, int rows, 
         if (d->paged && rows != d->cache.rows) fail(MFQB_ERR_ARG, "mfqb_decoder_layer: the cache has %d sequences, got %d rows", d->cache.rows, rows);
         if (!d->paged && d->cfg.max_ctx < 1) fail(MFQB_ERR_ARG, "mfqb_decoder_layer: the decoder has no cache of its own (max_ctx 0) and none is attached");
         MFQB_CUDA(cudaMemcpyAsync(d->h.p, h_in, bytes, cudaMemcpyDeviceToDevice, stream));
-        single_nodes(d);
+        single_nodes(d, stream);
         if (!d->paged) launch_rope_table(d, rows, stream);
         const float* delta = layer_forward(d, layer, rows, nullptr, stream);
         // fold the FFN output in with a norm whose bf16 output is discarded

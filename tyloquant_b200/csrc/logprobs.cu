@@ -41,6 +41,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float one_if_ge(float a, float b) {
+    float r;
+    asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ unsigned long long lp_key(float z, int token) { return (unsigned long long)ordered_f32(z) << 32 | (0xFFFFFFFFu - (unsigned)token); }
 
 // 16 bytes of logits as float32.
@@ -139,8 +144,8 @@ __device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
 // best: a bound that at least k logits reach comes from the maxima of 64 groups of threads (the k-th largest of them), and only the
 // vectors of threads whose own maximum reaches it are read again, a warp for each of those threads.  Where too many logits reach the
 // bound (equal ones, or all in a few threads' vectors) the cut is searched by counting instead.
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+template <typename T, int PER_SM>
+__global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int kN = LpVec<T>::kN;
     __shared__ LogprobShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -165,71 +170,84 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const __grid_co
     // A logit comes before the token's own if it is larger, or equal with a lower number.
     const float zt = there ? lp_float(z[token]) + 0.f : INFINITY;
     const float above = unordered_f32(ordered_f32(zt) + 1u);
-    LogprobSum s = {kLpLowest, 0.f, 0.f, 0};
-    uint64_t sum = 0ull, moment = 0ull;   // of the even and the odd ones of a vector
-    float most = -INFINITY;
-    uint4 next[kLpBatch];
-    auto ask = [&](int v0) {
-#pragma unroll
-        for (int u = 0; u < kLpBatch; ++u) {
-            if (v0 + u * kLpThreads < last) next[u] = fetch(v0 + u * kLpThreads);
-        }
-    };
-    ask(first + tid);
-    for (int v0 = first + tid; v0 < last; v0 += kLpThreads * kLpBatch) {
-        float x[kLpBatch][kN];
-#pragma unroll
-        for (int u = 0; u < kLpBatch; ++u) {
-            if (v0 + u * kLpThreads < last) {
-                LpVec<T>::widen(next[u], x[u]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kN; ++e) x[u][e] = -INFINITY;
-            }
-        }
-        ask(v0 + kLpThreads * kLpBatch);   // on its way while this one is worked on
+    // Of the CTA's vectors, those that lie wholly in the row are shared out over the threads; the row's ends go to two of them.
+    const bool head = first == 0 && skew > 0 && first < last, tail = last == vectors && (skew + a.vocab) % kN && !(head && last == 1) && first < last;
+    const int in0 = first + head, in1 = last - tail;
+    float high_of = kLpLowest, most = -INFINITY;   // what the sums are of; the largest of all
+    uint64_t sum = 0ull, moment = 0ull, before = 0ull;   // of the even and the odd ones of a vector
+    const int token_at = there ? (token + skew) / kN : -1;   // the token's vector; its own equals before the token are added below
+    auto take = [&](const auto& x, int v0, int step) {   // vectors v0, v0 + step ..
+        constexpr int kVectors = sizeof(x) / sizeof(x[0]);
         float high = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kLpBatch; ++u)
+        for (int u = 0; u < kVectors; ++u)
 #pragma unroll
             for (int e = 0; e < kN; ++e) high = fmaxf(high, x[u][e]);
         most = fmaxf(most, high);
-        if (high > s.top) {
-            const float d = fmaxf(s.top - high, kLpNone), f = exp2_approx(d * kLog2e);
+        if (high > high_of) {
+            const float d = fmaxf(high_of - high, kLpNone), f = exp2_approx(d * kLog2e);
             moment = fma_f32x2(fma_f32x2(pair_f32(d, d), sum, moment), pair_f32(f, f), 0ull);
             sum = fma_f32x2(sum, pair_f32(f, f), 0ull);
-            s.top = high;
+            high_of = high;
         }
-        const uint64_t down = pair_f32(-s.top, -s.top);
+        const uint64_t down = pair_f32(-high_of, -high_of), log2e = pair_f32(kLog2e, kLog2e);
 #pragma unroll
-        for (int u = 0; u < kLpBatch; ++u) {
-            const int at = (v0 + u * kLpThreads) * kN - skew;
-            if (v0 + u * kLpThreads >= last) break;
+        for (int u = 0; u < kVectors; ++u) {
+            const float line = v0 + u * step < token_at ? zt : above;
 #pragma unroll
             for (int e = 0; e < kN; e += 2) {
                 const float2 d = split_f32(add_f32x2(pair_f32(x[u][e], x[u][e + 1]), down));
                 const uint64_t dd = pair_f32(max_nan(d.x, kLpNone), max_nan(d.y, kLpNone));
-                const float2 y = split_f32(fma_f32x2(dd, pair_f32(kLog2e, kLog2e), 0ull));
+                const float2 y = split_f32(fma_f32x2(dd, log2e, 0ull));
                 const uint64_t p = pair_f32(exp2_approx(y.x), exp2_approx(y.y));
                 sum = add_f32x2(sum, p);
                 moment = fma_f32x2(p, dd, moment);
-            }
-            if (at + kN <= token || at > token) {
-                const float line = at > token ? above : zt;
-#pragma unroll
-                for (int e = 0; e < kN; ++e) s.before += x[u][e] >= line;
-            } else {
-#pragma unroll
-                for (int e = 0; e < kN; ++e) s.before += x[u][e] >= (at + e < token ? zt : above);
+                before = add_f32x2(before, pair_f32(one_if_ge(x[u][e], line), one_if_ge(x[u][e + 1], line)));   // at most vocab of them
             }
         }
-    }
-    if (first + tid == 0 && first < last && there && zt == -INFINITY) s.before -= skew;   // minus infinities that are not the row's
+    };
     {
-        const float2 x = split_f32(sum), y = split_f32(moment);
-        s.sum = x.x + x.y;
-        s.moment = y.x + y.y;
+        const uint4* at = reinterpret_cast<const uint4*>(z - skew) + in0 + tid;   // may point behind the row where there is nothing to read
+        const int mine = in0 + tid < in1 ? (in1 - in0 - tid + kLpThreads - 1) / kLpThreads : 0, batches = mine / kLpBatch;
+        uint4 next[kLpBatch];
+        auto ask = [&](int from) {
+#pragma unroll
+            for (int u = 0; u < kLpBatch; ++u) next[u] = __ldcg(at + (from + u) * kLpThreads);
+        };
+        if (batches) ask(0);
+        for (int i = 0; i < batches; ++i) {
+            float x[kLpBatch][kN];
+#pragma unroll
+            for (int u = 0; u < kLpBatch; ++u) LpVec<T>::widen(next[u], x[u]);
+            if (i + 1 < batches) ask((i + 1) * kLpBatch);   // on its way while this one is worked on
+            take(x, in0 + tid + i * kLpBatch * kLpThreads, kLpThreads);
+        }
+        const int left = mine - batches * kLpBatch;
+#pragma unroll
+        for (int u = 0; u < kLpBatch - 1; ++u)
+            if (u < left) next[u] = __ldcg(at + (batches * kLpBatch + u) * kLpThreads);
+#pragma unroll
+        for (int u = 0; u < kLpBatch - 1; ++u)
+            if (u < left) {
+                float x[1][kN];
+                LpVec<T>::widen(next[u], x[0]);
+                take(x, in0 + tid + (batches * kLpBatch + u) * kLpThreads, kLpThreads);
+            }
+        const int end = tid == 0 && head ? 0 : tid == 1 && tail ? vectors - 1 : -1;
+        if (end >= 0) {
+            float x[1][kN];
+            load(end, x[0]);
+            take(x, end, 0);
+        }
     }
+    LogprobSum s;
+    {
+        const float2 x = split_f32(sum), y = split_f32(moment), n = split_f32(before);
+        s = LogprobSum{high_of, x.x + x.y, y.x + y.y, (int)n.x + (int)n.y};
+    }
+    if (zt == -INFINITY && tid == 0 && head && token_at > 0) s.before -= skew;   // minus infinities that are not the row's
+    if (tid == 0 && token_at >= first && token_at < last)
+        for (int i = max(0, token_at * kN - skew); i < token; ++i) s.before += lp_float(z[i]) == zt;
     // ---- the CTA's sums
     LogprobSum joint = s;
     for (int o = 16; o > 0; o >>= 1) joint = lp_shuffle_join(joint, o);
@@ -256,11 +274,14 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const __grid_co
         }
         __syncthreads();
         const float bound = sh.bound;
-        if (first + tid < last && most >= bound) sh.hot[atomicAdd(&sh.hots, 1)] = tid;
+        if (most >= bound && (in0 + tid < in1 || (tid == 0 && head) || (tid == 1 && tail))) sh.hot[atomicAdd(&sh.hots, 1)] = tid;
         __syncthreads();
         const int hots = sh.hots;
         for (int h = warp; h < hots; h += kLpWarps) {
-            for (int v = first + sh.hot[h] + lane * kLpThreads; v < last; v += 32 * kLpThreads) {
+            const int thread = sh.hot[h], end = thread == 0 && head ? 0 : thread == 1 && tail ? vectors - 1 : -1;
+            const int count = (in0 + thread < in1 ? (in1 - in0 - thread + kLpThreads - 1) / kLpThreads : 0) + (end >= 0);
+            for (int i = lane; i < count; i += 32) {
+                const int v = end >= 0 && i == count - 1 ? end : in0 + thread + i * kLpThreads;
                 float x[kN];
                 load(v, x);
                 const int at = v * kN - skew;
@@ -295,10 +316,12 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const __grid_co
             if (tid == 0) sh.count = 0;
             __syncthreads();
             each([&](unsigned k, int token) {
-                if (cut.in(k, token)) sh.list[atomicAdd(&sh.count, 1)] = (unsigned long long)k << 32 | (0xFFFFFFFFu - (unsigned)token);   // a.top of them
+                if (!cut.in(k, token)) return;
+                const int i = atomicAdd(&sh.count, 1);   // a.top of them; the bounds are for logits that change meanwhile
+                if (i < kLpList) sh.list[i] = (unsigned long long)k << 32 | (0xFFFFFFFFu - (unsigned)token);
             });
             __syncthreads();
-            n = sh.count;
+            n = min(sh.count, kLpList);
         }
         // ---- the list in order: every key counts those above it
         const int keep = min(n, a.top);
@@ -365,10 +388,12 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     int device = 0;
     MFQB_CUDA(cudaGetDevice(&device));
     static std::once_flag once[64];
-    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); });
-    // CTAs of a row: until there are four for every SM, as long as a slice has a batch of vectors for every thread.
+    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, 3>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); });
+    // CTAs of a row: as many as are on the SMs at once, as long as a slice has a batch of vectors for every thread (77 rows of 32001 in bf16: 9.0 us with 4,
+    // 15.9 with 8, of which not all fit).  Rows that fill the SMs several times over have four CTAs on an SM, which read more at a time (1024 rows
+    // of 128256 in float32: 95 us, 110 with three), others three, with more registers (one row: 9.7 us, 10.3 with four).
     int ctas = 1;
-    while (ctas < kLpCtas && (int64_t)rows * ctas < 4 * 148 && a.vocab / (2 * ctas) >= kLpThreads * kLpBatch) ctas *= 2;
+    while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= 3 * 148 && a.vocab / (2 * ctas) >= kLpThreads * kLpBatch) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ctas);
     cfg.blockDim = dim3(kLpThreads);
@@ -381,7 +406,7 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    MFQB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a));
+    MFQB_CUDA(cudaLaunchKernelEx(&cfg, rows > 3 * 148 ? logprobs_kernel<T, 4> : logprobs_kernel<T, 3>, a));
 }
 
 }  // namespace mfqb

@@ -69,7 +69,8 @@ __device__ Cut select_cut(int want, unsigned low, unsigned high, int places, Cut
     unsigned base = __reduce_min_sync(0xffffffffu, sh.low[lane % kWarps]);
     unsigned range = __reduce_max_sync(0xffffffffu, sh.high[lane % kWarps]) - base;   // keys base .. base + range
     unsigned tied = 0;   // the key whose places are being sorted out, the first one the largest
-    for (;;) {
+    // At most three rounds by key and three by place.  The count is also what ends the search when keys change while it is under way.
+    for (int round = 0; round < 6; ++round) {
         const int shift = max(0, 21 - __clz(range | 1u));   // range >> shift is below 2048
         int4* own_bins = reinterpret_cast<int4*>(sh.bins + kCutBins - kOwn * ((int)threadIdx.x + 1));   // from the last one down
 #pragma unroll
@@ -117,8 +118,10 @@ __device__ Cut select_cut(int want, unsigned low, unsigned high, int places, Cut
             if (threadIdx.x == 0) sh.at = 0;
             __syncthreads();
             each([&](unsigned k, int place) {
-                if (tied ? k == tied && ~(unsigned)place - base <= range : k - base <= range)
-                    sh.few[atomicAdd(&sh.at, 1)] = (unsigned long long)k << 32 | ~(unsigned)place;
+                if (tied ? k == tied && ~(unsigned)place - base <= range : k - base <= range) {
+                    const int i = atomicAdd(&sh.at, 1);
+                    if (i < kCutFew) sh.few[i] = (unsigned long long)k << 32 | ~(unsigned)place;
+                }
             });
             __syncthreads();
             if ((int)threadIdx.x < inside) {
@@ -157,6 +160,7 @@ __device__ Cut select_cut(int want, unsigned low, unsigned high, int places, Cut
         }
         __syncthreads();
     }
+    return Cut{0xFFFFFFFFu, -1};
 }
 
 }  // namespace mfqb

@@ -57,7 +57,11 @@ struct WeighWalk {
         fresh = true;
         if (++kvh < a.kv_heads) return;
         kvh = 0;
-        seq = tree_seq(a, ++r);
+        if (++r >= a.rows) {   // only where lengths change meanwhile
+            left = 0;
+            return;
+        }
+        seq = tree_seq(a, r);
     }
 };
 

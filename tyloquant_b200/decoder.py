@@ -21,7 +21,7 @@ class Decoder:
         self.rank, self.world, self.device = rank, world, device
         self._comm = comm
         self._keep = []   # the weights are borrowed by the native object: keep them alive here
-        self._cache = None
+        self._cache, self._beside = None, None
         self._h = C.c_void_p()
         check(lib.mfqb_decoder_create(C.byref(self.cfg), rank, world, comm._h if comm is not None else None, device, C.byref(self._h)))
 
@@ -79,12 +79,26 @@ class Decoder:
         check(lib.mfqb_decoder_read_logits(self._h, rows, out.data_ptr(), _stream_ptr(self.device)))
         return out
 
-    def set_cache(self, cache) -> None:
+    def set_cache(self, cache, weights=None, dropped=None) -> None:
         """Runs over a :class:`PagedCache` from here on (``None``: over the decoder's own cache again); a row per sequence.  ``max_ctx=0`` at
         creation leaves the decoder without a cache of its own.  The decoder keeps the cache alive while it is attached; a graph that was
-        captured over it needs it as long as it is replayed."""
+        captured over it needs it as long as it is replayed.
+
+        ``weights`` (``cache.new_weights()``): every pass adds up in them how much each position was looked at, for ``cache.evict``.  ``dropped`` (int32
+        [rows]): what has been evicted of every sequence so far, added to its positions; add to it what ``evict`` returns.  Both are kept
+        alive like the cache; ``beam_step`` is refused with them."""
+        from .cache import _need
+        torch = _torch()
+        if cache is None and (weights is not None or dropped is not None):
+            raise ValueError("weights and dropped go with a cache")
+        if weights is not None:
+            cache._weights(weights)
+        if dropped is not None and _need(dropped, torch.int32, (cache.rows,), self.device, "dropped") is not dropped:
+            raise ValueError("dropped must be contiguous")
         check(lib.mfqb_decoder_set_cache(self._h, None if cache is None else C.byref(cache._view)))
-        self._cache = cache   # borrowed by the native object
+        self._cache, self._beside = cache, (weights, dropped)   # borrowed by the native object
+        if weights is not None or dropped is not None:
+            check(lib.mfqb_decoder_set_weights(self._h, None if weights is None else weights.data_ptr(), None if dropped is None else dropped.data_ptr()))
 
     def _rows(self, t, shape, dtype, what):
         from .cache import _need
