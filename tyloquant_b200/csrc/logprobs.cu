@@ -144,6 +144,9 @@ __device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
 // best: a bound that at least k logits reach comes from the maxima of 64 groups of threads (the k-th largest of them), and only the
 // vectors of threads whose own maximum reaches it are read again, a warp for each of those threads.  Where too many logits reach the
 // bound (equal ones, or all in a few threads' vectors) the cut is searched by counting instead.
+// Sums are float32, a thread's own of some hundred terms each, joined in a tree: log probabilities are off by about 1e-7 of themselves.  Many rows: bound by memory
+// and by issue (1024 rows of 128256 in float32: 95 us, 5.5 TB/s, 12 instructions a logit; with checks of the row's ends in the loop, 19 and 110 us).  One row: a
+// chain of trips (9.7 us: the logits, the hot threads' vectors again, the cluster's lists).
 template <typename T, int PER_SM>
 __global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int kN = LpVec<T>::kN;

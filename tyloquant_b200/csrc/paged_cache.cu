@@ -343,7 +343,8 @@ __device__ __forceinline__ uint2 rope_pack(float a, float b, float c, float d) {
 // How a thread's four pairs of a head lie: pairs (2j, 2j + 1); pairs (j, j + P) with P a multiple of four; with any P.
 enum RopeForm { kRopeNeighbours, kRopeHalves4, kRopeHalves };
 
-// cache_write_kernel's work for P <= 64 pairs, in other layouts and with a factor on what is turned.  Dims from 2P on pass, as pairs of neighbours: a head
+// cache_write_kernel's work for P <= 64 pairs, in other layouts and with a factor on what is turned.  (That one stays for whole heads in halves: 6.5 us where this takes 6.9,
+// for 64 nodes of 16 sequences with 48 heads in float32, and its sums round as they did; neighbouring pairs 7.0, any other number of pairs 10.3.)  Bound by memory.  Dims from 2P on pass, as pairs of neighbours: a head
 // has 64 pairs in all, of which thread t of 16 takes 4t .. 4t + 3 (kRopeHalves: t, t + 16, ..).
 template <typename T, RopeForm FORM>
 __global__ void __launch_bounds__(256) cache_rope_kernel(mfqb_cache c, int layer, const T* qkv, int hq, int nodes, const int* depths, const double* freqs, int pairs, float factor,

@@ -11,6 +11,8 @@ constexpr uint64_t kScoreBytes = 512ull << 20;     // as long as they take at mo
 constexpr int kWeighRows = 256;                    // rows of a pass over the keys
 constexpr int kWeighRing = 4, kWeighGroups = 4, kWeighThreads = 64 + 128 * kWeighGroups;   // a loader, an issuer, groups of four warps that sum
 
+// Scores are four bytes a row and position, written and read once: up to 32 rows that is less than the 256 bytes of a key, which the other form reads again; up
+// to 64 it saves a launch (kept: 1 to 3 us of the attention's time, the sums beside its merge).
 int64_t tree_score_stride(const mfqb_cache& c, int q_heads, int nodes) {
     const int64_t m_rows = (int64_t)nodes * (q_heads / c.kv_heads), stride = ((int64_t)c.width * c.page + kTile - 1) / kTile * kTile;
     return m_rows <= kScoreRows && 4ull * c.rows * c.kv_heads * m_rows * stride <= kScoreBytes ? stride : 0;
@@ -34,25 +36,39 @@ struct WeighShared {
 constexpr size_t kWeighSmem = (size_t)kWeighRing * kTileBytes + (size_t)kWeighRows * kHeadDim * 2 + sizeof(WeighShared);
 static_assert(kWeighSmem <= 227 * 1024, "shared memory of an SM");
 
-// A CTA's tiles in order: sequence, kv head, tile of 128 positions.
+// What tiles with nodes, which not every row sees, take in units of the others: they are shared out so (27 nodes of 13 sequences,
+// with the attention: 42 us, 48 with even shares).
+constexpr int kWeighNodes = 4;
+
+// A CTA's tiles in order: sequence, kv head, tile of 128 positions.  A tile belongs to the CTA in whose units its first one lies.
 struct WeighWalk {
     int r, kvh, t;
-    int64_t left;
-    bool fresh;   // the tile is the first of its head here
+    int64_t left;   // units from the head's first one to the CTA's last
+    bool fresh;     // the tile is the first of its head here
     TreeSeq seq;
+    static __device__ __forceinline__ int unit_of(const TreeSeq& s, int t) { return t + (kWeighNodes - 1) * max(0, t - s.len / kTile); }
+    static __device__ __forceinline__ int units_of(const TreeSeq& s) { return unit_of(s, s.tiles); }
     __device__ __forceinline__ void start(const TreeArgs& a, const WeighShared& sh) {
         left = sh.last - sh.first;
-        fresh = true;
         if (left <= 0) return;
         r = sh.row0;
         seq = tree_seq(a, r);
-        kvh = (int)quotient(sh.off, seq.tiles);
-        t = (int)(sh.off - (int64_t)kvh * seq.tiles);
+        const int units = units_of(seq);
+        kvh = (int)quotient(sh.off, units);
+        const int u0 = (int)(sh.off - (int64_t)kvh * units), plain = seq.len / kTile;
+        left += u0;
+        t = (u0 <= plain ? u0 : plain + (u0 - plain + kWeighNodes - 1) / kWeighNodes) - 1;
+        next(a);
+        fresh = true;
     }
     __device__ __forceinline__ void next(const TreeArgs& a) {
         fresh = false;
-        if (--left <= 0) return;
-        if (++t < seq.tiles) return;
+        if (++t < seq.tiles) {
+            if (unit_of(seq, t) >= left) left = 0;
+            return;
+        }
+        left = max(left - units_of(seq), (int64_t)0);
+        if (left == 0) return;
         t = 0;
         fresh = true;
         if (++kvh < a.kv_heads) return;
@@ -106,7 +122,14 @@ __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shif
 }
 
 // From the keys, by rows row0 .. row0 + rows of Q: S^T = K Q^T puts a position into each lane of tensor memory, so that the sum over the rows stays in
-// a thread.  One warp asks for the pages' keys, one issues tcgen05.mma, two groups of four warps take the tiles in turns.
+// a thread, and a tile of 128 positions is one product for up to 256 rows.  One warp asks for the pages' keys (a look into the table two tiles ahead: without it 8 us more
+// of 280), one issues tcgen05.mma, and of sixteen that sum a group of four has a half of the rows of every other tile; the second halves' sums
+// wait in shared memory until the first group's next tile.
+// weight = exp2(scale' s + shift), shift = - m - log2(l): one number per row, read from shared memory by all threads at once (two, m and 1 / l, made
+// it 8 us more; a shift of size 2^5 is off by 2^-20, the weight by 2^-20.5 of itself).
+// Bound by latency: the chain product - scores out of tensor memory (some 500 clocks a load) - exponentials - hand-over, with two tiles of scores in flight.  4
+// sequences at 32768 positions, 64 nodes in groups of 4, 8 kv heads: 124 us where the exponentials' unit needs 62 and the keys 41.  Eight warps with
+// loads of 32 rows ahead took 133 to 143, products of 128 rows each in four places 122 to 131 with slower short batches.
 __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap, int row0, int rows) {
     extern __shared__ __align__(1024) unsigned char ring[];
     unsigned char* q_tile = ring + (size_t)kWeighRing * kTileBytes;   // two halves of 64 dims, kWeighRows rows of 128 bytes each
@@ -138,7 +161,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
         int64_t tiles_of[kEach], mine = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            tiles_of[j] = kEach * tid + j < a.rows ? (int64_t)tree_seq(a, kEach * tid + j).tiles * a.kv_heads : 0;
+            tiles_of[j] = kEach * tid + j < a.rows ? (int64_t)WeighWalk::units_of(tree_seq(a, kEach * tid + j)) * a.kv_heads : 0;
             mine += tiles_of[j];
         }
         int64_t upto = mine;

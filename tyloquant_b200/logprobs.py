@@ -38,9 +38,10 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     z = logits if logits.stride(1) == 1 and logits.stride(0) >= vocab else logits.contiguous()
     t = _need(tokens, torch.int32, (rows,), dev, "tokens")
     top = int(top)
-    logprob, rank = z.new_empty((rows,), dtype=torch.float32), z.new_empty((rows,), dtype=torch.int32)
-    entropy = torch.empty_like(logprob)
-    top_logprobs, top_tokens = z.new_empty((rows, max(top, 0)), dtype=torch.float32), z.new_empty((rows, max(top, 0)), dtype=torch.int32)
+    # the host's part of a call is mostly these; sizes in positions and the type of a tensor at hand are the cheapest forms
+    logprob = z.new_empty(rows) if dtype == F32 else z.new_empty(rows, dtype=torch.float32)
+    entropy, rank = torch.empty_like(logprob), torch.empty_like(t)
+    top_logprobs, top_tokens = logprob.new_empty(rows, max(top, 0)), t.new_empty(rows, max(top, 0))
     if rows:
         _call(_fast.token_logprobs, dev, z.data_ptr(), dtype, rows, vocab, z.stride(0), t.data_ptr(), top, logprob.data_ptr(), entropy.data_ptr(),
               rank.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr())
