@@ -64,6 +64,8 @@ def rope_frequencies(theta: float = 500000.0, device="cuda", *, dims: int = HEAD
         return f / factor
     if scaling not in ("bands", "yarn"):
         raise ValueError(f"scaling must be None, 'linear', 'bands' or 'yarn', got {scaling!r}")
+    if scaling == "yarn" and not theta > 1.0:
+        raise ValueError(f"theta must be above 1, got {theta}")
     if original is None or original < 1:
         raise ValueError(f"{scaling!r} needs the original context length")
     high = high if high is not None else 4.0 if scaling == "bands" else 32.0

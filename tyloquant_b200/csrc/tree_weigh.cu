@@ -122,8 +122,8 @@ __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shif
 }
 
 // From the keys, by rows row0 .. row0 + rows of Q: S^T = K Q^T puts a position into each lane of tensor memory, so that the sum over the rows stays in
-// a thread, and a tile of 128 positions is one product for up to 256 rows.  One warp asks for the pages' keys (a look into the table two tiles ahead: without it 8 us more
-// of 280), one issues tcgen05.mma, and of sixteen that sum a group of four has a half of the rows of every other tile; the second halves' sums
+// a thread, and a tile of 128 positions is one product for up to 256 rows.  One warp asks for the pages' keys (a look into the table two tiles ahead: 3 us of
+// 280), one issues tcgen05.mma, and of sixteen that sum a group of four has a half of the rows of every other tile; the second halves' sums
 // wait in shared memory until the first group's next tile.
 // weight = exp2(scale' s + shift), shift = - m - log2(l): one number per row, read from shared memory by all threads at once (two, m and 1 / l, made
 // it 8 us more; a shift of size 2^5 is off by 2^-20, the weight by 2^-20.5 of itself).
