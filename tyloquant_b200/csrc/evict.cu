@@ -161,17 +161,19 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(mfqb_cache c, f
     };
     if (b > 0) {
         const int fours = (older + 3) / 4;
-        unsigned low = 0xFFFFFFFFu, high = 0u;
+        unsigned low = 0xFFFFFFFFu, high = 0u, above = 0xFFFFFFFFu;
 #pragma unroll 2
         for (int i = tid; i < fours; i += kEvictThreads) {
             const uint4 k = read(i);
             if (CACHED) s_keys[i] = k;
             low = min(min(low, k.x - 1u), min(k.y - 1u, min(k.z - 1u, k.w - 1u)));   // less 1, so that none is the largest
             high = max(max(high, k.x), max(k.y, max(k.z, k.w)));
+            above = min(min(above, k.x - kCutZero - 1u), min(k.y - kCutZero - 1u, min(k.z - kCutZero - 1u, k.w - kCutZero - 1u)));   // what is not above zero wraps
         }
         if (low != 0xFFFFFFFFu) ++low;
+        above = above < kCutZero - 1u ? above + kCutZero + 1u : 0xFFFFFFFFu;
         if (CACHED) sync_all();   // no CTA moves weights that another one has not read
-        const Cut cut = select_cut<kEvictThreads>(b, low, high, older, sh.cut, [&](auto f) {
+        const Cut cut = select_cut<kEvictThreads>(b, low, high, above, older, sh.cut, [&](auto f) {
 #pragma unroll 2
             for (int i = tid; i < fours; i += kEvictThreads) {
                 const uint4 k = keys(i);

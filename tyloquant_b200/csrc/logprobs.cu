@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __gr
                 low = min(low, k);
                 high = max(high, k);
             });
-            const Cut cut = select_cut<kLpThreads>(a.top, low, high, a.vocab, sh.cut, each);
+            const Cut cut = select_cut<kLpThreads>(a.top, low, high, 0xFFFFFFFFu, a.vocab, sh.cut, each);
             __syncthreads();
             if (tid == 0) sh.count = 0;
             __syncthreads();

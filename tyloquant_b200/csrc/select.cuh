@@ -39,11 +39,12 @@ struct Cut {
     __device__ __forceinline__ bool in(unsigned k, int place) const { return k > key || (k == key && place <= last); }
 };
 constexpr int kCutBins = 2048, kCutFew = 64;
+constexpr unsigned kCutZero = 0x80000000u;   // ordered_f32(0)
 struct CutShared {
     alignas(16) int bins[kCutBins];
     alignas(16) unsigned long long few[kCutFew];
     int sums[33], at, left, inside;
-    unsigned low[32], high[32];
+    unsigned low[32], high[32], above[32];
     Cut cut;
 };
 
@@ -51,32 +52,43 @@ struct CutShared {
 // thread's share of the keys, the same ones every time, at places 0 .. places - 1; a key 0 is none.  low and high are the smallest and the
 // largest of the thread's (all ones and 0 where there are none).  Bins divide the range from the smallest to the largest key: float32 values
 // that span orders of magnitude lie in many of them (by the first bits of the keys they would meet in a few counters, whose additions
-// wait for one another), and three rounds of 11 bits are enough for any range.  A round ends the search when all of its last bin is in, or
+// wait for one another), and three rounds of 11 bits are enough for any range.  Weights are mostly positive with some zeros, far below the others in this
+// order: the first round's first bin has all that is not above zero, the others divide the rest.  A round ends the search when all of its last bin is in, or
 // when that holds so few keys that they are better counted against each other.  The next one goes by what the keys of the bin span; where
 // they are equal, by their places.
 template <int THREADS, class Each>
-__device__ Cut select_cut(int want, unsigned low, unsigned high, int places, CutShared& sh, Each each) {
-    static_assert(kCutBins % (4 * THREADS) == 0 && kCutFew <= THREADS, "bins of a thread");
+__device__ Cut select_cut(int want, unsigned low, unsigned high, unsigned above, int places, CutShared& sh, Each each) {
+    static_assert(kCutBins % (4 * THREADS) == 0 && 2 * kCutFew <= THREADS, "bins of a thread");
     constexpr int kOwn = kCutBins / THREADS, kWarps = THREADS / 32;
     const int lane = threadIdx.x & 31;
     low = __reduce_min_sync(0xffffffffu, low);
     high = __reduce_max_sync(0xffffffffu, high);
+    above = __reduce_min_sync(0xffffffffu, above);
     if (lane == 0) {
         sh.low[threadIdx.x >> 5] = low;
         sh.high[threadIdx.x >> 5] = high;
+        sh.above[threadIdx.x >> 5] = above;
     }
     __syncthreads();
     unsigned base = __reduce_min_sync(0xffffffffu, sh.low[lane % kWarps]);
+    above = __reduce_min_sync(0xffffffffu, sh.above[lane % kWarps]);   // the smallest one above zero
     unsigned range = __reduce_max_sync(0xffffffffu, sh.high[lane % kWarps]) - base;   // keys base .. base + range
+    bool split = base <= kCutZero && above != 0xFFFFFFFFu;   // the first round
     unsigned tied = 0;   // the key whose places are being sorted out, the first one the largest
-    // At most three rounds by key and three by place.  The count is also what ends the search when keys change while it is under way.
-    for (int round = 0; round < 6; ++round) {
-        const int shift = max(0, 21 - __clz(range | 1u));   // range >> shift is below 2048
+    // At most four rounds by key (three, and one that splits at zero) and three by place.  The count is also what ends the search when keys change while it is under way.
+    for (int round = 0; round < 7; ++round) {
+        // range >> shift is below 2048, or, of what is above zero, below 2047
+        const int shift = split ? max(0, 21 - __clz((base + range - above) | 1u)) + ((base + range - above) >> max(0, 21 - __clz((base + range - above) | 1u)) == 2047u)
+                                : max(0, 21 - __clz(range | 1u));
         int4* own_bins = reinterpret_cast<int4*>(sh.bins + kCutBins - kOwn * ((int)threadIdx.x + 1));   // from the last one down
 #pragma unroll
         for (int j = 0; j < kOwn / 4; ++j) own_bins[j] = make_int4(0, 0, 0, 0);
         __syncthreads();
-        if (!tied) {
+        if (split) {
+            each([&](unsigned k, int) {
+                if (k) atomicAdd(&sh.bins[k >= above ? min((k - above) >> shift, 2046u) + 1 : 0u], 1);
+            });
+        } else if (!tied) {
             each([&](unsigned k, int) {
                 if (k - base <= range) atomicAdd(&sh.bins[(k - base) >> shift], 1);
             });
@@ -110,9 +122,14 @@ __device__ Cut select_cut(int want, unsigned low, unsigned high, int places, Cut
         __syncthreads();
         want = sh.left;
         const int inside = sh.inside;
-        base += (unsigned)sh.at << shift;
+        if (split && sh.at == 0) {
+            range = kCutZero - base;
+        } else {
+            base = split ? above + ((unsigned)(sh.at - 1) << shift) : base + ((unsigned)sh.at << shift);
+            range = (1u << shift) - 1u;
+        }
+        split = false;
         if (want == inside) return tied ? Cut{tied, (int)~base} : Cut{base - 1u, -1};   // no key of a value is 0
-        range = (1u << shift) - 1u;
         if (inside <= kCutFew) {
             __syncthreads();
             if (threadIdx.x == 0) sh.at = 0;
@@ -124,13 +141,15 @@ __device__ Cut select_cut(int want, unsigned low, unsigned high, int places, Cut
                 }
             });
             __syncthreads();
-            if ((int)threadIdx.x < inside) {
-                const unsigned long long x = sh.few[threadIdx.x];
-                int above = 0;
-#pragma unroll 4
-                for (int i = 0; i < inside; ++i) above += sh.few[i] > x;
-                if (above == want - 1) sh.cut = Cut{(unsigned)(x >> 32), (int)~(unsigned)x};
-            }
+            // Two or four threads count for a key.
+            const int each_key = inside <= THREADS / 4 ? 4 : 2, at = threadIdx.x / each_key, from = threadIdx.x % each_key;
+            int larger = 0;
+            const unsigned long long x = sh.few[min(at, kCutFew - 1)];
+            if (at < inside)
+                for (int i = from; i < inside; i += each_key) larger += sh.few[i] > x;
+            larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+            if (each_key == 4) larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+            if (at < inside && larger == want - 1) sh.cut = Cut{(unsigned)(x >> 32), (int)~(unsigned)x};
             __syncthreads();
             return sh.cut;
         }
