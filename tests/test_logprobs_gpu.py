@@ -59,10 +59,11 @@ def test_by_vocabulary(vocab, dtype):
 
 @pytest.mark.parametrize("rows", [1, 2, 5, 18, 19, 37, 74, 148, 296, 600])
 def test_by_rows(rows):
-    """Few rows are split over clusters of up to 16 CTAs."""
+    """Few rows are split over clusters of two CTAs, and longer ones of up to eight."""
     rng = np.random.default_rng(rows)
-    z = torch.from_numpy(2.5 * rng.standard_normal((rows, 33000), dtype=np.float32)).to(DEV)
-    _check(z, _tokens(rng, rows, 33000), 20)
+    for vocab in (33000, 70000, 130000) if rows <= 74 else (33000,):
+        z = torch.from_numpy(2.5 * rng.standard_normal((rows, vocab), dtype=np.float32)).to(DEV)
+        _check(z, _tokens(rng, rows, vocab), 20)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])

@@ -1,14 +1,13 @@
 // Log probabilities of given tokens, with entropy, rank and the best alternatives: one pass over the logits.
 #include <cuda_fp16.h>
 
-#include <mutex>
 
 #include "select.cuh"
 #include "tc05.cuh"
 
 namespace mfqb {
 
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4, kLpCtas = 16;
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4, kLpCtas = 8;
 constexpr int kLpVocab = 1 << 20;
 
 struct LogprobArgs {
@@ -145,8 +144,8 @@ __device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
 // vectors of threads whose own maximum reaches it are read again, a warp for each of those threads.  Where too many logits reach the
 // bound (equal ones, or all in a few threads' vectors) the cut is searched by counting instead.
 // Sums are float32, a thread's own of some hundred terms each, joined in a tree: log probabilities are off by about 1e-7 of themselves.  Many rows: bound by memory
-// and by issue (1024 rows of 128256 in float32: 95 us, 5.5 TB/s, 12 instructions a logit; with checks of the row's ends in the loop, 19 and 110 us).  One row: a
-// chain of trips (9.7 us: the logits, the hot threads' vectors again, the cluster's lists).
+// and by issue (1024 rows of 128256 in float32: 95 us, 5.5 TB/s, 12 instructions a logit; with checks of the ends of a row in the loop 19 instructions and 111 us).  One row: a
+// chain of trips (7.6 us: the logits, the hot threads' vectors again, the cluster's lists).
 template <typename T, int PER_SM>
 __global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int kN = LpVec<T>::kN;
@@ -356,7 +355,7 @@ __global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __gr
                 for (int o = ctas / 2; o > 0; o >>= 1) line = min(line, __shfl_xor_sync(0xffffffffu, line, o));
                 for (int i = tid; i < (int)ctas * kLpTop; i += kLpThreads) {
                     const unsigned long long key = sh.gathered[i / kLpTop][i % kLpTop];
-                    if (key && key >= line) sh.list[atomicAdd(&sh.count, 1)] = key;   // at most 16 lists of 32
+                    if (key && key >= line) sh.list[atomicAdd(&sh.count, 1)] = key;   // at most eight lists of 32
                 }
                 __syncthreads();
                 const int n = sh.count;
@@ -388,15 +387,13 @@ __global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __gr
 
 template <typename T>
 static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
-    int device = 0;
-    MFQB_CUDA(cudaGetDevice(&device));
-    static std::once_flag once[64];
-    std::call_once(once[device], [] { MFQB_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, 3>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); });
-    // CTAs of a row: as many as are on the SMs at once, as long as a slice has a batch of vectors for every thread (77 rows of 32001 in bf16: 9.0 us with 4,
-    // 15.9 with 8, of which not all fit).  Rows that fill the SMs several times over have four CTAs on an SM, which read more at a time (1024 rows
-    // of 128256 in float32: 95 us, 110 with three), others three, with more registers (one row: 9.7 us, 10.3 with four).
+    // CTAs of a row: two, four or eight, as long as all are on the SMs at once and a slice has more than 16000 logits.  Rows of 128256 in float32: one row 7.6 us with eight,
+    // 8.6 with four, 14.4 with one, 7.7 with 16; 64 rows 13.3 with eight, 25.8 with one; 230 rows 26 with two, 33 with one; 300 rows 35.5 with one, 43 with two.  Rows of
+    // 32001: 30 rows 6.9 with one, 7.6 with two, 8.1 with eight; 90 rows 7.5, 9.0, 15.
     int ctas = 1;
-    while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= 3 * 148 && a.vocab / (2 * ctas) >= kLpThreads * kLpBatch) ctas *= 2;
+    while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= 4 * 148 && a.vocab / (2 * ctas) > 16000) ctas *= 2;
+    // Four CTAs on an SM read more at a time (1024 rows of 128256 in float32: 92 us, 109 with three), three have more registers (one row: 10.3 and 9.7 us with 16 CTAs).
+    const bool four = (int64_t)rows * ctas > 3 * 148;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ctas);
     cfg.blockDim = dim3(kLpThreads);
@@ -409,7 +406,7 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    MFQB_CUDA(cudaLaunchKernelEx(&cfg, rows > 3 * 148 ? logprobs_kernel<T, 4> : logprobs_kernel<T, 3>, a));
+    MFQB_CUDA(cudaLaunchKernelEx(&cfg, four ? logprobs_kernel<T, 4> : logprobs_kernel<T, 3>, a));
 }
 
 }  // namespace mfqb
