@@ -455,7 +455,7 @@ int mfqb_decoder_read_logits(const mfqb_decoder* d, int rows, float* out, mfqb_s
 struct mfqb_cache;
 int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
 /* Passes over the attached pages that add up how much every position was looked at and go on behind evicted ones (mfqb_cache_evict): weights float32
- * [layers][rows][kv_heads][width * page] of mfqb_tree_attention_weigh (null: none), dropped int32 [rows] (null: none), what has been
+ * [layers][rows][kv_heads][width * page] of mfqb_tree_attention_weigh (16-byte aligned; null: none), dropped int32 [rows] (null: none), what has been
  * evicted of every sequence so far, which is added to its positions.  Both are the caller's memory on the decoder's device and must outlive the
  * passes; attaching a cache (mfqb_decoder_set_cache) takes them off again.  Allocates as mfqb_decoder_set_cache does.  Weights do not
  * move with sequences: mfqb_decoder_beam_step is refused meanwhile. */
@@ -552,7 +552,7 @@ int mfqb_tree_attention_weigh(const mfqb_cache* c, int layer, const void* q, int
 
 /* Eviction by weight: sequence r of n = lens[r] tokens is cut to k = keep[r] (device int32 [rows]) where 0 <= k < n; a negative entry, or
  * one that is not below n, leaves it.  Its last R = min(recent, k) positions stay, and of the older ones, for every kv head of
- * every layer by itself, the k - R with the largest weights (float32 [layers][rows][kv_heads][width * page], as above; a NaN ranks as minus infinity;
+ * every layer by itself, the k - R with the largest weights (float32 [layers][rows][kv_heads][width * page], as above, 16-byte aligned; a NaN ranks as minus infinity;
  * equal ones: the lower slot).  Of those, what lies in slots below k - R stays in its slot; the others go in ascending order to the
  * slots that this leaves free there, in ascending order; slot n - R + i goes to k - R + i.  Keys, values and weights move together; what
  * lies behind k is left as it was.  So the latest positions stay in order at the end, the older ones do not, and attention does not

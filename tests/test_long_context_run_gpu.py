@@ -228,3 +228,33 @@ def test_arguments_that_are_refused():
     with pytest.raises(ValueError, match="dropped"):
         dec.set_cache(own, dropped=torch.zeros(3, dtype=torch.int32, device=DEV))
     dec.free()
+
+
+def test_pools_past_32_bits():
+    """The same sequences on the last pages of pools of more than 2^31 values and 2^32 bytes: the same weights, eviction and writes as on the first ones."""
+    rng = np.random.default_rng(3)
+    heads, page, pages = 4, 64, 40000
+    st = _round_state(R.state(rng, [700, 300], extra=40, page=page, kv_heads=heads, layers=2, spare=2))
+    few = st["refs"].size
+    near = _cache(st)
+    big = [torch.zeros((2, pages, heads, page, 128), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    assert big[0].numel() > 2 ** 31
+    for x, name in zip(big, "kv"):
+        x[:, pages - few:] = getattr(near, name)
+    refs = torch.ones(pages, dtype=torch.int32, device=DEV)
+    refs[pages - few:] = near.refs
+    far = PagedCache(*big, torch.where(near.table >= 0, near.table + (pages - few), -1), near.lens.clone(), refs)
+    got = []
+    for cache in (near, far):
+        w = cache.new_weights()
+        for nodes, hq in ((1, 8), (40, 16)):
+            r = np.random.default_rng(nodes)
+            masks, _ = R.masks_depths(_random_trees(r, 2, nodes))
+            for layer in (0, 1):
+                cache.attend(layer, _bf(r.standard_normal((2, nodes, hq, 128))).to(DEV), _masks(masks), weights=w)
+        gone, status = cache.evict(w, 200, recent=30)
+        x = torch.from_numpy(np.random.default_rng(9).standard_normal((2, 3, 16 * 128), dtype=np.float32)).to(DEV)
+        q = cache.write(1, x, _i32(np.arange(3)[None]) + gone[:, None], rope_frequencies(device=DEV, dims=96), layout="interleaved")
+        got.append((w, gone, status, cache.lens, q, cache.k[:, -few:], cache.v[:, -few:]))
+    for a, b in zip(*got):
+        assert torch.equal(a.float().nan_to_num(5.0), b.float().nan_to_num(5.0))
