@@ -91,6 +91,17 @@ def test_equal_logits(vocab):
     _check(torch.cat([z] * 40), rng.integers(0, vocab, 40 * len(rows)).tolist(), 32)   # a CTA a row
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [1, 7, 40, 500, 8001])
+def test_many_short_rows(vocab, dtype):
+    """CTAs of 128 threads; a sixth of the rows all equal, a sixth of few values."""
+    rng = np.random.default_rng(vocab)
+    z = 2.5 * rng.standard_normal((600, vocab), dtype=np.float32)
+    z[::6] = 1.5
+    z[1::6] = np.round(z[1::6])
+    _check(torch.from_numpy(z).to(DEV, dtype), _tokens(rng, 600, vocab), min(32, vocab))
+
+
 def test_masked_logits_and_rows_without_a_log_sum():
     rng = np.random.default_rng(0)
     vocab = 9001

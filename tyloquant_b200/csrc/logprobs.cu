@@ -7,8 +7,8 @@
 
 namespace mfqb {
 
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4, kLpCtas = 8;
-constexpr int kLpVocab = 1 << 20;
+constexpr int kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4, kLpCtas = 8;
+constexpr int kLpVocab = 1 << 20, kLpBrief = 8192;
 
 struct LogprobArgs {
     const char* logits;
@@ -24,12 +24,16 @@ struct LogprobSum {
     float top, sum, moment;
     int before;
 };
+template <int THREADS>
 struct LogprobShared {
-    CutShared cut;
-    LogprobSum warp[kLpWarps], all;
+    union {   // the search for a cut is over when the list is made
+        CutShared cut;
+        unsigned long long list[kLpList];
+    };
+    LogprobSum warp[THREADS / 32], all;
     float group[kLpGroups], bound;
-    int hot[kLpThreads], hots, count;
-    unsigned long long list[kLpList], best[kLpTop], gathered[kLpCtas][kLpTop];   // 0: none
+    int hot[THREADS], hots, count;
+    unsigned long long best[kLpTop], gathered[kLpCtas][kLpTop];   // 0: none
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -146,10 +150,10 @@ __device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
 // Sums are float32, a thread's own of some hundred terms each, joined in a tree: log probabilities are off by about 1e-7 of themselves.  Many rows: bound by memory
 // and by issue (1024 rows of 128256 in float32: 95 us, 5.5 TB/s, 12 instructions a logit; with checks of the ends of a row in the loop 19 instructions and 111 us).  One row: a
 // chain of trips (7.6 us: the logits, the hot threads' vectors again, the cluster's lists).
-template <typename T, int PER_SM>
-__global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    constexpr int kN = LpVec<T>::kN;
-    __shared__ LogprobShared sh;
+template <typename T, int THREADS, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+    constexpr int kN = LpVec<T>::kN, kLpThreads = THREADS, kLpWarps = THREADS / 32;
+    __shared__ LogprobShared<THREADS> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned rank = cluster_rank(), ctas = cluster_size();
     const int64_t row = blockIdx.x / ctas;
@@ -394,9 +398,13 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= 4 * 148 && a.vocab / (2 * ctas) > 16000) ctas *= 2;
     // Four CTAs on an SM read more at a time (1024 rows of 128256 in float32: 92 us, 109 with three), three have more registers (one row: 10.3 and 9.7 us with 16 CTAs).
     const bool four = (int64_t)rows * ctas > 3 * 148;
+    // Many short rows are a chain each, of which more run at once in CTAs of 128 threads, eight on an SM: 4000 rows of 1000 in float32
+    // 20.5 us, 30 in CTAs of 256; 2000 of 8000 21.8 and 27.8; 1500 of 32001 47 and 44.
+    const bool brief = four && ctas == 1 && a.vocab <= kLpBrief;
+    const int threads = brief ? 128 : 256;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ctas);
-    cfg.blockDim = dim3(kLpThreads);
+    cfg.blockDim = dim3(threads);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -406,7 +414,7 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    MFQB_CUDA(cudaLaunchKernelEx(&cfg, four ? logprobs_kernel<T, 4> : logprobs_kernel<T, 3>, a));
+    MFQB_CUDA(cudaLaunchKernelEx(&cfg, brief ? logprobs_kernel<T, 128, 8> : four ? logprobs_kernel<T, 256, 4> : logprobs_kernel<T, 256, 3>, a));
 }
 
 }  // namespace mfqb
