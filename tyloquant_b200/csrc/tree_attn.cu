@@ -553,6 +553,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
                     group_sync();   // the scores of all rows too
                     if (!ok) break;
                     for (int pos = lane_l; pos < w.seq.end; pos += kTile) add_weights<1>(a, w.seq, w.r, kvh, sh.ml[1], m_rows, pos);
+                    __syncwarp();   // O comes out of tensor memory next, for all lanes at once
                 }
             }
             // What this copy's values are multiplied by: its maximum against the joint one, the sum where the row is complete.

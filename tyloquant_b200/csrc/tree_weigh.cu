@@ -90,6 +90,7 @@ __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shif
 #pragma unroll 1
     for (int c = 0; c < rows; c += 16) {
         uint32_t s[16];
+        __syncwarp();   // loads from tensor memory and their wait want the warp together; what lies between goes by the lane's position
         tmem_ld16_async(col + c, s);
         unsigned in = rows - c >= 16 ? 0xFFFFu : (1u << (rows - c)) - 1u;   // of these 16
         if (seen != ~0ull) {
@@ -102,6 +103,7 @@ __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shif
             }
             in &= by;
         }
+        __syncwarp();
         tmem_wait_ld16(s);
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
