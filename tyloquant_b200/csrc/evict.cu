@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(mfqb_cache c, f
     };
     auto keys = [&](int i) { return CACHED ? s_keys[i] : read(i); };
     auto sync_all = [&]() {
+        __syncwarp();   // the aligned form wants the warp together: lanes have read different numbers of keys
         if (parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         else __syncthreads();
     };

@@ -124,6 +124,7 @@ __device__ __forceinline__ unsigned cluster_size() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();   // the aligned form wants the warp together, whatever its lanes did before
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The address of this CTA's shared variable in another CTA of the cluster, and a load from there.
