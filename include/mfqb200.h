@@ -458,7 +458,8 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
  * [layers][rows][kv_heads][width * page] of mfqb_tree_attention_weigh (16-byte aligned; null: none), dropped int32 [rows] (null: none), what has been
  * evicted of every sequence so far, which is added to its positions.  Both are the caller's memory on the decoder's device and must outlive the
  * passes; attaching a cache (mfqb_decoder_set_cache) takes them off again.  Allocates as mfqb_decoder_set_cache does.  Weights do not
- * move with sequences: mfqb_decoder_beam_step is refused meanwhile. */
+ * move with sequences: mfqb_decoder_beam_step is refused meanwhile.  A branch that is kept of a tree (mfqb_decoder_verify) takes its weights along by
+ * mfqb_tree_accept_weigh; with mfqb_tree_accept its tokens would have those of the nodes whose places they take. */
 int mfqb_decoder_set_weights(mfqb_decoder* d, float* weights, const int32_t* dropped);
 int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream);
 int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, float* scores, int32_t* done, int eos, int32_t* ids_out,
@@ -543,7 +544,8 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
  * lens[r] + nodes (what the nodes' slots held is of tokens that are gone).  All else stays.  Probabilities are float32 here.  A position without a page
  * gets nothing (a node's: 0), nor does one whose score is minus infinity; a NaN or plus infinity among the scores of a row makes NaN of the weights
  * of all else that it sees.  Each sum is made in one order: a call repeats bit for bit.  out is the same as of
- * mfqb_tree_attention.  weights overlaps neither q, out nor work.  mfqb_tree_accept and mfqb_cache_fork move keys and values alone, not the weights.
+ * mfqb_tree_attention.  weights overlaps neither q, out nor work.  All nodes' queries count, those of drafted nodes that are rejected afterwards too.
+ * mfqb_tree_accept and mfqb_cache_fork move keys and values alone; mfqb_tree_accept_weigh moves a branch's weights along.
  * work: device memory of mfqb_tree_attention_weigh_work bytes, 16-byte aligned (with the scores of up to 64 query rows of a kv head, where
  * they take at most 512 MB). */
 int mfqb_tree_attention_weigh_work(const mfqb_cache* c, int q_heads, int nodes, uint64_t* bytes);
@@ -575,6 +577,11 @@ int mfqb_cache_evict(const mfqb_cache* c, float* weights, const int32_t* keep, i
  * other output may overlap an input).  An unused row has count 0, token -1 and keeps its length. */
 int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count,
                      int32_t* token, int32_t* path, int32_t* lens_out, mfqb_stream_t stream);
+/* mfqb_tree_accept, which also moves the branch's entries of weights (float32 [layers][rows][kv_heads][width * page] of
+ * mfqb_tree_attention_weigh): position lens[r] + i gets what node path[r][i] was given, so that mfqb_cache_evict goes by it.  Entries behind the new
+ * length are of tokens that are gone; the next pass writes over them.  What the queries of rejected nodes have added at positions below lens stays. */
+int mfqb_tree_accept_weigh(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count,
+                           int32_t* token, int32_t* path, int32_t* lens_out, float* weights, mfqb_stream_t stream);
 
 /* Beam selection: logits float32 [groups][beams][vocab], scores float32 [groups][beams].  The k best candidates of every group by
  * scores + log softmax(logits), largest first, into out_scores float32 [groups][k], out_rows int32 (group * beams + beam: what

@@ -112,6 +112,7 @@ _SIGNATURES = {
     "mfqb_token_logprobs": (_i, [_vp, _i, _i, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mfqb_tree_attention_work": (_i, [_P(CacheView), _i, _i, _P(_u64)]),
     "mfqb_tree_attention": (_i, [_P(CacheView), _i, _vp, _i, _i, _vp, C.c_float, _vp, _vp, _u64, _vp]),
+    "mfqb_tree_accept_weigh": (_i, [_P(CacheView), _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mfqb_tree_accept": (_i, [_P(CacheView), _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "mfqb_beam_select_work": (_i, [_i, _i, _i, _i, _P(_u64)]),
     "mfqb_beam_select": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _u64, _vp]),
@@ -155,7 +156,8 @@ from . import _fast  # noqa: E402  (built together with the library)
 
 _fast.bind(*(C.cast(getattr(lib, _name), C.c_void_p).value for _name in (
     "mfqb_mul_mat", "mfqb_moe_topk", "mfqb_moe_ffn", "mfqb_cache_extend", "mfqb_cache_fork", "mfqb_tree_masks", "mfqb_cache_write", "mfqb_tree_attention",
-    "mfqb_tree_accept", "mfqb_beam_select", "mfqb_cache_write_rope", "mfqb_tree_attention_weigh", "mfqb_cache_evict", "mfqb_token_logprobs")))
+    "mfqb_tree_accept", "mfqb_beam_select", "mfqb_cache_write_rope", "mfqb_tree_attention_weigh", "mfqb_cache_evict", "mfqb_token_logprobs",
+    "mfqb_tree_accept_weigh")))
 
 
 def check(status: int) -> None:

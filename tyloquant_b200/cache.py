@@ -203,8 +203,9 @@ class PagedCache:
         nothing.  ``scale`` is 1 / sqrt(128) unless given.
 
         ``weights`` (``new_weights``), changed in place: for every kv head of the layer, the probabilities that the nodes and the head's queries
-        give to a position are added to its entry; the nodes' own entries, at positions from ``lens`` on, are set.  ``accept`` and ``fork`` move keys
-        and values alone: entries of a branch, or of sequences that go on from others, are the caller's to move."""
+        give to a position are added to its entry; the nodes' own entries, at positions from ``lens`` on, are set.  All nodes count, those that are
+        rejected afterwards too.  ``accept`` moves a branch's entries where it is given the weights; ``fork`` moves keys and values alone: entries of
+        sequences that go on from others are the caller's to move (``weights[:, parents]``)."""
         torch = _torch()
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != HEAD_DIM:
             raise ValueError(f"q must be [{self.rows}, nodes, q_heads, 128], got {list(q.shape)}")
@@ -264,11 +265,13 @@ class PagedCache:
         _call(_fast.cache_evict, self.device, self._ptr, weights.data_ptr(), k.data_ptr(), recent, dropped.data_ptr(), status.data_ptr(), work.data_ptr(), self._evict_work)
         return dropped, status
 
-    def accept(self, ids, parents, targets, lens_out=None):
+    def accept(self, ids, parents, targets, lens_out=None, weights=None):
         """Keeps the branch of every tree that the model agrees with: from the root on the lowest child whose drafted token ``ids`` is the model's
         own ``targets`` of the node above (all int32 [rows, nodes]); its keys and values move to the slots behind ``lens``.  Returns
         (count [rows], next token [rows], path [rows, nodes], new lengths [rows]); the cache's own lengths change only where they
-        are given as ``lens_out``."""
+        are given as ``lens_out``.
+
+        ``weights`` (those of ``attend``, or of the decoder's ``verify``), changed in place: the branch's entries move along, as ``evict`` needs them."""
         if ids.dim() != 2:
             raise ValueError(f"ids must be an int32 tensor [{self.rows}, nodes]")
         torch, nodes = _torch(), ids.shape[1]
@@ -278,9 +281,14 @@ class PagedCache:
             lens_out = torch.empty_like(self.lens)
         elif self._int32(lens_out, (self.rows,), "lens_out") is not lens_out:
             raise ValueError("lens_out must be contiguous")
+        if weights is not None:
+            self._weights(weights)
         count, token, path = torch.empty_like(self.lens), torch.empty_like(self.lens), torch.empty_like(i)
-        _call(_fast.tree_accept, self.device, self._ptr, i.data_ptr(), p.data_ptr(), t.data_ptr(), nodes, count.data_ptr(), token.data_ptr(), path.data_ptr(),
-              lens_out.data_ptr())
+        given = self._ptr, i.data_ptr(), p.data_ptr(), t.data_ptr(), nodes, count.data_ptr(), token.data_ptr(), path.data_ptr(), lens_out.data_ptr()
+        if weights is None:
+            _call(_fast.tree_accept, self.device, *given)
+        else:
+            _call(_fast.tree_accept_weigh, self.device, *given, weights.data_ptr())
         return count, token, path, lens_out
 
 

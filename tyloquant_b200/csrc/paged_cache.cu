@@ -443,8 +443,9 @@ static void launch_cache_rope(const mfqb_cache& c, int layer, const void* qkv, i
 // written, since a slot that one node leaves is another one's place.  A chain from the lengths to the rows: one tree of 8 nodes 4.2 us, 16 of 48
 // with branches of 13 in 128 heads 8.6 (a launch for the walk and one for the rows: 5.0 and 9.0; with a CTA for each head of each layer 11).  Lengths
 // that change in place are a second launch, 0.7 and 1.1 us more.
+// weights (mfqb_tree_attention_weigh, or null): the branch's sums move along.
 __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* ids, const int* parents, const int* targets, int nodes, int* count, int* token,
-                                                     int* path, int* lens_out) {
+                                                     int* path, int* lens_out, float* weights) {
     chained_wait();
     __shared__ int s_path[kTreeNodes], s_n, s_token;
     __shared__ int64_t s_from[kTreeNodes], s_to[kTreeNodes];   // rows of the branch in 16-byte pieces, for head 0 of layer 0; -1: stays
@@ -513,6 +514,17 @@ __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* id
             kv[i][0] = static_cast<const uint4*>(c.k)[s_from[node] + at];
             kv[i][1] = static_cast<const uint4*>(c.v)[s_from[node] + at];
         }
+        float* sums = nullptr;   // of the head that this thread moves a sum of; positions have one whether they have a page or not
+        float sum = 0.f;
+        if (weights && t < each * n && h0 + t / n < heads) {
+            const int64_t head = h0 + t / n, layer = head / c.kv_heads;
+            const int node = t % n;
+            float* base = weights + ((layer * c.rows + r) * c.kv_heads + (head - layer * c.kv_heads)) * cap + len;
+            if (s_path[node] != node && len + s_path[node] < cap) {   // a node of a branch is never before its place
+                sum = __ldcg(base + s_path[node]);
+                sums = base + node;
+            }
+        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -520,6 +532,7 @@ __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* id
                 static_cast<uint4*>(c.k)[to[i]] = kv[i][0];
                 static_cast<uint4*>(c.v)[to[i]] = kv[i][1];
             }
+        if (sums) *sums = sum;
     }
 }
 
@@ -531,6 +544,20 @@ __global__ void __launch_bounds__(1024) accept_lens_kernel(mfqb_cache c, const i
     if (r < c.rows) len = (int)min(max((int64_t)c.lens[r], (int64_t)0), (int64_t)c.width * c.page) + __ldcg(count + r);
     __syncthreads();
     if (r < c.rows) lens_out[r] = len;
+}
+
+static void accept(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count, int32_t* token,
+                   int32_t* path, int32_t* lens_out, float* weights, cudaStream_t s, const char* who) {
+    check_cache(c, who);
+    check_nodes(c, nodes, who);
+    if (!ids || !parents || !targets || !count || !token || !path || !lens_out) fail(MFQB_ERR_ARG, "%s: null argument", who);
+    if ((int64_t)c->layers * c->kv_heads > (1ll << 30)) fail(MFQB_ERR_UNSUPPORTED, "%s: too many layers x heads", who);
+    // enough CTAs for the SMs, at least one head each (how many nodes a branch has is known on the device alone)
+    const int per_row = std::min(c->layers * c->kv_heads, std::max(1, 148 * 5 / c->rows));
+    const bool in_place = lens_out < c->lens + c->rows && c->lens < lens_out + c->rows;
+    launch_chained(accept_kernel, dim3((unsigned)per_row, c->rows), dim3(256), 0, s, *c, ids, parents, targets, nodes, count, token, path,
+                   in_place ? nullptr : lens_out, weights);
+    if (in_place) launch_chained(accept_lens_kernel, dim3(1), dim3(1024), 0, s, *c, static_cast<const int*>(count), lens_out);
 }
 
 }  // namespace mfqb
@@ -625,17 +652,15 @@ int mfqb_cache_write_rope(const mfqb_cache* c, int layer, const void* qkv, int q
 
 int mfqb_tree_accept(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count,
                      int32_t* token, int32_t* path, int32_t* lens_out, mfqb_stream_t stream) {
+    return guarded([&] { accept(c, ids, parents, targets, nodes, count, token, path, lens_out, nullptr, stream, "mfqb_tree_accept"); });
+}
+
+int mfqb_tree_accept_weigh(const mfqb_cache* c, const int32_t* ids, const int32_t* parents, const int32_t* targets, int nodes, int32_t* count,
+                           int32_t* token, int32_t* path, int32_t* lens_out, float* weights, mfqb_stream_t stream) {
     return guarded([&] {
-        check_cache(c, "mfqb_tree_accept");
-        check_nodes(c, nodes, "mfqb_tree_accept");
-        if (!ids || !parents || !targets || !count || !token || !path || !lens_out) fail(MFQB_ERR_ARG, "mfqb_tree_accept: null argument");
-        if ((int64_t)c->layers * c->kv_heads > (1ll << 30)) fail(MFQB_ERR_UNSUPPORTED, "mfqb_tree_accept: too many layers x heads");
-        // enough CTAs for the SMs, at least one head each (how many nodes a branch has is known on the device alone)
-        const int per_row = std::min(c->layers * c->kv_heads, std::max(1, 148 * 5 / c->rows));
-        const bool in_place = lens_out < c->lens + c->rows && c->lens < lens_out + c->rows;
-        launch_chained(accept_kernel, dim3((unsigned)per_row, c->rows), dim3(256), 0, stream, *c, ids, parents, targets, nodes, count, token, path,
-                       in_place ? nullptr : lens_out);
-        if (in_place) launch_chained(accept_lens_kernel, dim3(1), dim3(1024), 0, stream, *c, static_cast<const int*>(count), lens_out);
+        const char* who = "mfqb_tree_accept_weigh";
+        if (!weights || ((uintptr_t)weights & 3)) fail(MFQB_ERR_ARG, "%s: weights must be float32 values on 4-byte boundaries", who);
+        accept(c, ids, parents, targets, nodes, count, token, path, lens_out, weights, stream, who);
     });
 }
 

@@ -86,7 +86,8 @@ class Decoder:
 
         ``weights`` (``cache.new_weights()``): every pass adds up in them how much each position was looked at, for ``cache.evict``.  ``dropped`` (int32
         [rows]): what has been evicted of every sequence so far, added to its positions; add to it what ``evict`` returns.  Both are kept
-        alive like the cache; ``beam_step`` is refused with them."""
+        alive like the cache; ``beam_step`` is refused with them.  After ``verify`` give the weights to ``cache.accept`` too, which moves the kept
+        branch's; what the queries of rejected nodes have added to the context's positions stays."""
         from .cache import _need
         torch = _torch()
         if cache is None and (weights is not None or dropped is not None):
@@ -108,7 +109,8 @@ class Decoder:
 
     def verify(self, ids, parents):
         """The drafted trees of all sequences in one pass (``ids``, ``parents`` int32 [rows, nodes], see ``tree_masks``): returns the model's own
-        greedy token at every node.  Reserve ``nodes`` tokens first (``cache.extend``); ``cache.accept`` keeps the branch that agrees."""
+        greedy token at every node.  Reserve ``nodes`` tokens first (``cache.extend``); ``cache.accept`` keeps the branch that agrees (give it
+        the weights where some are attached)."""
         torch = _torch()
         if ids.dim() != 2:
             raise ValueError("ids must be an int32 tensor [rows, nodes]")

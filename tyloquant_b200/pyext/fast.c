@@ -22,6 +22,7 @@ typedef int (*beam_fn)(const void*, int, int, int, const void*, const void*, int
 typedef int (*rope_fn)(const void*, int, const void*, int, int, int, const void*, const void*, int, int, float, void*, void*);
 typedef int (*weigh_fn)(const void*, int, const void*, int, int, const void*, float, void*, void*, void*, uint64_t, void*);
 typedef int (*evict_fn)(const void*, void*, const void*, int, void*, void*, void*, uint64_t, void*);
+typedef int (*accept_weigh_fn)(const void*, const void*, const void*, const void*, int, void*, void*, void*, void*, void*, void*);
 typedef int (*logprobs_fn)(const void*, int, int, int, int64_t, const void*, int, void*, void*, void*, void*, void*, void*);
 
 static mul_mat_fn p_mul_mat;
@@ -38,6 +39,7 @@ static rope_fn p_rope;
 static weigh_fn p_weigh;
 static evict_fn p_evict;
 static logprobs_fn p_logprobs;
+static accept_weigh_fn p_accept_weigh;
 
 static void* address(PyObject* o) { return o == Py_None ? NULL : (void*)(uintptr_t)PyLong_AsUnsignedLongLong(o); }
 static int number(PyObject* o) {
@@ -53,7 +55,7 @@ static int arity(Py_ssize_t got, Py_ssize_t want) {
 
 static PyObject* bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
-    if (!arity(n, 14)) return NULL;
+    if (!arity(n, 15)) return NULL;
     p_mul_mat = (mul_mat_fn)address(a[0]);
     p_topk = (topk_fn)address(a[1]);
     p_ffn = (ffn_fn)address(a[2]);
@@ -68,6 +70,7 @@ static PyObject* bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     p_weigh = (weigh_fn)address(a[11]);
     p_evict = (evict_fn)address(a[12]);
     p_logprobs = (logprobs_fn)address(a[13]);
+    p_accept_weigh = (accept_weigh_fn)address(a[14]);
     if (PyErr_Occurred()) return NULL;
     Py_RETURN_NONE;
 }
@@ -233,6 +236,28 @@ static PyObject* tree_accept(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(rc);
 }
+/* cache, ids, parents, targets, nodes, count, token, path, lens_out, weights, stream */
+static PyObject* tree_accept_weigh(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    (void)self;
+    if (!arity(n, 11)) return NULL;
+    void* c = address(a[0]);
+    void* ids = address(a[1]);
+    void* pa = address(a[2]);
+    void* t = address(a[3]);
+    const int nodes = number(a[4]);
+    void* cnt = address(a[5]);
+    void* tok = address(a[6]);
+    void* path = address(a[7]);
+    void* lens = address(a[8]);
+    void* wt = address(a[9]);
+    void* s = address(a[10]);
+    if (PyErr_Occurred()) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_accept_weigh(c, ids, pa, t, nodes, cnt, tok, path, lens, wt, s);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
 /* logits, groups, beams, vocab, scores, done, eos, k, out_scores, out_rows, out_tokens, work, work_bytes, stream */
 static PyObject* beam_select(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
@@ -360,6 +385,7 @@ static PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH
                                 {"cache_write", (PyCFunction)(void (*)(void))cache_write, METH_FASTCALL, "mfqb_cache_write"},
                                 {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, "mfqb_tree_attention"},
                                 {"tree_accept", (PyCFunction)(void (*)(void))tree_accept, METH_FASTCALL, "mfqb_tree_accept"},
+                                {"tree_accept_weigh", (PyCFunction)(void (*)(void))tree_accept_weigh, METH_FASTCALL, "mfqb_tree_accept_weigh"},
                                 {"beam_select", (PyCFunction)(void (*)(void))beam_select, METH_FASTCALL, "mfqb_beam_select"},
                                 {"cache_write_rope", (PyCFunction)(void (*)(void))cache_write_rope, METH_FASTCALL, "mfqb_cache_write_rope"},
                                 {"tree_attention_weigh", (PyCFunction)(void (*)(void))tree_attention_weigh, METH_FASTCALL, "mfqb_tree_attention_weigh"},
