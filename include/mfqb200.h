@@ -459,7 +459,8 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
  * evicted of every sequence so far, which is added to its positions.  Both are the caller's memory on the decoder's device and must outlive the
  * passes; attaching a cache (mfqb_decoder_set_cache) takes them off again.  Allocates as mfqb_decoder_set_cache does.  Weights do not
  * move with sequences: mfqb_decoder_beam_step is refused meanwhile.  A branch that is kept of a tree (mfqb_decoder_verify) takes its weights along by
- * mfqb_tree_accept_weigh; with mfqb_tree_accept its tokens would have those of the nodes whose places they take. */
+ * mfqb_tree_accept_weigh; with mfqb_tree_accept its tokens would have those of the nodes whose places they take.  Nodes that are unused
+ * (mfqb_tree_masks), all of a sequence's or some, add nothing here, unlike in mfqb_tree_attention_weigh, where every node of the call has queries. */
 int mfqb_decoder_set_weights(mfqb_decoder* d, float* weights, const int32_t* dropped);
 int mfqb_decoder_verify(mfqb_decoder* d, const int32_t* ids, const int32_t* parents, int nodes, int32_t* targets, mfqb_stream_t stream);
 int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, float* scores, int32_t* done, int eos, int32_t* ids_out,
@@ -544,7 +545,8 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
  * lens[r] + nodes (what the nodes' slots held is of tokens that are gone).  All else stays.  Probabilities are float32 here.  A position without a page
  * gets nothing (a node's: 0), nor does one whose score is minus infinity; a NaN or plus infinity among the scores of a row makes NaN of the weights
  * of all else that it sees.  Each sum is made in one order: a call repeats bit for bit.  out is the same as of
- * mfqb_tree_attention.  weights overlaps neither q, out nor work.  All nodes' queries count, those of drafted nodes that are rejected afterwards too.
+ * mfqb_tree_attention.  weights overlaps neither q, out nor work.  All nodes' queries count: those of drafted nodes that are rejected
+ * afterwards, and those of nodes with mask 0, which see what is below lens (trees of different sizes in one call: call it for each size).
  * mfqb_tree_accept and mfqb_cache_fork move keys and values alone; mfqb_tree_accept_weigh moves a branch's weights along.
  * work: device memory of mfqb_tree_attention_weigh_work bytes, 16-byte aligned (with the scores of up to 64 query rows of a kv head, where
  * they take at most 512 MB). */

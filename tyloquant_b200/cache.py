@@ -204,7 +204,7 @@ class PagedCache:
 
         ``weights`` (``new_weights``), changed in place: for every kv head of the layer, the probabilities that the nodes and the head's queries
         give to a position are added to its entry; the nodes' own entries, at positions from ``lens`` on, are set.  All nodes count, those that are
-        rejected afterwards too.  ``accept`` moves a branch's entries where it is given the weights; ``fork`` moves keys and values alone: entries of
+        rejected afterwards too, and unused ones (mask 0), which see the context.  ``accept`` moves a branch's entries where it is given the weights; ``fork`` moves keys and values alone: entries of
         sequences that go on from others are the caller's to move (``weights[:, parents]``)."""
         torch = _torch()
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != HEAD_DIM:

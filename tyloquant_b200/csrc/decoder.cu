@@ -727,7 +727,7 @@ static void attend_pages(mfqb_decoder* d, int li, cudaStream_t s) {
     check(mfqb_cache_write(&d->write_to, li, static_cast<const float*>(d->qkv.p), d->nq, d->nodes, d->node_depths, static_cast<const double*>(d->freqs.p), d->q16.p, s));
     const float scale = 0.08838834764831845f;
     if (d->weights)
-        check(mfqb_tree_attention_weigh(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, scale, d->attn.p, d->weights, d->attn_work.p, d->attn_work_bytes, s));
+        tree_attention_weigh(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, scale, d->attn.p, d->weights, true, d->attn_work.p, d->attn_work_bytes, s);
     else
         check(mfqb_tree_attention(&d->read_from, li, d->q16.p, d->nq, d->nodes, d->node_masks, scale, d->attn.p, d->attn_work.p, d->attn_work_bytes, s));
 }

@@ -41,6 +41,10 @@ inline void check_apart(const void* out, uint64_t out_bytes, const void* in, uin
     if (o < i + in_bytes && i < o + out_bytes) fail(MFQB_ERR_ARG, "%s: %s overlap", who, what);
 }
 
+// mfqb_tree_attention_weigh; with `used`, nodes whose mask is 0 (mfqb_tree_masks: the tree has no such node) add nothing to the weights.
+void tree_attention_weigh(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights, bool used,
+                          void* work, uint64_t work_bytes, cudaStream_t s);
+
 // Launched with the programmatic-dependent-launch attribute: the kernel becomes resident while its predecessor runs and waits
 // (after_predecessor) until that one has completed.
 template <typename... KArgs, typename... Args>

@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             if constexpr (WEIGH && REP > 1) {
                 // All of the item is here (one token at context 100: 9.6 us, 11.7 with a launch for it); the other stream's place in sh.ml is free.
                 if (a.whole && a.scores) {
-                    if (live && copy == 0) sh.ml[1][row_l] = row_scale(sum.x, sum.y);
+                    if (live && copy == 0) sh.ml[1][row_l] = a.counts(mask) ? row_scale(sum.x, sum.y) : make_float2(0.f, 0.f);
                     group_sync();   // the scores of all rows too
                     if (!ok) break;
                     for (int pos = lane_l; pos < w.seq.end; pos += kTile) add_weights<1>(a, w.seq, w.r, kvh, sh.ml[1], m_rows, pos);
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             }
             if (live && copy == 0) {
                 if (!complete) a.part_ml[slot + row_l] = sum;
-                else if constexpr (WEIGH) a.row_ml[((int64_t)w.r * a.kv_heads + kvh) * m_rows + row] = row_scale(sum.x, sum.y);
+                else if constexpr (WEIGH) a.row_ml[((int64_t)w.r * a.kv_heads + kvh) * m_rows + row] = a.counts(mask) ? row_scale(sum.x, sum.y) : make_float2(0.f, 0.f);
                 if (bad) {
                     if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + a.row_at(w.r, kvh, row));
                     else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim);
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __gr
                     l += __shfl_xor_sync(0xffffffffu, l, o);
                     none += __shfl_xor_sync(0xffffffffu, none, o);
                 }
-                if (lane == 0) s_scale[row] = row_scale(high, high == -INFINITY ? none : l);
+                if (lane == 0) s_scale[row] = a.row_counts(r, row) ? row_scale(high, high == -INFINITY ? none : l) : make_float2(0.f, 0.f);
             }
             __syncthreads();
             for (int pos = ((at - item * stretches) * 32 * kMergeWarps + threadIdx.x) * 4; pos < seq.end; pos += stretches * 128 * kMergeWarps)
@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const __gr
         __syncwarp();   // the parts have been read before the next come in their place
     }
     if (m == -INFINITY) l = none;
-    if (a.row_ml && lane == 0) a.row_ml[((int64_t)r * a.kv_heads + kvh) * m_rows + row] = row_scale(m, l);
+    if (a.row_ml && lane == 0) a.row_ml[((int64_t)r * a.kv_heads + kvh) * m_rows + row] = a.row_counts(r, row) ? row_scale(m, l) : make_float2(0.f, 0.f);
     const float inv = 1.f / l;
     if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
     else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
@@ -813,9 +813,9 @@ static void check_attention(const mfqb_cache* c, int layer, const void* q, int q
     check_apart(out, bytes, q, bytes, who, "q and out");
 }
 
-// weights (of all layers): added up behind the attention, where given.
+// weights (of all layers): added up behind the attention, where given; used: of nodes with a mask alone.
 static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights,
-                                  void* work, cudaStream_t s) {
+                                  bool used, void* work, cudaStream_t s) {
     int device = 0;
     MFQB_CUDA(cudaGetDevice(&device));
     const int64_t per_layer = (int64_t)c.pages * c.kv_heads * c.page * kHeadDim;
@@ -850,6 +850,7 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
         a.weights = weights + (int64_t)layer * c.rows * c.kv_heads * c.width * c.page;
         a.score_stride = tree_score_stride(c, q_heads, nodes);
         a.scores = a.score_stride ? reinterpret_cast<float*>(more) : nullptr;
+        a.used = used;
         a.row_ml = reinterpret_cast<float2*>(more + 4ull * c.rows * c.kv_heads * m_rows * a.score_stride);
     }
     auto* kernel = weights ? ns == 2 ? tree_attn_kernel<2, 1, true> : m_rows > 64 ? tree_attn_kernel<1, 1, true> : m_rows > 32 ? tree_attn_kernel<1, 2, true> : tree_attn_kernel<1, 4, true>
@@ -882,6 +883,19 @@ static void launch_tree_attention(const mfqb_cache& c, int layer, const void* q,
     if (weights && !a.scores) launch_tree_weigh(c, a, s);
 }
 
+void tree_attention_weigh(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights, bool used,
+                          void* work, uint64_t work_bytes, cudaStream_t s) {
+    const char* who = "mfqb_tree_attention_weigh";
+    check_attention_shape(c, q_heads, nodes, who);
+    check_attention(c, layer, q, q_heads, nodes, masks, scale, out, work, work_bytes, weigh_work_bytes(*c, q_heads, nodes), who);
+    if (!weights || ((uintptr_t)weights & 3)) fail(MFQB_ERR_ARG, "%s: weights must be float32 values on 4-byte boundaries", who);
+    const uint64_t bytes = 256ull * c->rows * nodes * q_heads, all = 4ull * c->layers * c->rows * c->kv_heads * c->width * c->page;
+    check_apart(weights, all, q, bytes, who, "q and weights");   // q is read again for the weights
+    check_apart(weights, all, out, bytes, who, "out and weights");
+    check_apart(weights, all, work, work_bytes, who, "work and weights");
+    launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, weights, used, work, s);
+}
+
 }  // namespace mfqb
 
 using namespace mfqb;
@@ -903,7 +917,7 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
     return guarded([&] {
         check_attention_shape(c, q_heads, nodes, "mfqb_tree_attention");
         check_attention(c, layer, q, q_heads, nodes, masks, scale, out, work, work_bytes, tree_attention_work_bytes(*c, q_heads, nodes), "mfqb_tree_attention");
-        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, nullptr, work, stream);
+        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, nullptr, false, work, stream);
     });
 }
 
@@ -918,17 +932,7 @@ int mfqb_tree_attention_weigh_work(const mfqb_cache* c, int q_heads, int nodes, 
 
 int mfqb_tree_attention_weigh(const mfqb_cache* c, int layer, const void* q, int q_heads, int nodes, const uint64_t* masks, float scale, void* out, float* weights,
                               void* work, uint64_t work_bytes, mfqb_stream_t stream) {
-    return guarded([&] {
-        const char* who = "mfqb_tree_attention_weigh";
-        check_attention_shape(c, q_heads, nodes, who);
-        check_attention(c, layer, q, q_heads, nodes, masks, scale, out, work, work_bytes, weigh_work_bytes(*c, q_heads, nodes), who);
-        if (!weights || ((uintptr_t)weights & 3)) fail(MFQB_ERR_ARG, "%s: weights must be float32 values on 4-byte boundaries", who);
-        const uint64_t bytes = 256ull * c->rows * nodes * q_heads, all = 4ull * c->layers * c->rows * c->kv_heads * c->width * c->page;
-        check_apart(weights, all, q, bytes, who, "q and weights");   // q is read again for the weights
-        check_apart(weights, all, out, bytes, who, "out and weights");
-        check_apart(weights, all, work, work_bytes, who, "work and weights");
-        launch_tree_attention(*c, layer, q, q_heads, nodes, masks, scale, out, weights, work, stream);
-    });
+    return guarded([&] { tree_attention_weigh(c, layer, q, q_heads, nodes, masks, scale, out, weights, false, work, work_bytes, stream); });
 }
 
 #pragma GCC visibility pop

@@ -33,9 +33,13 @@ struct TreeArgs {
     float* scores;                // [rows][kv_heads][rows of Q][score_stride]: raw scores, minus infinity where a row does not see, or null
     int64_t score_stride;
     float* weights;               // of the layer: [rows][kv_heads][width * page], or null
+    bool used;                    // nodes whose mask is 0 stand for none: their rows' (maximum, 1 / sum) is (0, 0)
     unsigned group_inv;           // ceil(65536 / group): row / group = row * group_inv >> 16 for rows below 1024, groups up to 16
     float scale_log2;
     __device__ __forceinline__ int node_of(int row_of_q) const { return (int)((unsigned)row_of_q * group_inv >> 16); }
+    // Do a node's rows count among the weights?
+    __device__ __forceinline__ bool counts(unsigned long long mask) const { return !used || (nodes < 64 ? mask & ((1ull << nodes) - 1ull) : mask) != 0; }
+    __device__ __forceinline__ bool row_counts(int r, int row_of_q) const { return !used || counts(__ldcg(masks + (int64_t)r * nodes + node_of(row_of_q))); }
     // element offset of a row of Q (or of the output) of sequence r and kv head kvh
     __device__ __forceinline__ int64_t row_at(int r, int kvh, int row_of_q) const {
         const int node = node_of(row_of_q);
@@ -172,7 +176,7 @@ inline CUtensorMap page_map(const void* base, const mfqb_cache& c) {
 
 
 // What a position of sequence r gets, from the scores that the attention has kept: exp2(scale' score - x) y of every row's (x, y), in their order, nothing
-// for a score of minus infinity.  Positions pos .. pos + N - 1 lie in one page.
+// for a score of minus infinity, nor of a row with y = 0, whatever its scores are.  Positions pos .. pos + N - 1 lie in one page.
 template <int N>
 __device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& seq, int r, int kvh, const float2* scale, int m_rows, int pos) {
     const int64_t item = (int64_t)r * a.kv_heads + kvh;
@@ -197,7 +201,7 @@ __device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& se
             v[0] = __ldcg(scores + row * a.score_stride);
         }
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += v[e] == -INFINITY ? 0.f : exp2_approx(fmaf(v[e], a.scale_log2, -ml.x)) * ml.y;
+        for (int e = 0; e < N; ++e) sum[e] += v[e] == -INFINITY || ml.y == 0.f ? 0.f : exp2_approx(fmaf(v[e], a.scale_log2, -ml.x)) * ml.y;
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) {

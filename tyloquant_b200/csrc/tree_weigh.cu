@@ -81,7 +81,7 @@ struct WeighWalk {
     }
 };
 
-// A position that not every row sees, or (BAD) where weights of some rows are no numbers: a row counts where it sees the position and its score is
+// A position that not every row sees (or counts for), or (BAD) where weights of some rows are no numbers: a row counts where it sees the position and its score is
 // above minus infinity.
 template <bool BAD>
 __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shift, uint32_t col, int row0, int rows, unsigned long long seen) {
@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
         const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + g * kWeighRows + first_row;
         const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
         const unsigned long long every = a.nodes < 64 ? ~0ull << a.nodes : 0ull;   // nodes that there are not
+        unsigned long long counted = ~0ull;   // nodes whose rows count; all where there are none
         uint32_t j = 0, alls = 0;
         int items = 0;
         bool ok = true;
@@ -317,6 +318,8 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
                 {   // a lane has two nodes' masks, a warp makes the bits of four nodes
                     const unsigned long long* masks = a.masks + (int64_t)w.r * a.nodes;
                     const unsigned long long lo = lane < a.nodes ? __ldcg(masks + lane) : 0ull, hi = lane + 32 < a.nodes ? __ldcg(masks + lane + 32) : 0ull;
+                    if (a.used)
+                        counted = (unsigned long long)__ballot_sync(0xffffffffu, a.counts(hi)) << 32 | __ballot_sync(0xffffffffu, a.counts(lo)) | every;
 #pragma unroll
                     for (int u = 0; u < kTreeNodes / (4 * kWeighGroups); ++u) {
                         const int node = (warp - 2) * (kTreeNodes / (4 * kWeighGroups)) + u;
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
             const bool page = (good >> (at >> 4)) & 1u;
             float sum = 0.f;   // columns behind the last row are products with it too
             // What comes of a position behind the end or without a page is not used.
-            const unsigned long long seen = node < 0 || node >= a.nodes ? ~0ull : sh.seen_by[node] | every;
+            const unsigned long long seen = (node < 0 || node >= a.nodes ? ~0ull : sh.seen_by[node] | every) & counted;
             if (__all_sync(0xffffffffu, seen == ~0ull) && sh.bad != items) {   // every row sees all 32 positions
                 uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll 1
