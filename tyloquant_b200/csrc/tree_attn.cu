@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             if constexpr (WEIGH && REP > 1) {
                 // All of the item is here (one token at context 100: 9.6 us, 11.7 with a launch for it); the other stream's place in sh.ml is free.
                 if (a.whole && a.scores) {
-                    if (live && copy == 0) sh.ml[1][row_l] = a.counts(mask) ? row_scale(sum.x, sum.y) : make_float2(0.f, 0.f);
+                    if (live && copy == 0) sh.ml[1][row_l] = a.row_counts(w.r, row) ? row_scale(sum.x, sum.y) : make_float2(0.f, 0.f);
                     group_sync();   // the scores of all rows too
                     if (!ok) break;
                     for (int pos = lane_l; pos < w.seq.end; pos += kTile) add_weights<1>(a, w.seq, w.r, kvh, sh.ml[1], m_rows, pos);
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(tree_threads(NS), NS == 2 ? 1 : 2) tree_attn_k
             }
             if (live && copy == 0) {
                 if (!complete) a.part_ml[slot + row_l] = sum;
-                else if constexpr (WEIGH) a.row_ml[((int64_t)w.r * a.kv_heads + kvh) * m_rows + row] = a.counts(mask) ? row_scale(sum.x, sum.y) : make_float2(0.f, 0.f);
+                else if constexpr (WEIGH) a.row_ml[((int64_t)w.r * a.kv_heads + kvh) * m_rows + row] = a.row_counts(w.r, row) ? row_scale(sum.x, sum.y) : make_float2(0.f, 0.f);
                 if (bad) {
                     if (complete) add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.out + a.row_at(w.r, kvh, row));
                     else add_bad_nodes(a, bad, w.seq, w.r, kvh, row, sum.x, a.part + (slot + row_l) * kHeadDim);

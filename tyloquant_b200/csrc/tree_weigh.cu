@@ -26,7 +26,7 @@ struct WeighShared {
     uint64_t k_full[kWeighRing], k_empty[kWeighRing], q_full, s_full[2], s_empty[2], all, half[4];
     int64_t scan[kWeighThreads / 32], first, last, off;
     int row0, failed;
-    int bad;                         // the last head (its number in the CTA, from 1 on) with a row whose weights are no numbers
+    int bad;                         // the last head (its number in the CTA, from 1 on) with a row whose weights are no numbers, or that does not count
     uint32_t tmem;
     unsigned good[8];
     unsigned long long seen_by[kTreeNodes];   // by which nodes a node is
@@ -81,8 +81,8 @@ struct WeighWalk {
     }
 };
 
-// A position that not every row sees (or counts for), or (BAD) where weights of some rows are no numbers: a row counts where it sees the position and its score is
-// above minus infinity.
+// A position that not every row sees, or (BAD) where weights of some rows are no numbers or some do not count (a shift of minus infinity, whatever the
+// scores): a row counts where it sees the position and its score is above minus infinity.
 template <bool BAD>
 __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shift, uint32_t col, int row0, int rows, unsigned long long seen) {
     const int m_rows = a.nodes * a.group;
@@ -113,7 +113,7 @@ __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shif
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const float x = __uint_as_float(s[e + u]);
-                p[u] = (in >> (e + u)) & 1u && (!BAD || x != -INFINITY) ? exp2_approx(fmaf(x, a.scale_log2, shift[u])) : 0.f;
+                p[u] = (in >> (e + u)) & 1u && (!BAD || (x != -INFINITY && shift[u] != -INFINITY)) ? exp2_approx(fmaf(x, a.scale_log2, shift[u])) : 0.f;
             }
             sum2[0] = add_f32x2(sum2[0], pair_f32(p[0], p[1]));
             sum2[1] = add_f32x2(sum2[1], pair_f32(p[2], p[3]));
@@ -269,7 +269,6 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
         const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + g * kWeighRows + first_row;
         const uint64_t scale2 = pair_f32(a.scale_log2, a.scale_log2);
         const unsigned long long every = a.nodes < 64 ? ~0ull << a.nodes : 0ull;   // nodes that there are not
-        unsigned long long counted = ~0ull;   // nodes whose rows count; all where there are none
         uint32_t j = 0, alls = 0;
         int items = 0;
         bool ok = true;
@@ -313,13 +312,11 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
                     const float2 ml = __ldcg(a.row_ml + ((int64_t)w.r * a.kv_heads + w.kvh) * m_rows + min(row0 + t, row0 + rows - 1));
                     const float shift = t < rows ? log2f(ml.y) - ml.x : -INFINITY;
                     reinterpret_cast<float*>(sh.shift)[t] = shift;
-                    if (!(shift < INFINITY)) sh.bad = items;   // NaN too
+                    if (t < rows && !(fabsf(shift) < INFINITY)) sh.bad = items;   // NaN too
                 }
                 {   // a lane has two nodes' masks, a warp makes the bits of four nodes
                     const unsigned long long* masks = a.masks + (int64_t)w.r * a.nodes;
                     const unsigned long long lo = lane < a.nodes ? __ldcg(masks + lane) : 0ull, hi = lane + 32 < a.nodes ? __ldcg(masks + lane + 32) : 0ull;
-                    if (a.used)
-                        counted = (unsigned long long)__ballot_sync(0xffffffffu, a.counts(hi)) << 32 | __ballot_sync(0xffffffffu, a.counts(lo)) | every;
 #pragma unroll
                     for (int u = 0; u < kTreeNodes / (4 * kWeighGroups); ++u) {
                         const int node = (warp - 2) * (kTreeNodes / (4 * kWeighGroups)) + u;
@@ -342,7 +339,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) tree_weigh_kernel(const __gr
             const bool page = (good >> (at >> 4)) & 1u;
             float sum = 0.f;   // columns behind the last row are products with it too
             // What comes of a position behind the end or without a page is not used.
-            const unsigned long long seen = (node < 0 || node >= a.nodes ? ~0ull : sh.seen_by[node] | every) & counted;
+            const unsigned long long seen = node < 0 || node >= a.nodes ? ~0ull : sh.seen_by[node] | every;
             if (__all_sync(0xffffffffu, seen == ~0ull) && sh.bad != items) {   // every row sees all 32 positions
                 uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll 1
