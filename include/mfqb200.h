@@ -457,8 +457,8 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const struct mfqb_cache* cache);
 /* Passes over the attached pages that add up how much every position was looked at and go on behind evicted ones (mfqb_cache_evict): weights float32
  * [layers][rows][kv_heads][width * page] of mfqb_tree_attention_weigh (16-byte aligned; null: none), dropped int32 [rows] (null: none), what has been
  * evicted of every sequence so far, which is added to its positions.  Both are the caller's memory on the decoder's device and must outlive the
- * passes; attaching a cache (mfqb_decoder_set_cache) takes them off again.  Allocates as mfqb_decoder_set_cache does.  Weights do not
- * move with sequences: mfqb_decoder_beam_step is refused meanwhile.  A branch that is kept of a tree (mfqb_decoder_verify) takes its weights along by
+ * passes; attaching a cache (mfqb_decoder_set_cache) takes them off again.  Allocates as mfqb_decoder_set_cache does.  Neither
+ * moves with sequences: mfqb_decoder_beam_step is refused with either.  A branch that is kept of a tree (mfqb_decoder_verify) takes its weights along by
  * mfqb_tree_accept_weigh; with mfqb_tree_accept its tokens would have those of the nodes whose places they take.  Nodes that are unused
  * (mfqb_tree_masks), all of a sequence's or some, add nothing here, unlike in mfqb_tree_attention_weigh, where every node of the call has queries. */
 int mfqb_decoder_set_weights(mfqb_decoder* d, float* weights, const int32_t* dropped);

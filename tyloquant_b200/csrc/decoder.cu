@@ -1141,7 +1141,8 @@ int mfqb_decoder_beam_step(mfqb_decoder* d, const int32_t* ids_in, int beams, fl
         if (!d || !ids_in || !scores || !done || !ids_out || !parents_out || !status) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: null argument");
         if (!d->paged) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: needs a cache (mfqb_decoder_set_cache)");
         const int rows = d->cache.rows;
-        if (d->weights || d->dropped) fail(MFQB_ERR_UNSUPPORTED, "mfqb_decoder_beam_step: weights are attached, which do not move with sequences");
+        if (d->weights) fail(MFQB_ERR_UNSUPPORTED, "mfqb_decoder_beam_step: weights are attached, which do not move with sequences");
+        if (d->dropped) fail(MFQB_ERR_UNSUPPORTED, "mfqb_decoder_beam_step: counts of dropped positions are attached, which do not move with sequences");
         if (beams < 1 || rows % beams) fail(MFQB_ERR_ARG, "mfqb_decoder_beam_step: %d sequences do not make groups of %d beams", rows, beams);
         check_ready(d, rows, "mfqb_decoder_beam_step");
         DeviceGuard guard(d->device);
