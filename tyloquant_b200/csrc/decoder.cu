@@ -1031,6 +1031,8 @@ int mfqb_decoder_set_cache(mfqb_decoder* d, const mfqb_cache* cache) {
         if (!d) fail(MFQB_ERR_ARG, "mfqb_decoder_set_cache: null decoder");
         if (!cache) {
             d->paged = false;
+            d->weights = nullptr;
+            d->dropped = nullptr;
             return;
         }
         check_cache(cache, "mfqb_decoder_set_cache");

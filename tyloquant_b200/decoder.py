@@ -94,12 +94,19 @@ class Decoder:
             raise ValueError("weights and dropped go with a cache")
         if weights is not None:
             cache._weights(weights)
+            if weights.data_ptr() % 16:
+                raise ValueError("weights must be 16-byte aligned")
         if dropped is not None and _need(dropped, torch.int32, (cache.rows,), self.device, "dropped") is not dropped:
             raise ValueError("dropped must be contiguous")
         check(lib.mfqb_decoder_set_cache(self._h, None if cache is None else C.byref(cache._view)))
         self._cache, self._beside = cache, (weights, dropped)   # borrowed by the native object
         if weights is not None or dropped is not None:
-            check(lib.mfqb_decoder_set_weights(self._h, None if weights is None else weights.data_ptr(), None if dropped is None else dropped.data_ptr()))
+            try:
+                check(lib.mfqb_decoder_set_weights(self._h, None if weights is None else weights.data_ptr(), None if dropped is None else dropped.data_ptr()))
+            except Exception:   # no memory for what its passes need: no pages without what was asked for beside them
+                lib.mfqb_decoder_set_cache(self._h, None)
+                self._cache, self._beside = None, None
+                raise
 
     def _rows(self, t, shape, dtype, what):
         from .cache import _need
