@@ -63,3 +63,12 @@ def test_split_rows_of_equal_logits(vocab):
         x = _apart(z, skip, 1, torch.float32)
         for top in (1, 5, 32):
             _check(x, [0, vocab - 1, 9018, 3, vocab - 1], top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 32767), (1, 32769), (2, 65535), (2, 65537), (150, 66001), (149, 33001), (40, 80011), (38, 79993), (37, 80011)])
+def test_around_the_numbers_of_ctas(rows, vocab, dtype):
+    """One, two, four and eight CTAs a row, by bytes, rows and logits of a slice."""
+    rng = np.random.default_rng(vocab)
+    z = _apart(2.5 * rng.standard_normal((rows, vocab), dtype=np.float32), 1, 2, dtype)
+    _check(z, [(0, vocab - 1, vocab // 3, -1)[r % 4] for r in range(rows)], 7)

@@ -8,7 +8,7 @@
 namespace mfqb {
 
 constexpr int kLpTop = 32, kLpGroups = 64, kLpList = 1024, kLpBatch = 4, kLpCtas = 8;
-constexpr int kLpVocab = 1 << 20, kLpBrief = 8192;
+constexpr int kLpVocab = 1 << 20, kLpBrief = 8192, kLpSplit = 128 << 10, kLpSlice = 10000;
 
 struct LogprobArgs {
     const char* logits;
@@ -392,11 +392,15 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const __grid_
 
 template <typename T>
 static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
-    // CTAs of a row: two, four or eight, as long as all are on the SMs at once and a slice has more than 16000 logits.  Rows of 128256 in float32: one row 7.6 us with eight,
-    // 8.6 with four, 14.4 with one, 7.7 with 16; 64 rows 13.3 with eight, 25.8 with one; 230 rows 26 with two, 33 with one; 300 rows 35.5 with one, 43 with two.  Rows of
-    // 32001: 30 rows 6.9 with one, 7.6 with two, 8.1 with eight; 90 rows 7.5, 9.0, 15.
+    // CTAs of a row.  Joining them costs some 1 to 2 us, which rows of up to 128 KB do not earn: 30, 230 rows of 32768 in float32 6.4, 11.8 us with one and 6.9, 12.3 with two, of
+    // 40000 7.9, 14.3 and 7.5, 13.1; of 50257 in bfloat16 8.0, 13.8 and 8.0, 14.2, of 80000 10.3, 19.0 and 9.0, 17.9 (one row gains from 80 KB on: 64000 in bfloat16 8.0
+    // and 7.5).  Above that two, four: as long as all are on the SMs at once (300 rows of 128256: 35.5 with one, 43 with two).  Eight where a slice keeps 10000 logits and
+    // an SM has two of them at most: 30 rows of 64000 7.8 with four, 8.9 with eight, of 100000 10.5 and 9.7, of 262144 17.7 and 14.0; 70 rows of 128256 14.5 and 16.2;
+    // one row of 128256 14.4, 10.5, 8.5 and 7.5 with one, two, four, eight (five alternatives; twenty: 18.2, 12.6, 9.8, 8.8).
     int ctas = 1;
-    while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= 4 * 148 && a.vocab / (2 * ctas) > 16000) ctas *= 2;
+    const int64_t bytes = (int64_t)a.vocab * sizeof(T);
+    if (bytes > kLpSplit)
+        while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= (ctas < 4 ? 4 : 2) * 148 && (ctas < 4 || a.vocab / kLpCtas >= kLpSlice)) ctas *= 2;
     // Four CTAs on an SM read more at a time (1024 rows of 128256 in float32: 92 us, 109 with three), three have more registers (one row: 10.3 and 9.7 us with 16 CTAs).
     const bool four = (int64_t)rows * ctas > 3 * 148;
     // Many short rows are a chain each, of which more run at once in CTAs of 128 threads, eight on an SM: 4000 rows of 1000 in float32
