@@ -542,7 +542,8 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
 /* The same attention, which also adds up how much every position was looked at: weights float32 [layers][rows][kv_heads][width * page], of which the
  * call changes the layer's.  With p(i, h, t) the probability that node i's query head h gives position t, kv head g of sequence r
  * gets the sum over the nodes and over its query heads: added at positions t < lens[r], written over what was there at lens[r] <= t <
- * lens[r] + nodes (what the nodes' slots held is of tokens that are gone).  All else stays.  Probabilities are float32 here.  A position without a page
+ * lens[r] + nodes (what the nodes' slots held is of tokens that are gone).  All else stays.  Probabilities are float32 here, of float32
+ * scores: off by some 2^-23 of the largest |scale q.k| of their row.  A position without a page
  * gets nothing (a node's: 0), nor does one whose score is minus infinity; a NaN or plus infinity among the scores of a row makes NaN of the weights
  * of all else that it sees.  Each sum is made in one order: a call repeats bit for bit.  out is the same as of
  * mfqb_tree_attention.  weights overlaps neither q, out nor work.  All nodes' queries count: those of drafted nodes that are rejected

@@ -128,7 +128,8 @@ __device__ __noinline__ float weigh_some(const TreeArgs& a, const float4* s_shif
 // 280), one issues tcgen05.mma, and of sixteen that sum a group of four has a half of the rows of every other tile; the second halves' sums
 // wait in shared memory until the first group's next tile.
 // weight = exp2(scale' s + shift), shift = - m - log2(l): one number per row, read from shared memory by all threads at once (two, m and 1 / l, made
-// it 8 us more; a shift of size 2^5 is off by 2^-20, the weight by 2^-20.5 of itself).
+// it 8 us more).  Its rounding grows with the scores: a shift of size 2^5 is off by 2^-19 at most and the weight by 0.7 times that of itself, one of 2^10 by 2^-14.  That is
+// as much as a float32 score of this size is off by itself; weights from kept scores, which keep m and 1 / l apart, are nearer where scores happen to be exact.
 // Bound by latency: the chain product - scores out of tensor memory (some 500 clocks a load) - exponentials - hand-over, with two tiles of scores in flight.  4
 // sequences at 32768 positions, 64 nodes in groups of 4, 8 kv heads: 124 us where the exponentials' unit needs 62 and the keys 41.  Eight warps with
 // loads of 32 rows ahead took 133 to 143, products of 128 rows each in four places 122 to 131 with slower short batches.
