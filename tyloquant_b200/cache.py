@@ -205,7 +205,8 @@ class PagedCache:
         ``weights`` (``new_weights``), changed in place: for every kv head of the layer, the probabilities that the nodes and the head's queries
         give to a position are added to its entry; the nodes' own entries, at positions from ``lens`` on, are set.  All nodes count, those that are
         rejected afterwards too, and unused ones (mask 0), which see the context.  ``accept`` moves a branch's entries where it is given the weights; ``fork`` moves keys and values alone: entries of
-        sequences that go on from others are the caller's to move (``weights[:, parents]``)."""
+        sequences that go on from others are the caller's to move (``weights[:, parents]``).  With weights, and up to 64 nodes x query heads of a KV head, a
+        call allocates 4 bytes for each of them and each position of the table (up to 512 MB; more are made again from the keys)."""
         torch = _torch()
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != HEAD_DIM:
             raise ValueError(f"q must be [{self.rows}, nodes, q_heads, 128], got {list(q.shape)}")

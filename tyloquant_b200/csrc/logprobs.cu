@@ -1,7 +1,6 @@
 // Log probabilities of given tokens, with entropy, rank and the best alternatives: one pass over the logits.
 #include <cuda_fp16.h>
 
-
 #include "select.cuh"
 #include "tc05.cuh"
 
@@ -148,9 +147,10 @@ __device__ __forceinline__ unsigned long long remote_u64(uint32_t addr) {
 // best: a bound that at least k logits reach comes from the maxima of 64 groups of threads (the k-th largest of them), and only the
 // vectors of threads whose own maximum reaches it are read again, a warp for each of those threads.  Where too many logits reach the
 // bound (equal ones, or all in a few threads' vectors) the cut is searched by counting instead.
-// Sums are float32, a thread's own of some hundred terms each, joined in a tree: log probabilities are off by about 1e-7 of themselves.  Many rows: bound by memory
-// and by issue (1024 rows of 128256 in float32: 95 us, 5.5 TB/s, 12 instructions a logit; with checks of the ends of a row in the loop 19 instructions and 111 us).  One row: a
-// chain of trips (7.6 us: the logits, the hot threads' vectors again, the cluster's lists).
+// Sums are float32, a thread's own of some hundred terms each, joined in a tree: a log sum is off by some 1e-7 (the sum is 1 and more, so a log probability
+// below 6e-8 in size comes out as 0, and one of -1e-6 is off by a tenth of itself), an entropy likewise.  Many rows: bound by memory and by issue (1024 rows of 128256 in float32,
+// five alternatives: 92 us, 5.7 TB/s, 12.6 instructions a logit; with checks of the ends of a row in the loop 19 instructions and 111 us).  One row: a chain of trips (7.5 us,
+// with twenty alternatives 8.8: the logits, the hot threads' vectors again, the cluster's lists).
 template <typename T, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int kN = LpVec<T>::kN, kLpThreads = THREADS, kLpWarps = THREADS / 32;
@@ -401,10 +401,11 @@ static void launch_logprobs(const LogprobArgs& a, int rows, cudaStream_t s) {
     const int64_t bytes = (int64_t)a.vocab * sizeof(T);
     if (bytes > kLpSplit)
         while (ctas < kLpCtas && (int64_t)rows * ctas * 2 <= (ctas < 4 ? 4 : 2) * 148 && (ctas < 4 || a.vocab / kLpCtas >= kLpSlice)) ctas *= 2;
-    // Four CTAs on an SM read more at a time (1024 rows of 128256 in float32: 92 us, 109 with three), three have more registers (one row: 10.3 and 9.7 us with 16 CTAs).
+    // Four CTAs on an SM read more at a time (1024 rows of 128256 in float32 92 us, 108 with three; in bfloat16 60 with either), three have more registers (300 rows 35.3 us, 37.6 with
+    // four; in bfloat16 27.7 and 34.4).
     const bool four = (int64_t)rows * ctas > 3 * 148;
     // Many short rows are a chain each, of which more run at once in CTAs of 128 threads, eight on an SM: 4000 rows of 1000 in float32
-    // 20.5 us, 30 in CTAs of 256; 2000 of 8000 21.8 and 27.8; 1500 of 32001 47 and 44.
+    // 22 us, 33.6 in CTAs of 256; 2000 of 8000 21.6 and 27.7; 1500 of 32001 47 and 43 (600 of 16000 13.7 and 14.9, in bfloat16 14.6 and 14.0).
     const bool brief = four && ctas == 1 && a.vocab <= kLpBrief;
     const int threads = brief ? 128 : 256;
     cudaLaunchConfig_t cfg = {};

@@ -52,8 +52,8 @@ struct CutShared {
 // thread's share of the keys, the same ones every time, at places 0 .. places - 1; a key 0 is none.  low and high are the smallest and the
 // largest of the thread's (all ones and 0 where there are none).  Bins divide the range from the smallest to the largest key: float32 values
 // that span orders of magnitude lie in many of them (by the first bits of the keys they would meet in a few counters, whose additions
-// wait for one another), and three rounds of 11 bits are enough for any range.  Weights are mostly positive with some zeros, far below the others in this
-// order: the first round's first bin has all that is not above zero, the others divide the rest.  A round ends the search when all of its last bin is in, or
+// wait for one another), and three rounds of 11 bits are enough for any range, a fourth where the first one splits at zero.  Weights are mostly positive with some zeros, far below the
+// others in this order: the first round's first bin has all that is not above zero, the others divide the rest.  A round ends the search when all of its last bin is in, or
 // when that holds so few keys that they are better counted against each other.  The next one goes by what the keys of the bin span; where
 // they are equal, by their places.
 template <int THREADS, class Each>

@@ -87,7 +87,8 @@ class Decoder:
         ``weights`` (``cache.new_weights()``): every pass adds up in them how much each position was looked at, for ``cache.evict``.  ``dropped`` (int32
         [rows]): what has been evicted of every sequence so far, added to its positions; add to it what ``evict`` returns.  Both are kept
         alive like the cache; ``beam_step`` is refused with either.  After ``verify`` give the weights to ``cache.accept`` too, which moves the kept
-        branch's; what the queries of rejected nodes have added to the context's positions stays.  Unused nodes add nothing."""
+        branch's; what the queries of rejected nodes have added to the context's positions stays.  Unused nodes add nothing.  The passes' work memory, which
+        stays with the decoder, holds scores then: up to 512 MB (see ``PagedCache.attend``)."""
         from .cache import _need
         torch = _torch()
         if cache is None and (weights is not None or dropped is not None):
