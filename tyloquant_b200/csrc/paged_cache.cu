@@ -443,7 +443,9 @@ static void launch_cache_rope(const mfqb_cache& c, int layer, const void* qkv, i
 // written, since a slot that one node leaves is another one's place.  A chain from the lengths to the rows: one tree of 8 nodes 4.2 us, 16 of 48
 // with branches of 13 in 128 heads 8.6 (a launch for the walk and one for the rows: 5.0 and 9.0; with a CTA for each head of each layer 11).  Lengths
 // that change in place are a second launch, 0.7 and 1.1 us more.
-// weights (mfqb_tree_attention_weigh, or null): the branch's sums move along.
+// WEIGH: the branch's sums in weights (mfqb_tree_attention_weigh) move along.  A form of its own: as a pointer that may be null it took calls without weights from 9.0 to
+// 10.3 us (16 trees of 48 nodes).
+template <bool WEIGH>
 __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* ids, const int* parents, const int* targets, int nodes, int* count, int* token,
                                                      int* path, int* lens_out, float* weights) {
     chained_wait();
@@ -516,13 +518,15 @@ __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* id
         }
         float* sums = nullptr;   // of the head that this thread moves a sum of; positions have one whether they have a page or not
         float sum = 0.f;
-        if (weights && t < each * n && h0 + t / n < heads) {
-            const int64_t head = h0 + t / n, layer = head / c.kv_heads;
-            const int node = t % n;
-            float* base = weights + ((layer * c.rows + r) * c.kv_heads + (head - layer * c.kv_heads)) * cap + len;
-            if (s_path[node] != node && len + s_path[node] < cap) {   // a node of a branch is never before its place
-                sum = __ldcg(base + s_path[node]);
-                sums = base + node;
+        if constexpr (WEIGH) {
+            if (t < each * n && h0 + t / n < heads) {
+                const int64_t head = h0 + t / n, layer = head / c.kv_heads;
+                const int node = t % n;
+                float* base = weights + ((layer * c.rows + r) * c.kv_heads + (head - layer * c.kv_heads)) * cap + len;
+                if (s_path[node] != node && len + s_path[node] < cap) {   // a node of a branch is never before its place
+                    sum = __ldcg(base + s_path[node]);
+                    sums = base + node;
+                }
             }
         }
         __syncthreads();
@@ -532,7 +536,8 @@ __global__ void __launch_bounds__(256) accept_kernel(mfqb_cache c, const int* id
                 static_cast<uint4*>(c.k)[to[i]] = kv[i][0];
                 static_cast<uint4*>(c.v)[to[i]] = kv[i][1];
             }
-        if (sums) *sums = sum;
+        if constexpr (WEIGH)
+            if (sums) *sums = sum;
     }
 }
 
@@ -555,7 +560,7 @@ static void accept(const mfqb_cache* c, const int32_t* ids, const int32_t* paren
     // enough CTAs for the SMs, at least one head each (how many nodes a branch has is known on the device alone)
     const int per_row = std::min(c->layers * c->kv_heads, std::max(1, 148 * 5 / c->rows));
     const bool in_place = lens_out < c->lens + c->rows && c->lens < lens_out + c->rows;
-    launch_chained(accept_kernel, dim3((unsigned)per_row, c->rows), dim3(256), 0, s, *c, ids, parents, targets, nodes, count, token, path,
+    launch_chained(weights ? accept_kernel<true> : accept_kernel<false>, dim3((unsigned)per_row, c->rows), dim3(256), 0, s, *c, ids, parents, targets, nodes, count, token, path,
                    in_place ? nullptr : lens_out, weights);
     if (in_place) launch_chained(accept_lens_kernel, dim3(1), dim3(1024), 0, s, *c, static_cast<const int*>(count), lens_out);
 }
