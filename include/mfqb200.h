@@ -547,7 +547,7 @@ int mfqb_tree_attention(const mfqb_cache* c, int layer, const void* q, int q_hea
  * gets nothing (a node's: 0), nor does one whose score is minus infinity; a NaN or plus infinity among the scores of a row makes NaN of the weights
  * of all else that it sees.  Each sum is made in one order: a call repeats bit for bit.  out is the same as of
  * mfqb_tree_attention.  weights overlaps neither q, out nor work.  All nodes' queries count: those of drafted nodes that are rejected
- * afterwards, and those of nodes with mask 0, which see what is below lens (trees of different sizes in one call: call it for each size).
+ * afterwards, and those of nodes with mask 0, which see what is below lens (a decoder's passes leave these out: mfqb_decoder_set_weights).
  * mfqb_tree_accept and mfqb_cache_fork move keys and values alone; mfqb_tree_accept_weigh moves a branch's weights along.
  * work: device memory of mfqb_tree_attention_weigh_work bytes, 16-byte aligned (with the scores of up to 64 query rows of a kv head, where
  * they take at most 512 MB). */
